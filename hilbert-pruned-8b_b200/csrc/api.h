@@ -306,6 +306,26 @@ int hb_parallel_sum(float* x, long long ldx, const float* y, long long ldy, cons
 int hb_side_unit(const float* s, long long lds, const int* tokens, const void* table, int table_dtype, long long ldt, long long col0, int vocab,
                  void* out, int out_dtype, long long ldo, int dim, int n_out, int n_tokens, int* status, void* stream);
 
+// A bounded cache (attention_mass.cu, evict.cu): attention that also adds up every cached row's weight, for steps of many and of
+// few tokens; the choice of the rows that stay (kept, ascending, -1 behind the last); their move, in place (to_table null) or into
+// pages of their own.  before may be null or mass.
+int hb_attention_mass(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
+                      int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse,
+                      const float* before, float* mass, float* parts, int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles,
+                      int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* status, void* stream);
+int hb_attention_few_pairs(void);
+long long hb_attention_mass_few_floats(int n_tokens, int n_heads, int head_dim, int splits, int max_len);
+int hb_attention_mass_few(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
+                          int pt_width, const int* tok_seq, const int* positions, const int* seq_start, const int* seq_pos0, void* out,
+                          long long out_stride, float* scratch, const float* before, float* mass, int splits, int n_tokens, int n_seqs,
+                          int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages,
+                          int* status, void* stream);
+int hb_evict_select(const float* mass, const int* page_table, int pt_width, const int* lengths, int* kept, int entries, int n_seqs,
+                    int n_kv_heads, int n_pages, int first, int recent, int budget, int threads, int cluster, int* status, void* stream);
+int hb_evict_rows(const int* kept, void* k, int k_row_bytes, void* v, int v_row_bytes, float* mass, const int* from_table, int from_width,
+                  const int* to_table, int to_width, int entries, int n_seqs, int n_kv_heads, int n_pages, int budget, int sm_count,
+                  int* status, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

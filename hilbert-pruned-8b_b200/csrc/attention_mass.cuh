@@ -1,0 +1,80 @@
+// What the kernels of attention with accumulated weights share: where a block's queries or keys are, and how a key's sum of
+// weights is written.
+#pragma once
+#include "common.cuh"
+
+#define MASS_LOG2E 1.4426950408889634f
+#define MASS_FEW_PAIRS 512           // (tokens of a sequence) x (heads of a group) that a step of few tokens may have
+
+// before (null: nothing is added), mass: [n_pages][kv heads][64]; before may be mass.  parts: [shares][kv heads][places], where a
+// place is a key's number over all tiles of keys of the step.
+struct MassOut {
+    const float* before;
+    float* mass;
+    float* parts;
+};
+
+// distance, in floats, of the scores of two heads
+static __host__ __device__ inline long long mass_score_ld(int max_len) { return ((long long)max_len + 63) / 64 * 64; }
+
+// The sequence b and its block blk of `rows` new tokens that block number `at` of the step stands for.
+__device__ __forceinline__ bool mass_find_block(const int* __restrict__ seq_start, int n_seqs, int at, int rows, int& b, int& blk) {
+    for (b = 0; b < n_seqs; b++) {
+        const int nb = (seq_start[b + 1] - seq_start[b] + rows - 1) / rows;
+        if (at < nb) {
+            blk = at;
+            return true;
+        }
+        at -= nb;
+    }
+    return false;
+}
+
+// The sequence b and its tile kt of `tile` rows of the cache (those behind this step) that tile number `at` stands for.
+__device__ __forceinline__ bool mass_find_keys(const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, int n_seqs, int at, int tile,
+                                               int& b, int& kt) {
+    for (b = 0; b < n_seqs; b++) {
+        const int nb = (seq_pos0[b] + seq_start[b + 1] - seq_start[b] + tile - 1) / tile;
+        if (at < nb) {
+            kt = at;
+            return true;
+        }
+        at -= nb;
+    }
+    return false;
+}
+
+// The new tokens [n0, n1) of a sequence that see one of the keys [key0, key0 + keys): token i stands at pos0 + i.
+__device__ __forceinline__ void mass_queries(int key0, int keys, int pos0, int n_new, int window, int& n0, int& n1) {
+    n0 = max(0, key0 - pos0);
+    n1 = n_new;
+    if (window > 0) n1 = (int)min((long long)n_new, (long long)key0 + keys - 1 + window - pos0);
+    if (n1 <= n0) n1 = n0 = 0;
+}
+
+__device__ __forceinline__ void mass_write(const MassOut& mo, float sum, int g, int key, int page, int nkv, int n_pages, int pos0, int n_new) {
+    if (key >= pos0 + n_new || page < 0 || page >= n_pages) return;       // behind the end, or a page that was given back
+    const size_t at = ((size_t)page * nkv + g) * HB_PAGE_TOKENS + (key & (HB_PAGE_TOKENS - 1));
+    const float old = (key < pos0 && mo.before != nullptr) ? __ldcg(mo.before + at) : 0.0f;
+    mo.mass[at] = old + sum;
+}
+
+// a key's sum, or with several shares (S) share z of it
+__device__ __forceinline__ void mass_store(const MassOut& mo, float sum, int b, int g, int key, int page, int nkv, int n_pages, int pos0, int n_new,
+                                           int z, int S, size_t place, size_t places) {
+    if (S > 1) mo.parts[((size_t)z * nkv + g) * places + place] = sum;
+    else mass_write(mo, sum, g, key, page, nkv, n_pages, pos0, n_new);
+}
+
+__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+    const float4 v = *reinterpret_cast<const float4*>(p);
+    x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+__device__ __forceinline__ void load4(const bf16* p, float (&x)[4]) {
+    const uint2 v = *reinterpret_cast<const uint2*>(p);
+    x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+    x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+
+int mass_join(const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0, MassOut mo, int n_seqs, int nkv, int n_pages, int tile,
+              int key_tiles, int splits, cudaStream_t s);

@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import build
-from .plan import decode_splits
+from .plan import decode_splits, mass_splits, select_shape
 
 _c_int, _c_ll, _c_float, _c_ptr = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
 
@@ -79,6 +79,15 @@ _SIGNATURES = {
                              _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_prefill_tc": [_c_ptr, _c_ll, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_int,
                                 _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
+    "hb_attention_mass": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                          _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
+    "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr,
+                              _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr,
+                              _c_ptr],
+    "hb_evict_select": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr,
+                        _c_ptr],
+    "hb_evict_rows": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
+                      _c_int, _c_ptr, _c_ptr],
     "hb_random_normal": [_c_ptr, _c_int, _c_ll, ctypes.c_ulonglong, _c_float, _c_float, _c_ptr],
     "hb_argmax": [_c_ptr, _c_ll, _c_ptr, _c_int, _c_int, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr],
     "hb_sample": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_int, _c_ptr, _c_ptr],
@@ -176,6 +185,8 @@ def load_library():
         lib.hb_gemm_tc2_resident_pairs.argtypes, lib.hb_gemm_tc2_resident_pairs.restype = [_c_int], _c_int
         for name in ("hb_attention_decode_supported", "hb_attention_prefill_supported", "hb_attention_prefill_tc_supported"):
             getattr(lib, name).argtypes, getattr(lib, name).restype = [_c_int, _c_int, _c_int], _c_int
+        lib.hb_attention_few_pairs.argtypes, lib.hb_attention_few_pairs.restype = [], _c_int
+        lib.hb_attention_mass_few_floats.argtypes, lib.hb_attention_mass_few_floats.restype = [_c_int] * 5, _c_ll
         lib.hb_attention_sink_prefill_supported.argtypes, lib.hb_attention_sink_prefill_supported.restype = [_c_int] * 4, _c_int
         lib.hb_attention_sink_prefill_tc_supported.argtypes, lib.hb_attention_sink_prefill_tc_supported.restype = [_c_int] * 4, _c_int
         lib.hb_attention_group_supported.argtypes, lib.hb_attention_group_supported.restype = [_c_int] * 5, _c_int
@@ -1223,6 +1234,145 @@ class Ops:
                    step.tok_seq.data_ptr(), step.positions.data_ptr(), out.data_ptr(), _code(out),
                    _rows(out, "attention output"), T, heads, kv_heads, head_dim, float(scale), win, cache.k.shape[0],
                    self.status.data_ptr(), self._stream())
+        self.launches += 1
+
+    # ------------------------------------------------------------------ a bounded cache
+    MASS_FEW_TOKENS = 8             # a step whose sequences bring more tokens than this takes the kernels for many tokens
+
+    @staticmethod
+    def _mass_like(t, what: str, pages: int, kv_heads: int) -> None:
+        if t.dtype != torch.float32 or tuple(t.shape) != (pages, kv_heads, 64) or not t.is_contiguous():
+            raise KernelError(f"attention: {what} must be a contiguous float32 [{pages}, {kv_heads}, 64] (pages, kv heads, rows of a "
+                              f"page), got {t.dtype} {tuple(t.shape)}")
+
+    def attention_mass(self, qkv, heads: int, kv_heads: int, head_dim: int, cache, step, out, scale: float, window: Optional[int], mass,
+                       before=None, splits: Optional[int] = None) -> None:
+        """``attention``, and how much weight every cached row got: for each sequence of the step, kv head g and row j,
+        ``mass[page of j, g, j % 64] = before[the same] + the sum over the sequence's tokens in this step and the query heads of g of
+        their softmax weight of j`` in 32-bit; rows that this step itself appended start from zero, whatever ``before`` holds
+        there.  ``before``: None (this step's weights alone), another tensor, or ``mass`` itself (a running sum).  Rows that no
+        sequence of the step holds are neither read nor written.  The step's new keys and values are in the cache already, as for
+        ``attention``; queries, cache and output have one type.  The sums do not depend on what else runs (fixed order)."""
+        self._dev(qkv, cache.k, cache.v, out, mass, before)
+        T = qkv.shape[0]
+        pt = step.page_tables[cache.group]
+        pages = cache.k.shape[0]
+        if kv_heads < 1 or heads % kv_heads or not 0 < head_dim <= 256:
+            raise KernelError(f"attention: {heads} heads over {kv_heads} kv heads of size {head_dim} are not built (sizes up to 256)")
+        if qkv.shape[1] < heads * head_dim or out.shape[0] != T or out.shape[1] != heads * head_dim or T != step.num_tokens:
+            raise KernelError("attention: query or output shape does not match")
+        want = (pages, kv_heads, 64, head_dim)
+        if tuple(cache.k.shape) != want or tuple(cache.v.shape) != want or not cache.k.is_contiguous() or not cache.v.is_contiguous():
+            raise KernelError("attention: cache layer shape does not match the heads")
+        if not qkv.dtype == cache.k.dtype == cache.v.dtype == out.dtype:
+            raise KernelError("attention: queries, cache and output must have one dtype")
+        self._mass_like(mass, "mass", pages, kv_heads)
+        if before is not None:
+            self._mass_like(before, "before", pages, kv_heads)
+        if T == 0:
+            return
+        win = int(window) if window else 0
+        old = before.data_ptr() if before is not None else None
+        code, group = _code(qkv), heads // kv_heads
+        q_ld, out_ld = _rows(qkv, "attention queries"), _rows(out, "attention output")
+        # scratch of the call's own, from torch's allocator: two calls on two streams, or two captured graphs, share nothing
+        with torch.cuda.device(self.device):
+            if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * group <= self.lib.hb_attention_few_pairs():
+                max_pages = (step.max_len + 63) // 64
+                if splits is None:
+                    splits = decode_splits(T, kv_heads * -(-group // 8), max_pages, 3 * self.sm_count)
+                splits = max(1, min(splits, max_pages))
+                scratch = torch.empty(self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len), dtype=torch.float32,
+                                      device=self.device)
+                self._call("hb_attention_mass_few", qkv.data_ptr(), code, q_ld, cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(),
+                           pt.shape[1], step.tok_seq.data_ptr(), step.positions.data_ptr(), step.seq_start.data_ptr(),
+                           step.seq_pos0.data_ptr(), out.data_ptr(), out_ld, scratch.data_ptr(), old, mass.data_ptr(), splits, T, step.num_seqs,
+                           step.max_new, step.max_len, heads, kv_heads, head_dim, float(scale), win, pages, self.status.data_ptr(), self._stream())
+                self.launches += 2
+                return
+            lse = torch.empty(heads * T, dtype=torch.float32, device=self.device)
+            q_blocks = sum((n + 63) // 64 for n in step.host_new)
+            key_tiles = sum((n + 63) // 64 for n in step.host_len)
+            if splits is None:
+                splits = mass_splits(key_tiles, kv_heads, group * -(-step.max_new // 64), 2 * self.sm_count)
+            parts = torch.empty(splits * kv_heads * key_tiles * 64, dtype=torch.float32, device=self.device) if splits > 1 else None
+            self._call("hb_attention_mass", qkv.data_ptr(), code, q_ld, cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(), pt.shape[1],
+                       step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out.data_ptr(), out_ld, lse.data_ptr(), old, mass.data_ptr(),
+                       parts.data_ptr() if parts is not None else None, splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim,
+                       float(scale), win, pages, self.status.data_ptr(), self._stream())
+            self.launches += 2 if splits == 1 else 3
+
+    def evict_select(self, mass, page_table, lengths, first: int, recent: int, kept) -> None:
+        """Which rows of each sequence stay, for every entry and kv head by itself.  ``mass`` ``[entries, pages, kv_heads, 64]`` (or one
+        entry's ``[pages, kv_heads, 64]``), ``page_table`` int32 ``[sequences, width]``, ``lengths`` int32 rows of each sequence, ``kept``
+        int32 ``[entries, sequences, kv_heads, budget]`` (or without the first axis).  Of a sequence longer than the budget the first
+        ``first`` rows stay, the last ``recent``, and of those between the ones with the largest mass until the budget is full; equal
+        masses: the lower row; NaN counts below everything.  ``kept`` holds the rows in ascending order, -1 behind the last."""
+        self._dev(mass, page_table, lengths, kept)
+        entries = mass.shape[0] if mass.dim() == 4 else 1
+        if mass.dim() not in (3, 4) or mass.dtype != torch.float32 or mass.shape[-1] != 64 or not mass.is_contiguous():
+            raise KernelError(f"evict_select: mass must be a contiguous float32 [entries, pages, kv_heads, 64], got {mass.dtype} {tuple(mass.shape)}")
+        pages, kv_heads = mass.shape[-3], mass.shape[-2]
+        self._tables("evict_select", page_table)
+        B = page_table.shape[0]
+        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous():
+            raise KernelError("evict_select: one int32 length per row of the page table expected")
+        budget = self._kept("evict_select", kept, mass.dim(), entries, B, kv_heads)
+        first, recent = int(first), int(recent)
+        if first < 0 or recent < 0 or first + recent > budget:
+            raise KernelError(f"evict_select: the first {first} and the last {recent} rows do not fit a budget of {budget}")
+        if not entries * B * kv_heads:
+            return
+        threads, cluster = select_shape(entries * B * kv_heads, page_table.shape[1] * 64, self.sm_count)
+        with torch.cuda.device(self.device):
+            self._call("hb_evict_select", mass.data_ptr(), page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), kept.data_ptr(), entries,
+                       B, kv_heads, pages, first, recent, budget, threads, cluster, self.status.data_ptr(), self._stream())
+        self.launches += 1
+
+    @staticmethod
+    def _tables(op: str, table) -> None:
+        if table.dtype != torch.int32 or table.dim() != 2 or not table.is_contiguous() or table.shape[1] < 1:
+            raise KernelError(f"{op}: a page table is a contiguous int32 [sequences, width], got {table.dtype} {tuple(table.shape)}")
+
+    @staticmethod
+    def _kept(op: str, kept, dims: int, entries: int, sequences: int, kv_heads: int) -> int:
+        want = (entries, sequences, kv_heads)[4 - dims:]
+        if kept.dtype != torch.int32 or kept.dim() != dims or tuple(kept.shape[:-1]) != want or kept.shape[-1] < 1 or not kept.is_contiguous():
+            raise KernelError(f"{op}: kept must be a contiguous int32 [{', '.join(map(str, want))}, budget], got {kept.dtype} {tuple(kept.shape)}")
+        return kept.shape[-1]
+
+    def evict_rows(self, kept, k, v, mass, page_table, to_table=None) -> None:
+        """Row ``kept[.., j]`` of the keys, values and mass of (entry, sequence, kv head) becomes row j: in the sequence's own pages, or
+        with ``to_table`` (int32 ``[sequences, width]``, room for the budget) in other pages, which no row of ``page_table`` may name;
+        the rows of ``page_table`` then stay as they were.  ``k``, ``v`` ``[entries, pages, kv_heads, 64, head size]``, ``mass`` (may be None)
+        ``[entries, pages, kv_heads, 64]``, or all without the first axis.  ``kept`` as ``evict_select`` gives it: ascending, -1 behind
+        the last; rows behind what is kept stay as they were."""
+        self._dev(kept, k, v, mass, page_table, to_table)
+        if k.dim() not in (4, 5) or v.dim() != k.dim() or v.shape[:-1] != k.shape[:-1] or k.shape[-2] != 64 or k.dtype != v.dtype \
+                or not k.is_contiguous() or not v.is_contiguous():
+            raise KernelError("evict_rows: keys and values must be contiguous [entries, pages, kv_heads, 64, head size] of one dtype")
+        _code(k)
+        if mass is not None and (mass.dtype != torch.float32 or mass.shape != k.shape[:-1] or not mass.is_contiguous()):
+            raise KernelError(f"evict_rows: mass must be a contiguous float32 {list(k.shape[:-1])}, got {mass.dtype} {tuple(mass.shape)}")
+        entries = k.shape[0] if k.dim() == 5 else 1
+        pages, kv_heads = k.shape[-4], k.shape[-3]
+        self._tables("evict_rows", page_table)
+        B = page_table.shape[0]
+        budget = self._kept("evict_rows", kept, k.dim() - 1, entries, B, kv_heads)
+        if to_table is not None:
+            self._tables("evict_rows", to_table)
+            if to_table.shape[0] != B:
+                raise KernelError("evict_rows: the two page tables are of different numbers of sequences")
+        if to_table is not None and budget > 64 * to_table.shape[1]:
+            raise KernelError(f"evict_rows: a budget of {budget} rows does not fit a page table of {to_table.shape[1]} pages")
+        if not entries * B * kv_heads:
+            return
+        es = k.element_size()
+        with torch.cuda.device(self.device):
+            self._call("hb_evict_rows", kept.data_ptr(), k.data_ptr(), k.shape[-1] * es, v.data_ptr(), v.shape[-1] * es,
+                       mass.data_ptr() if mass is not None else None, page_table.data_ptr(), page_table.shape[1],
+                       to_table.data_ptr() if to_table is not None else None, to_table.shape[1] if to_table is not None else 0, entries, B, kv_heads,
+                       pages, budget, self.sm_count, self.status.data_ptr(), self._stream())
         self.launches += 1
 
     # ------------------------------------------------------------------ norms on a sublayer's output

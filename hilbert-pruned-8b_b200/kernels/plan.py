@@ -26,3 +26,25 @@ def decode_splits(sequences: int, kv_heads: int, max_pages: int, cta_slots: int)
             if -(-max_pages // s) >= 32 and fill(s) - 0.01 * s > fill(best) - 0.01 * best + 0.1:
                 best = s
     return best
+
+
+def mass_splits(key_tiles: int, kv_heads: int, items: int, cta_slots: int) -> int:
+    """Shares of the weights' kernel for ``key_tiles`` x ``kv_heads`` (tile of keys, kv head) pairs with up to ``items`` tiles of
+    queries each: under a causal mask the first keys are seen by every query and the last by few, so the work evens out only
+    over several blocks per slot.  Four times as many blocks as slots, at most 16 shares, and a share has work."""
+    pairs = max(1, key_tiles * kv_heads)
+    return max(1, min(16, items, -(-4 * max(1, cta_slots) // pairs)))
+
+
+def select_shape(lists: int, rows: int, sms: int):
+    """(threads, blocks in a cluster) for choosing among ``rows`` rows in each of ``lists`` lists.  A thread keeps up to 32 rows in
+    registers: 512 threads (two blocks to an SM) where that holds a list, else 1024 and a cluster that does.  With few lists, more
+    blocks to a list while the device has SMs without one and a thread would still have 8 rows or more."""
+    per_thread = 32
+    threads = 512 if rows <= 512 * per_thread and lists > sms // 2 else 1024
+    cluster = 1
+    while cluster < 8 and rows > cluster * threads * per_thread:
+        cluster *= 2
+    while cluster < 8 and 2 * cluster * lists <= sms and rows >= 2 * cluster * threads * 8:
+        cluster *= 2
+    return threads, cluster

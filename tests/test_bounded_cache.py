@@ -1,0 +1,541 @@
+"""The operators of a bounded cache against plain implementations in 64 bits: attention that adds up every cached row's weight,
+the choice of the rows that stay, and their move; alone, refused, and one after another as a program uses them."""
+import math
+import random
+import types
+
+import pytest
+import torch
+
+from conftest import require_gpu
+
+DEV = "cuda:0"
+PAGE = 64
+NAN = float("nan")
+
+
+@pytest.fixture(scope="module")
+def ops():
+    require_gpu()
+    from hilbert_pruned_8b_b200.kernels.ops import Ops
+    return Ops(torch.device(DEV))
+
+
+# ------------------------------------------------------------------------------------------------------- inputs
+def _pages(n):
+    return (n + PAGE - 1) // PAGE
+
+
+def _tables(lengths, seed, extra=2, width=None):
+    rng = random.Random(seed)
+    total = sum(_pages(n) for n in lengths) + extra
+    order = list(range(total))
+    rng.shuffle(order)
+    width = width or max(1, max(_pages(n) for n in lengths))
+    rows = []
+    for n in lengths:
+        mine = [order.pop() for _ in range(_pages(n))]
+        rows.append(mine + [-1] * (width - len(mine)))
+    return torch.tensor(rows, dtype=torch.int32, device=DEV), total, order
+
+
+def _ints(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def _step(past, new, table):
+    starts = [0]
+    for n in new:
+        starts.append(starts[-1] + n)
+    lens = [p + n for p, n in zip(past, new)]
+    return types.SimpleNamespace(
+        num_tokens=sum(new), num_seqs=len(new), page_tables=[table], positions=_ints([p + i for p, n in zip(past, new) for i in range(n)]),
+        tok_seq=_ints([b for b, n in enumerate(new) for _ in range(n)]), seq_start=_ints(starts), seq_pos0=_ints(past), seq_len=_ints(lens),
+        max_new=max(new), max_len=max(lens), is_decode=all(n == 1 for n in new), host_new=list(new), host_len=lens, shared={}, tag="")
+
+
+class Case:
+    """Queries as the first columns of wider rows, a paged cache whose rows behind the sequences' ends hold NaN."""
+
+    def __init__(self, dtype, heads, kv, hd, past, new, window, seed=0, strong=1.0, garbage=NAN):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        self.dtype, self.heads, self.kv, self.hd, self.window = dtype, heads, kv, hd, window
+        self.past, self.new = list(past), list(new)
+        self.lens = [p + n for p, n in zip(past, new)]
+        self.table, self.pages, _ = _tables(self.lens, seed)
+        T = sum(new)
+        # one more head than is used: rows are further apart than the queries are wide
+        self.qkv = (torch.randn(T, (heads + 1) * hd, generator=g, device=DEV) * strong).to(dtype)
+        self.k = torch.full((self.pages, kv, PAGE, hd), garbage, dtype=dtype, device=DEV)
+        self.v = torch.full((self.pages, kv, PAGE, hd), garbage, dtype=dtype, device=DEV)
+        for b, n in enumerate(self.lens):
+            j = torch.arange(n, device=DEV)
+            page = self.table[b].long()[j // PAGE]
+            self.k[page, :, j % PAGE] = torch.randn(n, kv, hd, generator=g, device=DEV).to(dtype)
+            self.v[page, :, j % PAGE] = torch.randn(n, kv, hd, generator=g, device=DEV).to(dtype)
+        self.before = torch.rand(self.pages, kv, PAGE, generator=g, device=DEV) * 3
+        self.step = _step(self.past, self.new, self.table)
+        self.cache = types.SimpleNamespace(k=self.k, v=self.v, group=0, window=window)
+        self.scale = 1.0 / math.sqrt(hd)
+
+    def run(self, ops, mass, before=None, out=None, **kw):
+        if out is None:
+            out = torch.full((sum(self.new), self.heads * self.hd), 7.0, dtype=self.dtype, device=DEV)
+        ops.attention_mass(self.qkv, self.heads, self.kv, self.hd, self.cache, self.step, out, self.scale, self.window, mass, before=before, **kw)
+        return out
+
+    def check(self, out, mass, before, start):
+        """``start``: what ``mass`` held before the call."""
+        G, t0, u = self.heads // self.kv, 0, 2.0 ** -24
+        untouched = torch.ones_like(mass, dtype=torch.bool)
+        for b, (p0, n) in enumerate(zip(self.past, self.new)):
+            ln = p0 + n
+            j = torch.arange(ln, device=DEV)
+            page = self.table[b].long()[j // PAGE]
+            i = torch.arange(p0, ln, device=DEV)
+            hidden = j[None] > i[:, None]
+            if self.window:
+                hidden |= j[None] <= i[:, None] - self.window
+            untouched[page, :, j % PAGE] = False
+            for g in range(self.kv):
+                k, v = self.k[page, g, j % PAGE].double(), self.v[page, g, j % PAGE].double()
+                total, slack = torch.zeros(ln, dtype=torch.float64, device=DEV), torch.zeros(ln, dtype=torch.float64, device=DEV)
+                for h in range(g * G, (g + 1) * G):
+                    q = self.qkv[t0: t0 + n, h * self.hd: (h + 1) * self.hd].double()
+                    w = torch.softmax((q @ k.T * self.scale).masked_fill(hidden, -math.inf), dim=-1)
+                    # A score is a sum of hd products in 32 bits: off by at most hd steps of the sum of their sizes, B at
+                    # most (the tensor cores' accumulation counts as two of them).  In units of log 2 it is rounded again, and so is
+                    # the log-sum, at most B log2(e) + log2(rows) large: a weight's relative error is at most
+                    rel = 0.0
+                    if n:
+                        B = float((q.abs() @ k.abs().T).max()) * self.scale
+                        rel = 2 * (2 * self.hd + 8) * u * B + 4 * u * (1.45 * B + math.log2(ln + 1)) + 16 * u
+                    total += w.sum(0)
+                    slack += w.sum(0) * rel
+                    got = out[t0: t0 + n, h * self.hd: (h + 1) * self.hd].double()
+                    want, size = w @ v, w @ v.abs()
+                    # a weight's error, its rounding for the product, the order of a sum of ln terms, the result's rounding
+                    half = torch.finfo(self.dtype).eps / 2
+                    tol = size * (2 * rel + (half if self.dtype == torch.bfloat16 else 0.0) + (ln + 16) * u) + want.abs() * half + 1e-30
+                    assert torch.isfinite(got).all()
+                    assert bool(((got - want).abs() <= tol).all()), float(((got - want).abs() / tol).max())
+                if before is not None:
+                    old = torch.where(j < p0, before[page, g, j % PAGE], torch.zeros_like(before[page, g, j % PAGE])).double()
+                    total += old
+                got = mass[page, g, j % PAGE].double()
+                tol = slack + total.abs() * (n * G + 20) * u + 1e-30
+                assert torch.isfinite(got).all()
+                assert bool(((got - total).abs() <= tol).all()), float(((got - total).abs() / tol).max())
+            t0 += n
+        assert torch.equal(mass[untouched], start[untouched])         # rows of nobody stay as they were
+
+
+MANY = [
+    # heads, kv heads, head size, rows before, new tokens, window
+    (4, 2, 64, [0], [9], None),
+    (4, 2, 64, [0, 63, 64, 65], [64, 65, 1, 63], None),
+    (8, 2, 128, [0, 1000], [200, 300], None),
+    (3, 1, 128, [129, 0, 700], [127, 128, 1], None),
+    (6, 3, 128, [500, 0], [300, 257], 100),
+    (2, 2, 64, [1000, 3], [40, 700], 1),
+    (16, 1, 64, [10], [150], None),
+    (17, 1, 64, [100], [30], 64),
+    (6, 2, 80, [0, 333], [190, 75], 200),
+    (5, 1, 33, [70, 0], [12, 130], None),
+    (2, 1, 256, [100], [70], None),
+    (4, 4, 200, [0, 64], [64, 100], 65),
+    (1, 1, 8, [0], [10], None),
+]
+FEW = [
+    (4, 2, 64, [0], [1], None),
+    (4, 2, 64, [62, 63, 64, 65, 127, 128], [1, 1, 1, 1, 1, 1], None),
+    (32, 8, 128, [3000, 1, 511], [1, 1, 1], None),
+    (32, 8, 64, [2999], [1], None),
+    (3, 1, 128, [900, 0, 64], [3, 8, 1], None),
+    (16, 1, 64, [700, 30], [2, 5], 100),
+    (17, 1, 64, [700], [1], None),
+    (40, 1, 128, [300], [8], 33),
+    (6, 2, 80, [1500, 7], [1, 1], 1),
+    (5, 5, 33, [200, 0], [4, 2], None),
+    (2, 1, 256, [513], [1], 4096),
+    (2, 2, 200, [100, 5000], [1, 2], 70),
+]
+TYPES = [torch.bfloat16, torch.float32]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,hd,past,new,window", MANY + FEW)
+def test_attention_mass(ops, dtype, heads, kv, hd, past, new, window):
+    c = Case(dtype, heads, kv, hd, past, new, window, seed=hd + len(past))
+    start = torch.full((c.pages, kv, PAGE), 5.0, device=DEV)
+    mass = start.clone()
+    out = c.run(ops, mass, before=c.before)
+    c.check(out, mass, c.before, start)
+    # this step's weights alone; then a running sum, in place
+    alone = start.clone()
+    out2 = c.run(ops, alone)
+    c.check(out2, alone, None, start)
+    assert torch.equal(out, out2)
+    running = c.before.clone()
+    c.run(ops, running, before=running)
+    seen = mass != start
+    assert torch.equal(running[seen], mass[seen])
+    again = start.clone()
+    assert torch.equal(c.run(ops, again, before=c.before), out) and torch.equal(again, mass)      # the same bits
+    ops.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("heads,kv,hd,past,new,window,splits", [
+    (8, 2, 128, [0, 1000], [200, 300], None, 1), (8, 2, 128, [0, 1000], [200, 300], None, 5), (6, 3, 64, [500, 0], [300, 257], 100, 7),
+    (6, 2, 80, [0, 333], [190, 75], 200, 3), (8, 2, 128, [3000, 10], [1, 1], None, 1), (8, 2, 128, [3000, 10], [2, 8], None, 16),
+    (6, 2, 80, [1500, 7], [1, 1], 100, 24)])
+def test_shares_of_the_work(ops, dtype, heads, kv, hd, past, new, window, splits):
+    """More shares than pages or tiles of queries, and one: the same sums."""
+    c = Case(dtype, heads, kv, hd, past, new, window, seed=5)
+    start = torch.zeros(c.pages, kv, PAGE, device=DEV)
+    mass = start.clone()
+    c.check(c.run(ops, mass, before=c.before, splits=splits), mass, c.before, start)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("new", [[70, 5], [1, 1]])
+def test_peaked_and_flat_rows(ops, dtype, new):
+    """Scores far apart (one row has nearly all the weight) and all alike."""
+    for strong in (30.0, 0.0):
+        c = Case(dtype, 8, 2, 128, [300, 64], new, None, seed=9, strong=strong)
+        mass = torch.zeros(c.pages, 2, PAGE, device=DEV)
+        c.check(c.run(ops, mass), mass, None, torch.zeros_like(mass))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[90, 3], [1, 1]])
+def test_output_rows_apart_and_unaligned_queries(ops, new):
+    c = Case(torch.bfloat16, 4, 2, 64, [100, 70], new, None, seed=3)
+    T = sum(new)
+    wide = torch.zeros(T, 4 * 64 + 24, dtype=torch.bfloat16, device=DEV)
+    mass = torch.zeros(c.pages, 2, PAGE, device=DEV)
+    out = c.run(ops, mass, out=wide[:, 8: 8 + 256])
+    c.check(out, mass, None, torch.zeros_like(mass))
+    assert not wide[:, :8].any() and not wide[:, 264:].any()
+    odd = torch.zeros(T, 4 * 64 + 3, dtype=torch.bfloat16, device=DEV)            # rows at odd places of memory
+    odd[:, 1:257] = c.qkv[:, :256]
+    was, c.qkv = c.qkv, odd[:, 1:]
+    m2 = torch.zeros_like(mass)
+    got = c.run(ops, m2)
+    c.qkv = was
+    c.check(got, m2, None, torch.zeros_like(mass))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[90, 3], [1, 2]])
+def test_a_sequence_without_new_tokens(ops, new):
+    """Rows of a sequence that brings nothing keep their earlier sum."""
+    c = Case(torch.bfloat16, 4, 2, 64, [100, 30, 70], [new[0], 0, new[1]], None, seed=4)
+    start = torch.zeros(c.pages, 2, PAGE, device=DEV)
+    mass = start.clone()
+    c.check(c.run(ops, mass, before=c.before), mass, c.before, start)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[90], [1]])
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.bfloat16, 80), (torch.float32, 64)])
+def test_attention_mass_notes_a_missing_page(ops, dtype, hd, new):
+    from hilbert_pruned_8b_b200.kernels.ops import KernelError
+    for bad in (-1, 10 ** 6):
+        c = Case(dtype, 4, 2, hd, [200], new, None, seed=1, garbage=0.0)
+        c.table[0, 1] = bad
+        ops.reset_status()
+        c.run(ops, torch.zeros(c.pages, 2, PAGE, device=DEV))
+        with pytest.raises(KernelError, match="page"):
+            ops.check_errors()
+    ops.reset_status()
+    # a page in front of every token's window was given back: nobody's fault, and its rows have no place
+    c = Case(dtype, 4, 2, hd, [200], new, 20, seed=1, garbage=0.0)
+    mass = torch.zeros(c.pages, 2, PAGE, device=DEV)
+    want = c.run(ops, mass.clone())
+    c.table[0, 0] = -1
+    assert torch.equal(c.run(ops, mass), want)
+    ops.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[90, 40], [1, 3]])
+def test_captured_and_replayed(ops, new):
+    """A captured call follows its inputs; two graphs that are replayed on two streams share nothing."""
+    cs = [Case(torch.bfloat16, 8, 2, 128, [300, 64], new, None, seed=s) for s in (1, 2)]
+    runs = []
+    for c in cs:
+        mass = torch.zeros(c.pages, 2, PAGE, device=DEV)
+        out = c.run(ops, mass, before=c.before)
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            c.run(ops, mass, before=c.before, out=out)
+        runs.append((c, graph, out, mass))
+    for c, _, out, mass in runs:
+        c.qkv.copy_(c.qkv.flip(0))
+        out.zero_()
+        mass.zero_()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(20):
+        for (c, graph, out, mass), st in zip(runs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+    torch.cuda.synchronize()
+    for c, _, out, mass in runs:
+        c.check(out, mass, c.before, torch.zeros_like(mass))
+
+
+# ------------------------------------------------------------------------------------------------------- the choice
+def _chosen(values, n, first, recent, budget):
+    """values: the rows' masses (a list)."""
+    if n <= budget:
+        return list(range(n)) + [-1] * (budget - n)
+    order = sorted(range(first, n - recent), key=lambda r: (0 if not math.isnan(values[r]) else 1, -values[r] if not math.isnan(values[r]) else 0.0, r))
+    rows = list(range(first)) + order[: budget - first - recent] + list(range(n - recent, n))
+    return sorted(rows)
+
+
+def _select_case(E, kv, lengths, seed, kind):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    table, pages, _ = _tables(lengths, seed)
+    m = torch.rand(E, pages, kv, PAGE, generator=g, device=DEV)
+    if kind == "ties":
+        m = (m * 5).round()
+    elif kind == "equal":
+        m.fill_(0.25)
+    elif kind == "wild":
+        m = torch.exp((m - 0.5) * 170)                      # zero to infinity
+        m[m > 1e36] = math.inf
+        m[m < 1e-36] = 0.0
+        m[torch.rand(m.shape, generator=g, device=DEV) < 0.05] = NAN
+        m[torch.rand(m.shape, generator=g, device=DEV) < 0.05] = -1.5
+        m[torch.rand(m.shape, generator=g, device=DEV) < 0.05] = -0.0
+        m[torch.rand(m.shape, generator=g, device=DEV) < 0.02] = -math.inf
+    return m, table
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["plain", "ties", "equal", "wild"])
+@pytest.mark.parametrize("E,kv,lengths,budget,first,recent", [
+    (1, 1, [1], 1, 0, 0), (1, 1, [2], 1, 0, 0), (1, 2, [2, 1], 1, 1, 0), (1, 2, [65, 64, 63], 64, 0, 1), (2, 3, [700, 100, 257], 128, 4, 32),
+    (2, 3, [700, 100, 257], 128, 100, 28), (1, 1, [0, 5, 300], 17, 3, 2), (3, 2, [5000, 1025], 1000, 0, 0), (1, 2, [40000], 4096, 4, 256),
+    (1, 1, [70001], 999, 1, 50), (12, 8, [16000, 300], 512, 4, 60), (1, 1, [300000], 70000, 4, 60)])
+def test_evict_select(ops, E, kv, lengths, budget, first, recent, kind):
+    m, table = _select_case(E, kv, lengths, 11, kind)
+    kept = torch.full((E, len(lengths), kv, budget), 99, dtype=torch.int32, device=DEV)
+    ops.evict_select(m, table, _ints(lengths), first, recent, kept)
+    host, t = m.cpu(), table.cpu()
+    for b, n in enumerate(lengths):
+        j = torch.arange(n)
+        page = t[b].long()[j // PAGE]
+        for e in range(0, E, 5):
+            for h in range(0, kv, 3):
+                assert kept[e, b, h].tolist() == _chosen(host[e, page, h, j % PAGE].tolist(), n, first, recent, budget)
+    # one entry alone, without the axis
+    alone = torch.full_like(kept[0], 99)
+    ops.evict_select(m[E - 1], table, _ints(lengths), first, recent, alone)
+    assert torch.equal(alone, kept[E - 1])
+    ops.check_errors()
+
+
+@pytest.mark.gpu
+def test_evict_select_takes_a_missing_page_for_no_mass(ops):
+    from hilbert_pruned_8b_b200.kernels.ops import KernelError
+    m, table = _select_case(1, 1, [300], 3, "plain")
+    table[0, 2] = -1
+    kept = torch.empty(1, 1, 1, 100, dtype=torch.int32, device=DEV)
+    ops.evict_select(m, table, _ints([300]), 0, 0, kept)
+    assert not ((kept >= 128) & (kept < 192)).any()
+    with pytest.raises(KernelError, match="page"):
+        ops.check_errors()
+    ops.reset_status()
+    ops.evict_select(m, table, _ints([10 ** 9]), 0, 0, kept)            # a length that the page table cannot hold
+    assert int(kept.max()) < 64 * table.shape[1] and int(kept.min()) >= 0
+    with pytest.raises(KernelError, match="page"):
+        ops.check_errors()
+    ops.reset_status()
+
+
+# --------------------------------------------------------------------------------------------------------- the move
+@pytest.mark.gpu
+@pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("E,kv,hd,v_hd,lengths,budget,first,recent", [
+    (1, 1, 64, 64, [1], 1, 0, 0), (2, 3, 128, 128, [700, 100, 257], 128, 4, 32), (1, 2, 80, 80, [3000, 65], 2990, 0, 5),
+    (1, 2, 33, 33, [300, 200], 100, 1, 1), (3, 2, 256, 128, [1000], 64, 4, 60), (1, 1, 7, 7, [5000], 1500, 4, 10), (8, 8, 128, 128, [2000, 900], 500, 4, 50)])
+def test_evict_rows(ops, dtype, E, kv, hd, v_hd, lengths, budget, first, recent, apart):
+    g = torch.Generator(device=DEV).manual_seed(2)
+    B, spare = len(lengths), _pages(budget)
+    table, pages, rest = _tables(lengths, 6, extra=B * spare + 2)
+    k = torch.randn(E, pages, kv, PAGE, hd, generator=g, device=DEV).to(dtype)
+    v = torch.randn(E, pages, kv, PAGE, v_hd, generator=g, device=DEV).to(dtype)
+    mass = torch.rand(E, pages, kv, PAGE, generator=g, device=DEV)
+    kept = torch.empty(E, B, kv, budget, dtype=torch.int32, device=DEV)
+    ops.evict_select(mass, table, _ints(lengths), first, recent, kept)
+    to = torch.tensor([rest[b * spare: (b + 1) * spare] for b in range(B)], dtype=torch.int32, device=DEV) if apart else None
+    want = [x.clone() for x in (k, v, mass)]
+    e, b, h, j = torch.nonzero(kept >= 0, as_tuple=True)
+    src = kept[e, b, h, j].long()
+    dest = (to if apart else table)[b, j // PAGE].long()
+    for x, y in zip((k, v, mass), want):
+        y[e, dest, h, j % PAGE] = x[e, table[b, src // PAGE].long(), h, src % PAGE]
+    ops.evict_rows(kept, k, v, mass, table, to_table=to)
+    for x, y in zip((k, v, mass), want):
+        assert torch.equal(x, y)
+    if not apart:
+        k1, v1 = k[0].clone(), v[0].clone()                   # one entry alone, without mass; rows that are in place stay
+        again = torch.where(kept[0] >= 0, torch.arange(budget, dtype=torch.int32, device=DEV), kept[0])
+        ops.evict_rows(again, k1, v1, None, table)
+        assert torch.equal(k1, k[0]) and torch.equal(v1, v[0])
+    ops.check_errors()
+
+
+@pytest.mark.gpu
+def test_evict_rows_skips_what_has_no_page(ops):
+    from hilbert_pruned_8b_b200.kernels.ops import KernelError
+    table, pages, _ = _tables([200], 1)
+    k = torch.randn(1, pages, 1, PAGE, 64, device=DEV)
+    v = torch.randn(1, pages, 1, PAGE, 64, device=DEV)
+    for where in (-1, 10 ** 6):
+        t, k2, v2 = table.clone(), k.clone(), v.clone()
+        t[0, 2] = where
+        kept = _ints([[[[0, 130, 3 + 10 ** 6]]]]).view(1, 1, 1, 3)
+        ops.evict_rows(kept, k2, v2, None, t)
+        assert torch.equal(k2, k) and torch.equal(v2, v)
+        with pytest.raises(KernelError, match="page"):
+            ops.check_errors()
+        ops.reset_status()
+
+
+# ------------------------------------------------------------------------------------------- one after another
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.float32, 80)])
+def test_a_conversation_with_a_bounded_cache(ops, dtype, hd):
+    """A prompt, single tokens, an eviction in place, more tokens: the attention behind the eviction is that over the rows that
+    stayed, and the sums go on from where they were."""
+    heads, kv, n, budget = 8, 2, 500, 150
+    c = Case(dtype, heads, kv, hd, [0, 0], [n, 90], None, seed=8, garbage=0.0)
+    mass = torch.zeros(c.pages, kv, PAGE, device=DEV)
+    c.run(ops, mass, before=mass)
+    kept = torch.empty(2, kv, budget, dtype=torch.int32, device=DEV)
+    ops.evict_select(mass, c.table, _ints(c.lens), 4, 20, kept)
+    rows = []
+    for b, ln in enumerate(c.lens):
+        for g in range(kv):
+            r = kept[b, g][kept[b, g] >= 0].long()
+            page = c.table[b].long()[r // PAGE]
+            rows.append((c.k[page, g, r % PAGE].clone(), c.v[page, g, r % PAGE].clone(), mass[page, g, r % PAGE].clone()))
+    ops.evict_rows(kept, c.k, c.v, mass, c.table)
+    lens = [min(ln, budget) for ln in c.lens]
+    d = Case(dtype, heads, kv, hd, lens, [1, 7], None, seed=21)       # the next tokens: their keys and values behind the kept rows
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    for b, (p, m) in enumerate(zip(lens, d.new)):
+        j = torch.arange(p, p + m, device=DEV)
+        page = c.table[b].long()[j // PAGE]
+        c.k[page, :, j % PAGE] = torch.randn(m, kv, hd, generator=gen, device=DEV).to(dtype)
+        c.v[page, :, j % PAGE] = torch.randn(m, kv, hd, generator=gen, device=DEV).to(dtype)
+        for g in range(kv):
+            k0, v0, m0 = rows[b * kv + g]
+            i = torch.arange(p, device=DEV)
+            page = c.table[b].long()[i // PAGE]
+            assert torch.equal(c.k[page, g, i % PAGE], k0) and torch.equal(c.v[page, g, i % PAGE], v0) and torch.equal(mass[page, g, i % PAGE], m0)
+    d.table, d.pages, d.k, d.v = c.table, c.pages, c.k, c.v
+    d.step, d.cache = _step(d.past, d.new, c.table), c.cache
+    start = mass.clone()
+    out = d.run(ops, mass, before=mass)
+    inside = torch.zeros_like(mass, dtype=torch.bool)
+    for b, ln in enumerate(d.lens):
+        j = torch.arange(ln, device=DEV)
+        inside[c.table[b].long()[j // PAGE], :, j % PAGE] = True
+    assert torch.equal(mass[~inside], start[~inside])
+    d.check(out, mass, start, start)
+    ops.check_errors()
+
+
+# ------------------------------------------------------------------------------------------------------- refusals
+class _Fake:
+    """An ``Ops`` without a device: the checks of arguments run, a call of the library would fail the test."""
+
+    def __new__(cls):
+        from hilbert_pruned_8b_b200.kernels.ops import Ops
+        o = object.__new__(Ops)
+        o.device, o.sm_count, o.launches = torch.device("cpu"), 148, 0
+        o.lib = None
+
+        def call(name, *a):
+            raise AssertionError("reached " + name)
+        o._call = call
+        return o
+
+
+def _attention_args(**kw):
+    n = types.SimpleNamespace
+    a = dict(qkv=torch.zeros(3, 64 * 6), heads=4, kv_heads=2, head_dim=64, k=torch.zeros(5, 2, 64, 64), v=torch.zeros(5, 2, 64, 64),
+             out=torch.zeros(3, 256), mass=torch.zeros(5, 2, 64), before=None, tokens=3)
+    a.update(kw)
+    step = n(num_tokens=a.pop("tokens"), num_seqs=1, page_tables=[torch.zeros(1, 2, dtype=torch.int32)], max_new=3, max_len=3, host_new=[3], host_len=[3])
+    cache = n(k=a.pop("k"), v=a.pop("v"), group=0, window=None)
+    return dict(a, cache=cache, step=step, scale=0.125, window=None)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(heads=5), "heads"), (dict(kv_heads=0), "heads"), (dict(head_dim=257), "heads"), (dict(head_dim=32), "shape"), (dict(tokens=4), "shape"),
+    (dict(out=torch.zeros(2, 256)), "shape"), (dict(out=torch.zeros(3, 255)), "shape"), (dict(qkv=torch.zeros(3, 255)), "shape"),
+    (dict(k=torch.zeros(5, 2, 32, 64)), "cache"), (dict(v=torch.zeros(5, 64, 2, 64).transpose(1, 2)), "cache"),
+    (dict(out=torch.zeros(3, 256, dtype=torch.bfloat16)), "dtype"), (dict(k=torch.zeros(5, 2, 64, 64).half()), "dtype"),
+    (dict(mass=torch.zeros(4, 2, 64)), "mass"), (dict(mass=torch.zeros(5, 2, 64).double()), "mass"), (dict(mass=torch.zeros(5, 64, 2).mT), "mass"),
+    (dict(before=torch.zeros(5, 2, 63)), "before")])
+def test_attention_mass_refuses(change, text):
+    from hilbert_pruned_8b_b200.kernels.ops import KernelError
+    with pytest.raises(KernelError, match=text):
+        _Fake().attention_mass(**_attention_args(**change))
+
+
+def test_attention_mass_of_no_tokens():
+    _Fake().attention_mass(**_attention_args(qkv=torch.zeros(0, 384), out=torch.zeros(0, 256), tokens=0))
+
+
+def _i32(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(mass=torch.zeros(2, 5, 3, 63)), "mass"), (dict(mass=torch.zeros(2, 5, 3, 64).double()), "mass"), (dict(mass=torch.zeros(5, 64)), "mass"),
+    (dict(page_table=_i32(4)), "page table"), (dict(page_table=torch.zeros(4, 2)), "page table"), (dict(page_table=_i32(4, 4)[:, ::2]), "page table"),
+    (dict(lengths=_i32(3)), "length"), (dict(lengths=torch.zeros(4, dtype=torch.int64)), "length"), (dict(kept=_i32(2, 4, 3, 0)), "kept"),
+    (dict(kept=_i32(2, 3, 4, 9)), "kept"), (dict(kept=torch.zeros(2, 4, 3, 9)), "kept"), (dict(kept=_i32(4, 3, 9)), "kept"),
+    (dict(first=5, recent=5), "budget"), (dict(first=-1), "budget"), (dict(recent=-1), "budget")])
+def test_evict_select_refuses(change, text):
+    from hilbert_pruned_8b_b200.kernels.ops import KernelError
+    a = dict(mass=torch.zeros(2, 5, 3, 64), page_table=_i32(4, 2), lengths=_i32(4), first=2, recent=3, kept=_i32(2, 4, 3, 9))
+    with pytest.raises(KernelError, match=text):
+        _Fake().evict_select(**dict(a, **change))
+
+
+@pytest.mark.parametrize("change,text", [
+    (dict(k=torch.zeros(2, 5, 3, 32, 16)), "keys"), (dict(v=torch.zeros(2, 5, 3, 64, 16).double()), "keys"), (dict(v=torch.zeros(2, 6, 3, 64, 16)), "keys"),
+    (dict(k=torch.zeros(2, 5, 3, 64, 32)[..., ::2]), "keys"), (dict(k=torch.zeros(2, 5, 3, 64, 16).half(), v=torch.zeros(2, 5, 3, 64, 16).half()), "dtype"),
+    (dict(mass=torch.zeros(2, 5, 3, 16)), "mass"), (dict(page_table=_i32(4)), "page table"), (dict(to_table=_i32(3, 2)), "page tables"),
+    (dict(to_table=_i32(4, 2).long()), "page table"), (dict(kept=_i32(2, 4, 3, 129), to_table=_i32(4, 2)), "budget"), (dict(kept=_i32(4, 3, 9)), "kept")])
+def test_evict_rows_refuses(change, text):
+    from hilbert_pruned_8b_b200.kernels.ops import KernelError
+    a = dict(kept=_i32(2, 4, 3, 9), k=torch.zeros(2, 5, 3, 64, 16), v=torch.zeros(2, 5, 3, 64, 16), mass=torch.zeros(2, 5, 3, 64),
+             page_table=_i32(4, 2), to_table=None)
+    with pytest.raises(KernelError, match=text):
+        _Fake().evict_rows(**dict(a, **change))
+
+
+def test_shapes_of_the_launches():
+    from hilbert_pruned_8b_b200.kernels.plan import mass_splits, select_shape
+    assert mass_splits(1000, 8, 100, 296) == 1 and mass_splits(1, 1, 1, 296) == 1 and mass_splits(1, 1, 100, 296) == 16
+    for rows in (1, 64, 1000, 16384, 16385, 70000, 131072, 300000, 10 ** 7):
+        for lists in (1, 2, 16, 74, 75, 148, 256, 4096):
+            threads, cluster = select_shape(lists, rows, 148)
+            assert threads in (512, 1024) and cluster in (1, 2, 4, 8)
+            assert cluster == 8 or rows <= threads * cluster * 32
