@@ -1,0 +1,283 @@
+// The weights of steps of many tokens on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), bfloat16, head size 64 or 128:
+// the second half of attention_mass.cu's arithmetic, behind the prompt attention that leaves each row's log-sum.
+//
+// One CTA = 256 consecutive rows of a sequence's cache x one kv head x a share of the (head, 128 queries) tiles that see them.
+// Keys are the M operand: a tile's 128 keys are the 128 lanes of tensor memory and the queries its columns, so that a key's sum over
+// queries and heads stays in one thread's registers from beginning to end and is written once: no atomics, no shuffles.
+//   warp 0      TMA producer: the two key tiles once, then query tiles (three stages)
+//   warp 1      owns tensor memory; one thread issues S = K Q^T of the two key tiles (head size / 16 steps each) into two pairs of buffers
+//   warps 2-17  weights: 8 warps per key tile, a thread has 64 queries of its key: w = 2^(s scale log2(e) - lse), added up
+// What bounds it: 16 exponentials a clock and SM (1024 clocks for 128 x 128 weights, against 512 for the product at head size
+// 128).  Two key tiles share a query tile because an SM takes about 32 bytes a clock from L2: with one, loading a 32 KB query tile would
+// last as long as its exponentials.
+//
+// Every wait is bounded; a wait that runs out sets *error_flag and the CTA drains and leaves.
+#include "api.h"
+#include "attention_mass.cuh"
+#include "attention_tc.cuh"
+
+#define MT_KEYS 256
+#define MT_THREADS 576
+#define MT_STAGES 3
+#define MT_WORKERS 512
+
+// A barrier of the workers that tells each of them whether any gave up: the same answer for all, so that none waits for one
+// that left.
+__device__ __forceinline__ bool workers_any(bool mine) {
+    uint32_t any;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 q, %1, 0;\n\t"
+        "bar.red.or.pred p, 2, 512, q;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(any)
+        : "r"((uint32_t)mine)
+        : "memory");
+    return any != 0;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(MT_THREADS, 1)
+mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const int* __restrict__ page_table, int pt_width,
+               const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* lse, MassOut mo, int n_tokens, int n_seqs, int nh,
+               int nkv, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    // [K tiles 2][Q stages 3][barriers]; a tile is 128 rows x HD
+    constexpr int HALVES = HD / 64, TILE = HALVES * FA_HALF_BYTES;
+    uint64_t* bars = (uint64_t*)(smem + (2 + MT_STAGES) * TILE);
+    uint32_t* tmem_slot = (uint32_t*)(bars + 16);
+    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
+    float* xlse = (float*)(tmem_slot + 4);                    // [2 buffers][128 queries]
+    float* xsum = xlse + 256;                                 // [2 key tiles][128]
+    const uint32_t smem_base = smem_u32(smem), q_smem = smem_base + 2 * TILE;
+    const uint32_t k_full = smem_u32(bars), q_full0 = smem_u32(bars + 1), q_empty0 = smem_u32(bars + 4);
+    const uint32_t s_full0 = smem_u32(bars + 7), s_empty0 = smem_u32(bars + 9);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = blockIdx.y, G = nh / nkv, z = blockIdx.z, S = gridDim.z;
+
+    int b = 0, kt = 0;
+    const bool has_work = mass_find_keys(seq_start, seq_pos0, n_seqs, blockIdx.x, MT_KEYS, b, kt);
+    const int t_begin = has_work ? seq_start[b] : 0, n_new = has_work ? seq_start[b + 1] - t_begin : 0, pos0 = has_work ? seq_pos0[b] : 0;
+    const int key0 = kt * MT_KEYS;
+    int n0 = 0, n1 = 0;
+    if (has_work) mass_queries(key0, MT_KEYS, pos0, n_new, window, n0, n1);
+    const int blocks = (n1 - n0 + 127) / 128;
+    const int it0 = (int)((long long)blocks * G * z / S), n_it = (int)((long long)blocks * G * (z + 1) / S) - it0;
+
+    if (threadIdx.x == 0) {
+        mbar_init(k_full, 1);
+        for (int s = 0; s < MT_STAGES; s++) {
+            mbar_init(q_full0 + 8 * s, 1);
+            mbar_init(q_empty0 + 8 * s, 1);
+        }
+        for (int s = 0; s < 2; s++) {
+            mbar_init(s_full0 + 8 * s, 1);
+            mbar_init(s_empty0 + 8 * s, MT_WORKERS);
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc(smem_u32(tmem_slot), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;                    // buffer s of key tile k at columns (2 s + k) * 128
+    pdl_trigger();
+    pdl_wait();
+
+    if (warp == 0) {
+        // ---------------------------------------------------------------- TMA producer
+        if (lane == 0 && n_it > 0) {
+            const int* pt = page_table + (size_t)b * pt_width;
+            mbar_expect_tx(k_full, 2 * TILE);
+            for (int pg = 0; pg < MT_KEYS / HB_PAGE_TOKENS; pg++) {
+                const int pi = kt * (MT_KEYS / HB_PAGE_TOKENS) + pg;
+                int page = pi < pt_width ? pt[pi] : -1;
+                if (page < 0 || page >= n_pages) {
+                    // a page that no token of the step sees (behind the end, or given back) may be missing
+                    int a, e;
+                    mass_queries(pi * HB_PAGE_TOKENS, HB_PAGE_TOKENS, pos0, n_new, window, a, e);
+                    if (e > a) hb_note(error_flag, HB_STATUS_PAGE, 1 + b);
+                    page = 0;                                       // never read outside the cache
+                }
+                const uint32_t dst = smem_base + (pg >> 1) * TILE + (pg & 1) * (FA_HALF_BYTES / 2);
+                for (int half = 0; half < HALVES; half++)
+                    tma_load_2d(dst + half * FA_HALF_BYTES, &map_k, k_full, half * 64, (page * nkv + g) * HB_PAGE_TOKENS);
+            }
+            int issued = 0;
+            for (int it = 0; it < n_it; it++) {
+                const int s = it % MT_STAGES;
+                if (!mbar_wait(q_empty0 + 8 * s, ((it / MT_STAGES) & 1) ^ 1)) {
+                    atomicExch(error_flag, 41);
+                    *abort_flag = 1;
+                    break;
+                }
+                const int item = it0 + it, head = g * G + item / blocks, q0 = n0 + (item % blocks) * 128;
+                mbar_expect_tx(q_full0 + 8 * s, TILE);
+                for (int half = 0; half < HALVES; half++)
+                    tma_load_2d(q_smem + s * TILE + half * FA_HALF_BYTES, &map_q, q_full0 + 8 * s, head * HD + half * 64, t_begin + q0);
+                issued = it + 1;
+            }
+            for (int it = max(0, issued - MT_STAGES); it < issued; it++)
+                if (!mbar_wait(q_full0 + 8 * (it % MT_STAGES), (it / MT_STAGES) & 1)) atomicExch(error_flag, 42);
+            if (!mbar_wait(k_full, 0)) atomicExch(error_flag, 42);
+        }
+    } else if (warp == 1) {
+        // ---------------------------------------------------------------- MMA issuer
+        if (lane == 0 && n_it > 0) {
+            constexpr uint32_t idesc = instr_desc_bf16_mn(128, 128);
+            bool alive = mbar_wait(k_full, 0);
+            if (!alive) {
+                atomicExch(error_flag, 43);
+                *abort_flag = 1;
+            }
+            for (int it = 0; it < n_it && alive; it++) {
+                const int s = it % MT_STAGES, sb = it & 1;
+                if (!mbar_wait(q_full0 + 8 * s, (it / MT_STAGES) & 1) || !mbar_wait(s_empty0 + 8 * sb, ((it >> 1) & 1) ^ 1)) {
+                    atomicExch(error_flag, 44);
+                    *abort_flag = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t qst = q_smem + s * TILE;
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int kk = 0; kk < HD / 16; kk++) {
+                        const uint32_t off = (kk >> 2) * FA_HALF_BYTES + (kk & 3) * 32;
+                        umma_bf16(tmem_base + (2 * sb + k) * 128, smem_desc_sw128(smem_base + k * TILE + off), smem_desc_sw128(qst + off), idesc,
+                                  kk ? 1u : 0u);
+                    }
+                umma_commit(q_empty0 + 8 * s);
+                umma_commit(s_full0 + 8 * sb);
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- weights
+        const int w = warp - 2, k = w >> 3;                    // key tile
+        const int quarter = warp & 3, r = quarter * 32 + lane;  // key of the tile = lane of tensor memory (a warp reads its own quarter)
+        const int hf = (w >> 2) & 1, et = threadIdx.x - 64;    // which 64 queries of a tile; the number among the workers
+        const int key = key0 + k * 128 + r;
+        const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
+        float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto lse_of = [&](int it) -> float {                   // of query et of the tile; 128 workers ask
+            const int item = it0 + it, head = g * G + item / blocks, t = n0 + (item % blocks) * 128 + et;
+            return t < n1 ? __ldcg(lse + (size_t)head * n_tokens + t_begin + t) : 0.0f;
+        };
+        if (n_it > 0) {
+            if (et < 128) xlse[et] = lse_of(0);
+            asm volatile("bar.sync 2, 512;" ::: "memory");
+        }
+        for (int it = 0; it < n_it; it++) {
+            const int sb = it & 1;
+            const float next = et < 128 && it + 1 < n_it ? lse_of(it + 1) : 0.0f;
+            if (!mbar_wait(s_full0 + 8 * sb, (it >> 1) & 1)) {
+                atomicExch(error_flag, 45);
+                *abort_flag = 1;
+            }
+            tc_fence_after();
+            const int q0 = n0 + ((it0 + it) % blocks) * 128 + hf * 64;       // this thread's first query
+            const int c_lo = key - pos0 - q0;                  // its queries [c_lo, c_hi] see the key
+            int c_hi = n1 - 1 - q0;
+            if (window > 0) c_hi = (int)min((long long)c_hi, (long long)key + window - 1 - pos0 - q0);
+            const uint32_t tm_s = tmem_base + (2 * sb + k) * 128 + lane_base + hf * 64;
+#pragma unroll
+            for (int part = 0; part < 2; part++) {
+                float sv[32];
+                tmem_ld32(tm_s + part * 32, sv);
+                if (part == 1) {
+                    tc_fence_before();
+                    mbar_arrive(s_empty0 + 8 * sb);            // all scores have been read
+                }
+                const float4* ls = reinterpret_cast<const float4*>(xlse + sb * 128 + hf * 64 + part * 32);
+                const int lo = c_lo - part * 32, hi = c_hi - part * 32;
+                if (lo <= 0 && hi >= 31) {
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {
+                        const float4 l4 = ls[c >> 2];
+                        sum4[0] += exp2_approx(fmaf(sv[c], scale_log2e, -l4.x));
+                        sum4[1] += exp2_approx(fmaf(sv[c + 1], scale_log2e, -l4.y));
+                        sum4[2] += exp2_approx(fmaf(sv[c + 2], scale_log2e, -l4.z));
+                        sum4[3] += exp2_approx(fmaf(sv[c + 3], scale_log2e, -l4.w));
+                    }
+                } else if (lo <= 31 && hi >= 0) {              // the causal diagonal, the window's edge, the last queries
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {
+                        const float4 l4 = ls[c >> 2];
+                        sum4[0] += c >= lo && c <= hi ? exp2_approx(fmaf(sv[c], scale_log2e, -l4.x)) : 0.0f;
+                        sum4[1] += c + 1 >= lo && c + 1 <= hi ? exp2_approx(fmaf(sv[c + 1], scale_log2e, -l4.y)) : 0.0f;
+                        sum4[2] += c + 2 >= lo && c + 2 <= hi ? exp2_approx(fmaf(sv[c + 2], scale_log2e, -l4.z)) : 0.0f;
+                        sum4[3] += c + 3 >= lo && c + 3 <= hi ? exp2_approx(fmaf(sv[c + 3], scale_log2e, -l4.w)) : 0.0f;
+                    }
+                }
+            }
+            if (et < 128) xlse[(sb ^ 1) * 128 + et] = next;    // read last in the round before, in front of its barrier
+            if (workers_any(*abort_flag != 0)) break;          // a barrier as well
+        }
+        const float mine = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+        if (hf == 1) xsum[k * 128 + r] = mine;
+        asm volatile("bar.sync 2, 512;" ::: "memory");
+        if (hf == 0 && has_work && !*abort_flag) {
+            const int pi = key / HB_PAGE_TOKENS;
+            const int page = pi < pt_width ? page_table[(size_t)b * pt_width + pi] : -1;
+            mass_store(mo, mine + xsum[k * 128 + r], b, g, key, page, nkv, n_pages, pos0, n_new, z, S, (size_t)blockIdx.x * MT_KEYS + k * 128 + r,
+                       (size_t)gridDim.x * MT_KEYS);
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+template <int HD>
+static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0,
+                          const float* lse, MassOut mo, int splits, int n_tokens, int n_seqs, int key_tiles, int nh, int nkv, float scale, int window,
+                          int n_pages, int* error_flag, cudaStream_t s) {
+    constexpr int SMEM = (2 + MT_STAGES) * (HD / 64) * FA_HALF_BYTES + 16 * 8 + 16 + (256 + 256) * 4 + 1024;
+    static_assert(SMEM <= 227 * 1024, "key and query tiles do not fit shared memory");
+    static bool done[HB_MAX_DEVICES] = {};
+    bool& set = done[hb_device_slot()];
+    if (!set) {
+        cudaError_t e = cudaFuncSetAttribute(mass_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e != cudaSuccess) return hb_fail("attention_mass_tc: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
+        set = true;
+    }
+    cudaError_t e = hb_launch(mass_tc_kernel<HD>, dim3(key_tiles, nkv, splits), dim3(MT_THREADS), SMEM, s, mq, mk, page_table, pt_width, seq_start,
+                              seq_pos0, lse, mo, n_tokens, n_seqs, nh, nkv, scale * FA_LOG2E, window, n_pages, error_flag);
+    if (e != cudaSuccess) return hb_fail("attention_mass_tc: launch failed: %s", cudaGetErrorString(e));
+    return hb_check_launch("attention_mass_tc");
+}
+
+extern "C" int hb_attention_mass_tc_keys(void) { return MT_KEYS; }
+
+// Sizes and types of hb_attention_prefill_tc, with the same alignment of queries and output.  q_blocks: sum over sequences of
+// ceil(new tokens / 128); key_tiles: sum of ceil(rows / 256); lse: n_heads * n_tokens floats; parts: splits * n_kv_heads *
+// key_tiles * 256 floats when splits > 1.
+extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
+                                    const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, const float* before,
+                                    float* mass, float* parts, int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads,
+                                    int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag, void* stream) {
+    if (n_seqs == 0 || n_tokens == 0) return 0;
+    HB_REQUIRE(lse != nullptr && mass != nullptr && n_kv_heads > 0 && n_kv_heads <= 65535 && key_tiles > 0 && splits >= 1 && splits <= 65535 &&
+                   (splits == 1 || parts != nullptr),
+               "attention_mass_tc: bad sizes");
+    if (attention_prefill_tc_lse(q, q_stride, n_tokens, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, n_seqs, q_blocks,
+                                 n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, lse, stream))
+        return 1;
+    CUtensorMap mq, mk;
+    if (tc_make_map(&mq, q, n_tokens, (long long)n_heads * head_dim, q_stride, 128)) return 1;
+    if (tc_make_map(&mk, k_cache, (long long)n_pages * n_kv_heads * HB_PAGE_TOKENS, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
+    MassOut mo = {before, mass, parts};
+    cudaStream_t s = (cudaStream_t)stream;
+    const int rc = head_dim == 128 ? launch_mass_tc<128>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, mo, splits, n_tokens, n_seqs, key_tiles,
+                                                         n_heads, n_kv_heads, scale, window, n_pages, error_flag, s)
+                                   : launch_mass_tc<64>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, mo, splits, n_tokens, n_seqs, key_tiles,
+                                                        n_heads, n_kv_heads, scale, window, n_pages, error_flag, s);
+    if (rc) return rc;
+    return splits > 1 ? mass_join(page_table, pt_width, seq_start, seq_pos0, mo, n_seqs, n_kv_heads, n_pages, MT_KEYS, key_tiles, splits, s) : 0;
+}

@@ -81,6 +81,8 @@ _SIGNATURES = {
                                 _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                           _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
+    "hb_attention_mass_tc": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+                             _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr,
                               _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr,
                               _c_ptr],
@@ -185,6 +187,7 @@ def load_library():
         lib.hb_gemm_tc2_resident_pairs.argtypes, lib.hb_gemm_tc2_resident_pairs.restype = [_c_int], _c_int
         for name in ("hb_attention_decode_supported", "hb_attention_prefill_supported", "hb_attention_prefill_tc_supported"):
             getattr(lib, name).argtypes, getattr(lib, name).restype = [_c_int, _c_int, _c_int], _c_int
+        lib.hb_attention_mass_tc_keys.argtypes, lib.hb_attention_mass_tc_keys.restype = [], _c_int
         lib.hb_attention_few_pairs.argtypes, lib.hb_attention_few_pairs.restype = [], _c_int
         lib.hb_attention_mass_few_floats.argtypes, lib.hb_attention_mass_few_floats.restype = [_c_int] * 5, _c_ll
         lib.hb_attention_sink_prefill_supported.argtypes, lib.hb_attention_sink_prefill_supported.restype = [_c_int] * 4, _c_int
@@ -1291,15 +1294,23 @@ class Ops:
                 self.launches += 2
                 return
             lse = torch.empty(heads * T, dtype=torch.float32, device=self.device)
-            q_blocks = sum((n + 63) // 64 for n in step.host_new)
-            key_tiles = sum((n + 63) // 64 for n in step.host_len)
+            tc = (self.use_fast_attention and self.use_tcgen05_attention and qkv.dtype == torch.bfloat16
+                  and self.lib.hb_attention_prefill_tc_supported(heads, kv_heads, head_dim) and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0
+                  and cache.k.data_ptr() % 16 == 0 and cache.v.data_ptr() % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0)
+            rows, keys = (128, self.lib.hb_attention_mass_tc_keys()) if tc else (64, 64)
+            q_blocks = sum(-(-n // rows) for n in step.host_new)
+            key_tiles = sum(-(-n // keys) for n in step.host_len)
             if splits is None:
-                splits = mass_splits(key_tiles, kv_heads, group * -(-step.max_new // 64), 2 * self.sm_count)
-            parts = torch.empty(splits * kv_heads * key_tiles * 64, dtype=torch.float32, device=self.device) if splits > 1 else None
-            self._call("hb_attention_mass", qkv.data_ptr(), code, q_ld, cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(), pt.shape[1],
-                       step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out.data_ptr(), out_ld, lse.data_ptr(), old, mass.data_ptr(),
-                       parts.data_ptr() if parts is not None else None, splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim,
-                       float(scale), win, pages, self.status.data_ptr(), self._stream())
+                splits = mass_splits(key_tiles, kv_heads, group * -(-step.max_new // rows), self.sm_count * (1 if tc else 2))
+            parts = torch.empty(splits * kv_heads * key_tiles * keys, dtype=torch.float32, device=self.device) if splits > 1 else None
+            sizes = (splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim, float(scale), win, pages, self.status.data_ptr(),
+                     self._stream())
+            buffers = (cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(),
+                       out.data_ptr(), out_ld, lse.data_ptr(), old, mass.data_ptr(), parts.data_ptr() if parts is not None else None)
+            if tc:
+                self._call("hb_attention_mass_tc", qkv.data_ptr(), q_ld, *buffers, *sizes)
+            else:
+                self._call("hb_attention_mass", qkv.data_ptr(), code, q_ld, *buffers, *sizes)
             self.launches += 2 if splits == 1 else 3
 
     def evict_select(self, mass, page_table, lengths, first: int, recent: int, kept) -> None:
