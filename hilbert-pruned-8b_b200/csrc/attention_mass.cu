@@ -574,12 +574,12 @@ static int launch_finish(const float* part_o, const float* part_ml, const float*
 }
 
 // Steps of few tokens (at most hb_attention_few_pairs() pairs of a sequence's tokens and a group's heads).  `scratch` holds
-// hb_attention_mass_few_floats floats; max_len bounds the rows of every sequence, max_new their new tokens.
+// hb_attention_mass_few_floats floats; tensor_cores: sizes of hb_attention_decode; max_len bounds the rows of every sequence, max_new their new tokens.
 extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
                                      int pt_width, const int* tok_seq, const int* positions, const int* seq_start, const int* seq_pos0, void* out,
                                      long long out_stride, float* scratch, const float* before, float* mass, int splits, int n_tokens, int n_seqs,
                                      int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages,
-                                     int* status, void* stream) {
+                                     int tensor_cores, int* status, void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0 && head_dim <= 256 && n_pages > 0 && pt_width > 0,
                "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, head_dim);
@@ -594,7 +594,14 @@ extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_strid
     cudaStream_t s = (cudaStream_t)stream;
     MassOut mo = {before, mass, nullptr};
     int rc;
-    if (dtype == HB_F32)
+    if (tensor_cores) {
+        HB_REQUIRE(dtype == HB_BF16 && hb_attention_decode_supported(n_heads, n_kv_heads, head_dim) && q_stride % 2 == 0 && ((uintptr_t)q & 3) == 0 &&
+                       (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0,
+                   "attention_mass: a head size of %d with %d heads over %d kv heads is not built for the tensor cores, or is not aligned", head_dim, n_heads,
+                   n_kv_heads);
+        rc = attention_decode_scores(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits,
+                                     n_tokens, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
+    } else if (dtype == HB_F32)
         rc = launch_few<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits,
                                n_tokens, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     else if (dtype == HB_BF16)

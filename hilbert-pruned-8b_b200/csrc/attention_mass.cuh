@@ -78,3 +78,9 @@ __device__ __forceinline__ void load4(const bf16* p, float (&x)[4]) {
 
 int mass_join(const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0, MassOut mo, int n_seqs, int nkv, int n_pages, int tile,
               int key_tiles, int splits, cudaStream_t s);
+
+// The first half of a step of few tokens on the tensor cores (attention_decode.cu): sizes of hb_attention_decode, queries 4-byte and
+// keys and values 16-byte aligned.
+int attention_decode_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* tok_seq,
+                            const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int n_tokens, int nh,
+                            int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);

@@ -330,7 +330,9 @@ __device__ __forceinline__ void evict_move(const EvictRows& p, U* data, int row_
 template <typename U>
 __global__ void __launch_bounds__(ER_THREADS)
 evict_rows_kernel(EvictRows p, U* k, int k_units, int k_slices, U* v, int v_units, int v_slices, uint32_t* mass, int rows_per_block) {
-    pdl_trigger();
+    // no pdl_trigger(): the decode attention kernels read pages of older tokens before their griddepcontrol.wait, and
+    // with small kernels in between they could be resident while rows still move.  Without the trigger, nothing behind this
+    // kernel starts before it has finished.
     pdl_wait();
     p.kept = pdl_fresh(p.kept);
     p.from_table = pdl_fresh(p.from_table);

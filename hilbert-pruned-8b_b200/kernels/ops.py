@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import build
-from .plan import decode_splits, mass_splits, select_shape
+from .plan import decode_splits, few_splits, mass_splits, select_shape
 
 _c_int, _c_ll, _c_float, _c_ptr = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
 
@@ -84,8 +84,8 @@ _SIGNATURES = {
     "hb_attention_mass_tc": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                              _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr,
-                              _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr,
-                              _c_ptr],
+                              _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int,
+                              _c_ptr, _c_ptr],
     "hb_evict_select": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr,
                         _c_ptr],
     "hb_evict_rows": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
@@ -1282,15 +1282,18 @@ class Ops:
         with torch.cuda.device(self.device):
             if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * group <= self.lib.hb_attention_few_pairs():
                 max_pages = (step.max_len + 63) // 64
+                tc = (self.use_fast_attention and qkv.dtype == torch.bfloat16 and self.lib.hb_attention_decode_supported(heads, kv_heads, head_dim)
+                      and q_ld % 2 == 0 and qkv.data_ptr() % 4 == 0 and cache.k.data_ptr() % 16 == 0 and cache.v.data_ptr() % 16 == 0)
                 if splits is None:
-                    splits = decode_splits(T, kv_heads * -(-group // 8), max_pages, 3 * self.sm_count)
+                    splits = few_splits(T, kv_heads if tc else kv_heads * -(-group // 8), max_pages, (2 if tc else 3) * self.sm_count)
                 splits = max(1, min(splits, max_pages))
                 scratch = torch.empty(self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len), dtype=torch.float32,
                                       device=self.device)
                 self._call("hb_attention_mass_few", qkv.data_ptr(), code, q_ld, cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(),
                            pt.shape[1], step.tok_seq.data_ptr(), step.positions.data_ptr(), step.seq_start.data_ptr(),
                            step.seq_pos0.data_ptr(), out.data_ptr(), out_ld, scratch.data_ptr(), old, mass.data_ptr(), splits, T, step.num_seqs,
-                           step.max_new, step.max_len, heads, kv_heads, head_dim, float(scale), win, pages, self.status.data_ptr(), self._stream())
+                           step.max_new, step.max_len, heads, kv_heads, head_dim, float(scale), win, pages, 1 if tc else 0, self.status.data_ptr(),
+                           self._stream())
                 self.launches += 2
                 return
             lse = torch.empty(heads * T, dtype=torch.float32, device=self.device)

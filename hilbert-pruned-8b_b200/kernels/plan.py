@@ -28,6 +28,13 @@ def decode_splits(sequences: int, kv_heads: int, max_pages: int, cta_slots: int)
     return best
 
 
+def few_splits(tokens: int, kv_heads: int, max_pages: int, cta_slots: int) -> int:
+    """Shares of a token's pages in a step of few tokens that keeps its scores: as ``decode_splits``, but down to a page each while
+    the device has room, since a second kernel follows in any case."""
+    room = max(1, cta_slots) // max(1, tokens * kv_heads)
+    return max(decode_splits(tokens, kv_heads, max_pages, cta_slots), min(max_pages, 16, room))
+
+
 def mass_splits(key_tiles: int, kv_heads: int, items: int, cta_slots: int) -> int:
     """Shares of the weights' kernel for ``key_tiles`` x ``kv_heads`` (tile of keys, kv head) pairs with up to ``items`` tiles of
     queries each: under a causal mask the first keys are seen by every query and the last by few, so the work evens out only

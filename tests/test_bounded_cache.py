@@ -532,7 +532,8 @@ def test_evict_rows_refuses(change, text):
 
 
 def test_shapes_of_the_launches():
-    from hilbert_pruned_8b_b200.kernels.plan import mass_splits, select_shape
+    from hilbert_pruned_8b_b200.kernels.plan import few_splits, mass_splits, select_shape
+    assert few_splits(1, 8, 5, 296) == 5 and few_splits(8, 8, 129, 296) == 4 and few_splits(1000, 8, 100, 296) == 1
     assert mass_splits(1000, 8, 100, 296) == 1 and mass_splits(1, 1, 1, 296) == 1 and mass_splits(1, 1, 100, 296) == 16
     for rows in (1, 64, 1000, 16384, 16385, 70000, 131072, 300000, 10 ** 7):
         for lists in (1, 2, 16, 74, 75, 148, 256, 4096):
