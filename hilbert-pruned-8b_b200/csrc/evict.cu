@@ -24,10 +24,33 @@ namespace cg = cooperative_groups;
 #define ES_ITEMS 32
 #define ES_BINS 2048
 
+// the value's place in the order of all values, 0 aside: that stands for a row that is not between the first and the last ones
 __device__ __forceinline__ uint32_t es_key(float f) {
-    if (isnan(f)) return 0u;                              // below everything, -inf included
     const uint32_t u = __float_as_uint(f + 0.0f);         // -0 counts as 0
-    return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+    const uint32_t k = u ^ (uint32_t)(((int32_t)u >> 31) | 0x80000000);
+    return isnan(f) ? 1u : k;                             // below everything, -inf (0x007fffff) included
+}
+
+// bits [from, to) of 32
+__device__ __forceinline__ uint32_t es_bits(int from, int to) {
+    from = min(max(from, 0), 32);
+    to = min(max(to, 0), 32);
+    return from < to ? (0xffffffffu >> (32 - (to - from))) << from : 0u;
+}
+
+// sums over the warps in front of this one of two counts, and over all warps
+template <int NW>
+__device__ __forceinline__ void es_scan(int& a, int& b, int& all_a, int& all_b, int (*scratch)[NW], int warp, int lane) {
+    if (lane == 0) {
+        scratch[0][warp] = a;
+        scratch[1][warp] = b;
+    }
+    __syncthreads();
+    const int x = lane < NW ? scratch[0][lane] : 0, y = lane < NW ? scratch[1][lane] : 0;
+    a = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
+    b = __reduce_add_sync(0xffffffffu, lane < warp ? y : 0);
+    all_a = __reduce_add_sync(0xffffffffu, x);
+    all_b = __reduce_add_sync(0xffffffffu, y);
 }
 
 template <int NT>
@@ -36,9 +59,8 @@ evict_select_kernel(const float* __restrict__ mass, const int* __restrict__ page
                     int* __restrict__ kept, int n_seqs, int nkv, int n_pages, int first, int recent, int budget, int* status) {
     constexpr int NW = NT / 32;
     __shared__ int hist[ES_BINS];
-    __shared__ int warp_keep[NW], warp_equal[NW];
+    __shared__ int sums[2][NW];
     __shared__ int totals[2];                             // this block's rows above the border, and at it
-    __shared__ int scan[33];
     __shared__ int chosen[2];                             // the digit, and how many are wanted of what has it
     pdl_trigger();
     pdl_wait();
@@ -59,55 +81,67 @@ evict_select_kernel(const float* __restrict__ mass, const int* __restrict__ page
         return;
     }
     const int* pt = page_table + (size_t)b * pt_width;
-    const float* base = mass + (size_t)e * n_pages * nkv * HB_PAGE_TOKENS;
-    // rows [w_begin, w_begin + 32 * items) are this warp's
-    const int items = (n + C * NT - 1) / (C * NT);
-    const int w_begin = (rank * NW + warp) * items * 32;
+    const float* base = mass + ((size_t)e * n_pages * nkv + g) * HB_PAGE_TOKENS + lane;
+    // rows [w_begin, w_begin + 32 * items) are this warp's, whole pages (an even number of 32 rows); row w_begin + 32 i + lane is
+    // item i of this lane
+    const int items = ((n + C * NT - 1) / (C * NT) + 1) & ~1;
+    const int w_begin = (rank * NW + warp) * items * 32, r0 = w_begin + lane;
     const int mid_end = n - recent;
     const int need = budget - first - recent;
+    auto item_of = [&](int r) { return (r - r0 + 31) >> 5; };             // the first item whose row is r or behind it
 
     bool bad = false;
-    auto value = [&](int i) -> uint32_t {
-        const int r = w_begin + i * 32 + lane;
-        if (r >= n) return 0u;
-        const int page = pt[r / HB_PAGE_TOKENS];
+    auto page_values = [&](int i) -> const float* {       // this lane's values of items i and i + 1, i even
+        const int pi = (w_begin + i * 32) / HB_PAGE_TOKENS;
+        const int page = pi * HB_PAGE_TOKENS < n ? pt[pi] : 0;
         if (page < 0 || page >= n_pages) {
             bad = true;
-            return 0u;
+            return nullptr;
         }
-        return es_key(__ldcg(base + ((size_t)page * nkv + g) * HB_PAGE_TOKENS + (r & (HB_PAGE_TOKENS - 1))));
+        return base + (size_t)page * nkv * HB_PAGE_TOKENS;
     };
     uint32_t key[ES_ITEMS];
+    const uint32_t middle = es_bits(item_of(first), item_of(mid_end));
 #pragma unroll
-    for (int i = 0; i < ES_ITEMS; i++) key[i] = i < items ? value(i) : 0u;
-    // calls f(row, key, is between first and recent) for every row of this thread; `i` is the same for the whole warp
-    auto each = [&](auto&& f) {
-#pragma unroll
-        for (int i = 0; i < ES_ITEMS; i++) {
-            const int r = w_begin + i * 32 + lane;
-            if (i < items) f(r, key[i], r >= first && r < mid_end);
+    for (int i = 0; i < ES_ITEMS; i += 2) {
+        key[i] = key[i + 1] = 0u;
+        if (i < items && (middle >> i & 3u)) {
+            const float* v = page_values(i);
+            if (middle >> i & 1u) key[i] = v != nullptr ? es_key(__ldcg(v)) : 1u;
+            if (middle >> (i + 1) & 1u) key[i + 1] = v != nullptr ? es_key(__ldcg(v + 32)) : 1u;
         }
-        for (int i = ES_ITEMS; i < items; i++) {
-            const int r = w_begin + i * 32 + lane;
-            f(r, value(i), r >= first && r < mid_end);
-        }
+    }
+    // what the registers do not hold: the same key of item i >= ES_ITEMS, from memory
+    auto far_key = [&](int i) -> uint32_t {
+        const int r = r0 + i * 32;
+        if (r < first || r >= mid_end) return 0u;
+        const float* v = page_values(i & ~1);
+        return v != nullptr ? es_key(__ldcg(v + (i & 1) * 32)) : 1u;
     };
 
-    uint32_t prefix = 0, prefix_mask = 0;
-    int want = need;                                      // of the values with this prefix, how many are still wanted
+    uint32_t border = need > 0 ? 0u : 0xffffffffu;        // the need-th largest key; no key is as large as the other
+    int want = need;                                      // of the keys that have the border's digits so far, how many stay
     if (need > 0) {
 #pragma unroll 1
         for (int pass = 0; pass < 3; pass++) {
             const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
             const int bins = pass == 2 ? 1024 : 2048;
+            const uint32_t mask = pass == 0 ? 0u : 0xffffffffu << (shift + (pass == 1 ? 11 : 10));
             for (int i = tid; i < ES_BINS; i += NT) hist[i] = 0;
             __syncthreads();
-            each([&](int, uint32_t k, bool middle) {
-                if (middle && (k & prefix_mask) == prefix) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
-            });
+            auto count = [&](uint32_t k) {
+                if (k != 0u && ((k ^ border) & mask) == 0u) atomicAdd(&hist[(k >> shift) & (bins - 1)], 1);
+            };
+#pragma unroll
+            for (int i = 0; i < ES_ITEMS; i += 2)
+                if (i < items) {
+                    count(key[i]);
+                    count(key[i + 1]);
+                }
+            for (int i = ES_ITEMS; i < items; i++) count(far_key(i));
             if (C > 1) cluster.sync();
             else __syncthreads();
-            // bins from the top, PER per thread: thread t has bins - 1 - t * PER and the PER - 1 below it
+            // bins from the top, PER per thread: thread t has bin bins - 1 - t * PER and the PER - 1 below it
             constexpr int PER = ES_BINS / NT;
             int mine[PER], sum = 0;
 #pragma unroll
@@ -128,19 +162,9 @@ evict_select_kernel(const float* __restrict__ mass, const int* __restrict__ page
                 const int u = __shfl_up_sync(0xffffffffu, inc, o);
                 if (lane >= o) inc += u;
             }
-            if (lane == 31) scan[warp] = inc;
-            __syncthreads();
-            if (warp == 0) {
-                int u = lane < NW ? scan[lane] : 0;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int w = __shfl_up_sync(0xffffffffu, u, o);
-                    if (lane >= o) u += w;
-                }
-                scan[lane] = u;
-            }
-            __syncthreads();
-            int before = inc - sum + (warp > 0 ? scan[warp - 1] : 0);
+            int of_warp = __shfl_sync(0xffffffffu, inc, 31), none = 0, all, all_none;
+            es_scan<NW>(of_warp, none, all, all_none, sums, warp, lane);
+            int before = of_warp + inc - sum;
 #pragma unroll
             for (int i = 0; i < PER; i++) {
                 if (before < want && before + mine[i] >= want) {
@@ -151,67 +175,85 @@ evict_select_kernel(const float* __restrict__ mass, const int* __restrict__ page
             }
             if (C > 1) cluster.sync();                    // nobody still reads this block's histogram
             else __syncthreads();
-            prefix |= (uint32_t)chosen[0] << shift;
-            prefix_mask |= (uint32_t)(bins - 1) << shift;
+            border |= (uint32_t)chosen[0] << shift;
             want = chosen[1];
         }
     }
-    // rows above the border stay, and the first `want` at it; with need == 0 no row between stays
-    const bool any = need > 0;
-    int above = 0, equal = 0;
-    each([&](int r, uint32_t k, bool middle) {
-        const bool in = r < n;
-        above += (in && (!middle || (any && k > prefix))) ? 1 : 0;
-        equal += (in && middle && any && k == prefix) ? 1 : 0;
-    });
-    above = __reduce_add_sync(0xffffffffu, above);
-    equal = __reduce_add_sync(0xffffffffu, equal);
-    if (lane == 0) {
-        warp_keep[warp] = above;
-        warp_equal[warp] = equal;
-    }
-    __syncthreads();
-    if (warp == 0) {
-        int a = lane < NW ? warp_keep[lane] : 0, q = lane < NW ? warp_equal[lane] : 0;
-        const int a0 = a, q0 = q;
+    // Rows that are not between stay, rows above the border stay, and the first `want` at it.  As bits of this lane's items.
+    uint32_t stay = es_bits(0, min(items, item_of(n))) & ~middle, equal = 0u;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int ua = __shfl_up_sync(0xffffffffu, a, o), uq = __shfl_up_sync(0xffffffffu, q, o);
-            if (lane >= o) {
-                a += ua;
-                q += uq;
-            }
+    for (int i = 0; i < ES_ITEMS; i++) {
+        stay |= key[i] > border ? 1u << i : 0u;
+        equal |= key[i] == border ? 1u << i : 0u;
+    }
+    int n_stay = __popc(stay), n_equal = __popc(equal);
+    auto far_stays = [&](int i, uint32_t k) { return r0 + i * 32 < n && (k == 0u || k > border); };
+    for (int i = ES_ITEMS; i < items; i++) {
+        const uint32_t k = far_key(i);
+        n_stay += far_stays(i, k) ? 1 : 0;
+        n_equal += k == border ? 1 : 0;
+    }
+    n_stay = __reduce_add_sync(0xffffffffu, n_stay);
+    n_equal = __reduce_add_sync(0xffffffffu, n_equal);
+    const int equal_here = n_equal;
+    int all_stay, all_equal;
+    es_scan<NW>(n_stay, n_equal, all_stay, all_equal, sums, warp, lane);
+    if (C > 1) {
+        if (tid == 0) {
+            totals[0] = all_stay;
+            totals[1] = all_equal;
         }
-        if (lane < NW) {
-            warp_keep[lane] = a - a0;
-            warp_equal[lane] = q - q0;
-        }
-        if (lane == 31) {
-            totals[0] = a;
-            totals[1] = q;
+        cluster.sync();
+        for (int o = 0; o < rank; o++) {
+            const int* t = cluster.map_shared_rank(totals, o);
+            n_stay += t[0];
+            n_equal += t[1];
         }
     }
-    if (C > 1) cluster.sync();
-    else __syncthreads();
-    int n_above = warp_keep[warp], n_equal = warp_equal[warp];
-    for (int o = 0; o < rank; o++) {
-        const int* t = cluster.map_shared_rank(totals, o);
-        n_above += t[0];
-        n_equal += t[1];
-    }
+    // n_stay, n_equal: how many stay, and how many lie at the border, in front of this warp's rows.  Does the limit for those at
+    // the border fall inside this warp's rows?
     const uint32_t below = (1u << lane) - 1u;
-    each([&](int r, uint32_t k, bool middle) {
-        const bool in = r < n;
-        const bool up = in && (!middle || (any && k > prefix)), eq = in && middle && any && k == prefix;
-        const uint32_t mu = __ballot_sync(0xffffffffu, up), me = __ballot_sync(0xffffffffu, eq);
-        const int eq_before = n_equal + __popc(me & below);
-        if (up || (eq && eq_before < want)) {
-            const int at = n_above + __popc(mu & below) + min(eq_before, want);
-            if (at < budget) out[at] = r;
+    int at = n_stay + min(n_equal, want);
+    if (n_equal >= want) {
+        equal = 0u;
+    } else if (n_equal + equal_here > want) {
+        uint32_t in = 0u;
+        int before = n_equal;
+#pragma unroll
+        for (int i = 0; i < ES_ITEMS; i++) {
+            const uint32_t m = __ballot_sync(0xffffffffu, equal >> i & 1u);
+            in |= (equal >> i & 1u) && before + __popc(m & below) < want ? 1u << i : 0u;
+            before += __popc(m);
         }
-        n_above += __popc(mu);
+        equal = in;
+        n_equal = before;                                 // in front of item ES_ITEMS
+    } else if (items > ES_ITEMS) {
+        n_equal += (int)__reduce_add_sync(0xffffffffu, (uint32_t)__popc(equal));
+    }
+    stay |= equal;
+#pragma unroll
+    for (int i = 0; i < ES_ITEMS; i++) {
+        if (i >= items) break;
+        const uint32_t m = __ballot_sync(0xffffffffu, stay >> i & 1u);
+        if (stay >> i & 1u) {
+            const int j = at + __popc(m & below);
+            if (j < budget) out[j] = r0 + i * 32;
+        }
+        at += __popc(m);
+    }
+    for (int i = ES_ITEMS; i < items; i++) {
+        const uint32_t k = far_key(i);
+        const bool up = far_stays(i, k), eq = k == border;
+        const uint32_t me = __ballot_sync(0xffffffffu, eq);
+        const bool in = up || (eq && n_equal + __popc(me & below) < want);
+        const uint32_t m = __ballot_sync(0xffffffffu, in);
+        if (in) {
+            const int j = at + __popc(m & below);
+            if (j < budget) out[j] = r0 + i * 32;
+        }
+        at += __popc(m);
         n_equal += __popc(me);
-    });
+    }
     if (bad) hb_note(status, HB_STATUS_PAGE, 1 + b);
     if (C > 1) cluster.sync();                            // a block's totals stay readable until all have read them
 }
@@ -288,23 +330,29 @@ __device__ __forceinline__ void evict_move(const EvictRows& p, U* data, int row_
     };
     U next[ER_UNROLL];
     bool have[ER_UNROLL];
-    auto load = [&](int c0) {
+    int src[ER_UNROLL];                                   // of the chunk behind the one that is loaded
+    auto sources = [&](int c0) {
 #pragma unroll
         for (int i = 0; i < ER_UNROLL; i++) {
             const int j = c0 + i * per + lead;
+            src[i] = lead < per && j < j1 ? kept[j] : -1;
+        }
+    };
+    auto load = [&](int c0) {
+#pragma unroll
+        for (int i = 0; i < ER_UNROLL; i++) {
             have[i] = false;
-            if (lead < per && j < j1) {
-                const int src = kept[j];
-                if (src >= 0 && !(p.in_place && src == j)) {
-                    const U* a = address(from, p.from_width, src);
-                    if (a != nullptr) {
-                        next[i] = __ldcg(a);
-                        have[i] = true;
-                    }
+            if (src[i] >= 0 && !(p.in_place && src[i] == c0 + i * per + lead)) {
+                const U* a = address(from, p.from_width, src[i]);
+                if (a != nullptr) {
+                    next[i] = __ldcg(a);
+                    have[i] = true;
                 }
             }
         }
+        sources(c0 + chunk);
     };
+    sources(j0);
     load(j0);
     for (int c0 = j0; c0 < j1; c0 += chunk) {
         U now[ER_UNROLL];
@@ -376,7 +424,11 @@ extern "C" int hb_evict_rows(const int* kept, void* k, int k_row_bytes, void* v,
         while ((ks + vs) * lists < 2LL * sm_count && k_row_bytes / (2 * ks) >= 64 && v_row_bytes / (2 * vs) >= 64) ks *= 2, vs *= 2;
         rows_per_block = budget;
     } else {
-        rows_per_block = 64;
+        // about four blocks to a slot (an SM holds four): a block's first chunk waits for three loads in a row (kept, page, row), the
+        // chunks behind it overlap with the one before
+        const long long lists_parts = lists * (ks + vs), want = (16LL * sm_count + lists_parts - 1) / lists_parts;
+        rows_per_block = (int)((budget + want - 1) / want);
+        rows_per_block = rows_per_block < 64 ? 64 : rows_per_block;
     }
     const long long blocks = (long long)((budget + rows_per_block - 1) / rows_per_block) * (ks + vs + (mass != nullptr ? 1 : 0));
     HB_REQUIRE(blocks <= 0x7fffffffLL, "evict_rows: too many rows for one launch");
