@@ -1,0 +1,394 @@
+// Attention of a chunk of new tokens over the paged cache on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), bfloat16, head
+// size 64 or 128, that leaves each row's log-sum for the weights' kernel (attention_mass_tc.cu): causal, grouped, with a window,
+// sequences with unequal numbers of new tokens, the keys cut into shares where there are few rows.
+//
+// One CTA = two tiles of 128 query rows that read the same keys and values: two heads of a kv head with an even group, else two
+// neighbouring blocks of one head's tokens.  A tile's rows are the 128 lanes of tensor memory.  What bounds it, per 128 x 128 scores at
+// head size 128: 1024 clocks of the two products, 1024 clocks of exponentials (16 a clock and SM), and 64 KB of keys and values, which at the
+// 32 bytes a clock that an SM takes from L2 would last 2048 clocks for one tile: hence two tiles, which halve that, and which take turns:
+// while one tile's weights are made, the tensor cores work on the other.
+//   warps 0-3, 4-7  softmax of tile 0 and 1, a thread per row: 128 scores from tensor memory into registers, running maximum and sum in
+//                   float32, weights as bfloat16 over the scores.  No exchange between threads.  The output accumulator is rescaled only
+//                   when a row's maximum grows by more than 2^8 (weights are taken against a maximum that may be stale by less).
+//   warp 8          TMA producer: the query tiles once, then key and value tiles of 128 rows (two pages), two stages each
+//   warp 9          owns tensor memory; one thread issues, per key tile and in this order: O0 += P0 V, S0 = Q0 K' (the next keys),
+//                   O1 += P1 V, S1 = Q1 K'.  P lies over S; the tensor cores take the products in order.
+// Weights are rounded to bfloat16 for the product with the values (the sum they are divided by is taken before that).
+//
+// Every wait is bounded; a wait that runs out sets *error_flag and the CTA drains and leaves.
+#include "api.h"
+#include "attention_mass.cuh"
+#include "attention_tc.cuh"
+
+#define CT_THREADS 320
+#define CT_STAGES 2
+
+template <int HD>
+__global__ void __launch_bounds__(CT_THREADS, 1)
+chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
+                bf16* __restrict__ out, long long out_stride, float* __restrict__ lse, float* __restrict__ part_o, float* __restrict__ part_ml,
+                int n_tokens, int n_seqs, int nh, int nkv, int head_pairs, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    // [Q tiles 2][K stages][V stages][barriers]; a tile is 128 rows x HD
+    constexpr int HALVES = HD / 64, TILE = HALVES * FA_HALF_BYTES;
+    uint64_t* bars = (uint64_t*)(smem + (2 + 2 * CT_STAGES) * TILE);
+    uint32_t* tmem_slot = (uint32_t*)(bars + 16);
+    const uint32_t smem_base = smem_u32(smem), k_smem = smem_base + 2 * TILE, v_smem = k_smem + CT_STAGES * TILE;
+    const uint32_t q_full = smem_u32(bars), k_full0 = smem_u32(bars + 1), k_empty0 = smem_u32(bars + 3), v_full0 = smem_u32(bars + 5),
+                   v_empty0 = smem_u32(bars + 7), s_full0 = smem_u32(bars + 9), p_full0 = smem_u32(bars + 11), o_full0 = smem_u32(bars + 13);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // The two tiles: heads head0 and head0 + 1 (head_pairs) of one block of tokens, or blocks 2 blk and 2 blk + 1 of head0.  Blocks
+    // are taken from the back and heads are the fast index: what sees the most keys starts first.
+    const int z = blockIdx.z, S = gridDim.z;
+    const int head0 = head_pairs ? 2 * blockIdx.x : blockIdx.x, g = head0 / (nh / nkv);
+    const int span = head_pairs ? FA_ROWS : 2 * FA_ROWS;
+    int b = 0, blk = 0;
+    const bool has_work = mass_find_block(seq_start, n_seqs, gridDim.y - 1 - blockIdx.y, span, b, blk);
+    const int t_begin = has_work ? seq_start[b] : 0, n_new = has_work ? seq_start[b + 1] - t_begin : 0, pos0 = has_work ? seq_pos0[b] : 0;
+    const int row0 = blk * span;                               // the first of the CTA's new tokens
+    const int first_pos = pos0 + row0, last_pos = pos0 + min(row0 + span, n_new) - 1;
+    const int lo_cta = hb_oldest_visible(first_pos, window, 0);
+    int jt0 = lo_cta / FA_KEYS, n_it = has_work ? last_pos / FA_KEYS + 1 - jt0 : 0;
+    {                                                          // this share's tiles of keys
+        const int a = (int)((long long)n_it * z / S), e = (int)((long long)n_it * (z + 1) / S);
+        jt0 += a;
+        n_it = e - a;
+    }
+
+    if (threadIdx.x == 0) {
+        mbar_init(q_full, 1);
+        for (int s = 0; s < 2; s++) {
+            mbar_init(k_full0 + 8 * s, 1);
+            mbar_init(k_empty0 + 8 * s, 1);
+            mbar_init(v_full0 + 8 * s, 1);
+            mbar_init(v_empty0 + 8 * s, 1);
+            mbar_init(s_full0 + 8 * s, 1);
+            mbar_init(p_full0 + 8 * s, 128);
+            mbar_init(o_full0 + 8 * s, 1);
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 9) tmem_alloc(smem_u32(tmem_slot), 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;                    // S0, S1 at columns 0 and 128, O0, O1 at 256 and 384
+    pdl_trigger();
+    pdl_wait();
+
+    if (warp == 8) {
+        // ---------------------------------------------------------------- TMA producer
+        if (lane == 0 && n_it > 0) {
+            const int* pt = page_table + (size_t)b * pt_width;
+            mbar_expect_tx(q_full, 2 * TILE);
+            for (int i = 0; i < 2; i++)
+                for (int half = 0; half < HALVES; half++)
+                    tma_load_2d(smem_base + i * TILE + half * FA_HALF_BYTES, &map_q, q_full, (head0 + (head_pairs ? i : 0)) * HD + half * 64,
+                                t_begin + row0 + (head_pairs ? 0 : i * FA_ROWS));
+            auto load_tile = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int it) {
+                mbar_expect_tx(bar, TILE);
+                for (int pg = 0; pg < 2; pg++) {
+                    const int pi = (jt0 + it) * 2 + pg;
+                    int page = pi < pt_width ? pt[pi] : -1;
+                    if (page < 0 || page >= n_pages) {
+                        // a page behind the last row's key or in front of the oldest that the first row sees may be missing
+                        if (page >= n_pages || (pi >= lo_cta / HB_PAGE_TOKENS && pi <= last_pos / HB_PAGE_TOKENS))
+                            hb_note(error_flag, HB_STATUS_PAGE, 1 + b);
+                        page = 0;                                   // never read outside the cache
+                    }
+                    for (int half = 0; half < HALVES; half++)
+                        tma_load_2d(dst + half * FA_HALF_BYTES + pg * (FA_HALF_BYTES / 2), map, bar, half * 64, (page * nkv + g) * HB_PAGE_TOKENS);
+                }
+            };
+            int k_issued = 0, v_issued = 0;
+            for (int it = 0; it < n_it; it++) {
+                const int s = it % CT_STAGES;
+                if (!mbar_wait(k_empty0 + 8 * s, ((it / CT_STAGES) & 1) ^ 1)) {
+                    atomicExch(error_flag, 51);
+                    break;
+                }
+                load_tile(k_smem + s * TILE, &map_k, k_full0 + 8 * s, it);
+                k_issued = it + 1;
+                if (!mbar_wait(v_empty0 + 8 * s, ((it / CT_STAGES) & 1) ^ 1)) {
+                    atomicExch(error_flag, 52);
+                    break;
+                }
+                load_tile(v_smem + s * TILE, &map_v, v_full0 + 8 * s, it);
+                v_issued = it + 1;
+            }
+            for (int it = max(0, k_issued - CT_STAGES); it < k_issued; it++)
+                if (!mbar_wait(k_full0 + 8 * (it % CT_STAGES), (it / CT_STAGES) & 1)) atomicExch(error_flag, 53);
+            for (int it = max(0, v_issued - CT_STAGES); it < v_issued; it++)
+                if (!mbar_wait(v_full0 + 8 * (it % CT_STAGES), (it / CT_STAGES) & 1)) atomicExch(error_flag, 53);
+            if (!mbar_wait(q_full, 0)) atomicExch(error_flag, 53);
+        }
+    } else if (warp == 9) {
+        // ---------------------------------------------------------------- MMA issuer
+        if (lane == 0 && n_it > 0) {
+            constexpr uint32_t idesc_qk = instr_desc_bf16_mn(128, FA_KEYS);
+            constexpr uint32_t idesc_pv = instr_desc_bf16_mn(128, HD) | (1u << 16);           // B is MN-major
+            auto scores = [&](int i, int it) {
+                const uint32_t kst = k_smem + (it % CT_STAGES) * TILE;
+#pragma unroll
+                for (int kk = 0; kk < HD / 16; kk++) {
+                    const uint32_t off = (kk >> 2) * FA_HALF_BYTES + (kk & 3) * 32;
+                    umma_bf16(tmem_base + i * 128, smem_desc_sw128(smem_base + i * TILE + off), smem_desc_sw128(kst + off), idesc_qk, kk ? 1u : 0u);
+                }
+                umma_commit(s_full0 + 8 * i);
+                if (i == 1) umma_commit(k_empty0 + 8 * (it % CT_STAGES));
+            };
+            bool alive = mbar_wait(q_full, 0) && mbar_wait(k_full0, 0);
+            if (alive) {
+                tc_fence_after();
+                scores(0, 0);
+                scores(1, 0);
+            } else {
+                atomicExch(error_flag, 54);
+            }
+            for (int it = 0; it < n_it && alive; it++) {
+                const int sv = it % CT_STAGES;
+                const uint32_t vst = v_smem + sv * TILE;
+#pragma unroll
+                for (int i = 0; i < 2 && alive; i++) {
+                    if (!mbar_wait(p_full0 + 8 * i, it & 1) || (i == 0 && !mbar_wait(v_full0 + 8 * sv, (it / CT_STAGES) & 1)) ||
+                        (i == 0 && it + 1 < n_it && !mbar_wait(k_full0 + 8 * ((it + 1) % CT_STAGES), ((it + 1) / CT_STAGES) & 1))) {
+                        atomicExch(error_flag, 55);
+                        alive = false;
+                        break;
+                    }
+                    tc_fence_after();
+#pragma unroll
+                    for (int kk = 0; kk < FA_KEYS / 16; kk++)
+                        umma_bf16_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + kk * 8, smem_desc_mn_sw128(vst + kk * 16 * 128, FA_HALF_BYTES, 1024),
+                                     idesc_pv, (it | kk) ? 1u : 0u);
+                    if (i == 1) umma_commit(v_empty0 + 8 * sv);
+                    if (it + 1 < n_it) scores(i, it + 1);
+                    else umma_commit(o_full0 + 8 * i);
+                }
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- softmax and output: a thread per row
+        const int i = warp >> 2, r = (warp & 3) * 32 + lane;   // tile, row of the tile = lane of tensor memory
+        const int head = head0 + (head_pairs ? i : 0), row = row0 + (head_pairs ? 0 : i * FA_ROWS) + r;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t tm_s = tmem_base + i * 128 + lane_base, tm_o = tmem_base + 256 + i * 128 + lane_base;
+        const int qpos = pos0 + row, lo = hb_oldest_visible(qpos, window, 0);
+        const bool valid = has_work && row < n_new;
+        float m_run = -INFINITY, l = 0.0f;
+        bool ok = true;
+        for (int it = 0; it < n_it; it++) {
+            if (!__all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * i, it & 1))) {
+                atomicExch(error_flag, 56);
+                ok = false;
+                break;
+            }
+            tc_fence_after();
+            float sv[128];
+            tmem_ld64(tm_s, sv);
+            tmem_ld64(tm_s + 64, sv + 64);
+            // this row sees keys lo..qpos; as columns of the tile: [c_lo, c_hi]
+            const int kbase = (jt0 + it) * FA_KEYS, c_lo = lo - kbase, c_hi = qpos - kbase;
+            if (c_lo > 0 || c_hi < 127) {                      // the causal diagonal or the window's edge
+#pragma unroll
+                for (int e = 0; e < 128; e++)
+                    if (e < c_lo || e > c_hi) sv[e] = -INFINITY;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 128; e += 8) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], fmaxf(sv[e + u], sv[e + 4 + u]));
+            }
+            const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2e;
+            if (it == 0) {
+                m_run = m_tile;
+            } else {
+                const bool grow = m_tile > m_run + FA_RESCALE_THRESHOLD;
+                if (__any_sync(0xffffffffu, grow)) {
+                    // S of this tile is complete, so is every product issued before it: nothing touches the accumulator now
+                    const float m_new = fmaxf(m_run, m_tile);
+                    const float corr = m_new == -INFINITY ? 1.0f : exp2f(m_run - m_new);
+                    m_run = m_new;
+                    l *= corr;
+#pragma unroll 1
+                    for (int c = 0; c < HD / 16; c++) {
+                        float v[16];
+                        tmem_ld16(tm_o + c * 16, v);
+                        uint32_t u[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) u[e] = __float_as_uint(v[e] * corr);
+                        tmem_st16u(tm_o + c * 16, u);
+                    }
+                    tmem_wait_st();
+                }
+            }
+            const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
+            float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t pk[16];
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    const float p0 = exp2_approx(fmaf(sv[c * 32 + e], scale_log2e, neg_m));
+                    const float p1 = exp2_approx(fmaf(sv[c * 32 + e + 1], scale_log2e, neg_m));
+                    sum4[e & 2] += p0;
+                    sum4[(e & 2) + 1] += p1;
+                    pk[e >> 1] = pack_bf16_pair(p0, p1);
+                }
+                tmem_st16u(tm_s + c * 16, pk);                 // P over S
+            }
+            l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+            if (i == 0 && (jt0 + it + 1) * FA_KEYS > pos0 + n_new) {
+                // the tile that holds the sequence's end: values behind it are whatever a page held before, and 0 * NaN is NaN
+                const int s = it % CT_STAGES;
+                if (!__all_sync(0xffffffffu, mbar_wait(v_full0 + 8 * s, (it / CT_STAGES) & 1))) {
+                    atomicExch(error_flag, 57);
+                    ok = false;
+                    break;
+                }
+                const int from = pos0 + n_new - kbase;         // rows from..127, 128 bytes of each half
+                for (int u = threadIdx.x + from * 8 * HALVES; u < FA_KEYS * 8 * HALVES; u += 128) {
+                    const int vr = u / (8 * HALVES), c = u % (8 * HALVES);
+                    *reinterpret_cast<uint4*>(smem + (2 + CT_STAGES + s) * TILE + (c >> 3) * FA_HALF_BYTES + vr * 128 + (c & 7) * 16) =
+                        make_uint4(0u, 0u, 0u, 0u);
+                }
+                fence_async_shared();                          // before the tensor core reads them (tile 0's product is issued first)
+            }
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(p_full0 + 8 * i);
+        }
+        const size_t at = ((size_t)z * nh + head) * n_tokens + t_begin + row;
+        if (n_it == 0) {                                       // a share without keys
+            if (valid && S > 1) {
+                part_ml[at * 2] = -INFINITY;
+                part_ml[at * 2 + 1] = 0.0f;
+            }
+        } else if (ok) {
+            if (!__all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * i, 0))) {
+                atomicExch(error_flag, 58);
+            } else {
+                tc_fence_after();
+                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+                bf16* dst = out + (size_t)(t_begin + row) * out_stride + (size_t)head * HD;
+                if (valid && S > 1) *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(m_run, l);
+                if (valid && S == 1) lse[at] = l > 0.0f ? m_run + log2f(l) : INFINITY;
+#pragma unroll 1
+                for (int c = 0; c < HD / 32; c++) {
+                    float v[32];
+                    tmem_ld32(tm_o + c * 32, v);
+                    if (!valid) continue;
+                    if (S > 1) {
+                        float4* po = reinterpret_cast<float4*>(part_o + at * HD + c * 32);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) po[e >> 2] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            uint4 o4;
+                            o4.x = pack_bf16_pair(v[e] * inv, v[e + 1] * inv);
+                            o4.y = pack_bf16_pair(v[e + 2] * inv, v[e + 3] * inv);
+                            o4.z = pack_bf16_pair(v[e + 4] * inv, v[e + 5] * inv);
+                            o4.w = pack_bf16_pair(v[e + 6] * inv, v[e + 7] * inv);
+                            *reinterpret_cast<uint4*>(dst + c * 32 + e) = o4;
+                        }
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// out = sum_z o_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), lse = M + log2 of that sum; a warp per (token, head)
+template <int HD>
+__global__ void __launch_bounds__(256)
+chunk_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, bf16* __restrict__ out, long long out_stride,
+                  float* __restrict__ lse, int n_tokens, int nh, int S) {
+    pdl_trigger();
+    pdl_wait();
+    const int t = blockIdx.x, lane = threadIdx.x & 31;
+    for (int head = blockIdx.y * 8 + (threadIdx.x >> 5); head < nh; head += gridDim.y * 8) {
+        const size_t at = (size_t)head * n_tokens + t, step = (size_t)nh * n_tokens;
+        float2 ml = make_float2(-INFINITY, 0.0f);              // of share `lane` (S <= 32)
+        if (lane < S) ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + at + lane * step);
+        const float M = warp_max(ml.x);
+        const float w = ml.x != -INFINITY ? exp2f(ml.x - M) : 0.0f;
+        const float L = warp_sum(ml.y * w);
+        float acc[HD / 32];
+#pragma unroll
+        for (int c = 0; c < HD / 32; c++) acc[c] = 0.0f;
+        for (int s = 0; s < S; s++) {
+            const float ws = __shfl_sync(0xffffffffu, w, s);
+            if (ws == 0.0f) continue;                          // its partial output may not have been written
+            const float* po = part_o + (at + s * step) * HD + lane;
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) acc[c] = fmaf(__ldcg(po + c * 32), ws, acc[c]);
+        }
+        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+        for (int c = 0; c < HD / 32; c++) out[(size_t)t * out_stride + (size_t)head * HD + c * 32 + lane] = __float2bfloat16_rn(acc[c] * inv);
+        if (lane == 0) lse[at] = L > 0.0f ? M + log2f(L) : INFINITY;
+    }
+}
+
+template <int HD>
+static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width, const int* seq_start,
+                        const int* seq_pos0, bf16* out, long long out_stride, float* lse, float* parts, int splits, int n_tokens, int n_seqs, int q_blocks,
+                        int nh, int nkv, int head_pairs, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
+    constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 16 * 8 + 16 + 1024;
+    static_assert(SMEM <= 227 * 1024, "attention tiles do not fit shared memory");
+    static bool done[HB_MAX_DEVICES] = {};
+    bool& set = done[hb_device_slot()];
+    if (!set) {
+        cudaError_t e = cudaFuncSetAttribute(chunk_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e != cudaSuccess) return hb_fail("attention_mass: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
+        set = true;
+    }
+    float* part_o = parts;
+    float* part_ml = parts == nullptr ? nullptr : parts + (size_t)splits * nh * n_tokens * HD;
+    cudaError_t e = hb_launch(chunk_tc_kernel<HD>, dim3(head_pairs ? nh / 2 : nh, q_blocks, splits), dim3(CT_THREADS), SMEM, s, mq, mk, mv, page_table,
+                              pt_width, seq_start, seq_pos0, out, out_stride, lse, part_o, part_ml, n_tokens, n_seqs, nh, nkv, head_pairs,
+                              scale * FA_LOG2E, window, n_pages, error_flag);
+    if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
+    if (hb_check_launch("attention_mass (chunk)")) return 1;
+    if (splits == 1) return 0;
+    e = hb_launch(chunk_join_kernel<HD>, dim3(n_tokens, (nh + 7) / 8), dim3(256), 0, s, part_o, part_ml, out, out_stride, lse, n_tokens, nh, splits);
+    if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
+    return hb_check_launch("attention_mass (join of the chunk)");
+}
+
+int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
+                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, float* parts, int splits, int n_tokens,
+                       int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
+                       cudaStream_t s) {
+    HB_REQUIRE(hb_attention_prefill_tc_supported(n_heads, n_kv_heads, head_dim), "attention_mass: head size %d is not built for the tensor cores (64, 128)",
+               head_dim);
+    HB_REQUIRE(q_blocks > 0 && q_blocks <= 65535 && error_flag != nullptr && splits >= 1 && splits <= 32 && (splits == 1 || parts != nullptr),
+               "attention_mass: the step is too large for one launch");
+    HB_REQUIRE(q_stride % 8 == 0 && ((uintptr_t)q & 15) == 0, "attention_mass: queries must have 16-byte aligned rows");
+    HB_REQUIRE(out_stride % 8 == 0 && ((uintptr_t)out & 15) == 0, "attention_mass: output must have 16-byte aligned rows");
+    HB_REQUIRE((((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0, "attention_mass: cache must be 16-byte aligned");
+    CUtensorMap mq, mk, mv;
+    const long long cache_rows = (long long)n_pages * n_kv_heads * HB_PAGE_TOKENS;
+    HB_REQUIRE(cache_rows <= 0x7fffffffLL, "attention_mass: the cache has too many rows for a tensor map");
+    if (tc_make_map(&mq, q, n_tokens, (long long)n_heads * head_dim, q_stride, FA_ROWS)) return 1;
+    if (tc_make_map(&mk, k_cache, cache_rows, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
+    if (tc_make_map(&mv, v_cache, cache_rows, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
+    const int head_pairs = (n_heads / n_kv_heads) % 2 == 0;
+    if (head_dim == 128)
+        return launch_chunk<128>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, parts, splits, n_tokens, n_seqs, q_blocks,
+                                 n_heads, n_kv_heads, head_pairs, scale, window, n_pages, error_flag, s);
+    return launch_chunk<64>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, parts, splits, n_tokens, n_seqs, q_blocks,
+                            n_heads, n_kv_heads, head_pairs, scale, window, n_pages, error_flag, s);
+}

@@ -84,3 +84,11 @@ int mass_join(const int* page_table, int pt_width, const int* seq_start, const i
 int attention_decode_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* tok_seq,
                             const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int n_tokens, int nh,
                             int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);
+
+// The first half of a step of many tokens on the tensor cores (attention_chunk_tc.cu): writes out and lse [heads][tokens].  q_blocks: sum
+// over sequences of ceil(new tokens / span), span 128 with an even group of heads and 256 with an odd one; parts: splits * n_heads *
+// n_tokens * (head_dim + 2) floats when splits > 1 (at most 32).
+int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
+                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, float* parts, int splits, int n_tokens,
+                       int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
+                       cudaStream_t s);

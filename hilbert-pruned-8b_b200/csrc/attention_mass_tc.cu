@@ -1,5 +1,5 @@
 // The weights of steps of many tokens on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), bfloat16, head size 64 or 128:
-// the second half of attention_mass.cu's arithmetic, behind the prompt attention that leaves each row's log-sum.
+// the second half of attention_mass.cu's arithmetic, behind the attention that leaves each row's log-sum (attention_chunk_tc.cu).
 //
 // One CTA = 256 consecutive rows of a sequence's cache x one kv head x a share of the (head, 128 queries) tiles that see them.
 // Keys are the M operand: a tile's 128 keys are the 128 lanes of tensor memory and the queries its columns, so that a key's sum over
@@ -255,25 +255,26 @@ static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const in
 
 extern "C" int hb_attention_mass_tc_keys(void) { return MT_KEYS; }
 
-// Sizes and types of hb_attention_prefill_tc, with the same alignment of queries and output.  q_blocks: sum over sequences of
-// ceil(new tokens / 128); key_tiles: sum of ceil(rows / 256); lse: n_heads * n_tokens floats; parts: splits * n_kv_heads *
-// key_tiles * 256 floats when splits > 1.
+// Sizes and types of hb_attention_prefill_tc, with the same alignment of queries and output.  q_blocks, chunk_parts, chunk_splits: as
+// attention_chunk_tc (attention_mass.cuh); key_tiles: sum over sequences of ceil(rows / 256); lse: n_heads * n_tokens floats; parts:
+// splits * n_kv_heads * key_tiles * 256 floats when splits > 1.
 extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
                                     const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, const float* before,
-                                    float* mass, float* parts, int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads,
-                                    int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag, void* stream) {
+                                    float* mass, float* parts, float* chunk_parts, int chunk_splits, int splits, int n_tokens, int n_seqs, int q_blocks,
+                                    int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
+                                    void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(lse != nullptr && mass != nullptr && n_kv_heads > 0 && n_kv_heads <= 65535 && key_tiles > 0 && splits >= 1 && splits <= 65535 &&
                    (splits == 1 || parts != nullptr),
-               "attention_mass_tc: bad sizes");
-    if (attention_prefill_tc_lse(q, q_stride, n_tokens, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, n_seqs, q_blocks,
-                                 n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, lse, stream))
+               "attention_mass: bad sizes");
+    cudaStream_t s = (cudaStream_t)stream;
+    if (attention_chunk_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, chunk_parts, chunk_splits,
+                           n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s))
         return 1;
     CUtensorMap mq, mk;
     if (tc_make_map(&mq, q, n_tokens, (long long)n_heads * head_dim, q_stride, 128)) return 1;
     if (tc_make_map(&mk, k_cache, (long long)n_pages * n_kv_heads * HB_PAGE_TOKENS, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     MassOut mo = {before, mass, parts};
-    cudaStream_t s = (cudaStream_t)stream;
     const int rc = head_dim == 128 ? launch_mass_tc<128>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, mo, splits, n_tokens, n_seqs, key_tiles,
                                                          n_heads, n_kv_heads, scale, window, n_pages, error_flag, s)
                                    : launch_mass_tc<64>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, mo, splits, n_tokens, n_seqs, key_tiles,

@@ -27,15 +27,13 @@
 #define FA_TILE_BYTES(HD) ((HD) / 64 * FA_HALF_BYTES) // 128 rows x head size, bf16
 #define FA_STAGES 3
 
-// LSE: the variant whose caller goes on with the rows' log-sums (attention_mass_tc.cu): it writes lse[head][token] = the log of
-// the row's sum of exponentials, in units of log 2, and takes rows of the cache behind the sequence's end for zero.
-template <int HD, bool LSE>
+template <int HD>
 __global__ void __launch_bounds__(FA_THREADS, 1)
 attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                        const __grid_constant__ CUtensorMap map_v, const int* __restrict__ page_table, int pt_width,
                        const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, bf16* __restrict__ out,
                        long long out_stride, int n_seqs, int nh, int nkv, float scale_log2e, int window, int n_pages,
-                       int* __restrict__ error_flag, float* __restrict__ lse, int n_tokens) {
+                       int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // [Q tile][K stages 3 x tile][V stages 3 x tile][barriers]; a tile is 128 rows x HD
@@ -306,21 +304,6 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 atomicExch(error_flag, 28);
                 *abort_flag = 1;
             }
-            if (LSE && (jt0 + it + 1) * FA_KEYS > pos0 + n_new) {
-                // the tile that holds the sequence's end: values behind it are whatever a page held before, and 0 * NaN is NaN
-                const int sv2 = it % FA_STAGES;
-                if (!mbar_wait(v_full0 + 8 * sv2, (it / FA_STAGES) & 1)) {
-                    atomicExch(error_flag, 30);
-                    *abort_flag = 1;
-                }
-                const int from = pos0 + n_new - (jt0 + it) * FA_KEYS;          // rows from..127, 128 bytes of each half
-                for (int i = (threadIdx.x - 64) + from * 8 * HALVES; i < FA_KEYS * 8 * HALVES; i += 256) {
-                    const int row = i / (8 * HALVES), c = i % (8 * HALVES);
-                    *reinterpret_cast<uint4*>(smem + TILE + FA_STAGES * TILE + sv2 * TILE + (c >> 3) * FA_HALF_BYTES + row * 128 + (c & 7) * 16) =
-                        make_uint4(0u, 0u, 0u, 0u);
-                }
-                fence_async_shared();                          // before the tensor core reads them
-            }
             tc_fence_before();
             mbar_arrive(p_full0 + 8 * s);
         }
@@ -336,7 +319,6 @@ attn_prefill_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
             tc_fence_after();
             const float lt = xrow[r] + xrow[128 + r];
             const float inv = lt > 0.0f ? 1.0f / lt : 0.0f;
-            if (LSE && hf == 0 && valid) lse[(size_t)head * n_tokens + t_begin + row_base + r] = lt > 0.0f ? m_run + log2f(lt) : INFINITY;
             bf16* dst = out + (size_t)(t_begin + row_base + r) * out_stride + (size_t)head * HD + hf * OC;
 #pragma unroll 1
             for (int c = 0; c < OC / 32; c++) {
@@ -368,23 +350,22 @@ extern "C" int hb_attention_prefill_tc_supported(int n_heads, int n_kv_heads, in
     return (head_dim == 64 || head_dim == 128) && n_kv_heads > 0 && n_heads % n_kv_heads == 0;
 }
 
-template <int HD, bool LSE>
+template <int HD>
 static int launch_prefill_tc(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width,
                              const int* seq_start, const int* seq_pos0, void* out, long long out_stride, int n_seqs, int q_blocks,
-                             int n_heads, int n_kv_heads, float scale, int window, int n_pages, int* error_flag, float* lse, int n_tokens,
-                             cudaStream_t stream) {
+                             int n_heads, int n_kv_heads, float scale, int window, int n_pages, int* error_flag, cudaStream_t stream) {
     constexpr int TILE = FA_TILE_BYTES(HD);
     constexpr int SMEM = TILE + FA_STAGES * 2 * TILE + 18 * 8 + 16 + 2 * 128 * 4 + 1024;
     static_assert(SMEM <= 227 * 1024, "attention tiles do not fit shared memory");
     static bool attr_set = false;
     if (!attr_set) {
-        cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc_kernel<HD, LSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        cudaError_t e = cudaFuncSetAttribute(attn_prefill_tc_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return hb_fail("attention_prefill_tc: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
         attr_set = true;
     }
-    cudaError_t e = hb_launch(attn_prefill_tc_kernel<HD, LSE>, dim3(n_heads, q_blocks), dim3(FA_THREADS), SMEM, stream, mq, mk, mv,
+    cudaError_t e = hb_launch(attn_prefill_tc_kernel<HD>, dim3(n_heads, q_blocks), dim3(FA_THREADS), SMEM, stream, mq, mk, mv,
                               page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, n_seqs, n_heads, n_kv_heads,
-                              scale * FA_LOG2E, window, n_pages, error_flag, lse, n_tokens);
+                              scale * FA_LOG2E, window, n_pages, error_flag);
     if (e != cudaSuccess) return hb_fail("attention_prefill_tc: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_prefill_tc");
 }
@@ -392,11 +373,12 @@ static int launch_prefill_tc(const CUtensorMap& mq, const CUtensorMap& mk, const
 // Tensor map over rows of `cols` bfloat16 with row stride `ld`: boxes of 64 columns x box_rows.
 // q: [tokens, q_stride] (head j at columns [j*hd, (j+1)*hd)); k_cache / v_cache: one layer,
 // [n_pages][n_kv_heads][64][hd]; seq_start / seq_pos0 as for hb_attention_prefill; q_blocks =
-// sum over sequences of ceil(new tokens / 128).  lse: null, or n_heads * n_tokens floats.
-int attention_prefill_tc_lse(const void* q, long long q_stride, long long n_tokens, const void* k_cache,
-                             const void* v_cache, const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0, void* out,
-                             long long out_stride, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale,
-                             int window, int n_pages, int* error_flag, float* lse, void* stream) {
+// sum over sequences of ceil(new tokens / 128).
+extern "C" int hb_attention_prefill_tc(const void* q, long long q_stride, long long n_tokens, const void* k_cache,
+                                       const void* v_cache, const int* page_table, int pt_width, const int* seq_start,
+                                       const int* seq_pos0, void* out, long long out_stride, int n_seqs, int q_blocks,
+                                       int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages,
+                                       int* error_flag, void* stream) {
     if (n_seqs == 0 || q_blocks == 0) return 0;
     HB_REQUIRE(hb_attention_prefill_tc_supported(n_heads, n_kv_heads, head_dim),
                "attention_prefill_tc: head size %d is not built (64, 128)", head_dim);
@@ -410,18 +392,9 @@ int attention_prefill_tc_lse(const void* q, long long q_stride, long long n_toke
     if (tc_make_map(&mk, k_cache, cache_rows, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     if (tc_make_map(&mv, v_cache, cache_rows, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     cudaStream_t st = (cudaStream_t)stream;
-#define HB_PREFILL_TC(HD, LSE)                                                                                                          \
-    launch_prefill_tc<HD, LSE>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, out, out_stride, n_seqs, q_blocks, n_heads, n_kv_heads, \
-                               scale, window, n_pages, error_flag, lse, (int)n_tokens, st)
-    if (head_dim == 128) return lse != nullptr ? HB_PREFILL_TC(128, true) : HB_PREFILL_TC(128, false);
-    return lse != nullptr ? HB_PREFILL_TC(64, true) : HB_PREFILL_TC(64, false);
-#undef HB_PREFILL_TC
-}
-
-extern "C" int hb_attention_prefill_tc(const void* q, long long q_stride, long long n_tokens, const void* k_cache, const void* v_cache,
-                                       const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0, void* out,
-                                       long long out_stride, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale,
-                                       int window, int n_pages, int* error_flag, void* stream) {
-    return attention_prefill_tc_lse(q, q_stride, n_tokens, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, n_seqs,
-                                    q_blocks, n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, nullptr, stream);
+    if (head_dim == 128)
+        return launch_prefill_tc<128>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, out, out_stride, n_seqs, q_blocks, n_heads,
+                                      n_kv_heads, scale, window, n_pages, error_flag, st);
+    return launch_prefill_tc<64>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, out, out_stride, n_seqs, q_blocks, n_heads,
+                                 n_kv_heads, scale, window, n_pages, error_flag, st);
 }

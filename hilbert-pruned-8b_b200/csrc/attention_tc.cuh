@@ -91,9 +91,3 @@ __device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t addr, uint32_t l
     d |= (uint64_t)2 << 61;
     return d;
 }
-
-// The prompt attention of attention_prefill_tc.cu; lse: null, or n_heads * n_tokens floats for the rows' log-sums in units of log 2
-// (the rows of the cache behind a sequence's end then count as zero whatever they hold).
-int attention_prefill_tc_lse(const void* q, long long q_stride, long long n_tokens, const void* k_cache, const void* v_cache, const int* page_table,
-                             int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, int n_seqs, int q_blocks,
-                             int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag, float* lse, void* stream);

@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import build
-from .plan import decode_splits, few_splits, mass_splits, select_shape
+from .plan import chunk_splits, decode_splits, few_splits, mass_splits, select_shape
 
 _c_int, _c_ll, _c_float, _c_ptr = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
 
@@ -82,7 +82,7 @@ _SIGNATURES = {
     "hb_attention_mass": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                           _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_tc": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
-                             _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
+                             _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr,
                               _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int,
                               _c_ptr, _c_ptr],
@@ -1272,6 +1272,8 @@ class Ops:
         self._mass_like(mass, "mass", pages, kv_heads)
         if before is not None:
             self._mass_like(before, "before", pages, kv_heads)
+        if not 0.0 < scale < float("inf"):
+            raise KernelError(f"attention: the scale must be positive and finite, got {scale}")
         if T == 0:
             return
         win = int(window) if window else 0
@@ -1300,18 +1302,22 @@ class Ops:
             tc = (self.use_fast_attention and self.use_tcgen05_attention and qkv.dtype == torch.bfloat16
                   and self.lib.hb_attention_prefill_tc_supported(heads, kv_heads, head_dim) and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0
                   and cache.k.data_ptr() % 16 == 0 and cache.v.data_ptr() % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0)
-            rows, keys = (128, self.lib.hb_attention_mass_tc_keys()) if tc else (64, 64)
+            # rows of a block of queries (two tiles of 128: two heads, or with an odd group two blocks of tokens), of a tile of keys
+            rows, keys = (128 if group % 2 == 0 else 256, self.lib.hb_attention_mass_tc_keys()) if tc else (64, 64)
             q_blocks = sum(-(-n // rows) for n in step.host_new)
             key_tiles = sum(-(-n // keys) for n in step.host_len)
             if splits is None:
-                splits = mass_splits(key_tiles, kv_heads, group * -(-step.max_new // rows), self.sm_count * (1 if tc else 2))
+                splits = mass_splits(key_tiles, kv_heads, group * -(-step.max_new // (128 if tc else 64)), self.sm_count * (1 if tc else 2))
             parts = torch.empty(splits * kv_heads * key_tiles * keys, dtype=torch.float32, device=self.device) if splits > 1 else None
             sizes = (splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim, float(scale), win, pages, self.status.data_ptr(),
                      self._stream())
             buffers = (cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(),
                        out.data_ptr(), out_ld, lse.data_ptr(), old, mass.data_ptr(), parts.data_ptr() if parts is not None else None)
             if tc:
-                self._call("hb_attention_mass_tc", qkv.data_ptr(), q_ld, *buffers, *sizes)
+                ways = chunk_splits((heads // 2 if group % 2 == 0 else heads) * q_blocks, step.max_len, self.sm_count)
+                shares = torch.empty(ways * heads * T * (head_dim + 2), dtype=torch.float32, device=self.device) if ways > 1 else None
+                self._call("hb_attention_mass_tc", qkv.data_ptr(), q_ld, *buffers, shares.data_ptr() if shares is not None else None, ways, *sizes)
+                self.launches += 0 if ways == 1 else 1
             else:
                 self._call("hb_attention_mass", qkv.data_ptr(), code, q_ld, *buffers, *sizes)
             self.launches += 2 if splits == 1 else 3

@@ -35,6 +35,14 @@ def few_splits(tokens: int, kv_heads: int, max_pages: int, cta_slots: int) -> in
     return max(decode_splits(tokens, kv_heads, max_pages, cta_slots), min(max_pages, 16, room))
 
 
+def chunk_splits(blocks: int, longest: int, sms: int) -> int:
+    """Shares of the keys in the attention of a chunk whose ``blocks`` (two tiles of queries each) take an SM each: one where they
+    fill half the device, else as many as fit it in one wave, with 4 tiles of 128 keys or more of the longest sequence to a share."""
+    if 2 * blocks > sms:
+        return 1
+    return max(1, min(32, sms // max(1, blocks), longest // 512))
+
+
 def mass_splits(key_tiles: int, kv_heads: int, items: int, cta_slots: int) -> int:
     """Shares of the weights' kernel for ``key_tiles`` x ``kv_heads`` (tile of keys, kv head) pairs with up to ``items`` tiles of
     queries each: under a causal mask the first keys are seen by every query and the last by few, so the work evens out only

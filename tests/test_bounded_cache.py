@@ -145,6 +145,10 @@ MANY = [
     (2, 1, 256, [100], [70], None),
     (4, 4, 200, [0, 64], [64, 100], 65),
     (1, 1, 8, [0], [10], None),
+    (4, 2, 128, [9000], [20], None),             # few rows, many keys: the keys are shared out
+    (3, 1, 64, [5000, 100], [30, 10], 2000),
+    (8, 8, 64, [0, 300], [513, 129], None),
+    (6, 2, 128, [0, 131], [400, 255], 130),
 ]
 FEW = [
     (4, 2, 64, [0], [1], None),
@@ -481,7 +485,7 @@ def _attention_args(**kw):
     a.update(kw)
     step = n(num_tokens=a.pop("tokens"), num_seqs=1, page_tables=[torch.zeros(1, 2, dtype=torch.int32)], max_new=3, max_len=3, host_new=[3], host_len=[3])
     cache = n(k=a.pop("k"), v=a.pop("v"), group=0, window=None)
-    return dict(a, cache=cache, step=step, scale=0.125, window=None)
+    return dict(dict(scale=0.125, window=None, cache=cache, step=step), **a)
 
 
 @pytest.mark.parametrize("change,text", [
@@ -490,7 +494,7 @@ def _attention_args(**kw):
     (dict(k=torch.zeros(5, 2, 32, 64)), "cache"), (dict(v=torch.zeros(5, 64, 2, 64).transpose(1, 2)), "cache"),
     (dict(out=torch.zeros(3, 256, dtype=torch.bfloat16)), "dtype"), (dict(k=torch.zeros(5, 2, 64, 64).half()), "dtype"),
     (dict(mass=torch.zeros(4, 2, 64)), "mass"), (dict(mass=torch.zeros(5, 2, 64).double()), "mass"), (dict(mass=torch.zeros(5, 64, 2).mT), "mass"),
-    (dict(before=torch.zeros(5, 2, 63)), "before")])
+    (dict(before=torch.zeros(5, 2, 63)), "before"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=NAN), "scale")])
 def test_attention_mass_refuses(change, text):
     from hilbert_pruned_8b_b200.kernels.ops import KernelError
     with pytest.raises(KernelError, match=text):
@@ -532,9 +536,11 @@ def test_evict_rows_refuses(change, text):
 
 
 def test_shapes_of_the_launches():
-    from hilbert_pruned_8b_b200.kernels.plan import few_splits, mass_splits, select_shape
+    from hilbert_pruned_8b_b200.kernels.plan import chunk_splits, few_splits, mass_splits, select_shape
     assert few_splits(1, 8, 5, 296) == 5 and few_splits(8, 8, 129, 296) == 4 and few_splits(1000, 8, 100, 296) == 1
     assert mass_splits(1000, 8, 100, 296) == 1 and mass_splits(1, 1, 1, 296) == 1 and mass_splits(1, 1, 100, 296) == 16
+    assert chunk_splits(100, 10 ** 6, 148) == 1 and chunk_splits(16, 100000, 148) == 9 and chunk_splits(16, 1100, 148) == 2 and chunk_splits(1, 300, 148) == 1
+    assert chunk_splits(1, 10 ** 6, 148) == 32
     for rows in (1, 64, 1000, 16384, 16385, 70000, 131072, 300000, 10 ** 7):
         for lists in (1, 2, 16, 74, 75, 148, 256, 4096):
             threads, cluster = select_shape(lists, rows, 148)
