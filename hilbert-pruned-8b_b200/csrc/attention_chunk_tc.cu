@@ -19,15 +19,41 @@
 #include "api.h"
 #include "attention_mass.cuh"
 #include "attention_tc.cuh"
+#include "exp2_pair.cuh"
 
 #define CT_THREADS 320
 #define CT_STAGES 2
+
+// The weights 2^(s scale log2(e) - m) of a row's 128 scores, as bfloat16 over the scores, and their sum.  POLY: two pairs in eight on the
+// FMA pipe (a masked score has to give exactly zero, which only the special-function unit does).
+template <bool POLY>
+__device__ __forceinline__ void chunk_weights(const float (&sv)[128], f32x2 scale2, f32x2 neg2, uint32_t tm_s, f32x2 (&sum)[2]) {
+#pragma unroll
+    for (int c = 0; c < 4; c++) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const f32x2 x = pair_fma(pair_of(sv[c * 32 + 2 * e], sv[c * 32 + 2 * e + 1]), scale2, neg2);
+            float a, d;
+            if (POLY && (e & 3) == 2) {
+                exp2_pair<4>(x, a, d);
+            } else {
+                pair_parts(x, a, d);
+                a = exp2_approx(a);
+                d = exp2_approx(d);
+            }
+            sum[e & 1] = pair_add(sum[e & 1], pair_of(a, d));
+            pk[e] = pack_bf16_pair(a, d);
+        }
+        tmem_st16u(tm_s + c * 16, pk);                         // P over S
+    }
+}
 
 template <int HD>
 __global__ void __launch_bounds__(CT_THREADS, 1)
 chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
-                bf16* __restrict__ out, long long out_stride, float* __restrict__ lse, float* __restrict__ part_o, float* __restrict__ part_ml,
+                bf16* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, float* __restrict__ part_o, float* __restrict__ part_ml,
                 int n_tokens, int n_seqs, int nh, int nkv, int head_pairs, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -193,7 +219,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             tmem_ld64(tm_s + 64, sv + 64);
             // this row sees keys lo..qpos; as columns of the tile: [c_lo, c_hi]
             const int kbase = (jt0 + it) * FA_KEYS, c_lo = lo - kbase, c_hi = qpos - kbase;
-            if (c_lo > 0 || c_hi < 127) {                      // the causal diagonal or the window's edge
+            const bool edge = __any_sync(0xffffffffu, c_lo > 0 || c_hi < 127);      // the causal diagonal or the window's edge
+            if (edge) {
 #pragma unroll
                 for (int e = 0; e < 128; e++)
                     if (e < c_lo || e > c_hi) sv[e] = -INFINITY;
@@ -228,21 +255,13 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 }
             }
             const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
-            float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t pk[16];
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    const float p0 = exp2_approx(fmaf(sv[c * 32 + e], scale_log2e, neg_m));
-                    const float p1 = exp2_approx(fmaf(sv[c * 32 + e + 1], scale_log2e, neg_m));
-                    sum4[e & 2] += p0;
-                    sum4[(e & 2) + 1] += p1;
-                    pk[e >> 1] = pack_bf16_pair(p0, p1);
-                }
-                tmem_st16u(tm_s + c * 16, pk);                 // P over S
-            }
-            l += (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+            f32x2 sum[2] = {0ull, 0ull};
+            const f32x2 scale2 = pair_of(scale_log2e, scale_log2e), neg2 = pair_of(neg_m, neg_m);
+            if (edge) chunk_weights<false>(sv, scale2, neg2, tm_s, sum);
+            else chunk_weights<true>(sv, scale2, neg2, tm_s, sum);
+            float s0, s1;
+            pair_parts(pair_add(sum[0], sum[1]), s0, s1);
+            l += s0 + s1;
             if (i == 0 && (jt0 + it + 1) * FA_KEYS > pos0 + n_new) {
                 // the tile that holds the sequence's end: values behind it are whatever a page held before, and 0 * NaN is NaN
                 const int s = it % CT_STAGES;
@@ -277,7 +296,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
                 bf16* dst = out + (size_t)(t_begin + row) * out_stride + (size_t)head * HD;
                 if (valid && S > 1) *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(m_run, l);
-                if (valid && S == 1) lse[at] = l > 0.0f ? m_run + log2f(l) : INFINITY;
+                if (valid && S == 1) {
+                    long long place = row;
+                    for (int a = 0; a < b; a++) place += mass_round128(seq_start[a + 1] - seq_start[a]);
+                    lse[head * lse_ld + place] = l > 0.0f ? m_run + log2f(l) : INFINITY;
+                }
 #pragma unroll 1
                 for (int c = 0; c < HD / 32; c++) {
                     float v[32];
@@ -314,10 +337,15 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 template <int HD>
 __global__ void __launch_bounds__(256)
 chunk_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, bf16* __restrict__ out, long long out_stride,
-                  float* __restrict__ lse, int n_tokens, int nh, int S) {
+                  float* __restrict__ lse, long long lse_ld, const int* __restrict__ seq_start, int n_seqs, int n_tokens, int nh, int S) {
     pdl_trigger();
     pdl_wait();
     const int t = blockIdx.x, lane = threadIdx.x & 31;
+    long long place = t;
+    for (int a = 0; a < n_seqs && seq_start[a + 1] <= t; a++) {
+        const int n = seq_start[a + 1] - seq_start[a];
+        place += mass_round128(n) - n;
+    }
     for (int head = blockIdx.y * 8 + (threadIdx.x >> 5); head < nh; head += gridDim.y * 8) {
         const size_t at = (size_t)head * n_tokens + t, step = (size_t)nh * n_tokens;
         float2 ml = make_float2(-INFINITY, 0.0f);              // of share `lane` (S <= 32)
@@ -338,13 +366,13 @@ chunk_join_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
         const float inv = L > 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
         for (int c = 0; c < HD / 32; c++) out[(size_t)t * out_stride + (size_t)head * HD + c * 32 + lane] = __float2bfloat16_rn(acc[c] * inv);
-        if (lane == 0) lse[at] = L > 0.0f ? M + log2f(L) : INFINITY;
+        if (lane == 0) lse[head * lse_ld + place] = L > 0.0f ? M + log2f(L) : INFINITY;
     }
 }
 
 template <int HD>
 static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width, const int* seq_start,
-                        const int* seq_pos0, bf16* out, long long out_stride, float* lse, float* parts, int splits, int n_tokens, int n_seqs, int q_blocks,
+                        const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, float* parts, int splits, int n_tokens, int n_seqs, int q_blocks,
                         int nh, int nkv, int head_pairs, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
     constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 16 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "attention tiles do not fit shared memory");
@@ -358,19 +386,20 @@ static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
     float* part_o = parts;
     float* part_ml = parts == nullptr ? nullptr : parts + (size_t)splits * nh * n_tokens * HD;
     cudaError_t e = hb_launch(chunk_tc_kernel<HD>, dim3(head_pairs ? nh / 2 : nh, q_blocks, splits), dim3(CT_THREADS), SMEM, s, mq, mk, mv, page_table,
-                              pt_width, seq_start, seq_pos0, out, out_stride, lse, part_o, part_ml, n_tokens, n_seqs, nh, nkv, head_pairs,
+                              pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, part_o, part_ml, n_tokens, n_seqs, nh, nkv, head_pairs,
                               scale * FA_LOG2E, window, n_pages, error_flag);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     if (hb_check_launch("attention_mass (chunk)")) return 1;
     if (splits == 1) return 0;
-    e = hb_launch(chunk_join_kernel<HD>, dim3(n_tokens, (nh + 7) / 8), dim3(256), 0, s, part_o, part_ml, out, out_stride, lse, n_tokens, nh, splits);
+    e = hb_launch(chunk_join_kernel<HD>, dim3(n_tokens, (nh + 7) / 8), dim3(256), 0, s, part_o, part_ml, out, out_stride, lse, lse_ld, seq_start,
+                  n_seqs, n_tokens, nh, splits);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (join of the chunk)");
 }
 
 int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
-                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, float* parts, int splits, int n_tokens,
-                       int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
+                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts, int splits,
+                       int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
                        cudaStream_t s) {
     HB_REQUIRE(hb_attention_prefill_tc_supported(n_heads, n_kv_heads, head_dim), "attention_mass: head size %d is not built for the tensor cores (64, 128)",
                head_dim);
@@ -387,8 +416,8 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
     if (tc_make_map(&mv, v_cache, cache_rows, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     const int head_pairs = (n_heads / n_kv_heads) % 2 == 0;
     if (head_dim == 128)
-        return launch_chunk<128>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, parts, splits, n_tokens, n_seqs, q_blocks,
+        return launch_chunk<128>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, parts, splits, n_tokens, n_seqs, q_blocks,
                                  n_heads, n_kv_heads, head_pairs, scale, window, n_pages, error_flag, s);
-    return launch_chunk<64>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, parts, splits, n_tokens, n_seqs, q_blocks,
+    return launch_chunk<64>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, parts, splits, n_tokens, n_seqs, q_blocks,
                             n_heads, n_kv_heads, head_pairs, scale, window, n_pages, error_flag, s);
 }

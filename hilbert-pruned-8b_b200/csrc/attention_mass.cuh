@@ -44,6 +44,8 @@ __device__ __forceinline__ bool mass_find_keys(const int* __restrict__ seq_start
     return false;
 }
 
+__host__ __device__ constexpr int mass_round128(int n) { return (n + 127) & ~127; }
+
 // The new tokens [n0, n1) of a sequence that see one of the keys [key0, key0 + keys): token i stands at pos0 + i.
 __device__ __forceinline__ void mass_queries(int key0, int keys, int pos0, int n_new, int window, int& n0, int& n1) {
     n0 = max(0, key0 - pos0);
@@ -85,10 +87,11 @@ int attention_decode_scores(const void* q, long long q_stride, const void* kc, c
                             const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int n_tokens, int nh,
                             int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);
 
-// The first half of a step of many tokens on the tensor cores (attention_chunk_tc.cu): writes out and lse [heads][tokens].  q_blocks: sum
+// The first half of a step of many tokens on the tensor cores (attention_chunk_tc.cu): writes out and the rows'
+// log-sums, lse[head][place]: a sequence's places begin at a multiple of 128, behind those of the sequences in front.  q_blocks: sum
 // over sequences of ceil(new tokens / span), span 128 with an even group of heads and 256 with an odd one; parts: splits * n_heads *
 // n_tokens * (head_dim + 2) floats when splits > 1 (at most 32).
 int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
-                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, float* parts, int splits, int n_tokens,
-                       int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
+                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts, int splits,
+                       int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
                        cudaStream_t s);

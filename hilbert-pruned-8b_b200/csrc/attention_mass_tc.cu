@@ -4,52 +4,43 @@
 // One CTA = 256 consecutive rows of a sequence's cache x one kv head x a share of the (head, 128 queries) tiles that see them.
 // Keys are the M operand: a tile's 128 keys are the 128 lanes of tensor memory and the queries its columns, so that a key's sum over
 // queries and heads stays in one thread's registers from beginning to end and is written once: no atomics, no shuffles.
-//   warp 0      TMA producer: the two key tiles once, then query tiles (three stages)
+//   warp 0      TMA producer: the two key tiles once, then query tiles with their log-sums (three stages)
 //   warp 1      owns tensor memory; one thread issues S = K Q^T of the two key tiles (head size / 16 steps each) into two pairs of buffers
 //   warps 2-17  weights: 8 warps per key tile, a thread has 64 queries of its key: w = 2^(s scale log2(e) - lse), added up
 // What bounds it: 16 exponentials a clock and SM (1024 clocks for 128 x 128 weights, against 512 for the product at head size
-// 128).  Two key tiles share a query tile because an SM takes about 32 bytes a clock from L2: with one, loading a 32 KB query tile would
-// last as long as its exponentials.
+// 128), so three pairs in eight are computed on the FMA pipe instead.  Two key tiles share a query tile because an SM takes about 32
+// bytes a clock from L2: with one, loading a 32 KB query tile would last as long as its exponentials.
 //
 // Every wait is bounded; a wait that runs out sets *error_flag and the CTA drains and leaves.
 #include "api.h"
 #include "attention_mass.cuh"
 #include "attention_tc.cuh"
+#include "exp2_pair.cuh"
 
 #define MT_KEYS 256
 #define MT_THREADS 576
 #define MT_STAGES 3
-#define MT_WORKERS 512
+#define MT_WORKER_WARPS 16
 
-// A barrier of the workers that tells each of them whether any gave up: the same answer for all, so that none waits for one
-// that left.
-__device__ __forceinline__ bool workers_any(bool mine) {
-    uint32_t any;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 q, %1, 0;\n\t"
-        "bar.red.or.pred p, 2, 512, q;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(any)
-        : "r"((uint32_t)mine)
-        : "memory");
-    return any != 0;
+// `bytes` from global into shared memory (both 16-byte aligned), counted on `bar`
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
 }
 
 template <int HD>
 __global__ void __launch_bounds__(MT_THREADS, 1)
 mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const int* __restrict__ page_table, int pt_width,
-               const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* lse, MassOut mo, int n_tokens, int n_seqs, int nh,
+               const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* lse, long long lse_ld, MassOut mo, int n_seqs, int nh,
                int nkv, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    // [K tiles 2][Q stages 3][barriers]; a tile is 128 rows x HD
+    // [K tiles 2][Q stages 3][log-sums of the stages][barriers]; a tile is 128 rows x HD
     constexpr int HALVES = HD / 64, TILE = HALVES * FA_HALF_BYTES;
-    uint64_t* bars = (uint64_t*)(smem + (2 + MT_STAGES) * TILE);
+    float* xlse = (float*)(smem + (2 + MT_STAGES) * TILE);     // [stages][128 queries]
+    uint64_t* bars = (uint64_t*)(xlse + MT_STAGES * 128);
     uint32_t* tmem_slot = (uint32_t*)(bars + 16);
-    volatile int* abort_flag = (volatile int*)(tmem_slot + 1);
-    float* xlse = (float*)(tmem_slot + 4);                    // [2 buffers][128 queries]
-    float* xsum = xlse + 256;                                 // [2 key tiles][128]
+    float* xsum = (float*)(tmem_slot + 4);                     // [2 key tiles][128]
     const uint32_t smem_base = smem_u32(smem), q_smem = smem_base + 2 * TILE;
     const uint32_t k_full = smem_u32(bars), q_full0 = smem_u32(bars + 1), q_empty0 = smem_u32(bars + 4);
     const uint32_t s_full0 = smem_u32(bars + 7), s_empty0 = smem_u32(bars + 9);
@@ -62,6 +53,7 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const int key0 = kt * MT_KEYS;
     int n0 = 0, n1 = 0;
     if (has_work) mass_queries(key0, MT_KEYS, pos0, n_new, window, n0, n1);
+    n0 &= ~127;                                                // whole blocks of 128 new tokens, as the log-sums lie
     const int blocks = (n1 - n0 + 127) / 128;
     const int it0 = (int)((long long)blocks * G * z / S), n_it = (int)((long long)blocks * G * (z + 1) / S) - it0;
 
@@ -69,13 +61,12 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         mbar_init(k_full, 1);
         for (int s = 0; s < MT_STAGES; s++) {
             mbar_init(q_full0 + 8 * s, 1);
-            mbar_init(q_empty0 + 8 * s, 1);
+            mbar_init(q_empty0 + 8 * s, 1 + MT_WORKER_WARPS);  // the products have read the queries, the workers the log-sums
         }
         for (int s = 0; s < 2; s++) {
             mbar_init(s_full0 + 8 * s, 1);
-            mbar_init(s_empty0 + 8 * s, MT_WORKERS);
+            mbar_init(s_empty0 + 8 * s, MT_WORKER_WARPS);
         }
-        *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -106,18 +97,20 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 for (int half = 0; half < HALVES; half++)
                     tma_load_2d(dst + half * FA_HALF_BYTES, &map_k, k_full, half * 64, (page * nkv + g) * HB_PAGE_TOKENS);
             }
+            long long lse0 = n0;                                    // where the log-sums of token n0 lie
+            for (int i = 0; i < b; i++) lse0 += mass_round128(seq_start[i + 1] - seq_start[i]);
             int issued = 0;
             for (int it = 0; it < n_it; it++) {
                 const int s = it % MT_STAGES;
                 if (!mbar_wait(q_empty0 + 8 * s, ((it / MT_STAGES) & 1) ^ 1)) {
                     atomicExch(error_flag, 41);
-                    *abort_flag = 1;
                     break;
                 }
-                const int item = it0 + it, head = g * G + item / blocks, q0 = n0 + (item % blocks) * 128;
-                mbar_expect_tx(q_full0 + 8 * s, TILE);
+                const int item = it0 + it, head = g * G + item / blocks, q0 = (item % blocks) * 128;
+                mbar_expect_tx(q_full0 + 8 * s, TILE + 512);
                 for (int half = 0; half < HALVES; half++)
-                    tma_load_2d(q_smem + s * TILE + half * FA_HALF_BYTES, &map_q, q_full0 + 8 * s, head * HD + half * 64, t_begin + q0);
+                    tma_load_2d(q_smem + s * TILE + half * FA_HALF_BYTES, &map_q, q_full0 + 8 * s, head * HD + half * 64, t_begin + n0 + q0);
+                bulk_load(smem_u32(xlse + s * 128), lse + (size_t)head * lse_ld + lse0 + q0, 512, q_full0 + 8 * s);
                 issued = it + 1;
             }
             for (int it = max(0, issued - MT_STAGES); it < issued; it++)
@@ -128,16 +121,12 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         // ---------------------------------------------------------------- MMA issuer
         if (lane == 0 && n_it > 0) {
             constexpr uint32_t idesc = instr_desc_bf16_mn(128, 128);
-            bool alive = mbar_wait(k_full, 0);
-            if (!alive) {
-                atomicExch(error_flag, 43);
-                *abort_flag = 1;
-            }
+            const bool alive = mbar_wait(k_full, 0);
+            if (!alive) atomicExch(error_flag, 43);
             for (int it = 0; it < n_it && alive; it++) {
                 const int s = it % MT_STAGES, sb = it & 1;
                 if (!mbar_wait(q_full0 + 8 * s, (it / MT_STAGES) & 1) || !mbar_wait(s_empty0 + 8 * sb, ((it >> 1) & 1) ^ 1)) {
                     atomicExch(error_flag, 44);
-                    *abort_flag = 1;
                     break;
                 }
                 tc_fence_after();
@@ -158,24 +147,19 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         // ---------------------------------------------------------------- weights
         const int w = warp - 2, k = w >> 3;                    // key tile
         const int quarter = warp & 3, r = quarter * 32 + lane;  // key of the tile = lane of tensor memory (a warp reads its own quarter)
-        const int hf = (w >> 2) & 1, et = threadIdx.x - 64;    // which 64 queries of a tile; the number among the workers
+        const int hf = (w >> 2) & 1;                           // which 64 queries of a tile
         const int key = key0 + k * 128 + r;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        float sum4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        auto lse_of = [&](int it) -> float {                   // of query et of the tile; 128 workers ask
-            const int item = it0 + it, head = g * G + item / blocks, t = n0 + (item % blocks) * 128 + et;
-            return t < n1 ? __ldcg(lse + (size_t)head * n_tokens + t_begin + t) : 0.0f;
-        };
-        if (n_it > 0) {
-            if (et < 128) xlse[et] = lse_of(0);
-            asm volatile("bar.sync 2, 512;" ::: "memory");
-        }
+        const f32x2 scale2 = pair_of(scale_log2e, scale_log2e), minus = pair_of(-1.0f, -1.0f);
+        f32x2 sum[4] = {0ull, 0ull, 0ull, 0ull};
+        bool ok = true;
         for (int it = 0; it < n_it; it++) {
-            const int sb = it & 1;
-            const float next = et < 128 && it + 1 < n_it ? lse_of(it + 1) : 0.0f;
-            if (!mbar_wait(s_full0 + 8 * sb, (it >> 1) & 1)) {
+            const int sb = it & 1, s = it % MT_STAGES;
+            // (the queries' barrier too: it says that the log-sums have arrived)
+            if (!__all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * sb, (it >> 1) & 1) && mbar_wait(q_full0 + 8 * s, (it / MT_STAGES) & 1))) {
                 atomicExch(error_flag, 45);
-                *abort_flag = 1;
+                ok = false;
+                break;
             }
             tc_fence_after();
             const int q0 = n0 + ((it0 + it) % blocks) * 128 + hf * 64;       // this thread's first query
@@ -189,37 +173,48 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 tmem_ld32(tm_s + part * 32, sv);
                 if (part == 1) {
                     tc_fence_before();
-                    mbar_arrive(s_empty0 + 8 * sb);            // all scores have been read
+                    if (lane == 0) mbar_arrive(s_empty0 + 8 * sb);           // all scores have been read (the load is the warp's)
                 }
-                const float4* ls = reinterpret_cast<const float4*>(xlse + sb * 128 + hf * 64 + part * 32);
+                const float4* ls = reinterpret_cast<const float4*>(xlse + s * 128 + hf * 64 + part * 32);
                 const int lo = c_lo - part * 32, hi = c_hi - part * 32;
                 if (lo <= 0 && hi >= 31) {
 #pragma unroll
                     for (int c = 0; c < 32; c += 4) {
                         const float4 l4 = ls[c >> 2];
-                        sum4[0] += exp2_approx(fmaf(sv[c], scale_log2e, -l4.x));
-                        sum4[1] += exp2_approx(fmaf(sv[c + 1], scale_log2e, -l4.y));
-                        sum4[2] += exp2_approx(fmaf(sv[c + 2], scale_log2e, -l4.z));
-                        sum4[3] += exp2_approx(fmaf(sv[c + 3], scale_log2e, -l4.w));
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const f32x2 x = pair_fma(pair_of(sv[c + 2 * u], sv[c + 2 * u + 1]), scale2,
+                                                     pair_fma(pair_of(u ? l4.z : l4.x, u ? l4.w : l4.y), minus, 0ull));
+                            const int pair = (c >> 1) + u;     // 0..15
+                            float a, d;
+                            if ((pair & 7) == 1 || (pair & 7) == 4 || (pair & 7) == 6) {
+                                exp2_pair<5>(x, a, d);
+                            } else {
+                                pair_parts(x, a, d);
+                                a = exp2_approx(a);
+                                d = exp2_approx(d);
+                            }
+                            sum[pair & 3] = pair_add(sum[pair & 3], pair_of(a, d));
+                        }
                     }
                 } else if (lo <= 31 && hi >= 0) {              // the causal diagonal, the window's edge, the last queries
 #pragma unroll
-                    for (int c = 0; c < 32; c += 4) {
-                        const float4 l4 = ls[c >> 2];
-                        sum4[0] += c >= lo && c <= hi ? exp2_approx(fmaf(sv[c], scale_log2e, -l4.x)) : 0.0f;
-                        sum4[1] += c + 1 >= lo && c + 1 <= hi ? exp2_approx(fmaf(sv[c + 1], scale_log2e, -l4.y)) : 0.0f;
-                        sum4[2] += c + 2 >= lo && c + 2 <= hi ? exp2_approx(fmaf(sv[c + 2], scale_log2e, -l4.z)) : 0.0f;
-                        sum4[3] += c + 3 >= lo && c + 3 <= hi ? exp2_approx(fmaf(sv[c + 3], scale_log2e, -l4.w)) : 0.0f;
+                    for (int c = 0; c < 32; c += 2) {
+                        const float a = c >= lo && c <= hi ? exp2_approx(fmaf(sv[c], scale_log2e, -xlse[s * 128 + hf * 64 + part * 32 + c])) : 0.0f;
+                        const float d = c + 1 >= lo && c + 1 <= hi ? exp2_approx(fmaf(sv[c + 1], scale_log2e, -xlse[s * 128 + hf * 64 + part * 32 + c + 1])) : 0.0f;
+                        sum[(c >> 1) & 3] = pair_add(sum[(c >> 1) & 3], pair_of(a, d));
                     }
                 }
             }
-            if (et < 128) xlse[(sb ^ 1) * 128 + et] = next;    // read last in the round before, in front of its barrier
-            if (workers_any(*abort_flag != 0)) break;          // a barrier as well
+            __syncwarp();
+            if (lane == 0) mbar_arrive(q_empty0 + 8 * s);      // and all log-sums
         }
-        const float mine = (sum4[0] + sum4[1]) + (sum4[2] + sum4[3]);
+        float a, d;
+        pair_parts(pair_add(pair_add(sum[0], sum[1]), pair_add(sum[2], sum[3])), a, d);
+        const float mine = a + d;
         if (hf == 1) xsum[k * 128 + r] = mine;
         asm volatile("bar.sync 2, 512;" ::: "memory");
-        if (hf == 0 && has_work && !*abort_flag) {
+        if (hf == 0 && has_work && ok) {
             const int pi = key / HB_PAGE_TOKENS;
             const int page = pi < pt_width ? page_table[(size_t)b * pt_width + pi] : -1;
             mass_store(mo, mine + xsum[k * 128 + r], b, g, key, page, nkv, n_pages, pos0, n_new, z, S, (size_t)blockIdx.x * MT_KEYS + k * 128 + r,
@@ -236,9 +231,9 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 
 template <int HD>
 static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0,
-                          const float* lse, MassOut mo, int splits, int n_tokens, int n_seqs, int key_tiles, int nh, int nkv, float scale, int window,
+                          const float* lse, long long lse_ld, MassOut mo, int splits, int n_seqs, int key_tiles, int nh, int nkv, float scale, int window,
                           int n_pages, int* error_flag, cudaStream_t s) {
-    constexpr int SMEM = (2 + MT_STAGES) * (HD / 64) * FA_HALF_BYTES + 16 * 8 + 16 + (256 + 256) * 4 + 1024;
+    constexpr int SMEM = (2 + MT_STAGES) * (HD / 64) * FA_HALF_BYTES + (MT_STAGES * 128 + 256) * 4 + 16 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "key and query tiles do not fit shared memory");
     static bool done[HB_MAX_DEVICES] = {};
     bool& set = done[hb_device_slot()];
@@ -248,7 +243,7 @@ static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const in
         set = true;
     }
     cudaError_t e = hb_launch(mass_tc_kernel<HD>, dim3(key_tiles, nkv, splits), dim3(MT_THREADS), SMEM, s, mq, mk, page_table, pt_width, seq_start,
-                              seq_pos0, lse, mo, n_tokens, n_seqs, nh, nkv, scale * FA_LOG2E, window, n_pages, error_flag);
+                              seq_pos0, lse, lse_ld, mo, n_seqs, nh, nkv, scale * FA_LOG2E, window, n_pages, error_flag);
     if (e != cudaSuccess) return hb_fail("attention_mass_tc: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass_tc");
 }
@@ -256,28 +251,30 @@ static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const in
 extern "C" int hb_attention_mass_tc_keys(void) { return MT_KEYS; }
 
 // Sizes and types of hb_attention_prefill_tc, with the same alignment of queries and output.  q_blocks, chunk_parts, chunk_splits: as
-// attention_chunk_tc (attention_mass.cuh); key_tiles: sum over sequences of ceil(rows / 256); lse: n_heads * n_tokens floats; parts:
+// attention_chunk_tc (attention_mass.cuh); key_tiles: sum over sequences of ceil(rows / 256); lse: n_heads * lse_ld
+// floats, lse_ld 128 * the sum of ceil(new tokens / 128); parts:
 // splits * n_kv_heads * key_tiles * 256 floats when splits > 1.
 extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
-                                    const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, const float* before,
+                                    const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, const float* before,
                                     float* mass, float* parts, float* chunk_parts, int chunk_splits, int splits, int n_tokens, int n_seqs, int q_blocks,
                                     int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
                                     void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
+    HB_REQUIRE(((uintptr_t)lse & 15) == 0 && lse_ld % 128 == 0, "attention_mass: the log-sums must be aligned");
     HB_REQUIRE(lse != nullptr && mass != nullptr && n_kv_heads > 0 && n_kv_heads <= 65535 && key_tiles > 0 && splits >= 1 && splits <= 65535 &&
                    (splits == 1 || parts != nullptr),
                "attention_mass: bad sizes");
     cudaStream_t s = (cudaStream_t)stream;
-    if (attention_chunk_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, chunk_parts, chunk_splits,
+    if (attention_chunk_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, chunk_parts, chunk_splits,
                            n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s))
         return 1;
     CUtensorMap mq, mk;
     if (tc_make_map(&mq, q, n_tokens, (long long)n_heads * head_dim, q_stride, 128)) return 1;
     if (tc_make_map(&mk, k_cache, (long long)n_pages * n_kv_heads * HB_PAGE_TOKENS, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     MassOut mo = {before, mass, parts};
-    const int rc = head_dim == 128 ? launch_mass_tc<128>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, mo, splits, n_tokens, n_seqs, key_tiles,
+    const int rc = head_dim == 128 ? launch_mass_tc<128>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, lse_ld, mo, splits, n_seqs, key_tiles,
                                                          n_heads, n_kv_heads, scale, window, n_pages, error_flag, s)
-                                   : launch_mass_tc<64>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, mo, splits, n_tokens, n_seqs, key_tiles,
+                                   : launch_mass_tc<64>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, lse_ld, mo, splits, n_seqs, key_tiles,
                                                         n_heads, n_kv_heads, scale, window, n_pages, error_flag, s);
     if (rc) return rc;
     return splits > 1 ? mass_join(page_table, pt_width, seq_start, seq_pos0, mo, n_seqs, n_kv_heads, n_pages, MT_KEYS, key_tiles, splits, s) : 0;

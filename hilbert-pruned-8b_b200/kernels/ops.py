@@ -81,7 +81,7 @@ _SIGNATURES = {
                                 _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
                           _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
-    "hb_attention_mass_tc": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
+    "hb_attention_mass_tc": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr,
                              _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr,
                               _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int,
@@ -1298,11 +1298,12 @@ class Ops:
                            self._stream())
                 self.launches += 2
                 return
-            lse = torch.empty(heads * T, dtype=torch.float32, device=self.device)
             tc = (self.use_fast_attention and self.use_tcgen05_attention and qkv.dtype == torch.bfloat16
                   and self.lib.hb_attention_prefill_tc_supported(heads, kv_heads, head_dim) and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0
                   and cache.k.data_ptr() % 16 == 0 and cache.v.data_ptr() % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0)
-            # rows of a block of queries (two tiles of 128: two heads, or with an odd group two blocks of tokens), of a tile of keys
+            # places of the log-sums; rows of a block of queries (two tiles of 128: two heads, or with an odd group two blocks of tokens), of a tile of keys
+            lse_ld = 128 * sum(-(-n // 128) for n in step.host_new) if tc else T
+            lse = torch.empty(heads * lse_ld, dtype=torch.float32, device=self.device)
             rows, keys = (128 if group % 2 == 0 else 256, self.lib.hb_attention_mass_tc_keys()) if tc else (64, 64)
             q_blocks = sum(-(-n // rows) for n in step.host_new)
             key_tiles = sum(-(-n // keys) for n in step.host_len)
@@ -1312,7 +1313,8 @@ class Ops:
             sizes = (splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim, float(scale), win, pages, self.status.data_ptr(),
                      self._stream())
             buffers = (cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(),
-                       out.data_ptr(), out_ld, lse.data_ptr(), old, mass.data_ptr(), parts.data_ptr() if parts is not None else None)
+                       out.data_ptr(), out_ld, lse.data_ptr(), *((lse_ld,) if tc else ()), old, mass.data_ptr(),
+                       parts.data_ptr() if parts is not None else None)
             if tc:
                 ways = chunk_splits((heads // 2 if group % 2 == 0 else heads) * q_blocks, step.max_len, self.sm_count)
                 shares = torch.empty(ways * heads * T * (head_dim + 2), dtype=torch.float32, device=self.device) if ways > 1 else None
