@@ -32,7 +32,7 @@ template <int HD>
 __global__ void __launch_bounds__(MT_THREADS, 1)
 mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const int* __restrict__ page_table, int pt_width,
                const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* lse, long long lse_ld, MassOut mo, int n_seqs, int nh,
-               int nkv, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
+               int nkv, float scale_log2e, int window, int n_pages, int S, int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // [K tiles 2][Q stages 3][log-sums of the stages][barriers]; a tile is 128 rows x HD
@@ -45,10 +45,12 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint32_t k_full = smem_u32(bars), q_full0 = smem_u32(bars + 1), q_empty0 = smem_u32(bars + 4);
     const uint32_t s_full0 = smem_u32(bars + 7), s_empty0 = smem_u32(bars + 9);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int g = blockIdx.y, G = nh / nkv, z = blockIdx.z, S = gridDim.z;
+    // Under a causal mask a sequence's first keys are seen by the most queries: with the tiles as the slowest index, the shares of the
+    // heaviest ones start first and what ends last is light.
+    const int z = blockIdx.x % S, g = blockIdx.x / S % nkv, G = nh / nkv, tile = blockIdx.x / (S * nkv);
 
     int b = 0, kt = 0;
-    const bool has_work = mass_find_keys(seq_start, seq_pos0, n_seqs, blockIdx.x, MT_KEYS, b, kt);
+    const bool has_work = mass_find_keys(seq_start, seq_pos0, n_seqs, tile, MT_KEYS, b, kt);
     const int t_begin = has_work ? seq_start[b] : 0, n_new = has_work ? seq_start[b + 1] - t_begin : 0, pos0 = has_work ? seq_pos0[b] : 0;
     const int key0 = kt * MT_KEYS;
     int n0 = 0, n1 = 0;
@@ -217,8 +219,8 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         if (hf == 0 && has_work && ok) {
             const int pi = key / HB_PAGE_TOKENS;
             const int page = pi < pt_width ? page_table[(size_t)b * pt_width + pi] : -1;
-            mass_store(mo, mine + xsum[k * 128 + r], b, g, key, page, nkv, n_pages, pos0, n_new, z, S, (size_t)blockIdx.x * MT_KEYS + k * 128 + r,
-                       (size_t)gridDim.x * MT_KEYS);
+            mass_store(mo, mine + xsum[k * 128 + r], b, g, key, page, nkv, n_pages, pos0, n_new, z, S, (size_t)tile * MT_KEYS + k * 128 + r,
+                       (size_t)(gridDim.x / (S * nkv)) * MT_KEYS);
         }
     }
     tc_fence_before();
@@ -242,8 +244,8 @@ static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const in
         if (e != cudaSuccess) return hb_fail("attention_mass_tc: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
         set = true;
     }
-    cudaError_t e = hb_launch(mass_tc_kernel<HD>, dim3(key_tiles, nkv, splits), dim3(MT_THREADS), SMEM, s, mq, mk, page_table, pt_width, seq_start,
-                              seq_pos0, lse, lse_ld, mo, n_seqs, nh, nkv, scale * FA_LOG2E, window, n_pages, error_flag);
+    cudaError_t e = hb_launch(mass_tc_kernel<HD>, dim3(key_tiles * nkv * splits), dim3(MT_THREADS), SMEM, s, mq, mk, page_table, pt_width, seq_start,
+                              seq_pos0, lse, lse_ld, mo, n_seqs, nh, nkv, scale * FA_LOG2E, window, n_pages, splits, error_flag);
     if (e != cudaSuccess) return hb_fail("attention_mass_tc: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass_tc");
 }
@@ -261,7 +263,7 @@ extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const voi
                                     void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(((uintptr_t)lse & 15) == 0 && lse_ld % 128 == 0, "attention_mass: the log-sums must be aligned");
-    HB_REQUIRE(lse != nullptr && mass != nullptr && n_kv_heads > 0 && n_kv_heads <= 65535 && key_tiles > 0 && splits >= 1 && splits <= 65535 &&
+    HB_REQUIRE(lse != nullptr && mass != nullptr && n_kv_heads > 0 && n_kv_heads <= 65535 && key_tiles > 0 && splits >= 1 && (long long)key_tiles * n_kv_heads * splits <= 0x7fffffffLL &&
                    (splits == 1 || parts != nullptr),
                "attention_mass: bad sizes");
     cudaStream_t s = (cudaStream_t)stream;
