@@ -70,8 +70,7 @@ template <int HD>
 __global__ void __launch_bounds__(CT_THREADS, 1)
 chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
-                bf16* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, float* __restrict__ part_o, float* __restrict__ part_ml,
-                int n_tokens, int n_seqs, int nh, int nkv, int head_pairs, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
+                bf16* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, Shares sh, int n_tokens, int n_seqs, int nh, int nkv, int head_pairs, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // [Q tiles 2][K stages][V stages][barriers]; a tile is 128 rows x HD
@@ -86,17 +85,18 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
     // The two tiles: heads head0 and head0 + 1 (head_pairs) of one block of tokens, or blocks 2 blk and 2 blk + 1 of head0.  Blocks
     // are taken from the back and heads are the fast index: what sees the most keys starts first.
-    const int z = blockIdx.z, S = gridDim.z;
+    const int z = blockIdx.z;
     const int head0 = head_pairs ? 2 * blockIdx.x : blockIdx.x, g = head0 / (nh / nkv);
     const int span = head_pairs ? FA_ROWS : 2 * FA_ROWS;
     int b = 0, blk = 0;
     const bool has_work = mass_find_block(seq_start, n_seqs, gridDim.y - 1 - blockIdx.y, span, b, blk);
-    const int t_begin = has_work ? seq_start[b] : 0, n_new = has_work ? seq_start[b + 1] - t_begin : 0, pos0 = has_work ? seq_pos0[b] : 0;
+    const int t_begin = has_work ? seq_start[b] : 0, n_new = has_work ? seq_start[b + 1] - t_begin : 1, pos0 = has_work ? seq_pos0[b] : 0;
     const int row0 = blk * span;                               // the first of the CTA's new tokens
     const int first_pos = pos0 + row0, last_pos = pos0 + min(row0 + span, n_new) - 1;
-    const int lo_cta = hb_oldest_visible(first_pos, window, 0);
-    int jt0 = lo_cta / FA_KEYS, n_it = has_work ? last_pos / FA_KEYS + 1 - jt0 : 0;
-    {                                                          // this share's tiles of keys
+    int jt0, n_it = key_tiles_of(first_pos, last_pos, window, FA_KEYS, jt0);
+    const int S = shares_of(sh, n_it), lo_cta = hb_oldest_visible(first_pos, window, 0);
+    if (!has_work || z >= S) return;
+    {                                                          // this share's tiles of keys (none is empty: S <= n_it)
         const int a = (int)((long long)n_it * z / S), e = (int)((long long)n_it * (z + 1) / S);
         jt0 += a;
         n_it = e - a;
@@ -110,7 +110,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             mbar_init(v_full0 + 8 * s, 1);
             mbar_init(v_empty0 + 8 * s, 1);
             mbar_init(s_full0 + 8 * s, 1);
-            mbar_init(p_full0 + 8 * s, 256);
+            mbar_init(p_full0 + 8 * s, 8);
             mbar_init(o_full0 + 8 * s, 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -126,7 +126,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
     if (warp == 16) {
         // ---------------------------------------------------------------- TMA producer
-        if (lane == 0 && n_it > 0) {
+        if (lane == 0) {
             const int* pt = page_table + (size_t)b * pt_width;
             mbar_expect_tx(q_full, 2 * TILE);
             for (int i = 0; i < 2; i++)
@@ -172,7 +172,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         }
     } else if (warp == 17) {
         // ---------------------------------------------------------------- MMA issuer
-        if (lane == 0 && n_it > 0) {
+        if (lane == 0) {
             constexpr uint32_t idesc_qk = instr_desc_bf16_mn(128, FA_KEYS);
             constexpr uint32_t idesc_pv = instr_desc_bf16_mn(128, HD) | (1u << 16);           // B is MN-major
             auto scores = [&](int i, int it) {
@@ -223,7 +223,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         const uint32_t tm_s = tmem_base + i * 128 + lane_base, tm_o = tmem_base + 256 + i * 128 + hf * (HD / 2) + lane_base;
         float* xmax = xrow + i * 256;
         const int qpos = pos0 + row, lo = hb_oldest_visible(qpos, window, 0);
-        const bool valid = has_work && row < n_new;
+        const bool valid = row < n_new;
         float m_run = -INFINITY, l = 0.0f;                     // l: this thread's columns only
         bool ok = true;
         for (int it = 0; it < n_it; it++) {
@@ -297,12 +297,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             }
             tmem_wait_st();
             tc_fence_before();
-            mbar_arrive(p_full0 + 8 * i);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_full0 + 8 * i);       // one arrival a warp: arrivals of single threads queue up
         }
         const size_t at = ((size_t)z * nh + head) * n_tokens + t_begin + row;
-        if (n_it == 0) {                                       // a share without keys
-            if (valid && S > 1 && hf == 0) *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(-INFINITY, 0.0f);
-        } else if (ok) {                                       // (the same for a tile's threads)
+        if (ok) {                                       // (the same for a tile's threads)
             const bool here = __all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * i, 0));
             xmax[hf * 128 + r] = l;                            // read last in front of the product that is complete now
             if (chunk_any(i, !here)) {
@@ -313,7 +312,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 const float inv = l > 0.0f ? 1.0f / l : 0.0f;
                 if (valid && hf == 0) {
                     if (S > 1) {
-                        *reinterpret_cast<float2*>(part_ml + at * 2) = make_float2(m_run, l);
+                        *reinterpret_cast<float2*>(sh.ml + at * 2) = make_float2(m_run, l);
                     } else {
                         int place = row;
                         for (int a = 0; a < b; a++) place += mass_round128(seq_start[a + 1] - seq_start[a]);
@@ -321,7 +320,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     }
                 }
                 bf16* dst = out + (size_t)(t_begin + row) * out_stride + (size_t)head * HD + hf * (HD / 2);
-                float4* po = reinterpret_cast<float4*>(part_o + at * HD + hf * (HD / 2));
+                float4* po = reinterpret_cast<float4*>(sh.o + at * HD + hf * (HD / 2));
 #pragma unroll 1
                 for (int c = 0; c < HD / 64; c++) {
                     float v[32];
@@ -353,46 +352,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
 }
 
-// out = sum_z o_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), lse = M + log2 of that sum; a warp per (token, head)
-template <int HD>
-__global__ void __launch_bounds__(256)
-chunk_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, bf16* __restrict__ out, long long out_stride,
-                  float* __restrict__ lse, long long lse_ld, const int* __restrict__ seq_start, int n_seqs, int n_tokens, int nh, int S) {
-    pdl_trigger();
-    pdl_wait();
-    const int t = blockIdx.x, lane = threadIdx.x & 31;
-    long long place = t;
-    for (int a = 0; a < n_seqs && seq_start[a + 1] <= t; a++) {
-        const int n = seq_start[a + 1] - seq_start[a];
-        place += mass_round128(n) - n;
-    }
-    for (int head = blockIdx.y * 8 + (threadIdx.x >> 5); head < nh; head += gridDim.y * 8) {
-        const size_t at = (size_t)head * n_tokens + t, step = (size_t)nh * n_tokens;
-        float2 ml = make_float2(-INFINITY, 0.0f);              // of share `lane` (S <= 32)
-        if (lane < S) ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + at + lane * step);
-        const float M = warp_max(ml.x);
-        const float w = ml.x != -INFINITY ? exp2f(ml.x - M) : 0.0f;
-        const float L = warp_sum(ml.y * w);
-        float acc[HD / 32];
-#pragma unroll
-        for (int c = 0; c < HD / 32; c++) acc[c] = 0.0f;
-        for (int s = 0; s < S; s++) {
-            const float ws = __shfl_sync(0xffffffffu, w, s);
-            if (ws == 0.0f) continue;                          // its partial output may not have been written
-            const float* po = part_o + (at + s * step) * HD + lane;
-#pragma unroll
-            for (int c = 0; c < HD / 32; c++) acc[c] = fmaf(__ldcg(po + c * 32), ws, acc[c]);
-        }
-        const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-#pragma unroll
-        for (int c = 0; c < HD / 32; c++) out[(size_t)t * out_stride + (size_t)head * HD + c * 32 + lane] = __float2bfloat16_rn(acc[c] * inv);
-        if (lane == 0) lse[head * lse_ld + place] = L > 0.0f ? M + log2f(L) : INFINITY;
-    }
-}
-
 template <int HD>
 static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width, const int* seq_start,
-                        const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, float* parts, int splits, int n_tokens, int n_seqs, int q_blocks,
+                        const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, Shares sh, int max_shares, int n_tokens, int n_seqs, int q_blocks,
                         int nh, int nkv, int head_pairs, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
     constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 16 * 8 + 16 + 512 * 4 + 1024;
     static_assert(SMEM <= 227 * 1024, "attention tiles do not fit shared memory");
@@ -403,27 +365,21 @@ static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
         if (e != cudaSuccess) return hb_fail("attention_mass: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
         set = true;
     }
-    float* part_o = parts;
-    float* part_ml = parts == nullptr ? nullptr : parts + (size_t)splits * nh * n_tokens * HD;
-    cudaError_t e = hb_launch(chunk_tc_kernel<HD>, dim3(head_pairs ? nh / 2 : nh, q_blocks, splits), dim3(CT_THREADS), SMEM, s, mq, mk, mv, page_table,
-                              pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, part_o, part_ml, n_tokens, n_seqs, nh, nkv, head_pairs,
+    cudaError_t e = hb_launch(chunk_tc_kernel<HD>, dim3(head_pairs ? nh / 2 : nh, q_blocks, max_shares), dim3(CT_THREADS), SMEM, s, mq, mk, mv, page_table,
+                              pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, sh, n_tokens, n_seqs, nh, nkv, head_pairs,
                               scale * FA_LOG2E, window, n_pages, error_flag);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
-    if (hb_check_launch("attention_mass (chunk)")) return 1;
-    if (splits == 1) return 0;
-    e = hb_launch(chunk_join_kernel<HD>, dim3(n_tokens, (nh + 7) / 8), dim3(256), 0, s, part_o, part_ml, out, out_stride, lse, lse_ld, seq_start,
-                  n_seqs, n_tokens, nh, splits);
-    if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
-    return hb_check_launch("attention_mass (join of the chunk)");
+    return hb_check_launch("attention_mass (chunk)");
 }
 
 int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
-                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts, int splits,
-                       int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
-                       cudaStream_t s) {
+                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts,
+                       int max_shares, int share_tiles, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale,
+                       int window, int n_pages, int* error_flag, cudaStream_t s) {
     HB_REQUIRE(hb_attention_prefill_tc_supported(n_heads, n_kv_heads, head_dim), "attention_mass: head size %d is not built for the tensor cores (64, 128)",
                head_dim);
-    HB_REQUIRE(q_blocks > 0 && q_blocks <= 65535 && error_flag != nullptr && splits >= 1 && splits <= 32 && (splits == 1 || parts != nullptr),
+    HB_REQUIRE(q_blocks > 0 && q_blocks <= 65535 && error_flag != nullptr && max_shares >= 1 && max_shares <= 32 && share_tiles >= 1 &&
+                   (max_shares == 1 || parts != nullptr),
                "attention_mass: the step is too large for one launch");
     HB_REQUIRE(q_stride % 8 == 0 && ((uintptr_t)q & 15) == 0, "attention_mass: queries must have 16-byte aligned rows");
     HB_REQUIRE(out_stride % 8 == 0 && ((uintptr_t)out & 15) == 0, "attention_mass: output must have 16-byte aligned rows");
@@ -435,9 +391,16 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
     if (tc_make_map(&mk, k_cache, cache_rows, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     if (tc_make_map(&mv, v_cache, cache_rows, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     const int head_pairs = (n_heads / n_kv_heads) % 2 == 0;
-    if (head_dim == 128)
-        return launch_chunk<128>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, parts, splits, n_tokens, n_seqs, q_blocks,
-                                 n_heads, n_kv_heads, head_pairs, scale, window, n_pages, error_flag, s);
-    return launch_chunk<64>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, parts, splits, n_tokens, n_seqs, q_blocks,
-                            n_heads, n_kv_heads, head_pairs, scale, window, n_pages, error_flag, s);
+    // one share: no block is cut, whatever it sees
+    const Shares sh = {parts, parts == nullptr ? nullptr : parts + (size_t)max_shares * n_heads * n_tokens * head_dim,
+                       max_shares == 1 ? 0x3fffffff : share_tiles};
+    const int rc = head_dim == 128 ? launch_chunk<128>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, sh,
+                                                       max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_pairs, scale, window, n_pages,
+                                                       error_flag, s)
+                                   : launch_chunk<64>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, sh,
+                                                      max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_pairs, scale, window, n_pages,
+                                                      error_flag, s);
+    if (rc || max_shares == 1) return rc;
+    return shares_join(sh, HB_BF16, out, out_stride, lse, lse_ld, 1, seq_start, seq_pos0, head_pairs ? FA_ROWS : 2 * FA_ROWS, FA_KEYS, window, n_tokens,
+                       n_seqs, n_heads, head_dim, s);
 }

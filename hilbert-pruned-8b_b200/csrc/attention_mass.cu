@@ -24,11 +24,42 @@
 #define AM_KEYS 64
 #define AM_THREADS 256
 
-// rows of float32 in shared memory, `ld` apart (a multiple of 4); columns behind hd are zero
-template <typename T>
-__device__ __forceinline__ void am_load_row(float* dst, const T* src, int hd, int ld, int lane, int step, bool there) {
-    for (int d = lane; d < ld - 4; d += step) dst[d] = (there && d < hd) ? to_f32(src[d]) : 0.0f;
-}
+// 64 rows of a tensor as float32 in shared memory, `ld` apart (a multiple of 4), in two halves so that the loads can be in flight while
+// something else is computed: registers (up to 4 NC numbers a thread), then shared memory.  Rows from `rows` on and columns
+// behind hd are zero.  vec: rows are aligned for four elements at a time.
+template <typename T, int NC>
+struct AmTile {
+    float4 x[NC];
+    __device__ __forceinline__ void load(const T* src, long long stride, int hd, int rows, bool vec, int tid) {
+        const int per = (hd + 3) >> 2;
+#pragma unroll
+        for (int u = 0; u < NC; u++) {
+            const int i = tid + u * AM_THREADS, r = i / per, d = (i - r * per) * 4;
+            x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (r < rows) {
+                const T* p = src + (size_t)r * stride + d;
+                if (vec) {
+                    float v[4];
+                    load4(p, v);
+                    x[u] = make_float4(v[0], v[1], v[2], v[3]);
+                } else {
+                    x[u].x = to_f32(p[0]);
+                    if (d + 1 < hd) x[u].y = to_f32(p[1]);
+                    if (d + 2 < hd) x[u].z = to_f32(p[2]);
+                    if (d + 3 < hd) x[u].w = to_f32(p[3]);
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void store(float* dst, int hd, int ld, int tid) const {
+        const int per = (hd + 3) >> 2;
+#pragma unroll
+        for (int u = 0; u < NC; u++) {
+            const int i = tid + u * AM_THREADS, r = i / per, d = (i - r * per) * 4;
+            if (r < 64) *reinterpret_cast<float4*>(dst + r * ld + d) = x[u];
+        }
+    }
+};
 
 // s[i][j] = sum_d a[ty + 16 i][d] b[tx + 16 j][d]
 __device__ __forceinline__ void am_scores(float (&s)[4][4], const float* a, const float* b, int ld, int tx, int ty) {
@@ -54,14 +85,14 @@ __device__ __forceinline__ void am_scores(float (&s)[4][4], const float* a, cons
     }
 }
 
-static __host__ __device__ inline int am_ld(int hd) { return ((hd + 3) & ~3) + 4; }      // 4 more: rows start in different banks
+static __host__ __device__ constexpr int am_ld(int hd) { return ((hd + 3) & ~3) + 4; }      // 4 more: rows start in different banks
 
 template <typename T, int NC>
 __global__ void __launch_bounds__(AM_THREADS)
 attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict__ kc, const T* __restrict__ vc,
                       const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
-                      T* __restrict__ out, long long out_stride, float* __restrict__ lse, int n_tokens, int n_seqs, int nh, int nkv, int hd,
-                      float scale_log2e, int window, int n_pages, int* status) {
+                      T* __restrict__ out, long long out_stride, float* __restrict__ lse, Shares sh, int n_tokens, int n_seqs, int nh, int nkv, int hd,
+                      float scale_log2e, int window, int n_pages, int vec_q, int vec_kv, int* status) {
     extern __shared__ __align__(16) float am_smem[];
     pdl_trigger();
     pdl_wait();
@@ -70,18 +101,36 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
     vc = pdl_fresh(vc);
     const int ld = am_ld(hd);
     float* qs = am_smem;                                 // [64][ld]
-    float* ks = qs + AM_ROWS * ld;                       // [64][ld]: keys, then values
-    float* ps = ks + AM_KEYS * ld;                       // [64 rows][68]: weights
+    float* ks = qs + AM_ROWS * ld;                       // [64][ld]
+    float* vs = ks + AM_KEYS * ld;                       // [64][ld]
+    float* ps = vs + AM_KEYS * ld;                       // [64 rows][68]: weights
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int head = blockIdx.x, g = head / (nh / nkv);
+    const int head = blockIdx.x, g = head / (nh / nkv), z = blockIdx.z;
     int b, blk;
     if (!mass_find_block(seq_start, n_seqs, gridDim.y - 1 - blockIdx.y, AM_ROWS, b, blk)) return;
     const int t0 = seq_start[b] + blk * AM_ROWS;
     const int rows = min(AM_ROWS, seq_start[b + 1] - t0);
     const int p0 = seq_pos0[b] + blk * AM_ROWS, p_last = p0 + rows - 1;
-    const int lo_first = hb_oldest_visible(p0, window, 0);
+    int page0;
+    const int n_all = key_tiles_of(p0, p_last, window, HB_PAGE_TOKENS, page0), S = shares_of(sh, n_all);
+    if (z >= S) return;
+    const int page1 = page0 + (int)((long long)n_all * (z + 1) / S);
+    page0 += (int)((long long)n_all * z / S);
     const int* pt = page_table + (size_t)b * pt_width;
-    for (int r = ty; r < AM_ROWS; r += 16) am_load_row(qs + r * ld, q + (size_t)(t0 + r) * q_stride + (size_t)head * hd, hd, ld, tx, 16, r < rows);
+    AmTile<T, NC> tile;
+    // rows of the cache that page pi holds of this sequence, and where; a page that is missing counts as no keys
+    auto page_of = [&](int pi, size_t& row0) -> int {
+        const int page = pi < pt_width ? pt[pi] : -1;
+        const bool held = page >= 0 && page < n_pages;
+        row0 = ((size_t)(held ? page : 0) * nkv + g) * HB_PAGE_TOKENS;
+        return held ? min(HB_PAGE_TOKENS, p_last + 1 - pi * HB_PAGE_TOKENS) : 0;
+    };
+    tile.load(q + (size_t)t0 * q_stride + (size_t)head * hd, q_stride, hd, rows, vec_q, tid);
+    tile.store(qs, hd, ld, tid);
+    size_t row0;
+    int held = page_of(page0, row0);
+    tile.load(kc + row0 * hd, hd, hd, held, vec_kv, tid);
+    tile.store(ks, hd, ld, tid);
     float m[4], l[4], acc[4][NC];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -90,22 +139,12 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
 #pragma unroll
         for (int c = 0; c < NC; c++) acc[i][c] = 0.0f;
     }
-    for (int pi = lo_first / HB_PAGE_TOKENS; pi <= p_last / HB_PAGE_TOKENS; pi++) {
-        int page = pi < pt_width ? pt[pi] : -1;
-        if (page < 0 || page >= n_pages) {
-            if (tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + b);
-            page = -1;                                  // its keys count as not there
-        }
-        const size_t row0 = ((size_t)max(page, 0) * nkv + g) * HB_PAGE_TOKENS;
-        __syncthreads();                                 // the values and weights of the page before are used up
-        for (int r = ty; r < AM_KEYS; r += 16)
-            am_load_row(ks + r * ld, kc + (row0 + r) * hd, hd, ld, tx, 16, page >= 0 && pi * HB_PAGE_TOKENS + r <= p_last);
-        __syncthreads();
+    for (int pi = page0; pi < page1; pi++) {
+        if (held == 0 && tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + b);
+        __syncthreads();                                 // the keys are there; values and weights of the page before are used up
+        tile.load(vc + row0 * hd, hd, hd, held, vec_kv, tid);
         float s[4][4];
         am_scores(s, qs, ks, ld, tx, ty);
-        __syncthreads();                                 // the keys are used up
-        for (int r = ty; r < AM_KEYS; r += 16)
-            am_load_row(ks + r * ld, vc + (row0 + r) * hd, hd, ld, tx, 16, page >= 0 && pi * HB_PAGE_TOKENS + r <= p_last);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int r = ty + 16 * i, p = p0 + r, lo = hb_oldest_visible(p, window, 0);
@@ -113,7 +152,7 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const int key = pi * HB_PAGE_TOKENS + tx + 16 * j;
-                s[i][j] = (page >= 0 && r < rows && key >= lo && key <= p) ? s[i][j] * scale_log2e : -INFINITY;
+                s[i][j] = (held > 0 && r < rows && key >= lo && key <= p) ? s[i][j] * scale_log2e : -INFINITY;
                 top = fmaxf(top, s[i][j]);
             }
 #pragma unroll
@@ -132,7 +171,12 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
 #pragma unroll
             for (int c = 0; c < NC; c++) acc[i][c] *= corr;
         }
-        __syncthreads();
+        tile.store(vs, hd, ld, tid);
+        __syncthreads();                                 // values and weights are there; the keys are used up
+        if (pi + 1 < page1) {
+            held = page_of(pi + 1, row0);
+            tile.load(kc + row0 * hd, hd, hd, held, vec_kv, tid);
+        }
         for (int e = 0; e < AM_KEYS; e += 4) {
             float4 w[4];
 #pragma unroll
@@ -141,7 +185,7 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
             for (int c = 0; c < NC; c++) {
                 const int d = tx + 16 * c;
                 if (d >= hd) break;
-                const float v0 = ks[e * ld + d], v1 = ks[(e + 1) * ld + d], v2 = ks[(e + 2) * ld + d], v3 = ks[(e + 3) * ld + d];
+                const float v0 = vs[e * ld + d], v1 = vs[(e + 1) * ld + d], v2 = vs[(e + 2) * ld + d], v3 = vs[(e + 3) * ld + d];
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
                     acc[i][c] = fmaf(w[i].x, v0, acc[i][c]);
@@ -151,6 +195,7 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
                 }
             }
         }
+        if (pi + 1 < page1) tile.store(ks, hd, ld, tid);
     }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -158,6 +203,17 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], o);
         if (r >= rows) continue;
+        if (S > 1) {
+            const size_t at = ((size_t)z * nh + head) * n_tokens + t0 + r;
+#pragma unroll
+            for (int c = 0; c < NC; c++)
+                if (tx + 16 * c < hd) sh.o[at * hd + tx + 16 * c] = acc[i][c];
+            if (tx == 0) {
+                sh.ml[at * 2] = m[i];
+                sh.ml[at * 2 + 1] = l[i];
+            }
+            continue;
+        }
         const float inv = l[i] > 0.0f ? 1.0f / l[i] : 0.0f;
         T* o = out + (size_t)(t0 + r) * out_stride + (size_t)head * hd;
 #pragma unroll
@@ -167,13 +223,61 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
     }
 }
 
+// out = sum_z o_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), lse = M + log2 of that sum, for the rows whose block has several shares; a
+// warp per (token, head)
+template <typename T>
+__global__ void __launch_bounds__(256)
+shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, int rounded,
+                   const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh,
+                   int hd) {
+    __shared__ float ws[8][32];
+    pdl_trigger();
+    pdl_wait();
+    const int t = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * 8 + (threadIdx.x >> 5);
+    int b = 0, place = t;
+    for (; b < n_seqs - 1 && seq_start[b + 1] <= t; b++) {
+        const int n = seq_start[b + 1] - seq_start[b];
+        if (rounded) place += mass_round128(n) - n;
+    }
+    const int n_new = seq_start[b + 1] - seq_start[b], row0 = (t - seq_start[b]) / span * span;
+    int tile0;
+    const int S = shares_of(sh, key_tiles_of(seq_pos0[b] + row0, seq_pos0[b] + min(row0 + span, n_new) - 1, window, keys, tile0));
+    if (S == 1 || head >= nh) return;
+    const size_t at = (size_t)head * n_tokens + t, step = (size_t)nh * n_tokens;
+    float2 ml = make_float2(-INFINITY, 0.0f);                  // of share `lane` (at most 32)
+    if (lane < S) ml = __ldcg(reinterpret_cast<const float2*>(sh.ml) + at + lane * step);
+    const float M = warp_max(ml.x);
+    const float w = ml.x != -INFINITY ? exp2f(ml.x - M) : 0.0f;
+    const float L = warp_sum(ml.y * w), inv = L > 0.0f ? 1.0f / L : 0.0f;
+    float* mine = ws[threadIdx.x >> 5];
+    mine[lane] = w;
+    __syncwarp();
+    for (int d = lane; d < hd; d += 32) {
+        float acc = 0.0f;
+        for (int z = 0; z < S; z++) acc = fmaf(__ldcg(sh.o + (at + z * step) * hd + d), mine[z], acc);
+        out[(size_t)t * out_stride + (size_t)head * hd + d] = from_f32<T>(acc * inv);
+    }
+    if (lane == 0) lse[head * lse_ld + place] = L > 0.0f ? M + log2f(L) : INFINITY;
+}
+
+int shares_join(Shares sh, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded, const int* seq_start,
+                const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s) {
+    const dim3 grid(n_tokens, (nh + 7) / 8);
+    cudaError_t e = dtype == HB_BF16 ? hb_launch(shares_join_kernel<bf16>, grid, dim3(256), 0, s, sh, (bf16*)out, out_stride, lse, lse_ld, rounded,
+                                                 seq_start, seq_pos0, span, keys, window, n_tokens, n_seqs, nh, hd)
+                                     : hb_launch(shares_join_kernel<float>, grid, dim3(256), 0, s, sh, (float*)out, out_stride, lse, lse_ld, rounded,
+                                                 seq_start, seq_pos0, span, keys, window, n_tokens, n_seqs, nh, hd);
+    if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
+    return hb_check_launch("attention_mass (join of the shares)");
+}
+
 // A block per (64 keys = a page, kv head, share of the work): the scores of these keys with the queries that see them, in tiles
 // of 64 queries of one head.
-template <typename T>
+template <typename T, int NC>
 __global__ void __launch_bounds__(AM_THREADS)
 mass_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict__ kc, const int* __restrict__ page_table, int pt_width,
                  const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* __restrict__ lse, MassOut mo, int n_tokens,
-                 int n_seqs, int nh, int nkv, int hd, float scale_log2e, int window, int n_pages, int* status) {
+                 int n_seqs, int nh, int nkv, int hd, float scale_log2e, int window, int n_pages, int vec_q, int vec_kv, int* status) {
     extern __shared__ __align__(16) float am_smem[];
     pdl_trigger();
     pdl_wait();
@@ -200,13 +304,22 @@ mass_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restric
     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};             // of keys tx + 16 j, over rows ty + 16 i
     if (held && items > 0) {
         const size_t row0 = ((size_t)page * nkv + g) * HB_PAGE_TOKENS;
-        for (int r = ty; r < AM_KEYS; r += 16) am_load_row(ks + r * ld, kc + (row0 + r) * hd, hd, ld, tx, 16, pi * HB_PAGE_TOKENS + r < pos0 + n_new);
-        for (int it = (int)((long long)items * z / S); it < (int)((long long)items * (z + 1) / S); it++) {
+        AmTile<T, NC> tile;
+        tile.load(kc + row0 * hd, hd, hd, min(HB_PAGE_TOKENS, pos0 + n_new - pi * HB_PAGE_TOKENS), vec_kv, tid);
+        tile.store(ks, hd, ld, tid);
+        const int it1 = (int)((long long)items * (z + 1) / S);
+        auto load = [&](int it) {
+            const int q0 = n0 + (it % blocks) * AM_ROWS;
+            tile.load(q + (size_t)(t_begin + q0) * q_stride + (size_t)(g * G + it / blocks) * hd, q_stride, hd, min(AM_ROWS, n1 - q0), vec_q, tid);
+        };
+        int it = (int)((long long)items * z / S);
+        if (it < it1) load(it);
+        for (; it < it1; it++) {
             const int head = g * G + it / blocks, q0 = n0 + (it % blocks) * AM_ROWS;
             __syncthreads();
-            for (int r = ty; r < AM_ROWS; r += 16)
-                am_load_row(qs + r * ld, q + (size_t)(t_begin + q0 + r) * q_stride + (size_t)head * hd, hd, ld, tx, 16, q0 + r < n1);
+            tile.store(qs, hd, ld, tid);
             __syncthreads();
+            if (it + 1 < it1) load(it + 1);
             float s[4][4];
             am_scores(s, qs, ks, ld, tx, ty);
 #pragma unroll
@@ -269,65 +382,64 @@ static int am_reserve(F* kernel, int bytes, bool (&done)[HB_MAX_DEVICES]) {
     return 0;
 }
 
-#define AM_SMEM_ROWS(hd) ((2 * 64 * am_ld(hd) + 64 * 68) * 4)
+#define AM_SMEM_ROWS(hd) ((3 * 64 * am_ld(hd) + 64 * 68) * 4)
 #define AM_SMEM_MASS(hd) (2 * 64 * am_ld(hd) * 4)
 
 template <typename T, int NC>
 static int launch_rows(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                       const int* seq_pos0, void* out, long long out_stride, float* lse, int n_tokens, int n_seqs, int q_blocks, int nh, int nkv,
-                       int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
-    static bool done[HB_MAX_DEVICES] = {};
+                       const int* seq_pos0, void* out, long long out_stride, float* lse, Shares sh, int max_shares, MassOut mo, int splits, int n_tokens,
+                       int n_seqs, int q_blocks, int key_tiles, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+    static_assert(AM_SMEM_ROWS(256) <= 227 * 1024, "attention tiles do not fit shared memory");
+    static bool done[HB_MAX_DEVICES] = {}, done_mass[HB_MAX_DEVICES] = {};
     if (am_reserve(attention_rows_kernel<T, NC>, AM_SMEM_ROWS(16 * NC), done)) return 1;
-    cudaError_t e = hb_launch(attention_rows_kernel<T, NC>, dim3(nh, q_blocks), dim3(AM_THREADS), AM_SMEM_ROWS(hd), s, (const T*)q, q_stride,
-                              (const T*)kc, (const T*)vc, page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, lse, n_tokens, n_seqs, nh,
-                              nkv, hd, scale * MASS_LOG2E, window, n_pages, status);
+    if (am_reserve(mass_rows_kernel<T, NC>, AM_SMEM_MASS(16 * NC), done_mass)) return 1;
+    const uintptr_t four = 4 * sizeof(T);                      // four elements at a time where rows and heads begin at a multiple of that
+    const int vec_kv = hd % 4 == 0 && (((uintptr_t)kc | (uintptr_t)vc) & (four - 1)) == 0;
+    const int vec_q = hd % 4 == 0 && q_stride % 4 == 0 && ((uintptr_t)q & (four - 1)) == 0;
+    cudaError_t e = hb_launch(attention_rows_kernel<T, NC>, dim3(nh, q_blocks, max_shares), dim3(AM_THREADS), AM_SMEM_ROWS(hd), s, (const T*)q, q_stride,
+                              (const T*)kc, (const T*)vc, page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, lse, sh, n_tokens, n_seqs, nh,
+                              nkv, hd, scale * MASS_LOG2E, window, n_pages, vec_q, vec_kv, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
-    return hb_check_launch("attention_mass (rows)");
-}
-
-template <typename T>
-static int launch_general(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width,
-                          const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, MassOut mo, int splits, int n_tokens,
-                          int n_seqs, int q_blocks, int key_tiles, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status,
-                          cudaStream_t s) {
-    const int rc = hd <= 64 ? launch_rows<T, 4>(q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, n_tokens, n_seqs,
-                                                q_blocks, nh, nkv, hd, scale, window, n_pages, status, s)
-                   : hd <= 128 ? launch_rows<T, 8>(q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, n_tokens,
-                                                   n_seqs, q_blocks, nh, nkv, hd, scale, window, n_pages, status, s)
-                               : launch_rows<T, 16>(q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, n_tokens,
-                                                    n_seqs, q_blocks, nh, nkv, hd, scale, window, n_pages, status, s);
-    if (rc) return rc;
-    static bool done[HB_MAX_DEVICES] = {};
-    if (am_reserve(mass_rows_kernel<T>, AM_SMEM_MASS(256), done)) return 1;
-    cudaError_t e = hb_launch(mass_rows_kernel<T>, dim3(key_tiles, nkv, splits), dim3(AM_THREADS), AM_SMEM_MASS(hd), s, (const T*)q, q_stride,
-                              (const T*)kc, page_table, pt_width, seq_start, seq_pos0, (const float*)lse, mo, n_tokens, n_seqs, nh, nkv, hd,
-                              scale * MASS_LOG2E, window, n_pages, status);
+    if (hb_check_launch("attention_mass (rows)")) return 1;
+    if (max_shares > 1 && shares_join(sh, sizeof(T) == 4 ? HB_F32 : HB_BF16, out, out_stride, lse, n_tokens, 0, seq_start, seq_pos0, AM_ROWS,
+                                      HB_PAGE_TOKENS, window, n_tokens, n_seqs, nh, hd, s))
+        return 1;
+    e = hb_launch(mass_rows_kernel<T, NC>, dim3(key_tiles, nkv, splits), dim3(AM_THREADS), AM_SMEM_MASS(hd), s, (const T*)q, q_stride, (const T*)kc,
+                  page_table, pt_width, seq_start, seq_pos0, (const float*)lse, mo, n_tokens, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window, n_pages,
+                  vec_q, vec_kv, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     if (hb_check_launch("attention_mass (weights)")) return 1;
     return splits > 1 ? mass_join(page_table, pt_width, seq_start, seq_pos0, mo, n_seqs, nkv, n_pages, AM_KEYS, key_tiles, splits, s) : 0;
 }
 
 // Steps of many tokens.  q_blocks: sum over sequences of ceil(new tokens / 64); key_tiles: sum of ceil(rows / 64); lse:
-// n_heads * n_tokens floats; parts: splits * n_kv_heads * key_tiles * 64 floats when splits > 1.  before may be null or mass.
+// n_heads * n_tokens floats; max_shares: the most blocks that a block of queries takes, share_tiles: the most pages of one of them;
+// chunk_parts: max_shares * n_heads * n_tokens * (head_dim + 2) floats when max_shares > 1; parts: splits * n_kv_heads * key_tiles * 64
+// floats when splits > 1.  before may be null or mass.
 extern "C" int hb_attention_mass(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
                                  int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse,
-                                 const float* before, float* mass, float* parts, int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles,
-                                 int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* status, void* stream) {
+                                 const float* before, float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int splits,
+                                 int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window,
+                                 int n_pages, int* status, void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0 && head_dim <= 256 && n_pages > 0 && pt_width > 0,
                "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, head_dim);
-    HB_REQUIRE(n_kv_heads <= 65535 && q_blocks <= 65535 && key_tiles > 0 && splits >= 1 && splits <= 65535 && (splits == 1 || parts != nullptr),
+    HB_REQUIRE(n_kv_heads <= 65535 && q_blocks <= 65535 && key_tiles > 0 && splits >= 1 && splits <= 65535 && (splits == 1 || parts != nullptr) &&
+                   max_shares >= 1 && max_shares <= 32 && share_tiles >= 1 && (max_shares == 1 || chunk_parts != nullptr),
                "attention_mass: the step is too large for one launch");
     HB_REQUIRE(lse != nullptr && mass != nullptr, "attention_mass: missing buffers");
+    HB_REQUIRE(dtype == HB_F32 || dtype == HB_BF16, "attention_mass: unsupported dtype %d", dtype);
     MassOut mo = {before, mass, parts};
+    // (maximum, sum) pairs in front: 8-byte aligned whatever the head size; one share: no block is cut, whatever it sees
+    const Shares sh = {chunk_parts == nullptr ? nullptr : chunk_parts + (size_t)max_shares * n_heads * n_tokens * 2, chunk_parts,
+                       max_shares == 1 ? 0x3fffffff : share_tiles};
     cudaStream_t s = (cudaStream_t)stream;
-    if (dtype == HB_F32)
-        return launch_general<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, mo, splits, n_tokens,
-                                     n_seqs, q_blocks, key_tiles, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
-    if (dtype == HB_BF16)
-        return launch_general<bf16>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, mo, splits, n_tokens,
-                                    n_seqs, q_blocks, key_tiles, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
-    return hb_fail("attention_mass: unsupported dtype %d", dtype);
+#define HB_AM_LAUNCH(T, NC)                                                                                                                     \
+    launch_rows<T, NC>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, sh, max_shares, mo, splits, \
+                       n_tokens, n_seqs, q_blocks, key_tiles, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s)
+    if (dtype == HB_F32) return head_dim <= 64 ? HB_AM_LAUNCH(float, 4) : head_dim <= 128 ? HB_AM_LAUNCH(float, 8) : HB_AM_LAUNCH(float, 16);
+    return head_dim <= 64 ? HB_AM_LAUNCH(bf16, 4) : head_dim <= 128 ? HB_AM_LAUNCH(bf16, 8) : HB_AM_LAUNCH(bf16, 16);
+#undef HB_AM_LAUNCH
 }
 
 // -------------------------------------------------------------------------------------------- few tokens, every head size

@@ -87,6 +87,41 @@ int attention_decode_scores(const void* q, long long q_stride, const void* kc, c
                             const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int n_tokens, int nh,
                             int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);
 
+// The keys of a block of queries, shared out: a block that sees n tiles of keys takes ceil(n / tiles) CTAs, and where those are several each
+// leaves its unnormalised outputs and (maximum, sum) of its rows: o[(share * heads + head) * tokens + token][head size], ml likewise.
+struct Shares {
+    float* o;
+    float* ml;
+    int tiles;
+};
+__device__ __forceinline__ int shares_of(const Shares& sh, int n_tiles) { return max(1, (n_tiles + sh.tiles - 1) / sh.tiles); }
+// how many tiles of `keys` keys a block of queries at positions first..last sees, and the first of them
+__device__ __forceinline__ int key_tiles_of(int first, int last, int window, int keys, int& tile0) {
+    tile0 = hb_oldest_visible(first, window, 0) / keys;
+    return last / keys + 1 - tile0;
+}
+
+// joins the shares (attention_mass.cu): out and lse of the rows whose block has several.  Blocks of `span` tokens, tiles of `keys`
+// keys; lse[head * lse_ld + place], places in blocks of 128 per sequence (`rounded`) or the token's number
+int shares_join(Shares sh, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded, const int* seq_start,
+                const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s);
+
+// The first half of a step of many tokens on the tensor cores (attention_chunk_tc.cu): writes out and the rows'
+// log-sums, lse[head][place]: a sequence's places begin at a multiple of 128, behind those of the sequences in front.  q_blocks: sum
+// over sequences of ceil(new tokens / span), span 128 with an even group of heads and 256 with an odd one; max_shares: the most CTAs
+// that a block of queries takes, share_tiles: the most tiles of 128 keys of one of them; parts: max_shares * n_heads * n_tokens *
+// (head_dim + 2) floats when max_shares > 1.
+int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
+                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts,
+                       int max_shares, int share_tiles, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale,
+                       int window, int n_pages, int* error_flag, cudaStream_t s);
+
+// The first half of a step of few tokens on the tensor cores (attention_decode.cu): sizes of hb_attention_decode, queries 4-byte and
+// keys and values 16-byte aligned.
+int attention_decode_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* tok_seq,
+                            const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int n_tokens, int nh,
+                            int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);
+
 // The first half of a step of many tokens on the tensor cores (attention_chunk_tc.cu): writes out and the rows'
 // log-sums, lse[head][place]: a sequence's places begin at a multiple of 128, behind those of the sequences in front.  q_blocks: sum
 // over sequences of ceil(new tokens / span), span 128 with an even group of heads and 256 with an odd one; parts: splits * n_heads *

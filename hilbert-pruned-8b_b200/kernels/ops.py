@@ -19,7 +19,7 @@ from typing import Optional
 import torch
 
 from . import build
-from .plan import chunk_splits, decode_splits, few_splits, mass_splits, select_shape
+from .plan import chunk_shares, decode_splits, few_splits, mass_splits, select_shape
 
 _c_int, _c_ll, _c_float, _c_ptr = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
 
@@ -80,9 +80,9 @@ _SIGNATURES = {
     "hb_attention_prefill_tc": [_c_ptr, _c_ll, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_int,
                                 _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
-                          _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
+                          _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_tc": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr,
-                             _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
+                             _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr,
                               _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_int,
                               _c_ptr, _c_ptr],
@@ -1315,13 +1315,15 @@ class Ops:
             buffers = (cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(),
                        out.data_ptr(), out_ld, lse.data_ptr(), *((lse_ld,) if tc else ()), old, mass.data_ptr(),
                        parts.data_ptr() if parts is not None else None)
+            shares, tiles = chunk_shares(step.host_new, step.host_len, win, rows, 128 if tc else 64, heads // 2 if tc and group % 2 == 0 else heads,
+                                         heads * (head_dim + 2), self.sm_count * (1 if tc or head_dim > 64 else 2))
+            partial = torch.empty(shares * heads * T * (head_dim + 2), dtype=torch.float32, device=self.device) if shares > 1 else None
+            cut = (partial.data_ptr() if partial is not None else None, shares, tiles)
             if tc:
-                ways = chunk_splits((heads // 2 if group % 2 == 0 else heads) * q_blocks, step.max_len, self.sm_count)
-                shares = torch.empty(ways * heads * T * (head_dim + 2), dtype=torch.float32, device=self.device) if ways > 1 else None
-                self._call("hb_attention_mass_tc", qkv.data_ptr(), q_ld, *buffers, shares.data_ptr() if shares is not None else None, ways, *sizes)
-                self.launches += 0 if ways == 1 else 1
+                self._call("hb_attention_mass_tc", qkv.data_ptr(), q_ld, *buffers, *cut, *sizes)
             else:
-                self._call("hb_attention_mass", qkv.data_ptr(), code, q_ld, *buffers, *sizes)
+                self._call("hb_attention_mass", qkv.data_ptr(), code, q_ld, *buffers, *cut, *sizes)
+            self.launches += 0 if shares == 1 else 1
             self.launches += 2 if splits == 1 else 3
 
     def evict_select(self, mass, page_table, lengths, first: int, recent: int, kept) -> None:

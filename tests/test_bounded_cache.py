@@ -536,11 +536,18 @@ def test_evict_rows_refuses(change, text):
 
 
 def test_shapes_of_the_launches():
-    from hilbert_pruned_8b_b200.kernels.plan import chunk_splits, few_splits, mass_splits, select_shape
+    from hilbert_pruned_8b_b200.kernels.plan import chunk_shares, few_splits, mass_splits, select_shape
     assert few_splits(1, 8, 5, 296) == 5 and few_splits(8, 8, 129, 296) == 4 and few_splits(1000, 8, 100, 296) == 1
     assert mass_splits(1000, 8, 100, 296) == 1 and mass_splits(1, 1, 1, 296) == 1 and mass_splits(1, 1, 100, 296) == 16
-    assert chunk_splits(100, 10 ** 6, 148) == 1 and chunk_splits(16, 100000, 148) == 9 and chunk_splits(16, 1100, 148) == 2 and chunk_splits(1, 300, 148) == 1
-    assert chunk_splits(1, 10 ** 6, 148) == 32
+    assert chunk_shares([4096], [4096], 0, 128, 128, 16, 4160, 148) == (1, 32)                 # enough blocks for everybody
+    shares, tiles = chunk_shares([128], [100000], 0, 128, 128, 16, 4160, 148)                  # 16 blocks of 782 tiles
+    assert 8 <= shares <= 32 and (shares - 1) * tiles < 782 <= shares * tiles
+    assert chunk_shares([10, 0], [100, 7], 0, 128, 128, 16, 4160, 148) == (1, 1) and chunk_shares([], [], 0, 128, 128, 16, 4160, 148) == (1, 1)
+    for window in (0, 1000):
+        for new, lens in (([700, 33, 1], [700, 550, 5000]), ([2000] * 5, [9000] * 5), ([9], [10 ** 6])):
+            shares, tiles = chunk_shares(new, lens, window, 256, 64, 5, 100, 148)
+            seen = max(min(ln, window + 256) if window else ln for ln in lens)
+            assert 1 <= shares <= 32 and shares * tiles * 64 >= seen               # the device cuts a block into at most that many
     for rows in (1, 64, 1000, 16384, 16385, 70000, 131072, 300000, 10 ** 7):
         for lists in (1, 2, 16, 74, 75, 148, 256, 4096):
             threads, cluster = select_shape(lists, rows, 148)
