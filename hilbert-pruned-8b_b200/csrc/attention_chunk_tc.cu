@@ -8,9 +8,8 @@
 // 32 bytes a clock that an SM takes from L2 would last 2048 clocks for one tile: hence two tiles, which halve that, and which take turns:
 // while one tile's weights are made, the tensor cores work on the other.
 //   warps 0-7, 8-15 softmax of tile 0 and 1, two threads per row: 64 scores each from tensor memory into registers, the row's maximum agreed
-//                   on through shared memory, running maximum and sum in float32, weights as bfloat16 over the scores.  (With one
-//                   thread per row and 8 warps in all, latencies showed: 1054 us against XXX for 2048 tokens behind 30001 rows of the 8B
-//                   sizes.)  The output accumulator is rescaled only when a row's maximum grows by more than 2^8 (weights are
+//                   on through shared memory, running maximum and sum in float32, weights as bfloat16 over the scores.  (One thread
+//                   per row needs no exchange but leaves two warps to a quarter of the SM: the same time.)  The output accumulator is rescaled only when a row's maximum grows by more than 2^8 (weights are
 //                   taken against a maximum that may be stale by less).
 //   warp 16         TMA producer: the query tiles once, then key and value tiles of 128 rows (two pages), two stages each
 //   warp 17         owns tensor memory; one thread issues, per key tile and in this order: O0 += P0 V, S0 = Q0 K' (the next keys),
@@ -88,8 +87,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int z = blockIdx.z;
     const int head0 = head_pairs ? 2 * blockIdx.x : blockIdx.x, g = head0 / (nh / nkv);
     const int span = head_pairs ? FA_ROWS : 2 * FA_ROWS;
-    int b = 0, blk = 0;
-    const bool has_work = mass_find_block(seq_start, n_seqs, gridDim.y - 1 - blockIdx.y, span, b, blk);
+    int b, blk, place0;
+    const bool has_work = mass_find_block(seq_start, n_seqs, gridDim.y - 1 - blockIdx.y, span, b, blk, place0);
     const int t_begin = has_work ? seq_start[b] : 0, n_new = has_work ? seq_start[b + 1] - t_begin : 1, pos0 = has_work ? seq_pos0[b] : 0;
     const int row0 = blk * span;                               // the first of the CTA's new tokens
     const int first_pos = pos0 + row0, last_pos = pos0 + min(row0 + span, n_new) - 1;
@@ -171,48 +170,49 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (!mbar_wait(q_full, 0)) atomicExch(error_flag, 53);
         }
     } else if (warp == 17) {
-        // ---------------------------------------------------------------- MMA issuer
-        if (lane == 0) {
-            constexpr uint32_t idesc_qk = instr_desc_bf16_mn(128, FA_KEYS);
-            constexpr uint32_t idesc_pv = instr_desc_bf16_mn(128, HD) | (1u << 16);           // B is MN-major
-            auto scores = [&](int i, int it) {
-                const uint32_t kst = k_smem + (it % CT_STAGES) * TILE;
+        // ---------------------------------------------------------------- MMA issuer: the warp waits, one lane issues
+        constexpr uint32_t idesc_qk = instr_desc_bf16_mn(128, FA_KEYS);
+        constexpr uint32_t idesc_pv = instr_desc_bf16_mn(128, HD) | (1u << 16);               // B is MN-major
+        // descriptors of the tiles' beginnings; a step along a tile adds its bytes / 16
+        const uint64_t q_desc = smem_desc_sw128(smem_base), k_desc = smem_desc_sw128(k_smem), v_desc = smem_desc_mn_sw128(v_smem, FA_HALF_BYTES, 1024);
+        auto scores = [&](int i, int it) {
+            const int st = it % CT_STAGES;
 #pragma unroll
-                for (int kk = 0; kk < HD / 16; kk++) {
-                    const uint32_t off = (kk >> 2) * FA_HALF_BYTES + (kk & 3) * 32;
-                    umma_bf16(tmem_base + i * 128, smem_desc_sw128(smem_base + i * TILE + off), smem_desc_sw128(kst + off), idesc_qk, kk ? 1u : 0u);
-                }
-                umma_commit(s_full0 + 8 * i);
-                if (i == 1) umma_commit(k_empty0 + 8 * (it % CT_STAGES));
-            };
-            bool alive = mbar_wait(q_full, 0) && mbar_wait(k_full0, 0);
-            if (alive) {
-                tc_fence_after();
-                scores(0, 0);
-                scores(1, 0);
-            } else {
-                atomicExch(error_flag, 54);
+            for (int kk = 0; kk < HD / 16; kk++) {
+                const uint32_t off = (kk >> 2) * FA_HALF_BYTES + (kk & 3) * 32;
+                umma_bf16(tmem_base + i * 128, q_desc + ((i * TILE + off) >> 4), k_desc + ((st * TILE + off) >> 4), idesc_qk, kk ? 1u : 0u);
             }
-            for (int it = 0; it < n_it && alive; it++) {
-                const int sv = it % CT_STAGES;
-                const uint32_t vst = v_smem + sv * TILE;
+            umma_commit(s_full0 + 8 * i);
+            if (i == 1) umma_commit(k_empty0 + 8 * st);
+        };
+        bool alive = __all_sync(0xffffffffu, mbar_wait(q_full, 0) && mbar_wait(k_full0, 0));
+        if (!alive) atomicExch(error_flag, 54);
+        tc_fence_after();
+        if (alive && elect_one()) {
+            scores(0, 0);
+            scores(1, 0);
+        }
+        for (int it = 0; it < n_it && alive; it++) {
+            const int sv = it % CT_STAGES;
 #pragma unroll
-                for (int i = 0; i < 2 && alive; i++) {
-                    if (!mbar_wait(p_full0 + 8 * i, it & 1) || (i == 0 && !mbar_wait(v_full0 + 8 * sv, (it / CT_STAGES) & 1)) ||
-                        (i == 0 && it + 1 < n_it && !mbar_wait(k_full0 + 8 * ((it + 1) % CT_STAGES), ((it + 1) / CT_STAGES) & 1))) {
-                        atomicExch(error_flag, 55);
-                        alive = false;
-                        break;
-                    }
-                    tc_fence_after();
+            for (int i = 0; i < 2; i++) {
+                alive = __all_sync(0xffffffffu, mbar_wait(p_full0 + 8 * i, it & 1) && (i == 1 || mbar_wait(v_full0 + 8 * sv, (it / CT_STAGES) & 1)) &&
+                                                    (i == 1 || it + 1 == n_it || mbar_wait(k_full0 + 8 * ((it + 1) % CT_STAGES), ((it + 1) / CT_STAGES) & 1)));
+                if (!alive) {
+                    atomicExch(error_flag, 55);
+                    break;
+                }
+                tc_fence_after();
+                if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < FA_KEYS / 16; kk++)
-                        umma_bf16_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + kk * 8, smem_desc_mn_sw128(vst + kk * 16 * 128, FA_HALF_BYTES, 1024),
-                                     idesc_pv, (it | kk) ? 1u : 0u);
+                        umma_bf16_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + kk * 8, v_desc + ((sv * TILE + kk * 16 * 128) >> 4), idesc_pv,
+                                     (it | kk) ? 1u : 0u);
                     if (i == 1) umma_commit(v_empty0 + 8 * sv);
                     if (it + 1 < n_it) scores(i, it + 1);
                     else umma_commit(o_full0 + 8 * i);
                 }
+                __syncwarp();
             }
         }
     } else {
@@ -314,9 +314,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     if (S > 1) {
                         *reinterpret_cast<float2*>(sh.ml + at * 2) = make_float2(m_run, l);
                     } else {
-                        int place = row;
-                        for (int a = 0; a < b; a++) place += mass_round128(seq_start[a + 1] - seq_start[a]);
-                        lse[head * lse_ld + place] = l > 0.0f ? m_run + log2f(l) : INFINITY;
+                        lse[head * lse_ld + place0 + row] = l > 0.0f ? m_run + log2f(l) : INFINITY;
                     }
                 }
                 bf16* dst = out + (size_t)(t_begin + row) * out_stride + (size_t)head * HD + hf * (HD / 2);

@@ -106,8 +106,8 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
     float* ps = vs + AM_KEYS * ld;                       // [64 rows][68]: weights
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int head = blockIdx.x, g = head / (nh / nkv), z = blockIdx.z;
-    int b, blk;
-    if (!mass_find_block(seq_start, n_seqs, gridDim.y - 1 - blockIdx.y, AM_ROWS, b, blk)) return;
+    int b, blk, place0;
+    if (!mass_find_block(seq_start, n_seqs, gridDim.y - 1 - blockIdx.y, AM_ROWS, b, blk, place0)) return;
     const int t0 = seq_start[b] + blk * AM_ROWS;
     const int rows = min(AM_ROWS, seq_start[b + 1] - t0);
     const int p0 = seq_pos0[b] + blk * AM_ROWS, p_last = p0 + rows - 1;
@@ -234,11 +234,9 @@ shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* 
     pdl_trigger();
     pdl_wait();
     const int t = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * 8 + (threadIdx.x >> 5);
-    int b = 0, place = t;
-    for (; b < n_seqs - 1 && seq_start[b + 1] <= t; b++) {
-        const int n = seq_start[b + 1] - seq_start[b];
-        if (rounded) place += mass_round128(n) - n;
-    }
+    int b, i, place0;
+    if (!mass_find_block(seq_start, n_seqs, t, 1, b, i, place0)) return;
+    const int place = rounded ? place0 + i : t;
     const int n_new = seq_start[b + 1] - seq_start[b], row0 = (t - seq_start[b]) / span * span;
     int tile0;
     const int S = shares_of(sh, key_tiles_of(seq_pos0[b] + row0, seq_pos0[b] + min(row0 + span, n_new) - 1, window, keys, tile0));
@@ -289,8 +287,8 @@ mass_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restric
     float* qs = ks + AM_KEYS * ld;                       // [64][ld]
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
     const int g = blockIdx.y, G = nh / nkv, S = gridDim.z, z = blockIdx.z;
-    int b, pi;
-    if (!mass_find_keys(seq_start, seq_pos0, n_seqs, blockIdx.x, AM_KEYS, b, pi)) return;
+    int b, pi, place0;
+    if (!mass_find_keys(seq_start, seq_pos0, n_seqs, blockIdx.x, AM_KEYS, b, pi, place0)) return;
     const int page = pi < pt_width ? page_table[(size_t)b * pt_width + pi] : -1;
     const bool held = page >= 0 && page < n_pages;
     const int t_begin = seq_start[b], n_new = seq_start[b + 1] - t_begin, pos0 = seq_pos0[b];
@@ -354,8 +352,8 @@ __global__ void mass_join_kernel(const int* __restrict__ page_table, int pt_widt
     pdl_trigger();
     pdl_wait();
     const int g = blockIdx.y, tid = threadIdx.x;
-    int b, kt;
-    if (!mass_find_keys(seq_start, seq_pos0, n_seqs, blockIdx.x, tile, b, kt)) return;
+    int b, kt, place0;
+    if (!mass_find_keys(seq_start, seq_pos0, n_seqs, blockIdx.x, tile, b, kt, place0)) return;
     const int key = kt * tile + tid, pi = key / HB_PAGE_TOKENS;
     const int page = pi < pt_width ? page_table[(size_t)b * pt_width + pi] : -1;
     const size_t place = (size_t)blockIdx.x * tile + tid, places = (size_t)gridDim.x * tile;

@@ -17,34 +17,53 @@ struct MassOut {
 // distance, in floats, of the scores of two heads
 static __host__ __device__ inline long long mass_score_ld(int max_len) { return ((long long)max_len + 63) / 64 * 64; }
 
-// The sequence b and its block blk of `rows` new tokens that block number `at` of the step stands for.
-__device__ __forceinline__ bool mass_find_block(const int* __restrict__ seq_start, int n_seqs, int at, int rows, int& b, int& blk) {
-    for (b = 0; b < n_seqs; b++) {
-        const int nb = (seq_start[b + 1] - seq_start[b] + rows - 1) / rows;
-        if (at < nb) {
-            blk = at;
+// A step's sequences are looked through 32 at a time, a lane each: which of them element number `at` of `count(b)` elements each belongs
+// to, its number there, and the sum of `other(b)` over the sequences in front.  Called by whole warps; the same answer in every lane.
+template <typename F, typename H>
+__device__ __forceinline__ bool mass_find(int n_seqs, int at, F&& count, H&& other, int& b, int& inside, int& others) {
+    const int lane = threadIdx.x & 31;
+    int front = 0;
+    others = 0;
+    for (int b0 = 0; b0 < n_seqs; b0 += 32) {
+        const bool there = b0 + lane < n_seqs;
+        const int n = there ? count(b0 + lane) : 0, o = there ? other(b0 + lane) : 0;
+        int sum = n;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += u;
+        }
+        const unsigned behind = __ballot_sync(0xffffffffu, at < front + sum);
+        if (behind != 0u) {
+            const int i = __ffs(behind) - 1;
+            b = b0 + i;
+            inside = at - front - (__shfl_sync(0xffffffffu, sum, i) - __shfl_sync(0xffffffffu, n, i));
+            others += (int)__reduce_add_sync(0xffffffffu, (unsigned)(lane < i ? o : 0));
             return true;
         }
-        at -= nb;
+        front += __shfl_sync(0xffffffffu, sum, 31);
+        others += (int)__reduce_add_sync(0xffffffffu, (unsigned)o);
     }
+    b = inside = 0;
     return false;
+}
+
+// where the log-sums of a sequence's rows begin, in blocks of 128 rows (attention_chunk_tc below)
+__host__ __device__ constexpr int mass_round128(int n) { return (n + 127) & ~127; }
+
+// The sequence b and its block blk of `rows` new tokens that block number `at` of the step stands for; place0: mass_round128 of the
+// new tokens of the sequences in front, added up.
+__device__ __forceinline__ bool mass_find_block(const int* __restrict__ seq_start, int n_seqs, int at, int rows, int& b, int& blk, int& place0) {
+    return mass_find(n_seqs, at, [&](int i) { return (seq_start[i + 1] - seq_start[i] + rows - 1) / rows; },
+                     [&](int i) { return mass_round128(seq_start[i + 1] - seq_start[i]); }, b, blk, place0);
 }
 
 // The sequence b and its tile kt of `tile` rows of the cache (those behind this step) that tile number `at` stands for.
 __device__ __forceinline__ bool mass_find_keys(const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, int n_seqs, int at, int tile,
-                                               int& b, int& kt) {
-    for (b = 0; b < n_seqs; b++) {
-        const int nb = (seq_pos0[b] + seq_start[b + 1] - seq_start[b] + tile - 1) / tile;
-        if (at < nb) {
-            kt = at;
-            return true;
-        }
-        at -= nb;
-    }
-    return false;
+                                               int& b, int& kt, int& place0) {
+    return mass_find(n_seqs, at, [&](int i) { return (seq_pos0[i] + seq_start[i + 1] - seq_start[i] + tile - 1) / tile; },
+                     [&](int i) { return mass_round128(seq_start[i + 1] - seq_start[i]); }, b, kt, place0);
 }
-
-__host__ __device__ constexpr int mass_round128(int n) { return (n + 127) & ~127; }
 
 // The new tokens [n0, n1) of a sequence that see one of the keys [key0, key0 + keys): token i stands at pos0 + i.
 __device__ __forceinline__ void mass_queries(int key0, int keys, int pos0, int n_new, int window, int& n0, int& n1) {

@@ -49,8 +49,8 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     // heaviest ones start first and what ends last is light.
     const int z = blockIdx.x % S, g = blockIdx.x / S % nkv, G = nh / nkv, tile = blockIdx.x / (S * nkv);
 
-    int b = 0, kt = 0;
-    const bool has_work = mass_find_keys(seq_start, seq_pos0, n_seqs, tile, MT_KEYS, b, kt);
+    int b, kt, place0;
+    const bool has_work = mass_find_keys(seq_start, seq_pos0, n_seqs, tile, MT_KEYS, b, kt, place0);
     const int t_begin = has_work ? seq_start[b] : 0, n_new = has_work ? seq_start[b + 1] - t_begin : 0, pos0 = has_work ? seq_pos0[b] : 0;
     const int key0 = kt * MT_KEYS;
     int n0 = 0, n1 = 0;
@@ -99,8 +99,7 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 for (int half = 0; half < HALVES; half++)
                     tma_load_2d(dst + half * FA_HALF_BYTES, &map_k, k_full, half * 64, (page * nkv + g) * HB_PAGE_TOKENS);
             }
-            long long lse0 = n0;                                    // where the log-sums of token n0 lie
-            for (int i = 0; i < b; i++) lse0 += mass_round128(seq_start[i + 1] - seq_start[i]);
+            const int lse0 = place0 + n0;                           // where the log-sums of token n0 lie
             int issued = 0;
             for (int it = 0; it < n_it; it++) {
                 const int s = it % MT_STAGES;
@@ -120,30 +119,33 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             if (!mbar_wait(k_full, 0)) atomicExch(error_flag, 42);
         }
     } else if (warp == 1) {
-        // ---------------------------------------------------------------- MMA issuer
-        if (lane == 0 && n_it > 0) {
-            constexpr uint32_t idesc = instr_desc_bf16_mn(128, 128);
-            const bool alive = mbar_wait(k_full, 0);
-            if (!alive) atomicExch(error_flag, 43);
-            for (int it = 0; it < n_it && alive; it++) {
-                const int s = it % MT_STAGES, sb = it & 1;
-                if (!mbar_wait(q_full0 + 8 * s, (it / MT_STAGES) & 1) || !mbar_wait(s_empty0 + 8 * sb, ((it >> 1) & 1) ^ 1)) {
-                    atomicExch(error_flag, 44);
-                    break;
-                }
-                tc_fence_after();
-                const uint32_t qst = q_smem + s * TILE;
+        // ---------------------------------------------------------------- MMA issuer: the warp waits, one lane issues
+        constexpr uint32_t idesc = instr_desc_bf16_mn(128, 128);
+        const uint64_t k_desc = smem_desc_sw128(smem_base), q_desc = smem_desc_sw128(q_smem);     // a step along a tile adds its bytes / 16
+        bool alive = n_it > 0;
+        if (alive && !__all_sync(0xffffffffu, mbar_wait(k_full, 0))) {
+            atomicExch(error_flag, 43);
+            alive = false;
+        }
+        for (int it = 0; it < n_it && alive; it++) {
+            const int s = it % MT_STAGES, sb = it & 1;
+            if (!__all_sync(0xffffffffu, mbar_wait(q_full0 + 8 * s, (it / MT_STAGES) & 1) && mbar_wait(s_empty0 + 8 * sb, ((it >> 1) & 1) ^ 1))) {
+                atomicExch(error_flag, 44);
+                break;
+            }
+            tc_fence_after();
+            if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < 2; k++)
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; kk++) {
                         const uint32_t off = (kk >> 2) * FA_HALF_BYTES + (kk & 3) * 32;
-                        umma_bf16(tmem_base + (2 * sb + k) * 128, smem_desc_sw128(smem_base + k * TILE + off), smem_desc_sw128(qst + off), idesc,
-                                  kk ? 1u : 0u);
+                        umma_bf16(tmem_base + (2 * sb + k) * 128, k_desc + ((k * TILE + off) >> 4), q_desc + ((s * TILE + off) >> 4), idesc, kk ? 1u : 0u);
                     }
                 umma_commit(q_empty0 + 8 * s);
                 umma_commit(s_full0 + 8 * sb);
             }
+            __syncwarp();
         }
     } else {
         // ---------------------------------------------------------------- weights
