@@ -11,7 +11,6 @@
 //
 // Sizes: head size 64 or 128, group size up to 16; anything else is the general kernel's.
 #include "api.h"
-#include "attention_mass.cuh"
 #include "mma.cuh"
 
 #define AD_THREADS 128
@@ -31,19 +30,16 @@
 // happens before the first request of that page, or after the prologue.  -1: the caller
 // has waited already.  `after_wait` runs right after the wait (the place to write that page).
 // `status`, `batch_row`: where a page number outside the cache is noted (common.cuh).
-// SAVE: every score (in units of log 2, -inf where the query does not see the key) of head row r goes to
-// scores[r * score_ld + key], and value rows behind the sequence's end count as zero whatever the page holds there.
 // `patch_page` (>= 0): when that page has arrived, row `patch_row` of its key and value tiles is
 // overwritten with k_new / v_new (HD values each, in shared memory): the new token's key and
 // value, for a page that was requested before they existed.
-template <int HD, int STAGES, bool SAVE = false, typename F, typename W>
+template <int HD, int STAGES, typename F, typename W>
 __device__ __forceinline__ void decode_split_core(uint32_t (&qf)[HD / 16][4], const bf16* kc, const bf16* vc,
                                                   const int* __restrict__ pt, int n_pages, int nkv, int g, int lo,
                                                   int len, int p_begin, int p_end, float scale_log2e, uint8_t* smem,
                                                   F&& after_prologue, int fresh_page, W&& after_wait, int patch_page = -1,
                                                   int patch_row = 0, const bf16* k_new = nullptr, const bf16* v_new = nullptr,
-                                                  int* status = nullptr, int batch_row = 0, float* scores = nullptr,
-                                                  long long score_ld = 0, int n_heads_here = 0) {
+                                                  int* status = nullptr, int batch_row = 0) {
     constexpr int ROW_BYTES = HD * 2;
     constexpr int TILE_BYTES = HB_PAGE_TOKENS * ROW_BYTES;        // one page of K (or V) of one kv head
     constexpr int CHUNKS = ROW_BYTES / 16;
@@ -68,8 +64,7 @@ __device__ __forceinline__ void decode_split_core(uint32_t (&qf)[HD / 16][4], co
                 const int row = i / CHUNKS, ch = i % CHUNKS;
                 const uint32_t off = swizzled<ROW_BYTES>(row, ch);
                 cp_async_16(kdst + off, ksrc + (size_t)i * 16);
-                if (SAVE) cp_async_16_or_zero(vdst + off, vsrc + (size_t)i * 16, page_idx * HB_PAGE_TOKENS + row < len);
-                else cp_async_16(vdst + off, vsrc + (size_t)i * 16);
+                cp_async_16(vdst + off, vsrc + (size_t)i * 16);
             }
         }
         cp_async_commit();
@@ -134,17 +129,6 @@ __device__ __forceinline__ void decode_split_core(uint32_t (&qf)[HD / 16][4], co
                 s[nt][e] = v;
                 mx[e >> 1] = fmaxf(mx[e >> 1], v);
             }
-        if (SAVE) {
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int r = (lane >> 2) + 8 * h;
-                if (r < n_heads_here) {
-#pragma unroll
-                    for (int nt = 0; nt < 2; nt++)
-                        *reinterpret_cast<float2*>(scores + r * score_ld + key0 + nt * 8) = make_float2(s[nt][2 * h], s[nt][2 * h + 1]);
-                }
-            }
-        }
         uint32_t pa[4];
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -377,107 +361,6 @@ attn_decode_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* _
     }
     if (COMBINE && S > 1)
         combine_by_last_split<HD>(b, g, G, S, nh, nkv, part_o, part_ml, counters, out, out_stride, w_split, l_split, &is_last);
-}
-
-// The split-K attention of a step of few tokens that keeps the scores (attention_mass.cu joins the splits and turns the scores
-// into weights).  One query token t of sequence tok_seq[t] takes a CTA row; a sequence with several tokens has its pages read once
-// per token, from L2 after the first.  Everything waits for the kernel in front: what it moved or wrote may be any page.
-template <int HD>
-__global__ void __launch_bounds__(AD_THREADS)
-attn_decode_scores_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __restrict__ kc, const bf16* __restrict__ vc,
-                          const int* __restrict__ page_table, int pt_width, const int* __restrict__ tok_seq, const int* __restrict__ positions,
-                          float* part_o, float* part_ml, float* scores, long long score_ld, int nh, int nkv, float scale_log2e, int window,
-                          int n_pages, int* status) {
-    constexpr int KSTEPS = HD / 16;
-    extern __shared__ __align__(128) uint8_t smem[];
-    pdl_trigger();
-    pdl_wait();
-    q = pdl_fresh(q);
-    const int z = blockIdx.x, g = blockIdx.y, t = blockIdx.z, S = gridDim.x;
-    const int tid = threadIdx.x, lane = tid & 31;
-    const int G = nh / nkv, b = tok_seq[t];
-    const int len = positions[t] + 1;
-    const int lo = (window > 0 && len - window > 0) ? len - window : 0;
-    const int width = (int)min((long long)pt_width, score_ld / HB_PAGE_TOKENS);       // no score is written behind its head's
-    int p_begin, p_end, pages_per_split;
-    split_pages(z, S, lo, len, width, p_begin, p_end, pages_per_split);
-    if (z == 0 && tid == 0 && len > width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
-    if (p_begin >= p_end) {
-        if (tid < G) {
-            float* ml = part_ml + (((size_t)t * nh + g * G + tid) * S + z) * 2;
-            ml[0] = -INFINITY;
-            ml[1] = 0.0f;
-        }
-        return;
-    }
-    uint32_t qf[KSTEPS][4];
-    decode_split_core<HD, AD_STAGES, true>(qf, kc, vc, page_table + (size_t)b * pt_width, n_pages, nkv, g, lo, len, p_begin, p_end, scale_log2e, smem, [&] {
-        const int r0 = lane >> 2, c = (lane & 3) * 2;
-        const unsigned int* q0 = reinterpret_cast<const unsigned int*>(q + (size_t)t * q_stride + (size_t)(g * G + r0) * HD + c);
-        const unsigned int* q1 = q0 + 8 * HD / 2;
-#pragma unroll
-        for (int ks = 0; ks < KSTEPS; ks++) {
-            qf[ks][0] = r0 < G ? __ldcg(q0 + ks * 8) : 0u;
-            qf[ks][1] = r0 + 8 < G ? __ldcg(q1 + ks * 8) : 0u;
-            qf[ks][2] = r0 < G ? __ldcg(q0 + ks * 8 + 4) : 0u;
-            qf[ks][3] = r0 + 8 < G ? __ldcg(q1 + ks * 8 + 4) : 0u;
-        }
-    }, -1, [] {}, -1, 0, nullptr, nullptr, status, b, scores + ((size_t)t * nh + g * G) * score_ld, score_ld, G);
-    const float* so = reinterpret_cast<const float*>(smem);
-    const float* sm = so + 4 * 16 * HD;
-    const float* sl = sm + 4 * 16;
-    for (int idx = tid; idx < G * HD; idx += AD_THREADS) {
-        const int r = idx / HD, d = idx - r * HD;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w * 16 + r]);
-        float acc = 0.0f, L = 0.0f;
-        if (M != -INFINITY) {
-#pragma unroll
-            for (int w = 0; w < 4; w++) {
-                const float e = exp2f(sm[w * 16 + r] - M);
-                acc += so[(size_t)(w * 16 + r) * HD + d] * e;
-                L += sl[w * 16 + r] * e;
-            }
-        }
-        const size_t base = ((size_t)t * nh + g * G + r) * S + z;
-        part_o[base * HD + d] = acc;
-        if (d == 0) {
-            part_ml[base * 2] = M;
-            part_ml[base * 2 + 1] = L;
-        }
-    }
-}
-
-template <int HD>
-static int launch_decode_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width,
-                                const int* tok_seq, const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld,
-                                int splits, int n_tokens, int nh, int nkv, float scale, int window, int n_pages, int* status, cudaStream_t s) {
-    constexpr int PIPE = AD_STAGES * 2 * HB_PAGE_TOKENS * HD * 2;
-    constexpr int MERGE = (4 * 16 * HD + 2 * 4 * 16) * 4;
-    constexpr int SMEM = PIPE > MERGE ? PIPE : MERGE;
-    static bool attr_done[HB_MAX_DEVICES] = {};
-    bool& attr_set = attr_done[hb_device_slot()];
-    if (!attr_set) {
-        cudaError_t e = cudaFuncSetAttribute(attn_decode_scores_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
-        if (e != cudaSuccess) return hb_fail("attention_mass: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
-        attr_set = true;
-    }
-    cudaError_t e = hb_launch(attn_decode_scores_kernel<HD>, dim3(splits, nkv, n_tokens), dim3(AD_THREADS), SMEM, s, (const bf16*)q, q_stride,
-                              (const bf16*)kc, (const bf16*)vc, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, nh, nkv,
-                              scale * AD_LOG2E, window, n_pages, status);
-    if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
-    return hb_check_launch("attention_mass (few tokens, tensor cores)");
-}
-
-int attention_decode_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* tok_seq,
-                            const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int n_tokens, int nh,
-                            int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s) {
-    if (head_dim == 128)
-        return launch_decode_scores<128>(q, q_stride, kc, vc, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits, n_tokens,
-                                         nh, nkv, scale, window, n_pages, status, s);
-    return launch_decode_scores<64>(q, q_stride, kc, vc, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits, n_tokens, nh,
-                                    nkv, scale, window, n_pages, status, s);
 }
 
 // The attention of a decode step without a rotation kernel in front: rotate the new token's

@@ -1,0 +1,273 @@
+// The first half of a step of few tokens with accumulated weights (attention_mass.cu) on the tensor cores, bfloat16, head size 64 or
+// 128: partial results over shares of the keys, and the scores themselves, for the kernel that joins the shares and turns the
+// scores into weights.
+//
+// A CTA = a share of the pages x one kv head x a block of a sequence's new tokens: the rows of the mma.sync tiles (16 RT of them) are the
+// (token, head) pairs of the block, so a page is read once for all of them.  Bound by memory: 2 head sizes of keys and values per row of
+// the cache against 4 bytes of score per pair.  The pages stream through three cp.async stages; each of the four warps takes a
+// quarter of every page's keys with its own running maximum and sum, joined through shared memory at the end.
+// (With a CTA per token, as for single tokens, 17 drafted tokens of four sequences took 82 us; their pages came from L2 17 times.)
+#include "api.h"
+#include "attention_mass.cuh"
+#include "mma.cuh"
+
+#define FT_THREADS 128
+#define FT_STAGES 3
+
+template <int HD, int RT>
+__global__ void __launch_bounds__(FT_THREADS)
+few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __restrict__ kc, const bf16* __restrict__ vc,
+              const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* part_o,
+              float* part_ml, float* scores, long long score_ld, int tokens_per_block, int n_seqs, int nh, int nkv, float scale_log2e, int window,
+              int n_pages, int* status) {
+    constexpr int ROW_BYTES = HD * 2, TILE_BYTES = HB_PAGE_TOKENS * ROW_BYTES, CHUNKS = ROW_BYTES / 16, KSTEPS = HD / 16, ROWS = 16 * RT;
+    extern __shared__ __align__(128) uint8_t smem[];
+    pdl_trigger();
+    pdl_wait();
+    q = pdl_fresh(q);
+    const int z = blockIdx.x, g = blockIdx.y, S = gridDim.x;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int G = nh / nkv;
+    int b, blk, place0;
+    if (!mass_find_block(seq_start, n_seqs, blockIdx.z, tokens_per_block, b, blk, place0)) return;
+    const int t0 = seq_start[b] + blk * tokens_per_block, n_tok = min(tokens_per_block, seq_start[b + 1] - t0);
+    const int p0 = seq_pos0[b] + blk * tokens_per_block, p_last = p0 + n_tok - 1;
+    const int width = (int)min((long long)pt_width, score_ld / HB_PAGE_TOKENS);       // no score is written behind its head's
+    const int first = hb_oldest_visible(p0, window, 0) / HB_PAGE_TOKENS, last = min(p_last / HB_PAGE_TOKENS + 1, width);
+    const int per = max(1, (last - first + S - 1) / S), page0 = first + z * per, page1 = min(page0 + per, last);
+    const int* pt = page_table + (size_t)b * pt_width;
+    if (z == 0 && tid == 0 && p_last >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
+    const int pairs = n_tok * G;                           // row r is head r % G of token r / G
+    if (page0 >= page1) {                                  // a share without keys
+        for (int r = tid; r < pairs; r += FT_THREADS) {
+            float* ml = part_ml + (((size_t)(t0 + r / G) * nh + g * G + r % G) * S + z) * 2;
+            ml[0] = -INFINITY;
+            ml[1] = 0.0f;
+        }
+        return;
+    }
+    const uint32_t smem_base = (uint32_t)__cvta_generic_to_shared(smem);
+    bool bad_page = false;
+    auto load_page = [&](int stage, int pi) {
+        if (pi < page1) {
+            int page = pt[pi];
+            if (page < 0 || page >= n_pages) {
+                bad_page = true;
+                page = 0;                                   // never read outside the cache
+            }
+            const uint8_t* ksrc = (const uint8_t*)(kc + ((size_t)page * nkv + g) * HB_PAGE_TOKENS * HD);
+            const uint8_t* vsrc = (const uint8_t*)(vc + ((size_t)page * nkv + g) * HB_PAGE_TOKENS * HD);
+            const uint32_t kdst = smem_base + stage * 2 * TILE_BYTES, vdst = kdst + TILE_BYTES;
+#pragma unroll
+            for (int i = tid; i < HB_PAGE_TOKENS * CHUNKS; i += FT_THREADS) {
+                const int row = i / CHUNKS, ch = i % CHUNKS;
+                const uint32_t off = swizzled<ROW_BYTES>(row, ch);
+                cp_async_16(kdst + off, ksrc + (size_t)i * 16);
+                // values behind the last key are whatever the page held before, and 0 * NaN is NaN
+                cp_async_16_or_zero(vdst + off, vsrc + (size_t)i * 16, pi * HB_PAGE_TOKENS + row <= p_last);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < FT_STAGES - 1; s++) load_page(s, page0 + s);
+
+    // this thread's rows: r = 16 rt + 8 h + lane / 4
+    uint32_t qf[RT][KSTEPS][4];
+    int row_lo[RT][2], row_end[RT][2];                     // the row sees the keys [row_lo, row_end)
+    float* row_scores[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = rt * 16 + h * 8 + (lane >> 2);
+            const bool there = r < pairs;
+            const int i = there ? r / G : 0, head = g * G + (there ? r - i * G : 0);
+            row_lo[rt][h] = hb_oldest_visible(p0 + i, window, 0);
+            row_end[rt][h] = there ? p0 + i + 1 : 0;
+            row_scores[rt][h] = scores + ((size_t)(t0 + i) * nh + head) * score_ld;
+            const unsigned int* src = reinterpret_cast<const unsigned int*>(q + (size_t)(t0 + i) * q_stride + (size_t)head * HD + (lane & 3) * 2);
+#pragma unroll
+            for (int ks = 0; ks < KSTEPS; ks++) {
+                qf[rt][ks][h] = there ? __ldcg(src + ks * 8) : 0u;
+                qf[rt][ks][h + 2] = there ? __ldcg(src + ks * 8 + 4) : 0u;
+            }
+        }
+    float o[RT][HD / 8][4], m[RT][2], l[RT][2];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+        for (int i = 0; i < HD / 8; i++) o[rt][i][0] = o[rt][i][1] = o[rt][i][2] = o[rt][i][3] = 0.0f;
+        m[rt][0] = m[rt][1] = -INFINITY;
+        l[rt][0] = l[rt][1] = 0.0f;
+    }
+    for (int pi = page0; pi < page1; pi++) {
+        const int it = pi - page0;
+        cp_async_wait<FT_STAGES - 2>();
+        __syncthreads();
+        load_page((it + FT_STAGES - 1) % FT_STAGES, pi + FT_STAGES - 1);
+        const uint32_t kt = smem_base + (it % FT_STAGES) * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
+        float s[RT][2][4];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+            for (int nt = 0; nt < 2; nt++) s[rt][nt][0] = s[rt][nt][1] = s[rt][nt][2] = s[rt][nt][3] = 0.0f;
+        const int key_row = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
+#pragma unroll
+        for (int ks = 0; ks < KSTEPS; ks++) {
+            uint32_t kf[4];
+            ldmatrix_x4(kf, kt + swizzled<ROW_BYTES>(key_row, 2 * ks + ((lane >> 3) & 1)));
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                mma_bf16_16816(s[rt][0], qf[rt][ks], kf[0], kf[1]);
+                mma_bf16_16816(s[rt][1], qf[rt][ks], kf[2], kf[3]);
+            }
+        }
+        const int key0 = pi * HB_PAGE_TOKENS + warp * 16 + (lane & 3) * 2;
+        uint32_t pa[RT][4];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                float top = -INFINITY;
+#pragma unroll
+                for (int nt = 0; nt < 2; nt++) {
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int key = key0 + nt * 8 + e;
+                        const float v = key >= row_lo[rt][h] && key < row_end[rt][h] ? s[rt][nt][2 * h + e] * scale_log2e : -INFINITY;
+                        s[rt][nt][2 * h + e] = v;
+                        top = fmaxf(top, v);
+                    }
+                    if (row_end[rt][h] > 0)
+                        *reinterpret_cast<float2*>(row_scores[rt][h] + key0 + nt * 8) = make_float2(s[rt][nt][2 * h], s[rt][nt][2 * h + 1]);
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float m_new = fmaxf(m[rt][h], top), m_safe = m_new == -INFINITY ? 0.0f : m_new;
+                const float corr = exp2f(m[rt][h] - m_safe);
+                m[rt][h] = m_new;
+                float sum = 0.0f;
+#pragma unroll
+                for (int nt = 0; nt < 2; nt++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const float w = exp2f(s[rt][nt][2 * h + e] - m_safe);
+                        s[rt][nt][2 * h + e] = w;
+                        sum += w;
+                    }
+                l[rt][h] = l[rt][h] * corr + sum;
+                if (__any_sync(0xffffffffu, corr != 1.0f)) {       // a maximum grew: rarely, after the first pages
+#pragma unroll
+                    for (int i = 0; i < HD / 8; i++) {
+                        o[rt][i][2 * h] *= corr;
+                        o[rt][i][2 * h + 1] *= corr;
+                    }
+                }
+            }
+            pa[rt][0] = pack_bf16(s[rt][0][0], s[rt][0][1]);
+            pa[rt][1] = pack_bf16(s[rt][0][2], s[rt][0][3]);
+            pa[rt][2] = pack_bf16(s[rt][1][0], s[rt][1][1]);
+            pa[rt][3] = pack_bf16(s[rt][1][2], s[rt][1][3]);
+        }
+        const int v_row = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
+#pragma unroll
+        for (int dn = 0; dn < HD / 16; dn++) {
+            uint32_t vf[4];
+            ldmatrix_x4_trans(vf, vt + swizzled<ROW_BYTES>(v_row, 2 * dn + (lane >> 4)));
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                mma_bf16_16816(o[rt][2 * dn], pa[rt], vf[0], vf[1]);
+                mma_bf16_16816(o[rt][2 * dn + 1], pa[rt], vf[2], vf[3]);
+            }
+        }
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    if (bad_page && tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + b);
+
+    float* so = reinterpret_cast<float*>(smem);                        // [4 warps][ROWS][HD]
+    float* sm = so + 4 * ROWS * HD;                                    // [4][ROWS]
+    float* sl = sm + 4 * ROWS;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int r = rt * 16 + h * 8 + (lane >> 2);
+            float sum = l[rt][h];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+            for (int i = 0; i < HD / 8; i++)
+                *reinterpret_cast<float2*>(so + (size_t)(warp * ROWS + r) * HD + i * 8 + (lane & 3) * 2) = make_float2(o[rt][i][2 * h], o[rt][i][2 * h + 1]);
+            if ((lane & 3) == 0) {
+                sm[warp * ROWS + r] = m[rt][h];
+                sl[warp * ROWS + r] = sum;
+            }
+        }
+    __syncthreads();
+    for (int idx = tid; idx < pairs * HD; idx += FT_THREADS) {
+        const int r = idx / HD, d = idx - r * HD, i = r / G;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w * ROWS + r]);
+        float acc = 0.0f, L = 0.0f;
+        if (M != -INFINITY) {
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float e = exp2f(sm[w * ROWS + r] - M);
+                acc += so[(size_t)(w * ROWS + r) * HD + d] * e;
+                L += sl[w * ROWS + r] * e;
+            }
+        }
+        const size_t base = ((size_t)(t0 + i) * nh + g * G + (r - i * G)) * S + z;
+        part_o[base * HD + d] = acc;
+        if (d == 0) {
+            part_ml[base * 2] = M;
+            part_ml[base * 2 + 1] = L;
+        }
+    }
+}
+
+template <int HD, int RT>
+static int launch_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
+                         const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks,
+                         int tokens_per_block, int n_seqs, int nh, int nkv, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+    constexpr int PIPE = FT_STAGES * 2 * HB_PAGE_TOKENS * HD * 2, MERGE = (4 * 16 * RT * HD + 2 * 4 * 16 * RT) * 4, SMEM = PIPE > MERGE ? PIPE : MERGE;
+    static bool done[HB_MAX_DEVICES] = {};
+    bool& set = done[hb_device_slot()];
+    if (!set) {
+        cudaError_t e = cudaFuncSetAttribute(few_tc_kernel<HD, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        if (e != cudaSuccess) return hb_fail("attention_mass: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
+        set = true;
+    }
+    cudaError_t e = hb_launch(few_tc_kernel<HD, RT>, dim3(splits, nkv, token_blocks), dim3(FT_THREADS), SMEM, s, (const bf16*)q, q_stride,
+                              (const bf16*)kc, (const bf16*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld,
+                              tokens_per_block, n_seqs, nh, nkv, scale * MASS_LOG2E, window, n_pages, status);
+    if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
+    return hb_check_launch("attention_mass (few tokens, tensor cores)");
+}
+
+extern "C" int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_dim, int max_new) {
+    if ((head_dim != 64 && head_dim != 128) || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 32 || max_new < 1) return 0;
+    const int G = n_heads / n_kv_heads, rows = G * max_new <= 16 ? 16 : 32;
+    return rows / G;
+}
+
+int attention_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
+                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks, int max_new,
+                     int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+    const int tokens = hb_attention_few_tc_tokens(nh, nkv, head_dim, max_new);
+    HB_REQUIRE(tokens > 0, "attention_mass: head size %d with %d heads over %d kv heads is not built for the tensor cores (64 or 128, groups up to 32)",
+               head_dim, nh, nkv);
+    HB_REQUIRE(q_stride % 2 == 0 && ((uintptr_t)q & 3) == 0 && (((uintptr_t)kc | (uintptr_t)vc) & 15) == 0,
+               "attention_mass: queries must be 4-byte and the cache 16-byte aligned");
+    HB_REQUIRE(token_blocks <= 65535, "attention_mass: too many tokens for one launch");
+    const bool two = nh / nkv * tokens > 16;
+#define HB_FT_LAUNCH(HD, RT)                                                                                                                  \
+    launch_few_tc<HD, RT>(q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, token_blocks, \
+                          tokens, n_seqs, nh, nkv, scale, window, n_pages, status, s)
+    if (head_dim == 128) return two ? HB_FT_LAUNCH(128, 2) : HB_FT_LAUNCH(128, 1);
+    return two ? HB_FT_LAUNCH(64, 2) : HB_FT_LAUNCH(64, 1);
+#undef HB_FT_LAUNCH
+}

@@ -580,14 +580,33 @@ few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict
     }
 }
 
-// The second half of a step of few tokens.  grid: (blocks of 256 keys + tokens of a sequence, kv heads, sequences).  A block of
-// keys first joins the log-sums of the sequence's tokens and heads from the shares' maxima and sums, then turns its keys'
-// scores into weights; the blocks behind them join a token's partial outputs.
+// maximum and sum of a (token, head) over its S shares; every lane of the warp gets them
+__device__ __forceinline__ void join_stats(const float* __restrict__ part_ml, size_t base, int S, int lane, float& M, float& L) {
+    M = -INFINITY;
+    L = 0.0f;
+    for (int z = lane; z < S; z += 32) {
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + base + z);
+        const float m = fmaxf(M, ml.x);
+        if (m != -INFINITY) L = L * exp2f(M - m) + ml.y * exp2f(ml.x - m);
+        M = m;
+    }
+    const float top = warp_max(M);
+    L = warp_sum(M != -INFINITY ? L * exp2f(M - top) : 0.0f);
+    M = top;
+}
+
+// The second half of a step of few tokens.  grid: (tokens of a sequence + blocks of FF_KEYS keys, kv heads, sequences).  The first blocks
+// join a token's partial outputs; a block of keys joins the log-sums of the sequence's tokens and heads from the shares' maxima
+// and sums, then turns its keys' scores into weights, four keys a thread.  (With 256 keys to a block the log-sums' round trips took most of the time:
+// 55 us for two sequences of 100000 and 65538 rows.)
+#define FF_THREADS 256
+#define FF_KEYS 1024
+
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(FF_THREADS)
 few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const float* __restrict__ scores, long long score_ld,
                   const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, T* __restrict__ out,
-                  long long out_stride, MassOut mo, int key_blocks, int nh, int nkv, int hd, int S, int window, int n_pages) {
+                  long long out_stride, MassOut mo, int token_rows, int nh, int nkv, int hd, int S, int window, int n_pages, int vec) {
     __shared__ float lse[MASS_FEW_PAIRS];
     pdl_trigger();
     pdl_wait();
@@ -596,59 +615,72 @@ few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
     scores = pdl_fresh(scores);
     const int g = blockIdx.y, b = blockIdx.z, G = nh / nkv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int t0 = seq_start[b], n_new = seq_start[b + 1] - t0, pos0 = seq_pos0[b];
-    if ((int)blockIdx.x >= key_blocks) {
-        const int i = blockIdx.x - key_blocks;
+    if ((int)blockIdx.x < token_rows) {
+        const int i = blockIdx.x;
         if (i >= n_new) return;
         const int t = t0 + i;
-        for (int h = warp; h < G; h += 8) {
+        for (int h = warp; h < G; h += FF_THREADS / 32) {
             const size_t base = ((size_t)t * nh + g * G + h) * S;
-            float M = -INFINITY;
-            for (int z = lane; z < S; z += 32) M = fmaxf(M, __ldcg(part_ml + (base + z) * 2));
-            M = warp_max(M);
-            float L = 0.0f;
-            for (int z = lane; z < S; z += 32) {
-                const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + base + z);
-                if (ml.x != -INFINITY) L += ml.y * exp2f(ml.x - M);
-            }
-            L = warp_sum(L);
+            float M, L;
+            join_stats(part_ml, base, S, lane, M, L);
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-            for (int d = lane; d < hd; d += 32) {
-                float acc = 0.0f;
+            for (int d0 = 0; d0 < hd; d0 += 128) {             // four columns a lane, all shares' loads in flight
+                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
                 for (int z = 0; z < S; z++) {
                     const float mz = __ldcg(part_ml + (base + z) * 2);
-                    if (mz != -INFINITY) acc += __ldcg(part_o + (base + z) * hd + d) * exp2f(mz - M);
+                    const float w = mz != -INFINITY ? exp2f(mz - M) : 0.0f;
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const int d = d0 + u * 32 + lane;
+                        const float x = d < hd ? __ldcg(part_o + (base + z) * hd + d) : 0.0f;
+                        if (w != 0.0f) acc[u] = fmaf(x, w, acc[u]);          // a share without keys has written no output
+                    }
                 }
-                out[(size_t)t * out_stride + (size_t)(g * G + h) * hd + d] = from_f32<T>(acc * inv);
+#pragma unroll
+                for (int u = 0; u < 4; u++) {
+                    const int d = d0 + u * 32 + lane;
+                    if (d < hd) out[(size_t)t * out_stride + (size_t)(g * G + h) * hd + d] = from_f32<T>(acc[u] * inv);
+                }
             }
         }
         return;
     }
-    const int n = pos0 + n_new;
-    if ((int)blockIdx.x * 256 >= n) return;
-    for (int i = warp; i < n_new * G; i += 8) {
-        const size_t base = ((size_t)(t0 + i / G) * nh + g * G + i % G) * S;
-        float M = -INFINITY, L = 0.0f;
-        for (int z = lane; z < S; z += 32) M = fmaxf(M, __ldcg(part_ml + (base + z) * 2));
-        M = warp_max(M);
-        for (int z = lane; z < S; z += 32) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_ml) + base + z);
-            if (ml.x != -INFINITY) L += ml.y * exp2f(ml.x - M);
-        }
-        L = warp_sum(L);
+    const int n = (int)min((long long)(pos0 + n_new), score_ld), key0 = ((int)blockIdx.x - token_rows) * FF_KEYS;
+    if (key0 >= n) return;
+    for (int i = warp; i < n_new * G; i += FF_THREADS / 32) {
+        float M, L;
+        join_stats(part_ml, ((size_t)(t0 + i / G) * nh + g * G + i % G) * S, S, lane, M, L);
         if (lane == 0) lse[i] = L > 0.0f ? M + log2f(L) : INFINITY;
     }
     __syncthreads();
-    const int key = blockIdx.x * 256 + tid;
-    if (key >= n || key >= score_ld) return;
-    float s = 0.0f;
+    const int key = key0 + tid * 4;                            // this thread's four keys, on one page
+    if (key >= n) return;
+    float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int i = 0; i < n_new; i++) {
-        const int p = pos0 + i;
-        if (key > p || key < hb_oldest_visible(p, window, 0)) continue;
-        for (int h = 0; h < G; h++) s += exp2f(__ldcg(scores + ((size_t)(t0 + i) * nh + g * G + h) * score_ld + key) - lse[i * G + h]);
+        const int p = pos0 + i, lo = hb_oldest_visible(p, window, 0);
+        if (key > p || key + 3 < lo) continue;
+        const float* row = scores + ((size_t)(t0 + i) * nh + g * G) * score_ld + key;
+#pragma unroll 4
+        for (int h = 0; h < G; h++) {
+            const float4 x = __ldcg(reinterpret_cast<const float4*>(row + h * score_ld));
+            const float e = lse[i * G + h];
+            s[0] += key >= lo ? exp2f(x.x - e) : 0.0f;
+            s[1] += key + 1 >= lo && key + 1 <= p ? exp2f(x.y - e) : 0.0f;
+            s[2] += key + 2 >= lo && key + 2 <= p ? exp2f(x.z - e) : 0.0f;
+            s[3] += key + 3 >= lo && key + 3 <= p ? exp2f(x.w - e) : 0.0f;
+        }
     }
     const int pi = key / HB_PAGE_TOKENS;
     const int page = pi < pt_width ? page_table[(size_t)b * pt_width + pi] : -1;
-    mass_write(mo, s, g, key, page, nkv, n_pages, pos0, n_new);
+    if (vec && key + 3 < pos0 && page >= 0 && page < n_pages) {
+        const size_t at = ((size_t)page * nkv + g) * HB_PAGE_TOKENS + (key & (HB_PAGE_TOKENS - 1));
+        const float4 old = mo.before != nullptr ? __ldcg(reinterpret_cast<const float4*>(mo.before + at)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        *reinterpret_cast<float4*>(mo.mass + at) = make_float4(old.x + s[0], old.y + s[1], old.z + s[2], old.w + s[3]);
+    } else {
+#pragma unroll
+        for (int u = 0; u < 4; u++) mass_write(mo, s[u], g, key + u, page, nkv, n_pages, pos0, n_new);
+    }
 }
 
 extern "C" int hb_attention_few_pairs(void) { return MASS_FEW_PAIRS; }
@@ -676,20 +708,21 @@ template <typename T>
 static int launch_finish(const float* part_o, const float* part_ml, const float* scores, long long score_ld, const int* page_table, int pt_width,
                          const int* seq_start, const int* seq_pos0, void* out, long long out_stride, MassOut mo, int max_len, int max_new, int n_seqs,
                          int nh, int nkv, int hd, int splits, int window, int n_pages, cudaStream_t s) {
-    const int key_blocks = (max_len + 255) / 256;
-    cudaError_t e = hb_launch(few_finish_kernel<T>, dim3(key_blocks + max_new, nkv, n_seqs), dim3(256), 0, s, part_o, part_ml, scores, score_ld,
-                              page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, mo, key_blocks, nh, nkv, hd, splits, window, n_pages);
+    const int key_blocks = (max_len + FF_KEYS - 1) / FF_KEYS;
+    const int vec = (((uintptr_t)mo.before | (uintptr_t)mo.mass) & 15) == 0;
+    cudaError_t e = hb_launch(few_finish_kernel<T>, dim3(max_new + key_blocks, nkv, n_seqs), dim3(FF_THREADS), 0, s, part_o, part_ml, scores, score_ld,
+                              page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, mo, max_new, nh, nkv, hd, splits, window, n_pages, vec);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (finish)");
 }
 
 // Steps of few tokens (at most hb_attention_few_pairs() pairs of a sequence's tokens and a group's heads).  `scratch` holds
-// hb_attention_mass_few_floats floats; tensor_cores: sizes of hb_attention_decode; max_len bounds the rows of every sequence, max_new their new tokens.
+// hb_attention_mass_few_floats floats; token_blocks: 0, or for the tensor cores as attention_few_tc; max_len bounds the rows of every sequence, max_new their new tokens.
 extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
                                      int pt_width, const int* tok_seq, const int* positions, const int* seq_start, const int* seq_pos0, void* out,
                                      long long out_stride, float* scratch, const float* before, float* mass, int splits, int n_tokens, int n_seqs,
                                      int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages,
-                                     int tensor_cores, int* status, void* stream) {
+                                     int token_blocks, int* status, void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0 && head_dim <= 256 && n_pages > 0 && pt_width > 0,
                "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, head_dim);
@@ -698,19 +731,16 @@ extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_strid
     HB_REQUIRE(n_tokens <= 65535 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && max_len >= 1 && scratch != nullptr && mass != nullptr,
                "attention_mass: bad sizes");
     const size_t rows = (size_t)n_tokens * n_heads * splits;
-    float *part_ml = scratch, *part_o = part_ml + rows * 2, *scores = part_o + rows * head_dim;
     const long long score_ld = mass_score_ld(max_len);
-    HB_REQUIRE(((uintptr_t)scratch & 7) == 0, "attention_mass: scratch must be 8-byte aligned");
+    float *scores = scratch, *part_ml = scores + (size_t)n_tokens * n_heads * score_ld, *part_o = part_ml + rows * 2;
+    HB_REQUIRE(((uintptr_t)scratch & 15) == 0, "attention_mass: scratch must be 16-byte aligned");
     cudaStream_t s = (cudaStream_t)stream;
     MassOut mo = {before, mass, nullptr};
     int rc;
-    if (tensor_cores) {
-        HB_REQUIRE(dtype == HB_BF16 && hb_attention_decode_supported(n_heads, n_kv_heads, head_dim) && q_stride % 2 == 0 && ((uintptr_t)q & 3) == 0 &&
-                       (((uintptr_t)k_cache | (uintptr_t)v_cache) & 15) == 0,
-                   "attention_mass: a head size of %d with %d heads over %d kv heads is not built for the tensor cores, or is not aligned", head_dim, n_heads,
-                   n_kv_heads);
-        rc = attention_decode_scores(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits,
-                                     n_tokens, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
+    if (token_blocks > 0) {
+        HB_REQUIRE(dtype == HB_BF16, "attention_mass: the tensor cores take bfloat16");
+        rc = attention_few_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits,
+                              token_blocks, max_new, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     } else if (dtype == HB_F32)
         rc = launch_few<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits,
                                n_tokens, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);

@@ -100,12 +100,6 @@ __device__ __forceinline__ void load4(const bf16* p, float (&x)[4]) {
 int mass_join(const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0, MassOut mo, int n_seqs, int nkv, int n_pages, int tile,
               int key_tiles, int splits, cudaStream_t s);
 
-// The first half of a step of few tokens on the tensor cores (attention_decode.cu): sizes of hb_attention_decode, queries 4-byte and
-// keys and values 16-byte aligned.
-int attention_decode_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* tok_seq,
-                            const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int n_tokens, int nh,
-                            int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);
-
 // The keys of a block of queries, shared out: a block that sees n tiles of keys takes ceil(n / tiles) CTAs, and where those are several each
 // leaves its unnormalised outputs and (maximum, sum) of its rows: o[(share * heads + head) * tokens + token][head size], ml likewise.
 struct Shares {
@@ -135,17 +129,8 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
                        int max_shares, int share_tiles, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale,
                        int window, int n_pages, int* error_flag, cudaStream_t s);
 
-// The first half of a step of few tokens on the tensor cores (attention_decode.cu): sizes of hb_attention_decode, queries 4-byte and
-// keys and values 16-byte aligned.
-int attention_decode_scores(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* tok_seq,
-                            const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int n_tokens, int nh,
-                            int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);
-
-// The first half of a step of many tokens on the tensor cores (attention_chunk_tc.cu): writes out and the rows'
-// log-sums, lse[head][place]: a sequence's places begin at a multiple of 128, behind those of the sequences in front.  q_blocks: sum
-// over sequences of ceil(new tokens / span), span 128 with an even group of heads and 256 with an odd one; parts: splits * n_heads *
-// n_tokens * (head_dim + 2) floats when splits > 1 (at most 32).
-int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
-                       const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts, int splits,
-                       int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
-                       cudaStream_t s);
+// The first half of a step of few tokens on the tensor cores (attention_few_tc.cu): token_blocks, the sum over sequences of ceil(new
+// tokens / hb_attention_few_tc_tokens(...)); queries 4-byte, keys and values 16-byte aligned.
+int attention_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
+                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks, int max_new,
+                     int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);

@@ -188,6 +188,7 @@ def load_library():
         for name in ("hb_attention_decode_supported", "hb_attention_prefill_supported", "hb_attention_prefill_tc_supported"):
             getattr(lib, name).argtypes, getattr(lib, name).restype = [_c_int, _c_int, _c_int], _c_int
         lib.hb_attention_mass_tc_keys.argtypes, lib.hb_attention_mass_tc_keys.restype = [], _c_int
+        lib.hb_attention_few_tc_tokens.argtypes, lib.hb_attention_few_tc_tokens.restype = [_c_int] * 4, _c_int
         lib.hb_attention_few_pairs.argtypes, lib.hb_attention_few_pairs.restype = [], _c_int
         lib.hb_attention_mass_few_floats.argtypes, lib.hb_attention_mass_few_floats.restype = [_c_int] * 5, _c_ll
         lib.hb_attention_sink_prefill_supported.argtypes, lib.hb_attention_sink_prefill_supported.restype = [_c_int] * 4, _c_int
@@ -1284,17 +1285,24 @@ class Ops:
         with torch.cuda.device(self.device):
             if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * group <= self.lib.hb_attention_few_pairs():
                 max_pages = (step.max_len + 63) // 64
-                tc = (self.use_fast_attention and qkv.dtype == torch.bfloat16 and self.lib.hb_attention_decode_supported(heads, kv_heads, head_dim)
-                      and q_ld % 2 == 0 and qkv.data_ptr() % 4 == 0 and cache.k.data_ptr() % 16 == 0 and cache.v.data_ptr() % 16 == 0)
+                at_once = 0                 # tokens that a block of the tensor-core kernel takes; 0: the general kernel, one
+                if self.use_fast_attention and qkv.dtype == torch.bfloat16 and q_ld % 2 == 0 and qkv.data_ptr() % 4 == 0 \
+                        and cache.k.data_ptr() % 16 == 0 and cache.v.data_ptr() % 16 == 0:
+                    at_once = self.lib.hb_attention_few_tc_tokens(heads, kv_heads, head_dim, step.max_new)
+                blocks = 0 if not at_once else step.num_seqs if step.max_new == 1 else sum(-(-n // at_once) for n in step.host_new)
                 if splits is None:
-                    splits = few_splits(T, kv_heads if tc else kv_heads * -(-group // 8), max_pages, (2 if tc else 3) * self.sm_count)
+                    # (single tokens: from the page table's width alone, so that a captured step and an eager one sum alike)
+                    lens = [step.max_len] * step.num_seqs if step.max_new == 1 else step.host_len
+                    each = at_once or 1
+                    seen = [-(-(min(ln, win + n) if win else ln) // 64) for ln, n in zip(lens, step.host_new) for _ in range(-(-n // each))]
+                    splits = few_splits(seen, kv_heads if at_once else kv_heads * -(-group // 8), (2 if at_once else 3) * self.sm_count)
                 splits = max(1, min(splits, max_pages))
                 scratch = torch.empty(self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len), dtype=torch.float32,
                                       device=self.device)
                 self._call("hb_attention_mass_few", qkv.data_ptr(), code, q_ld, cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(),
                            pt.shape[1], step.tok_seq.data_ptr(), step.positions.data_ptr(), step.seq_start.data_ptr(),
                            step.seq_pos0.data_ptr(), out.data_ptr(), out_ld, scratch.data_ptr(), old, mass.data_ptr(), splits, T, step.num_seqs,
-                           step.max_new, step.max_len, heads, kv_heads, head_dim, float(scale), win, pages, 1 if tc else 0, self.status.data_ptr(),
+                           step.max_new, step.max_len, heads, kv_heads, head_dim, float(scale), win, pages, blocks, self.status.data_ptr(),
                            self._stream())
                 self.launches += 2
                 return

@@ -163,6 +163,10 @@ FEW = [
     (5, 5, 33, [200, 0], [4, 2], None),
     (2, 1, 256, [513], [1], 4096),
     (2, 2, 200, [100, 5000], [1, 2], 70),
+    (32, 1, 128, [500, 64], [1, 1], None),
+    (33, 1, 64, [500], [1], None),
+    (6, 2, 128, [2000, 0, 61, 63], [8, 7, 6, 1], 50),
+    (12, 1, 64, [130, 1000], [3, 8], None),
 ]
 TYPES = [torch.bfloat16, torch.float32]
 
@@ -537,7 +541,8 @@ def test_evict_rows_refuses(change, text):
 
 def test_shapes_of_the_launches():
     from hilbert_pruned_8b_b200.kernels.plan import chunk_shares, few_splits, mass_splits, select_shape
-    assert few_splits(1, 8, 5, 296) == 5 and few_splits(8, 8, 129, 296) == 4 and few_splits(1000, 8, 100, 296) == 1
+    assert few_splits([5], 8, 296) == 5 and few_splits([129] * 8, 8, 296) == 4 and few_splits([100] * 1000, 8, 296) == 1
+    assert few_splits([33, 126, 9, 65], 8, 296) == 18 and few_splits([], 8, 296) == 1 and few_splits([1], 1, 296) == 1
     assert mass_splits(1000, 8, 100, 296) == 1 and mass_splits(1, 1, 1, 296) == 1 and mass_splits(1, 1, 100, 296) == 16
     assert chunk_shares([4096], [4096], 0, 128, 128, 16, 4160, 148) == (1, 32)                 # enough blocks for everybody
     shares, tiles = chunk_shares([128], [100000], 0, 128, 128, 16, 4160, 148)                  # 16 blocks of 782 tiles
