@@ -368,6 +368,9 @@ class Ops:
         self.sm_count = sms.value
         if major.value != 10:
             raise KernelError(f"the kernels are built for sm_100a; device {idx} is sm_{major.value}{minor.value}")
+        self._index = idx
+        self._mass_plans = {}                                    # how steps of attention_mass are cut, by their sizes
+        self.MASS_FEW_PAIRS = self.lib.hb_attention_few_pairs()   # (tokens of a sequence) x (heads of a group) of a step of few tokens
         self.launches = 0  # kernels launched through this object (a claim bench.py reports)
         self.use_tensor_cores = True   # tests switch this off to compare the two matrix-product kernels
         self.use_pair_gemm = True      # many-token products on CTA pairs (cta_group::2)
@@ -1242,12 +1245,64 @@ class Ops:
 
     # ------------------------------------------------------------------ a bounded cache
     MASS_FEW_TOKENS = 8             # a step whose sequences bring more tokens than this takes the kernels for many tokens
+    MASS_PLANS = 512                # plans kept: steps of the same sizes are cut alike
+
+    def _on(self, *tensors) -> None:
+        for t in tensors:
+            if t is not None and t.get_device() != self._index:
+                raise KernelError(f"tensor on {t.device}, kernels bound to {self.device}")
+
+    def _elsewhere(self) -> bool:
+        """Whether another device than this object's is the current one (a launch has to be made with its own current)."""
+        return torch.cuda.current_device() != self._index
 
     @staticmethod
-    def _mass_like(t, what: str, pages: int, kv_heads: int) -> None:
-        if t.dtype != torch.float32 or tuple(t.shape) != (pages, kv_heads, 64) or not t.is_contiguous():
-            raise KernelError(f"attention: {what} must be a contiguous float32 [{pages}, {kv_heads}, 64] (pages, kv heads, rows of a "
-                              f"page), got {t.dtype} {tuple(t.shape)}")
+    def _mass_like(t, what: str, want) -> None:
+        if t.dtype != torch.float32 or t.shape != want or not t.is_contiguous():
+            raise KernelError(f"attention: {what} must be a contiguous float32 {list(want)} (pages, kv heads, rows of a page), got {t.dtype} "
+                              f"{tuple(t.shape)}")
+
+    def _mass_plan(self, few: bool, tc: bool, heads: int, kv_heads: int, head_dim: int, win: int, step, splits: Optional[int]):
+        """How a step of ``attention_mass`` is cut, from its sizes alone: few tokens: (blocks of tokens for the tensor cores or 0, shares of
+        the pages, floats of scratch); many: (shares of the keys' sums, blocks of queries, tiles of keys, most shares of a block of
+        queries, tiles of keys in one, distance of two heads' log-sums, floats of the log-sums, of the sums' shares, of the partial results)."""
+        T, group = step.num_tokens, heads // kv_heads
+        # (single tokens: from the page table's width alone, so that a captured step and an eager one sum alike)
+        single = step.max_new == 1 and few
+        key = (few, tc, heads, kv_heads, head_dim, win, splits, T, step.num_seqs, step.max_len, step.max_new,
+               None if single else (tuple(step.host_new), tuple(step.host_len)))
+        plan = self._mass_plans.get(key)
+        if plan is not None:
+            return plan
+        if few:
+            at_once = self.lib.hb_attention_few_tc_tokens(heads, kv_heads, head_dim, step.max_new) if tc else 0
+            blocks = 0 if not at_once else step.num_seqs if single else sum(-(-n // at_once) for n in step.host_new)
+            if splits is None:
+                seqs = [(1, step.max_len)] * step.num_seqs if single else zip(step.host_new, step.host_len)
+                seen = [-(-(min(ln, win + n) if win else ln) // 64) for n, ln in seqs for _ in range(-(-n // (at_once or 1)))]
+                splits = few_splits(seen, kv_heads if at_once else kv_heads * -(-group // 8), (2 if at_once else 3) * self.sm_count)
+            splits = max(1, min(splits, (step.max_len + 63) // 64))
+            plan = (blocks, splits, self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len))
+        else:
+            # the tensor cores take two tiles of 128 queries at a time: two heads, or with an odd group two blocks of tokens
+            rows, keys = (128 if group % 2 == 0 else 256, self.lib.hb_attention_mass_tc_keys()) if tc else (64, 64)
+            q_blocks = sum(-(-n // rows) for n in step.host_new)
+            key_tiles = sum(-(-n // keys) for n in step.host_len)
+            if splits is None:
+                splits = mass_splits(key_tiles, kv_heads, group * -(-step.max_new // (128 if tc else 64)), self.sm_count * (1 if tc else 2))
+            shares, tiles = chunk_shares(step.host_new, step.host_len, win, rows, 128 if tc else 64, heads // 2 if tc and group % 2 == 0 else heads,
+                                         heads * (head_dim + 2), self.sm_count * (1 if tc or head_dim > 64 else 2))
+            lse_ld = 128 * sum(-(-n // 128) for n in step.host_new) if tc else T
+
+            def round128(n: int) -> int:
+                return (n + 127) & ~127
+            plan = (splits, q_blocks, key_tiles, shares, tiles, lse_ld, round128(heads * lse_ld),
+                    round128(splits * kv_heads * key_tiles * keys) if splits > 1 else 0,
+                    shares * heads * T * (head_dim + 2) if shares > 1 else 0)
+        if len(self._mass_plans) >= self.MASS_PLANS:
+            self._mass_plans.clear()
+        self._mass_plans[key] = plan
+        return plan
 
     def attention_mass(self, qkv, heads: int, kv_heads: int, head_dim: int, cache, step, out, scale: float, window: Optional[int], mass,
                        before=None, splits: Optional[int] = None) -> None:
@@ -1257,82 +1312,57 @@ class Ops:
         there.  ``before``: None (this step's weights alone), another tensor, or ``mass`` itself (a running sum).  Rows that no
         sequence of the step holds are neither read nor written.  The step's new keys and values are in the cache already, as for
         ``attention``; queries, cache and output have one type.  The sums do not depend on what else runs (fixed order)."""
-        self._dev(qkv, cache.k, cache.v, out, mass, before)
-        T = qkv.shape[0]
-        pt = step.page_tables[cache.group]
-        pages = cache.k.shape[0]
-        if kv_heads < 1 or heads % kv_heads or not 0 < head_dim <= 256:
+        k, v = cache.k, cache.v
+        self._on(qkv, k, v, out, mass, before)
+        T, pages = qkv.shape[0], k.shape[0]
+        if kv_heads < 1 or heads < 1 or heads % kv_heads or not 0 < head_dim <= 256:
             raise KernelError(f"attention: {heads} heads over {kv_heads} kv heads of size {head_dim} are not built (sizes up to 256)")
-        if qkv.shape[1] < heads * head_dim or out.shape[0] != T or out.shape[1] != heads * head_dim or T != step.num_tokens:
+        if qkv.shape[1] < heads * head_dim or out.shape != (T, heads * head_dim) or T != step.num_tokens:
             raise KernelError("attention: query or output shape does not match")
         want = (pages, kv_heads, 64, head_dim)
-        if tuple(cache.k.shape) != want or tuple(cache.v.shape) != want or not cache.k.is_contiguous() or not cache.v.is_contiguous():
+        if k.shape != want or v.shape != want or not k.is_contiguous() or not v.is_contiguous():
             raise KernelError("attention: cache layer shape does not match the heads")
-        if not qkv.dtype == cache.k.dtype == cache.v.dtype == out.dtype:
+        dtype = qkv.dtype
+        if not dtype == k.dtype == v.dtype == out.dtype:
             raise KernelError("attention: queries, cache and output must have one dtype")
-        self._mass_like(mass, "mass", pages, kv_heads)
+        self._mass_like(mass, "mass", want[:3])
         if before is not None:
-            self._mass_like(before, "before", pages, kv_heads)
+            self._mass_like(before, "before", want[:3])
         if not 0.0 < scale < float("inf"):
             raise KernelError(f"attention: the scale must be positive and finite, got {scale}")
         if T == 0:
             return
-        win = int(window) if window else 0
-        old = before.data_ptr() if before is not None else None
-        code, group = _code(qkv), heads // kv_heads
-        q_ld, out_ld = _rows(qkv, "attention queries"), _rows(out, "attention output")
+        if self._elsewhere():
+            with torch.cuda.device(self._index):
+                return self.attention_mass(qkv, heads, kv_heads, head_dim, cache, step, out, scale, window, mass, before, splits)
+        pt, win = step.page_tables[cache.group], int(window) if window else 0
+        code, q_ld, out_ld = _code(qkv), _rows(qkv, "attention queries"), _rows(out, "attention output")
+        q_at, k_at, v_at, out_at = qkv.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
+        fast = self.use_fast_attention and dtype == torch.bfloat16 and (k_at | v_at) % 16 == 0
+        old, new, status, stream = before.data_ptr() if before is not None else None, mass.data_ptr(), self.status.data_ptr(), self._stream()
         # scratch of the call's own, from torch's allocator: two calls on two streams, or two captured graphs, share nothing
-        with torch.cuda.device(self.device):
-            if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * group <= self.lib.hb_attention_few_pairs():
-                max_pages = (step.max_len + 63) // 64
-                at_once = 0                 # tokens that a block of the tensor-core kernel takes; 0: the general kernel, one
-                if self.use_fast_attention and qkv.dtype == torch.bfloat16 and q_ld % 2 == 0 and qkv.data_ptr() % 4 == 0 \
-                        and cache.k.data_ptr() % 16 == 0 and cache.v.data_ptr() % 16 == 0:
-                    at_once = self.lib.hb_attention_few_tc_tokens(heads, kv_heads, head_dim, step.max_new)
-                blocks = 0 if not at_once else step.num_seqs if step.max_new == 1 else sum(-(-n // at_once) for n in step.host_new)
-                if splits is None:
-                    # (single tokens: from the page table's width alone, so that a captured step and an eager one sum alike)
-                    lens = [step.max_len] * step.num_seqs if step.max_new == 1 else step.host_len
-                    each = at_once or 1
-                    seen = [-(-(min(ln, win + n) if win else ln) // 64) for ln, n in zip(lens, step.host_new) for _ in range(-(-n // each))]
-                    splits = few_splits(seen, kv_heads if at_once else kv_heads * -(-group // 8), (2 if at_once else 3) * self.sm_count)
-                splits = max(1, min(splits, max_pages))
-                scratch = torch.empty(self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len), dtype=torch.float32,
-                                      device=self.device)
-                self._call("hb_attention_mass_few", qkv.data_ptr(), code, q_ld, cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(),
-                           pt.shape[1], step.tok_seq.data_ptr(), step.positions.data_ptr(), step.seq_start.data_ptr(),
-                           step.seq_pos0.data_ptr(), out.data_ptr(), out_ld, scratch.data_ptr(), old, mass.data_ptr(), splits, T, step.num_seqs,
-                           step.max_new, step.max_len, heads, kv_heads, head_dim, float(scale), win, pages, blocks, self.status.data_ptr(),
-                           self._stream())
-                self.launches += 2
-                return
-            tc = (self.use_fast_attention and self.use_tcgen05_attention and qkv.dtype == torch.bfloat16
-                  and self.lib.hb_attention_prefill_tc_supported(heads, kv_heads, head_dim) and qkv.data_ptr() % 16 == 0 and out.data_ptr() % 16 == 0
-                  and cache.k.data_ptr() % 16 == 0 and cache.v.data_ptr() % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0)
-            # places of the log-sums; rows of a block of queries (two tiles of 128: two heads, or with an odd group two blocks of tokens), of a tile of keys
-            lse_ld = 128 * sum(-(-n // 128) for n in step.host_new) if tc else T
-            lse = torch.empty(heads * lse_ld, dtype=torch.float32, device=self.device)
-            rows, keys = (128 if group % 2 == 0 else 256, self.lib.hb_attention_mass_tc_keys()) if tc else (64, 64)
-            q_blocks = sum(-(-n // rows) for n in step.host_new)
-            key_tiles = sum(-(-n // keys) for n in step.host_len)
-            if splits is None:
-                splits = mass_splits(key_tiles, kv_heads, group * -(-step.max_new // (128 if tc else 64)), self.sm_count * (1 if tc else 2))
-            parts = torch.empty(splits * kv_heads * key_tiles * keys, dtype=torch.float32, device=self.device) if splits > 1 else None
-            sizes = (splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim, float(scale), win, pages, self.status.data_ptr(),
-                     self._stream())
-            buffers = (cache.k.data_ptr(), cache.v.data_ptr(), pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(),
-                       out.data_ptr(), out_ld, lse.data_ptr(), *((lse_ld,) if tc else ()), old, mass.data_ptr(),
-                       parts.data_ptr() if parts is not None else None)
-            shares, tiles = chunk_shares(step.host_new, step.host_len, win, rows, 128 if tc else 64, heads // 2 if tc and group % 2 == 0 else heads,
-                                         heads * (head_dim + 2), self.sm_count * (1 if tc or head_dim > 64 else 2))
-            partial = torch.empty(shares * heads * T * (head_dim + 2), dtype=torch.float32, device=self.device) if shares > 1 else None
-            cut = (partial.data_ptr() if partial is not None else None, shares, tiles)
-            if tc:
-                self._call("hb_attention_mass_tc", qkv.data_ptr(), q_ld, *buffers, *cut, *sizes)
-            else:
-                self._call("hb_attention_mass", qkv.data_ptr(), code, q_ld, *buffers, *cut, *sizes)
-            self.launches += 0 if shares == 1 else 1
-            self.launches += 2 if splits == 1 else 3
+        if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * (heads // kv_heads) <= self.MASS_FEW_PAIRS:
+            blocks, splits, floats = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, heads, kv_heads, head_dim, win, step, splits)
+            scratch = torch.empty(floats, dtype=torch.float32, device=self.device)
+            self._call("hb_attention_mass_few", q_at, code, q_ld, k_at, v_at, pt.data_ptr(), pt.shape[1], step.tok_seq.data_ptr(),
+                       step.positions.data_ptr(), step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out_at, out_ld, scratch.data_ptr(), old, new,
+                       splits, T, step.num_seqs, step.max_new, step.max_len, heads, kv_heads, head_dim, scale, win, pages, blocks, status, stream)
+            self.launches += 2
+            return
+        tc = bool(fast and self.use_tcgen05_attention and (q_at | out_at) % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0
+                  and self.lib.hb_attention_prefill_tc_supported(heads, kv_heads, head_dim))
+        splits, q_blocks, key_tiles, shares, tiles, lse_ld, n_lse, n_parts, n_cut = self._mass_plan(False, tc, heads, kv_heads, head_dim, win, step, splits)
+        scratch = torch.empty(n_lse + n_parts + n_cut, dtype=torch.float32, device=self.device)
+        lse = scratch.data_ptr()
+        parts, cut = lse + 4 * n_lse if n_parts else None, lse + 4 * (n_lse + n_parts) if n_cut else None
+        where = (k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out_at, out_ld, lse)
+        sizes = (old, new, parts, cut, shares, tiles, splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim, scale, win, pages, status,
+                 stream)
+        if tc:
+            self._call("hb_attention_mass_tc", q_at, q_ld, *where, lse_ld, *sizes)
+        else:
+            self._call("hb_attention_mass", q_at, code, q_ld, *where, *sizes)
+        self.launches += 2 + (splits > 1) + (shares > 1)
 
     def evict_select(self, mass, page_table, lengths, first: int, recent: int, kept) -> None:
         """Which rows of each sequence stay, for every entry and kv head by itself.  ``mass`` ``[entries, pages, kv_heads, 64]`` (or one
@@ -1340,25 +1370,28 @@ class Ops:
         int32 ``[entries, sequences, kv_heads, budget]`` (or without the first axis).  Of a sequence longer than the budget the first
         ``first`` rows stay, the last ``recent``, and of those between the ones with the largest mass until the budget is full; equal
         masses: the lower row; NaN counts below everything.  ``kept`` holds the rows in ascending order, -1 behind the last."""
-        self._dev(mass, page_table, lengths, kept)
-        entries = mass.shape[0] if mass.dim() == 4 else 1
-        if mass.dim() not in (3, 4) or mass.dtype != torch.float32 or mass.shape[-1] != 64 or not mass.is_contiguous():
+        self._on(mass, page_table, lengths, kept)
+        dims = mass.dim()
+        if dims not in (3, 4) or mass.dtype != torch.float32 or mass.shape[-1] != 64 or not mass.is_contiguous():
             raise KernelError(f"evict_select: mass must be a contiguous float32 [entries, pages, kv_heads, 64], got {mass.dtype} {tuple(mass.shape)}")
-        pages, kv_heads = mass.shape[-3], mass.shape[-2]
+        entries, pages, kv_heads = mass.shape[0] if dims == 4 else 1, mass.shape[-3], mass.shape[-2]
         self._tables("evict_select", page_table)
-        B = page_table.shape[0]
-        if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or not lengths.is_contiguous():
+        B, width = page_table.shape
+        if lengths.dtype != torch.int32 or lengths.shape != (B,) or not lengths.is_contiguous():
             raise KernelError("evict_select: one int32 length per row of the page table expected")
-        budget = self._kept("evict_select", kept, mass.dim(), entries, B, kv_heads)
+        budget = self._kept("evict_select", kept, dims, entries, B, kv_heads)
         first, recent = int(first), int(recent)
         if first < 0 or recent < 0 or first + recent > budget:
             raise KernelError(f"evict_select: the first {first} and the last {recent} rows do not fit a budget of {budget}")
-        if not entries * B * kv_heads:
+        lists = entries * B * kv_heads
+        if not lists:
             return
-        threads, cluster = select_shape(entries * B * kv_heads, page_table.shape[1] * 64, self.sm_count)
-        with torch.cuda.device(self.device):
-            self._call("hb_evict_select", mass.data_ptr(), page_table.data_ptr(), page_table.shape[1], lengths.data_ptr(), kept.data_ptr(), entries,
-                       B, kv_heads, pages, first, recent, budget, threads, cluster, self.status.data_ptr(), self._stream())
+        if self._elsewhere():
+            with torch.cuda.device(self._index):
+                return self.evict_select(mass, page_table, lengths, first, recent, kept)
+        threads, cluster = select_shape(lists, width * 64, self.sm_count)
+        self._call("hb_evict_select", mass.data_ptr(), page_table.data_ptr(), width, lengths.data_ptr(), kept.data_ptr(), entries, B, kv_heads, pages,
+                   first, recent, budget, threads, cluster, self.status.data_ptr(), self._stream())
         self.launches += 1
 
     @staticmethod
@@ -1369,7 +1402,7 @@ class Ops:
     @staticmethod
     def _kept(op: str, kept, dims: int, entries: int, sequences: int, kv_heads: int) -> int:
         want = (entries, sequences, kv_heads)[4 - dims:]
-        if kept.dtype != torch.int32 or kept.dim() != dims or tuple(kept.shape[:-1]) != want or kept.shape[-1] < 1 or not kept.is_contiguous():
+        if kept.dtype != torch.int32 or kept.dim() != dims or kept.shape[:-1] != want or kept.shape[-1] < 1 or not kept.is_contiguous():
             raise KernelError(f"{op}: kept must be a contiguous int32 [{', '.join(map(str, want))}, budget], got {kept.dtype} {tuple(kept.shape)}")
         return kept.shape[-1]
 
@@ -1379,32 +1412,34 @@ class Ops:
         the rows of ``page_table`` then stay as they were.  ``k``, ``v`` ``[entries, pages, kv_heads, 64, head size]``, ``mass`` (may be None)
         ``[entries, pages, kv_heads, 64]``, or all without the first axis.  ``kept`` as ``evict_select`` gives it: ascending, -1 behind
         the last; rows behind what is kept stay as they were."""
-        self._dev(kept, k, v, mass, page_table, to_table)
-        if k.dim() not in (4, 5) or v.dim() != k.dim() or v.shape[:-1] != k.shape[:-1] or k.shape[-2] != 64 or k.dtype != v.dtype \
+        self._on(kept, k, v, mass, page_table, to_table)
+        dims = k.dim()
+        if dims not in (4, 5) or v.dim() != dims or v.shape[:-1] != k.shape[:-1] or k.shape[-2] != 64 or k.dtype != v.dtype \
                 or not k.is_contiguous() or not v.is_contiguous():
             raise KernelError("evict_rows: keys and values must be contiguous [entries, pages, kv_heads, 64, head size] of one dtype")
         _code(k)
         if mass is not None and (mass.dtype != torch.float32 or mass.shape != k.shape[:-1] or not mass.is_contiguous()):
             raise KernelError(f"evict_rows: mass must be a contiguous float32 {list(k.shape[:-1])}, got {mass.dtype} {tuple(mass.shape)}")
-        entries = k.shape[0] if k.dim() == 5 else 1
-        pages, kv_heads = k.shape[-4], k.shape[-3]
+        entries, pages, kv_heads = k.shape[0] if dims == 5 else 1, k.shape[-4], k.shape[-3]
         self._tables("evict_rows", page_table)
         B = page_table.shape[0]
-        budget = self._kept("evict_rows", kept, k.dim() - 1, entries, B, kv_heads)
+        budget = self._kept("evict_rows", kept, dims - 1, entries, B, kv_heads)
         if to_table is not None:
             self._tables("evict_rows", to_table)
             if to_table.shape[0] != B:
                 raise KernelError("evict_rows: the two page tables are of different numbers of sequences")
-        if to_table is not None and budget > 64 * to_table.shape[1]:
-            raise KernelError(f"evict_rows: a budget of {budget} rows does not fit a page table of {to_table.shape[1]} pages")
+            if budget > 64 * to_table.shape[1]:
+                raise KernelError(f"evict_rows: a budget of {budget} rows does not fit a page table of {to_table.shape[1]} pages")
         if not entries * B * kv_heads:
             return
+        if self._elsewhere():
+            with torch.cuda.device(self._index):
+                return self.evict_rows(kept, k, v, mass, page_table, to_table)
         es = k.element_size()
-        with torch.cuda.device(self.device):
-            self._call("hb_evict_rows", kept.data_ptr(), k.data_ptr(), k.shape[-1] * es, v.data_ptr(), v.shape[-1] * es,
-                       mass.data_ptr() if mass is not None else None, page_table.data_ptr(), page_table.shape[1],
-                       to_table.data_ptr() if to_table is not None else None, to_table.shape[1] if to_table is not None else 0, entries, B, kv_heads,
-                       pages, budget, self.sm_count, self.status.data_ptr(), self._stream())
+        self._call("hb_evict_rows", kept.data_ptr(), k.data_ptr(), k.shape[-1] * es, v.data_ptr(), v.shape[-1] * es,
+                   mass.data_ptr() if mass is not None else None, page_table.data_ptr(), page_table.shape[1],
+                   to_table.data_ptr() if to_table is not None else None, to_table.shape[1] if to_table is not None else 0, entries, B, kv_heads,
+                   pages, budget, self.sm_count, self.status.data_ptr(), self._stream())
         self.launches += 1
 
     # ------------------------------------------------------------------ norms on a sublayer's output

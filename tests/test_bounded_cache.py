@@ -473,7 +473,7 @@ class _Fake:
     def __new__(cls):
         from hilbert_pruned_8b_b200.kernels.ops import Ops
         o = object.__new__(Ops)
-        o.device, o.sm_count, o.launches = torch.device("cpu"), 148, 0
+        o.device, o._index, o.sm_count, o.launches = torch.device("cpu"), -1, 148, 0
         o.lib = None
 
         def call(name, *a):
