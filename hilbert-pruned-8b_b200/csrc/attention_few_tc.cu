@@ -4,29 +4,31 @@
 //
 // A CTA = a share of the pages x one kv head x a block of a sequence's new tokens: the rows of the mma.sync tiles (16 RT of them) are the
 // (token, head) pairs of the block, so a page is read once for all of them.  Bound by memory: 2 head sizes of keys and values per row of
-// the cache against 4 bytes of score per pair.  The pages stream through three cp.async stages; each of the four warps takes a
-// quarter of every page's keys with its own running maximum and sum, joined through shared memory at the end.
-// (With a CTA per token, as for single tokens, 17 drafted tokens of four sequences took 82 us; their pages came from L2 17 times.)
+// the cache against 4 bytes of score per pair.  The pages stream through three cp.async stages; a warp takes a quarter of every page's
+// keys for one tile of 16 rows, with its own running maximum and sum, joined through shared memory at the end.  (Two tiles of rows in one
+// warp leave two warps to a quarter of the SM: 38 us for 17 drafted tokens of four sequences,
+// latencies unhidden, against 34.)
+// (With a CTA per token, as for single tokens, 17 drafted tokens of four sequences took 82 us in all instead of 46; their pages came
+// from L2 17 times.)
 #include "api.h"
 #include "attention_mass.cuh"
 #include "mma.cuh"
 
-#define FT_THREADS 128
 #define FT_STAGES 3
 
 template <int HD, int RT>
-__global__ void __launch_bounds__(FT_THREADS)
+__global__ void __launch_bounds__(128 * RT, 2)
 few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __restrict__ kc, const bf16* __restrict__ vc,
               const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* part_o,
-              float* part_ml, float* scores, long long score_ld, int tokens_per_block, int n_seqs, int nh, int nkv, float scale_log2e, int window,
-              int n_pages, int* status) {
-    constexpr int ROW_BYTES = HD * 2, TILE_BYTES = HB_PAGE_TOKENS * ROW_BYTES, CHUNKS = ROW_BYTES / 16, KSTEPS = HD / 16, ROWS = 16 * RT;
+              float* part_ml, float* scores, long long score_ld, int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, float scale_log2e,
+              int window, int n_pages, int* status) {
+    constexpr int ROW_BYTES = HD * 2, TILE_BYTES = HB_PAGE_TOKENS * ROW_BYTES, CHUNKS = ROW_BYTES / 16, KSTEPS = HD / 16, ROWS = 16 * RT, THREADS = 128 * RT;
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_trigger();
     pdl_wait();
     q = pdl_fresh(q);
     const int z = blockIdx.x, g = blockIdx.y, S = gridDim.x;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) & 3, rt = tid >> 7;       // quarter of a page's keys, tile of rows
     const int G = nh / nkv;
     int b, blk, place0;
     if (!mass_find_block(seq_start, n_seqs, blockIdx.z, tokens_per_block, b, blk, place0)) return;
@@ -34,12 +36,13 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
     const int p0 = seq_pos0[b] + blk * tokens_per_block, p_last = p0 + n_tok - 1;
     const int width = (int)min((long long)pt_width, score_ld / HB_PAGE_TOKENS);       // no score is written behind its head's
     const int first = hb_oldest_visible(p0, window, 0) / HB_PAGE_TOKENS, last = min(p_last / HB_PAGE_TOKENS + 1, width);
-    const int per = max(1, (last - first + S - 1) / S), page0 = first + z * per, page1 = min(page0 + per, last);
+    int page0, page1;
+    mass_share(first, last, z, S, share_pages, page0, page1);
     const int* pt = page_table + (size_t)b * pt_width;
     if (z == 0 && tid == 0 && p_last >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
     const int pairs = n_tok * G;                           // row r is head r % G of token r / G
     if (page0 >= page1) {                                  // a share without keys
-        for (int r = tid; r < pairs; r += FT_THREADS) {
+        for (int r = tid; r < pairs; r += THREADS) {
             float* ml = part_ml + (((size_t)(t0 + r / G) * nh + g * G + r % G) * S + z) * 2;
             ml[0] = -INFINITY;
             ml[1] = 0.0f;
@@ -59,7 +62,7 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
             const uint8_t* vsrc = (const uint8_t*)(vc + ((size_t)page * nkv + g) * HB_PAGE_TOKENS * HD);
             const uint32_t kdst = smem_base + stage * 2 * TILE_BYTES, vdst = kdst + TILE_BYTES;
 #pragma unroll
-            for (int i = tid; i < HB_PAGE_TOKENS * CHUNKS; i += FT_THREADS) {
+            for (int i = tid; i < HB_PAGE_TOKENS * CHUNKS; i += THREADS) {
                 const int row = i / CHUNKS, ch = i % CHUNKS;
                 const uint32_t off = swizzled<ROW_BYTES>(row, ch);
                 cp_async_16(kdst + off, ksrc + (size_t)i * 16);
@@ -73,140 +76,113 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
     for (int s = 0; s < FT_STAGES - 1; s++) load_page(s, page0 + s);
 
     // this thread's rows: r = 16 rt + 8 h + lane / 4
-    uint32_t qf[RT][KSTEPS][4];
-    int row_lo[RT][2], row_end[RT][2];                     // the row sees the keys [row_lo, row_end)
-    float* row_scores[RT][2];
+    uint32_t qf[KSTEPS][4];
+    int row_lo[2], row_end[2];                             // the row sees the keys [row_lo, row_end)
+    float* row_scores[2];
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++)
+    for (int h = 0; h < 2; h++) {
+        const int r = rt * 16 + h * 8 + (lane >> 2);
+        const bool there = r < pairs;
+        const int i = there ? r / G : 0, head = g * G + (there ? r - i * G : 0);
+        row_lo[h] = hb_oldest_visible(p0 + i, window, 0);
+        row_end[h] = there ? p0 + i + 1 : 0;
+        row_scores[h] = scores + ((size_t)(t0 + i) * nh + head) * score_ld;
+        const unsigned int* src = reinterpret_cast<const unsigned int*>(q + (size_t)(t0 + i) * q_stride + (size_t)head * HD + (lane & 3) * 2);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int r = rt * 16 + h * 8 + (lane >> 2);
-            const bool there = r < pairs;
-            const int i = there ? r / G : 0, head = g * G + (there ? r - i * G : 0);
-            row_lo[rt][h] = hb_oldest_visible(p0 + i, window, 0);
-            row_end[rt][h] = there ? p0 + i + 1 : 0;
-            row_scores[rt][h] = scores + ((size_t)(t0 + i) * nh + head) * score_ld;
-            const unsigned int* src = reinterpret_cast<const unsigned int*>(q + (size_t)(t0 + i) * q_stride + (size_t)head * HD + (lane & 3) * 2);
-#pragma unroll
-            for (int ks = 0; ks < KSTEPS; ks++) {
-                qf[rt][ks][h] = there ? __ldcg(src + ks * 8) : 0u;
-                qf[rt][ks][h + 2] = there ? __ldcg(src + ks * 8 + 4) : 0u;
-            }
+        for (int ks = 0; ks < KSTEPS; ks++) {
+            qf[ks][h] = there ? __ldcg(src + ks * 8) : 0u;
+            qf[ks][h + 2] = there ? __ldcg(src + ks * 8 + 4) : 0u;
         }
-    float o[RT][HD / 8][4], m[RT][2], l[RT][2];
-#pragma unroll
-    for (int rt = 0; rt < RT; rt++) {
-#pragma unroll
-        for (int i = 0; i < HD / 8; i++) o[rt][i][0] = o[rt][i][1] = o[rt][i][2] = o[rt][i][3] = 0.0f;
-        m[rt][0] = m[rt][1] = -INFINITY;
-        l[rt][0] = l[rt][1] = 0.0f;
     }
+    float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+#pragma unroll
+    for (int i = 0; i < HD / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
     for (int pi = page0; pi < page1; pi++) {
         const int it = pi - page0;
         cp_async_wait<FT_STAGES - 2>();
         __syncthreads();
         load_page((it + FT_STAGES - 1) % FT_STAGES, pi + FT_STAGES - 1);
         const uint32_t kt = smem_base + (it % FT_STAGES) * 2 * TILE_BYTES, vt = kt + TILE_BYTES;
-        float s[RT][2][4];
-#pragma unroll
-        for (int rt = 0; rt < RT; rt++)
-#pragma unroll
-            for (int nt = 0; nt < 2; nt++) s[rt][nt][0] = s[rt][nt][1] = s[rt][nt][2] = s[rt][nt][3] = 0.0f;
+        float s[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
         const int key_row = warp * 16 + ((lane >> 4) << 3) + (lane & 7);
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ks++) {
             uint32_t kf[4];
             ldmatrix_x4(kf, kt + swizzled<ROW_BYTES>(key_row, 2 * ks + ((lane >> 3) & 1)));
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                mma_bf16_16816(s[rt][0], qf[rt][ks], kf[0], kf[1]);
-                mma_bf16_16816(s[rt][1], qf[rt][ks], kf[2], kf[3]);
-            }
+            mma_bf16_16816(s[0], qf[ks], kf[0], kf[1]);
+            mma_bf16_16816(s[1], qf[ks], kf[2], kf[3]);
         }
         const int key0 = pi * HB_PAGE_TOKENS + warp * 16 + (lane & 3) * 2;
-        uint32_t pa[RT][4];
 #pragma unroll
-        for (int rt = 0; rt < RT; rt++) {
+        for (int h = 0; h < 2; h++) {
+            float top = -INFINITY;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float top = -INFINITY;
+            for (int nt = 0; nt < 2; nt++) {
 #pragma unroll
-                for (int nt = 0; nt < 2; nt++) {
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int key = key0 + nt * 8 + e;
-                        const float v = key >= row_lo[rt][h] && key < row_end[rt][h] ? s[rt][nt][2 * h + e] * scale_log2e : -INFINITY;
-                        s[rt][nt][2 * h + e] = v;
-                        top = fmaxf(top, v);
-                    }
-                    if (row_end[rt][h] > 0)
-                        *reinterpret_cast<float2*>(row_scores[rt][h] + key0 + nt * 8) = make_float2(s[rt][nt][2 * h], s[rt][nt][2 * h + 1]);
+                for (int e = 0; e < 2; e++) {
+                    const int key = key0 + nt * 8 + e;
+                    const float v = key >= row_lo[h] && key < row_end[h] ? s[nt][2 * h + e] * scale_log2e : -INFINITY;
+                    s[nt][2 * h + e] = v;
+                    top = fmaxf(top, v);
                 }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float m_new = fmaxf(m[rt][h], top), m_safe = m_new == -INFINITY ? 0.0f : m_new;
-                const float corr = exp2f(m[rt][h] - m_safe);
-                m[rt][h] = m_new;
-                float sum = 0.0f;
+                if (row_end[h] > 0) *reinterpret_cast<float2*>(row_scores[h] + key0 + nt * 8) = make_float2(s[nt][2 * h], s[nt][2 * h + 1]);
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const float m_new = fmaxf(m[h], top), m_safe = m_new == -INFINITY ? 0.0f : m_new;
+            const float corr = exp2f(m[h] - m_safe);
+            m[h] = m_new;
+            float sum = 0.0f;
 #pragma unroll
-                for (int nt = 0; nt < 2; nt++)
+            for (int nt = 0; nt < 2; nt++)
 #pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const float w = exp2f(s[rt][nt][2 * h + e] - m_safe);
-                        s[rt][nt][2 * h + e] = w;
-                        sum += w;
-                    }
-                l[rt][h] = l[rt][h] * corr + sum;
-                if (__any_sync(0xffffffffu, corr != 1.0f)) {       // a maximum grew: rarely, after the first pages
+                for (int e = 0; e < 2; e++) {
+                    const float w = exp2f(s[nt][2 * h + e] - m_safe);
+                    s[nt][2 * h + e] = w;
+                    sum += w;
+                }
+            l[h] = l[h] * corr + sum;
+            if (__any_sync(0xffffffffu, corr != 1.0f)) {   // a maximum grew: rarely, after the first pages
 #pragma unroll
-                    for (int i = 0; i < HD / 8; i++) {
-                        o[rt][i][2 * h] *= corr;
-                        o[rt][i][2 * h + 1] *= corr;
-                    }
+                for (int i = 0; i < HD / 8; i++) {
+                    o[i][2 * h] *= corr;
+                    o[i][2 * h + 1] *= corr;
                 }
             }
-            pa[rt][0] = pack_bf16(s[rt][0][0], s[rt][0][1]);
-            pa[rt][1] = pack_bf16(s[rt][0][2], s[rt][0][3]);
-            pa[rt][2] = pack_bf16(s[rt][1][0], s[rt][1][1]);
-            pa[rt][3] = pack_bf16(s[rt][1][2], s[rt][1][3]);
         }
+        const uint32_t pa[4] = {pack_bf16(s[0][0], s[0][1]), pack_bf16(s[0][2], s[0][3]), pack_bf16(s[1][0], s[1][1]), pack_bf16(s[1][2], s[1][3])};
         const int v_row = warp * 16 + (((lane >> 3) & 1) << 3) + (lane & 7);
 #pragma unroll
         for (int dn = 0; dn < HD / 16; dn++) {
             uint32_t vf[4];
             ldmatrix_x4_trans(vf, vt + swizzled<ROW_BYTES>(v_row, 2 * dn + (lane >> 4)));
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                mma_bf16_16816(o[rt][2 * dn], pa[rt], vf[0], vf[1]);
-                mma_bf16_16816(o[rt][2 * dn + 1], pa[rt], vf[2], vf[3]);
-            }
+            mma_bf16_16816(o[2 * dn], pa, vf[0], vf[1]);
+            mma_bf16_16816(o[2 * dn + 1], pa, vf[2], vf[3]);
         }
     }
     cp_async_wait<0>();
     __syncthreads();
     if (bad_page && tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + b);
 
-    float* so = reinterpret_cast<float*>(smem);                        // [4 warps][ROWS][HD]
+    float* so = reinterpret_cast<float*>(smem);                        // [4 quarters][ROWS][HD]
     float* sm = so + 4 * ROWS * HD;                                    // [4][ROWS]
     float* sl = sm + 4 * ROWS;
 #pragma unroll
-    for (int rt = 0; rt < RT; rt++)
+    for (int h = 0; h < 2; h++) {
+        const int r = rt * 16 + h * 8 + (lane >> 2);
+        float sum = l[h];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const int r = rt * 16 + h * 8 + (lane >> 2);
-            float sum = l[rt][h];
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-            for (int i = 0; i < HD / 8; i++)
-                *reinterpret_cast<float2*>(so + (size_t)(warp * ROWS + r) * HD + i * 8 + (lane & 3) * 2) = make_float2(o[rt][i][2 * h], o[rt][i][2 * h + 1]);
-            if ((lane & 3) == 0) {
-                sm[warp * ROWS + r] = m[rt][h];
-                sl[warp * ROWS + r] = sum;
-            }
+        for (int i = 0; i < HD / 8; i++)
+            *reinterpret_cast<float2*>(so + (size_t)(warp * ROWS + r) * HD + i * 8 + (lane & 3) * 2) = make_float2(o[i][2 * h], o[i][2 * h + 1]);
+        if ((lane & 3) == 0) {
+            sm[warp * ROWS + r] = m[h];
+            sl[warp * ROWS + r] = sum;
         }
+    }
     __syncthreads();
-    for (int idx = tid; idx < pairs * HD; idx += FT_THREADS) {
+    for (int idx = tid; idx < pairs * HD; idx += THREADS) {
         const int r = idx / HD, d = idx - r * HD, i = r / G;
         float M = -INFINITY;
 #pragma unroll
@@ -232,7 +208,7 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
 template <int HD, int RT>
 static int launch_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                          const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks,
-                         int tokens_per_block, int n_seqs, int nh, int nkv, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+                         int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, float scale, int window, int n_pages, int* status, cudaStream_t s) {
     constexpr int PIPE = FT_STAGES * 2 * HB_PAGE_TOKENS * HD * 2, MERGE = (4 * 16 * RT * HD + 2 * 4 * 16 * RT) * 4, SMEM = PIPE > MERGE ? PIPE : MERGE;
     static bool done[HB_MAX_DEVICES] = {};
     bool& set = done[hb_device_slot()];
@@ -241,9 +217,9 @@ static int launch_few_tc(const void* q, long long q_stride, const void* kc, cons
         if (e != cudaSuccess) return hb_fail("attention_mass: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
         set = true;
     }
-    cudaError_t e = hb_launch(few_tc_kernel<HD, RT>, dim3(splits, nkv, token_blocks), dim3(FT_THREADS), SMEM, s, (const bf16*)q, q_stride,
+    cudaError_t e = hb_launch(few_tc_kernel<HD, RT>, dim3(splits, nkv, token_blocks), dim3(128 * RT), SMEM, s, (const bf16*)q, q_stride,
                               (const bf16*)kc, (const bf16*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld,
-                              tokens_per_block, n_seqs, nh, nkv, scale * MASS_LOG2E, window, n_pages, status);
+                              tokens_per_block, share_pages, n_seqs, nh, nkv, scale * MASS_LOG2E, window, n_pages, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (few tokens, tensor cores)");
 }
@@ -255,7 +231,7 @@ extern "C" int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_
 }
 
 int attention_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks, int max_new,
+                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int token_blocks, int max_new,
                      int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s) {
     const int tokens = hb_attention_few_tc_tokens(nh, nkv, head_dim, max_new);
     HB_REQUIRE(tokens > 0, "attention_mass: head size %d with %d heads over %d kv heads is not built for the tensor cores (64 or 128, groups up to 32)",
@@ -266,7 +242,7 @@ int attention_few_tc(const void* q, long long q_stride, const void* kc, const vo
     const bool two = nh / nkv * tokens > 16;
 #define HB_FT_LAUNCH(HD, RT)                                                                                                                  \
     launch_few_tc<HD, RT>(q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, token_blocks, \
-                          tokens, n_seqs, nh, nkv, scale, window, n_pages, status, s)
+                          tokens, share_pages, n_seqs, nh, nkv, scale, window, n_pages, status, s)
     if (head_dim == 128) return two ? HB_FT_LAUNCH(128, 2) : HB_FT_LAUNCH(128, 1);
     return two ? HB_FT_LAUNCH(64, 2) : HB_FT_LAUNCH(64, 1);
 #undef HB_FT_LAUNCH

@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(AF_THREADS)
 few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict__ kc, const T* __restrict__ vc, const int* __restrict__ page_table,
                 int pt_width, const int* __restrict__ tok_seq, const int* __restrict__ positions, float* __restrict__ part_o,
                 float* __restrict__ part_ml, float* __restrict__ scores, long long score_ld, int nh, int nkv, int hd, int head_blocks,
-                float scale_log2e, int window, int n_pages, int* status) {
+                int share_pages, float scale_log2e, int window, int n_pages, int* status) {
     extern __shared__ __align__(16) float am_smem[];
     __shared__ float sc[AF_HEADS][HB_PAGE_TOKENS + 1];   // a page's scores
     __shared__ float w8[HB_PAGE_TOKENS][AF_HEADS];       // and weights
@@ -468,7 +468,8 @@ few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict
     const int* pt = page_table + (size_t)b * pt_width;
     const int width = (int)min((long long)pt_width, score_ld / HB_PAGE_TOKENS);      // no score is written behind its head's
     const int first = lo / HB_PAGE_TOKENS, last = min(p / HB_PAGE_TOKENS + 1, width);
-    const int per = max(1, (last - first + S - 1) / S), p_begin = first + z * per, p_end = min(p_begin + per, last);
+    int p_begin, p_end;
+    mass_share(first, last, z, S, share_pages, p_begin, p_end);
     if (z == 0 && tid == 0 && p >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
     const int hd4 = (hd + 3) & ~3;
     float* qs = am_smem;                                  // [8][hd4]
@@ -692,13 +693,13 @@ extern "C" long long hb_attention_mass_few_floats(int n_tokens, int n_heads, int
 
 template <typename T>
 static int launch_few(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* tok_seq,
-                      const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int n_tokens, int nh, int nkv,
-                      int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+                      const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int n_tokens, int nh,
+                      int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
     const int hd4 = (hd + 3) & ~3, slices = AF_THREADS / hd > 1 ? AF_THREADS / hd : 1, hb = (nh / nkv + AF_HEADS - 1) / AF_HEADS;
     const int smem = (AF_HEADS * hd4 + slices * AF_HEADS * hd) * 4;        // at most 16 KB
     HB_REQUIRE((long long)nkv * hb <= 65535, "attention_mass: too many heads for one launch");
     cudaError_t e = hb_launch(few_rows_kernel<T>, dim3(splits, nkv * hb, n_tokens), dim3(AF_THREADS), smem, s, (const T*)q, q_stride, (const T*)kc,
-                              (const T*)vc, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, nh, nkv, hd, hb,
+                              (const T*)vc, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, nh, nkv, hd, hb, share_pages,
                               scale * MASS_LOG2E, window, n_pages, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (few tokens)");
@@ -717,18 +718,19 @@ static int launch_finish(const float* part_o, const float* part_ml, const float*
 }
 
 // Steps of few tokens (at most hb_attention_few_pairs() pairs of a sequence's tokens and a group's heads).  `scratch` holds
-// hb_attention_mass_few_floats floats; token_blocks: 0, or for the tensor cores as attention_few_tc; max_len bounds the rows of every sequence, max_new their new tokens.
+// hb_attention_mass_few_floats floats; token_blocks: 0, or for the tensor cores as attention_few_tc; a
+// sequence's pages go into at most `splits` shares, of share_pages or more; max_len bounds the rows of every sequence, max_new their new tokens.
 extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
                                      int pt_width, const int* tok_seq, const int* positions, const int* seq_start, const int* seq_pos0, void* out,
-                                     long long out_stride, float* scratch, const float* before, float* mass, int splits, int n_tokens, int n_seqs,
-                                     int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages,
+                                     long long out_stride, float* scratch, const float* before, float* mass, int splits, int share_pages, int n_tokens,
+                                     int n_seqs, int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages,
                                      int token_blocks, int* status, void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0 && head_dim <= 256 && n_pages > 0 && pt_width > 0,
                "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, head_dim);
     HB_REQUIRE((long long)max_new * (n_heads / n_kv_heads) <= MASS_FEW_PAIRS, "attention_mass: %d tokens of %d heads are no step of few tokens",
                max_new, n_heads / n_kv_heads);
-    HB_REQUIRE(n_tokens <= 65535 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && max_len >= 1 && scratch != nullptr && mass != nullptr,
+    HB_REQUIRE(n_tokens <= 65535 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && max_len >= 1 && share_pages >= 1 && scratch != nullptr && mass != nullptr,
                "attention_mass: bad sizes");
     const size_t rows = (size_t)n_tokens * n_heads * splits;
     const long long score_ld = mass_score_ld(max_len);
@@ -739,13 +741,13 @@ extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_strid
     int rc;
     if (token_blocks > 0) {
         HB_REQUIRE(dtype == HB_BF16, "attention_mass: the tensor cores take bfloat16");
-        rc = attention_few_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits,
+        rc = attention_few_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, share_pages,
                               token_blocks, max_new, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     } else if (dtype == HB_F32)
-        rc = launch_few<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits,
+        rc = launch_few<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits, share_pages,
                                n_tokens, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     else if (dtype == HB_BF16)
-        rc = launch_few<bf16>(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits, n_tokens,
+        rc = launch_few<bf16>(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits, share_pages, n_tokens,
                               n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     else
         return hb_fail("attention_mass: unsupported dtype %d", dtype);

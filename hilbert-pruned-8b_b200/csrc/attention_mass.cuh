@@ -100,6 +100,13 @@ __device__ __forceinline__ void load4(const bf16* p, float (&x)[4]) {
 int mass_join(const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0, MassOut mo, int n_seqs, int nkv, int n_pages, int tile,
               int key_tiles, int splits, cudaStream_t s);
 
+// Share z of S of the pages [first, last): at most S equal shares of this sequence's pages, and no more than of `least` pages each.
+__device__ __forceinline__ void mass_share(int first, int last, int z, int S, int least, int& page0, int& page1) {
+    const int n = last - first, shares = max(1, min(S, (n + least - 1) / least)), per = max(1, (n + shares - 1) / shares);
+    page0 = first + z * per;
+    page1 = min(page0 + per, last);
+}
+
 // The keys of a block of queries, shared out: a block that sees n tiles of keys takes ceil(n / tiles) CTAs, and where those are several each
 // leaves its unnormalised outputs and (maximum, sum) of its rows: o[(share * heads + head) * tokens + token][head size], ml likewise.
 struct Shares {
@@ -132,5 +139,5 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
 // The first half of a step of few tokens on the tensor cores (attention_few_tc.cu): token_blocks, the sum over sequences of ceil(new
 // tokens / hb_attention_few_tc_tokens(...)); queries 4-byte, keys and values 16-byte aligned.
 int attention_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks, int max_new,
+                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int token_blocks, int max_new,
                      int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);

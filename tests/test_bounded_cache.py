@@ -541,8 +541,11 @@ def test_evict_rows_refuses(change, text):
 
 def test_shapes_of_the_launches():
     from hilbert_pruned_8b_b200.kernels.plan import chunk_shares, few_splits, mass_splits, select_shape
-    assert few_splits([5], 8, 296) == 5 and few_splits([129] * 8, 8, 296) == 4 and few_splits([100] * 1000, 8, 296) == 1
-    assert few_splits([33, 126, 9, 65], 8, 296) == 18 and few_splits([], 8, 296) == 1 and few_splits([1], 1, 296) == 1
+    assert few_splits([5], 8, 296) == (5, 1) and few_splits([129] * 8, 8, 296) == (4, 1) and few_splits([100] * 1000, 8, 296) == (1, 1)
+    assert few_splits([], 8, 296) == (1, 1) and few_splits([1], 1, 296) == (1, 1)
+    for pages in ([33, 126, 9, 65], [1, 1, 2000], [7] * 50 + [900]):
+        splits, least = few_splits(pages, 8, 296)
+        assert 1 <= splits <= 32 and splits * least >= max(pages)
     assert mass_splits(1000, 8, 100, 296) == 1 and mass_splits(1, 1, 1, 296) == 1 and mass_splits(1, 1, 100, 296) == 16
     assert chunk_shares([4096], [4096], 0, 128, 128, 16, 4160, 148) == (1, 32)                 # enough blocks for everybody
     shares, tiles = chunk_shares([128], [100000], 0, 128, 128, 16, 4160, 148)                  # 16 blocks of 782 tiles
