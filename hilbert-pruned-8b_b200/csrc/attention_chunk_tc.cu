@@ -22,28 +22,13 @@
 #include "attention_tc.cuh"
 #include "exp2_pair.cuh"
 
-#define CT_THREADS 576
+#define CT_THREADS 320
 #define CT_STAGES 2
-
-// A barrier of the 256 softmax threads of a tile that tells each of them whether any gave up: the same answer for all, so that none
-// waits for one that left.
-__device__ __forceinline__ bool chunk_any(int tile, bool mine) {
-    uint32_t any;
-    asm volatile(
-        "{\n\t.reg .pred p, q;\n\t"
-        "setp.ne.u32 q, %2, 0;\n\t"
-        "bar.red.or.pred p, %1, 256, q;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(any)
-        : "r"(2 + tile), "r"((uint32_t)mine)
-        : "memory");
-    return any != 0;
-}
 
 // The weights 2^(s scale log2(e) - m) of 64 scores of a row, as bfloat16 over the scores, and their sum.  POLY: a quarter of the pairs on
 // the FMA pipe (a masked score has to give exactly zero, which only the special-function unit does).
 template <bool POLY>
-__device__ __forceinline__ void chunk_weights(const float (&sv)[64], f32x2 scale2, f32x2 neg2, uint32_t tm_p, f32x2 (&sum)[2]) {
+__device__ __forceinline__ void chunk_weights(const float* sv, f32x2 scale2, f32x2 neg2, uint32_t tm_p, f32x2 (&sum)[2]) {
 #pragma unroll
     for (int c = 0; c < 2; c++) {
         uint32_t pk[16];
@@ -75,11 +60,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     // [Q tiles 2][K stages][V stages][barriers]; a tile is 128 rows x HD
     constexpr int HALVES = HD / 64, TILE = HALVES * FA_HALF_BYTES;
     uint64_t* bars = (uint64_t*)(smem + (2 + 2 * CT_STAGES) * TILE);
-    uint32_t* tmem_slot = (uint32_t*)(bars + 16);
-    float* xrow = (float*)(tmem_slot + 4);                     // [2 tiles][2 halves][128 rows]: row maxima, at the end row sums
+    uint32_t* tmem_slot = (uint32_t*)(bars + 18);
     const uint32_t smem_base = smem_u32(smem), k_smem = smem_base + 2 * TILE, v_smem = k_smem + CT_STAGES * TILE;
     const uint32_t q_full = smem_u32(bars), k_full0 = smem_u32(bars + 1), k_empty0 = smem_u32(bars + 3), v_full0 = smem_u32(bars + 5),
-                   v_empty0 = smem_u32(bars + 7), s_full0 = smem_u32(bars + 9), p_full0 = smem_u32(bars + 11), o_full0 = smem_u32(bars + 13);
+                   v_empty0 = smem_u32(bars + 7), s_full0 = smem_u32(bars + 9), p_full0 = smem_u32(bars + 11), o_full0 = smem_u32(bars + 15);   // p_full: [2 tiles][2 halves of the keys]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // The two tiles: heads head0 and head0 + 1 (head_pairs) of one block of tokens, or blocks 2 blk and 2 blk + 1 of head0.  Blocks
@@ -109,13 +93,14 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             mbar_init(v_full0 + 8 * s, 1);
             mbar_init(v_empty0 + 8 * s, 1);
             mbar_init(s_full0 + 8 * s, 1);
-            mbar_init(p_full0 + 8 * s, 8);
+            mbar_init(p_full0 + 16 * s, 4);
+            mbar_init(p_full0 + 16 * s + 8, 4);
             mbar_init(o_full0 + 8 * s, 1);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    if (warp == 17) tmem_alloc(smem_u32(tmem_slot), 512);
+    if (warp == 9) tmem_alloc(smem_u32(tmem_slot), 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -123,7 +108,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     pdl_trigger();
     pdl_wait();
 
-    if (warp == 16) {
+    if (warp == 8) {
         // ---------------------------------------------------------------- TMA producer
         if (lane == 0) {
             const int* pt = page_table + (size_t)b * pt_width;
@@ -169,7 +154,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 if (!mbar_wait(v_full0 + 8 * (it % CT_STAGES), (it / CT_STAGES) & 1)) atomicExch(error_flag, 53);
             if (!mbar_wait(q_full, 0)) atomicExch(error_flag, 53);
         }
-    } else if (warp == 17) {
+    } else if (warp == 9) {
         // ---------------------------------------------------------------- MMA issuer: the warp waits, one lane issues
         constexpr uint32_t idesc_qk = instr_desc_bf16_mn(128, FA_KEYS);
         constexpr uint32_t idesc_pv = instr_desc_bf16_mn(128, HD) | (1u << 16);               // B is MN-major
@@ -196,63 +181,66 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const int sv = it % CT_STAGES;
 #pragma unroll
             for (int i = 0; i < 2; i++) {
-                alive = __all_sync(0xffffffffu, mbar_wait(p_full0 + 8 * i, it & 1) && (i == 1 || mbar_wait(v_full0 + 8 * sv, (it / CT_STAGES) & 1)) &&
-                                                    (i == 1 || it + 1 == n_it || mbar_wait(k_full0 + 8 * ((it + 1) % CT_STAGES), ((it + 1) / CT_STAGES) & 1)));
-                if (!alive) {
-                    atomicExch(error_flag, 55);
-                    break;
-                }
-                tc_fence_after();
-                if (elect_one()) {
 #pragma unroll
-                    for (int kk = 0; kk < FA_KEYS / 16; kk++)
-                        umma_bf16_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + kk * 8, v_desc + ((sv * TILE + kk * 16 * 128) >> 4), idesc_pv,
-                                     (it | kk) ? 1u : 0u);
-                    if (i == 1) umma_commit(v_empty0 + 8 * sv);
-                    if (it + 1 < n_it) scores(i, it + 1);
-                    else umma_commit(o_full0 + 8 * i);
+                for (int half = 0; half < 2; half++) {         // the weights of a tile's first 64 keys, then the others
+                    alive = alive && __all_sync(0xffffffffu, mbar_wait(p_full0 + 16 * i + 8 * half, it & 1) &&
+                                                                 (i + half > 0 || mbar_wait(v_full0 + 8 * sv, (it / CT_STAGES) & 1)) &&
+                                                                 (i > 0 || half == 0 || it + 1 == n_it ||
+                                                                  mbar_wait(k_full0 + 8 * ((it + 1) % CT_STAGES), ((it + 1) / CT_STAGES) & 1)));
+                    if (!alive) break;
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int kk = half * 4; kk < half * 4 + 4; kk++)
+                            umma_bf16_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + kk * 8, v_desc + ((sv * TILE + kk * 16 * 128) >> 4), idesc_pv,
+                                         (it | kk) ? 1u : 0u);
+                        if (half == 1) {
+                            if (i == 1) umma_commit(v_empty0 + 8 * sv);
+                            if (it + 1 < n_it) scores(i, it + 1);
+                            else umma_commit(o_full0 + 8 * i);
+                        }
+                    }
+                    __syncwarp();
                 }
-                __syncwarp();
             }
+            if (!alive) atomicExch(error_flag, 55);
         }
     } else {
-        // ---------------------------------------------------------------- softmax and output
-        const int i = warp >> 3, hf = (warp >> 2) & 1, r = (warp & 3) * 32 + lane;   // tile, half of its columns, row = lane of tensor memory
+        // ---------------------------------------------------------------- softmax and output: a thread per row
+        const int i = warp >> 2, r = (warp & 3) * 32 + lane;   // tile, row = lane of tensor memory
         const int head = head0 + (head_pairs ? i : 0), row = row0 + (head_pairs ? 0 : i * FA_ROWS) + r;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t tm_s = tmem_base + i * 128 + lane_base, tm_o = tmem_base + 256 + i * 128 + hf * (HD / 2) + lane_base;
-        float* xmax = xrow + i * 256;
+        const uint32_t tm_s = tmem_base + i * 128 + lane_base, tm_o = tmem_base + 256 + i * 128 + lane_base;
         const int qpos = pos0 + row, lo = hb_oldest_visible(qpos, window, 0);
         const bool valid = row < n_new;
-        float m_run = -INFINITY, l = 0.0f;                     // l: this thread's columns only
+        const f32x2 scale2 = pair_of(scale_log2e, scale_log2e);
+        float m_run = -INFINITY, l = 0.0f;
         bool ok = true;
         for (int it = 0; it < n_it; it++) {
-            const bool here = __all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * i, it & 1));
-            tc_fence_after();
-            // this row sees keys lo..qpos; as columns of its half of the tile: [c_lo, c_hi]
-            const int kbase = (jt0 + it) * FA_KEYS, c_lo = lo - kbase - hf * 64, c_hi = qpos - kbase - hf * 64;
-            float sv[64];
-            tmem_ld64(tm_s + hf * 64, sv);
-            const bool edge = __any_sync(0xffffffffu, c_lo > 0 || c_hi < 63);       // the causal diagonal or the window's edge
-            if (edge) {
-#pragma unroll
-                for (int e = 0; e < 64; e++)
-                    if (e < c_lo || e > c_hi) sv[e] = -INFINITY;
-            }
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int e = 0; e < 64; e += 8) {
-#pragma unroll
-                for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], fmaxf(sv[e + u], sv[e + 4 + u]));
-            }
-            xmax[hf * 128 + r] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-            // the tile's threads have their scores in registers now (P may overwrite S), and the other half's maximum is visible
-            if (chunk_any(i, !here)) {
+            if (!__all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * i, it & 1))) {
                 atomicExch(error_flag, 56);
                 ok = false;
                 break;
             }
-            const float m_tile = fmaxf(xmax[r], xmax[128 + r]) * scale_log2e;
+            tc_fence_after();
+            float sv[128];
+            tmem_ld64(tm_s, sv);
+            tmem_ld64(tm_s + 64, sv + 64);
+            // this row sees keys lo..qpos; as columns of the tile: [c_lo, c_hi]
+            const int kbase = (jt0 + it) * FA_KEYS, c_lo = lo - kbase, c_hi = qpos - kbase;
+            const bool edge = __any_sync(0xffffffffu, c_lo > 0 || c_hi < 127);      // the causal diagonal or the window's edge
+            if (edge) {
+#pragma unroll
+                for (int e = 0; e < 128; e++)
+                    if (e < c_lo || e > c_hi) sv[e] = -INFINITY;
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int e = 0; e < 128; e += 8) {
+#pragma unroll
+                for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], fmaxf(sv[e + u], sv[e + 4 + u]));
+            }
+            const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2e;
             if (it == 0) {
                 m_run = m_tile;
             } else {
@@ -264,7 +252,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                     m_run = m_new;
                     l *= corr;
 #pragma unroll 1
-                    for (int c = 0; c < HD / 32; c++) {
+                    for (int c = 0; c < HD / 16; c++) {
                         float v[16];
                         tmem_ld16(tm_o + c * 16, v);
                         uint32_t u[16];
@@ -277,66 +265,64 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             }
             const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
             f32x2 sum[2] = {0ull, 0ull};
-            const f32x2 scale2 = pair_of(scale_log2e, scale_log2e), neg2 = pair_of(neg_m, neg_m);
-            if (edge) chunk_weights<false>(sv, scale2, neg2, tm_s + hf * 32, sum);
-            else chunk_weights<true>(sv, scale2, neg2, tm_s + hf * 32, sum);
-            float s0, s1;
-            pair_parts(pair_add(sum[0], sum[1]), s0, s1);
-            l += s0 + s1;
+            const f32x2 neg2 = pair_of(neg_m, neg_m);
             if (i == 0 && (jt0 + it + 1) * FA_KEYS > pos0 + n_new) {
                 // the tile that holds the sequence's end: values behind it are whatever a page held before, and 0 * NaN is NaN
                 const int s = it % CT_STAGES;
                 if (!mbar_wait(v_full0 + 8 * s, (it / CT_STAGES) & 1)) atomicExch(error_flag, 57);
                 const int from = pos0 + n_new - kbase;         // rows from..127, 128 bytes of each half
-                for (int u = threadIdx.x + from * 8 * HALVES; u < FA_KEYS * 8 * HALVES; u += 256) {
+                for (int u = threadIdx.x + from * 8 * HALVES; u < FA_KEYS * 8 * HALVES; u += 128) {
                     const int vr = u / (8 * HALVES), c = u % (8 * HALVES);
                     *reinterpret_cast<uint4*>(smem + (2 + CT_STAGES + s) * TILE + (c >> 3) * FA_HALF_BYTES + vr * 128 + (c & 7) * 16) =
                         make_uint4(0u, 0u, 0u, 0u);
                 }
                 fence_async_shared();                          // before the tensor core reads them (tile 0's product is issued first)
+                __syncwarp();
             }
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_full0 + 8 * i);       // one arrival a warp: arrivals of single threads queue up
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                if (edge) chunk_weights<false>(sv + 64 * half, scale2, neg2, tm_s + half * 32, sum);
+                else chunk_weights<true>(sv + 64 * half, scale2, neg2, tm_s + half * 32, sum);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_full0 + 16 * i + 8 * half);       // one arrival a warp: arrivals of single threads queue up
+            }
+            float s0, s1;
+            pair_parts(pair_add(sum[0], sum[1]), s0, s1);
+            l += s0 + s1;
         }
         const size_t at = ((size_t)z * nh + head) * n_tokens + t_begin + row;
-        if (ok) {                                       // (the same for a tile's threads)
-            const bool here = __all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * i, 0));
-            xmax[hf * 128 + r] = l;                            // read last in front of the product that is complete now
-            if (chunk_any(i, !here)) {
-                atomicExch(error_flag, 58);
-            } else {
-                tc_fence_after();
-                l = xmax[r] + xmax[128 + r];
-                const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-                if (valid && hf == 0) {
-                    if (S > 1) {
-                        *reinterpret_cast<float2*>(sh.ml + at * 2) = make_float2(m_run, l);
-                    } else {
-                        lse[head * lse_ld + place0 + row] = l > 0.0f ? m_run + log2f(l) : INFINITY;
-                    }
-                }
-                bf16* dst = out + (size_t)(t_begin + row) * out_stride + (size_t)head * HD + hf * (HD / 2);
-                float4* po = reinterpret_cast<float4*>(sh.o + at * HD + hf * (HD / 2));
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * i, 0))) {
+            atomicExch(error_flag, 58);
+            ok = false;
+        }
+        if (ok) {
+            tc_fence_after();
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            if (valid) {
+                if (S > 1) *reinterpret_cast<float2*>(sh.ml + at * 2) = make_float2(m_run, l);
+                else lse[head * lse_ld + place0 + row] = l > 0.0f ? m_run + log2f(l) : INFINITY;
+            }
+            bf16* dst = out + (size_t)(t_begin + row) * out_stride + (size_t)head * HD;
+            float4* po = reinterpret_cast<float4*>(sh.o + at * HD);
 #pragma unroll 1
-                for (int c = 0; c < HD / 64; c++) {
-                    float v[32];
-                    tmem_ld32(tm_o + c * 32, v);
-                    if (!valid) continue;
-                    if (S > 1) {
+            for (int c = 0; c < HD / 32; c++) {
+                float v[32];
+                tmem_ld32(tm_o + c * 32, v);
+                if (!valid) continue;
+                if (S > 1) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 4) po[c * 8 + (e >> 2)] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                    } else {
+                    for (int e = 0; e < 32; e += 4) po[c * 8 + (e >> 2)] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                } else {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            uint4 o4;
-                            o4.x = pack_bf16_pair(v[e] * inv, v[e + 1] * inv);
-                            o4.y = pack_bf16_pair(v[e + 2] * inv, v[e + 3] * inv);
-                            o4.z = pack_bf16_pair(v[e + 4] * inv, v[e + 5] * inv);
-                            o4.w = pack_bf16_pair(v[e + 6] * inv, v[e + 7] * inv);
-                            *reinterpret_cast<uint4*>(dst + c * 32 + e) = o4;
-                        }
+                    for (int e = 0; e < 32; e += 8) {
+                        uint4 o4;
+                        o4.x = pack_bf16_pair(v[e] * inv, v[e + 1] * inv);
+                        o4.y = pack_bf16_pair(v[e + 2] * inv, v[e + 3] * inv);
+                        o4.z = pack_bf16_pair(v[e + 4] * inv, v[e + 5] * inv);
+                        o4.w = pack_bf16_pair(v[e + 6] * inv, v[e + 7] * inv);
+                        *reinterpret_cast<uint4*>(dst + c * 32 + e) = o4;
                     }
                 }
             }
@@ -344,7 +330,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 17) {
+    if (warp == 9) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
     }
@@ -354,7 +340,7 @@ template <int HD>
 static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width, const int* seq_start,
                         const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, Shares sh, int max_shares, int n_tokens, int n_seqs, int q_blocks,
                         int nh, int nkv, int head_pairs, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
-    constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 16 * 8 + 16 + 512 * 4 + 1024;
+    constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 18 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "attention tiles do not fit shared memory");
     static bool done[HB_MAX_DEVICES] = {};
     bool& set = done[hb_device_slot()];
