@@ -1,5 +1,5 @@
 // Attention of a chunk of new tokens over the paged cache on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), bfloat16, head
-// size 64 or 128, that leaves each row's log-sum for the weights' kernel (attention_mass_tc.cu): causal, grouped, with a window,
+// size 64 or 128, that leaves each row's log-sum, negated, for the weights' kernel (attention_mass_tc.cu): causal, grouped, with a window,
 // sequences with unequal numbers of new tokens, the keys cut into shares where there are few rows.
 //
 // One CTA = two tiles of 128 query rows that read the same keys and values: two heads of a kv head with an even group, else two
@@ -7,13 +7,14 @@
 // head size 128: 1024 clocks of the two products, 1024 clocks of exponentials (16 a clock and SM), and 64 KB of keys and values, which at the
 // 32 bytes a clock that an SM takes from L2 would last 2048 clocks for one tile: hence two tiles, which halve that, and which take turns:
 // while one tile's weights are made, the tensor cores work on the other.
-//   warps 0-7, 8-15 softmax of tile 0 and 1, two threads per row: 64 scores each from tensor memory into registers, the row's maximum agreed
-//                   on through shared memory, running maximum and sum in float32, weights as bfloat16 over the scores.  (One thread
-//                   per row needs no exchange but leaves two warps to a quarter of the SM: the same time.)  The output accumulator is rescaled only when a row's maximum grows by more than 2^8 (weights are
-//                   taken against a maximum that may be stale by less).
-//   warp 16         TMA producer: the query tiles once, then key and value tiles of 128 rows (two pages), two stages each
-//   warp 17         owns tensor memory; one thread issues, per key tile and in this order: O0 += P0 V, S0 = Q0 K' (the next keys),
-//                   O1 += P1 V, S1 = Q1 K'.  P lies over S; the tensor cores take the products in order.
+//   warps 0-3, 4-7  softmax of tile 0 and 1, a thread per row: 128 scores from tensor memory into registers, running maximum and sum in
+//                   float32, weights as bfloat16, handed over in two halves.  No exchange between threads (two threads per row, which agree
+//                   on the maximum through shared memory: 2.09 instead of 1.77 us for the two tiles at head size 128, 1.73 instead of 1.62 at
+//                   64).  The output accumulator is rescaled only when a row's maximum grows by more than 2^8 (weights are taken against a
+//                   maximum that may be stale by less).
+//   warp 8          TMA producer: the query tiles once, then key and value tiles of 128 rows (two pages), two stages each
+//   warp 9          owns tensor memory; one thread issues, per key tile and in this order: O0 += P0 V, S0 = Q0 K' (the next keys),
+//                   O1 += P1 V, S1 = Q1 K'; with head size 64, whose weights do not lie over the scores, a tile's S before its O.
 // Weights are rounded to bfloat16 for the product with the values (the sum they are divided by is taken before that).
 //
 // Every wait is bounded; a wait that runs out sets *error_flag and the CTA drains and leaves.
@@ -25,7 +26,7 @@
 #define CT_THREADS 320
 #define CT_STAGES 2
 
-// The weights 2^(s scale log2(e) - m) of 64 scores of a row, as bfloat16 over the scores, and their sum.  POLY: a quarter of the pairs on
+// The weights 2^(s scale log2(e) - m) of 64 scores of a row, as bfloat16 over the scores, and their sum.  POLY: an eighth of the pairs on
 // the FMA pipe (a masked score has to give exactly zero, which only the special-function unit does).
 template <bool POLY>
 __device__ __forceinline__ void chunk_weights(const float* sv, f32x2 scale2, f32x2 neg2, uint32_t tm_p, f32x2 (&sum)[2]) {
@@ -36,7 +37,7 @@ __device__ __forceinline__ void chunk_weights(const float* sv, f32x2 scale2, f32
         for (int e = 0; e < 16; e++) {
             const f32x2 x = pair_fma(pair_of(sv[c * 32 + 2 * e], sv[c * 32 + 2 * e + 1]), scale2, neg2);
             float a, d;
-            if (POLY && (e & 3) == 2) {
+            if (POLY && (e & 7) == 2) {
                 exp2_pair<4>(x, a, d);
             } else {
                 pair_parts(x, a, d);
@@ -60,10 +61,11 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     // [Q tiles 2][K stages][V stages][barriers]; a tile is 128 rows x HD
     constexpr int HALVES = HD / 64, TILE = HALVES * FA_HALF_BYTES;
     uint64_t* bars = (uint64_t*)(smem + (2 + 2 * CT_STAGES) * TILE);
-    uint32_t* tmem_slot = (uint32_t*)(bars + 18);
+    uint32_t* tmem_slot = (uint32_t*)(bars + 22);
     const uint32_t smem_base = smem_u32(smem), k_smem = smem_base + 2 * TILE, v_smem = k_smem + CT_STAGES * TILE;
     const uint32_t q_full = smem_u32(bars), k_full0 = smem_u32(bars + 1), k_empty0 = smem_u32(bars + 3), v_full0 = smem_u32(bars + 5),
-                   v_empty0 = smem_u32(bars + 7), s_full0 = smem_u32(bars + 9), p_full0 = smem_u32(bars + 11), o_full0 = smem_u32(bars + 15);   // p_full: [2 tiles][2 halves of the keys]
+                   v_empty0 = smem_u32(bars + 7), s_full0 = smem_u32(bars + 9), p_full0 = smem_u32(bars + 11), pv_done0 = smem_u32(bars + 15),
+                   s_free0 = smem_u32(bars + 17);              // p_full: [2 tiles][2 halves of the keys]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     // The two tiles: heads head0 and head0 + 1 (head_pairs) of one block of tokens, or blocks 2 blk and 2 blk + 1 of head0.  Blocks
@@ -95,7 +97,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             mbar_init(s_full0 + 8 * s, 1);
             mbar_init(p_full0 + 16 * s, 4);
             mbar_init(p_full0 + 16 * s + 8, 4);
-            mbar_init(o_full0 + 8 * s, 1);
+            mbar_init(pv_done0 + 8 * s, 1);
+            mbar_init(s_free0 + 8 * s, 4);
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -104,7 +107,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem_base = *tmem_slot;                    // S0, S1 at columns 0 and 128, O0, O1 at 256 and 384
+    // S0, S1 at columns 0 and 128; head size 128: O0, O1 at 256 and 384, P over S; 64: O0, O1 at 256 and 320, P0, P1 at 384 and 448, so that
+    // the next scores can be computed as soon as these have been read
+    constexpr bool APART = HD == 64;
+    const uint32_t tmem_base = *tmem_slot;
     pdl_trigger();
     pdl_wait();
 
@@ -171,46 +177,55 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             if (i == 1) umma_commit(k_empty0 + 8 * st);
         };
         bool alive = __all_sync(0xffffffffu, mbar_wait(q_full, 0) && mbar_wait(k_full0, 0));
-        if (!alive) atomicExch(error_flag, 54);
         tc_fence_after();
         if (alive && elect_one()) {
             scores(0, 0);
             scores(1, 0);
         }
+        __syncwarp();
         for (int it = 0; it < n_it && alive; it++) {
             const int sv = it % CT_STAGES;
+            const bool more = it + 1 < n_it;
+            const uint32_t next_k = k_full0 + 8 * ((it + 1) % CT_STAGES), next_parity = ((it + 1) / CT_STAGES) & 1;
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
+            for (int i = 0; i < 2 && alive; i++) {
+                if (APART && more) {                           // the next scores, once the softmax has these in registers
+                    alive = __all_sync(0xffffffffu, mbar_wait(s_free0 + 8 * i, it & 1) && (i > 0 || mbar_wait(next_k, next_parity)));
+                    if (!alive) break;
+                    tc_fence_after();
+                    if (elect_one()) scores(i, it + 1);
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int half = 0; half < 2; half++) {         // the weights of a tile's first 64 keys, then the others
                     alive = alive && __all_sync(0xffffffffu, mbar_wait(p_full0 + 16 * i + 8 * half, it & 1) &&
                                                                  (i + half > 0 || mbar_wait(v_full0 + 8 * sv, (it / CT_STAGES) & 1)) &&
-                                                                 (i > 0 || half == 0 || it + 1 == n_it ||
-                                                                  mbar_wait(k_full0 + 8 * ((it + 1) % CT_STAGES), ((it + 1) / CT_STAGES) & 1)));
+                                                                 (APART || i > 0 || half == 0 || !more || mbar_wait(next_k, next_parity)));
                     if (!alive) break;
                     tc_fence_after();
                     if (elect_one()) {
 #pragma unroll
                         for (int kk = half * 4; kk < half * 4 + 4; kk++)
-                            umma_bf16_ts(tmem_base + 256 + i * 128, tmem_base + i * 128 + kk * 8, v_desc + ((sv * TILE + kk * 16 * 128) >> 4), idesc_pv,
-                                         (it | kk) ? 1u : 0u);
+                            umma_bf16_ts(tmem_base + 256 + i * HD, tmem_base + (APART ? 384 + i * 64 : i * 128) + kk * 8,
+                                         v_desc + ((sv * TILE + kk * 16 * 128) >> 4), idesc_pv, (it | kk) ? 1u : 0u);
                         if (half == 1) {
                             if (i == 1) umma_commit(v_empty0 + 8 * sv);
-                            if (it + 1 < n_it) scores(i, it + 1);
-                            else umma_commit(o_full0 + 8 * i);
+                            if (!APART && more) scores(i, it + 1);
+                            if (APART || !more) umma_commit(pv_done0 + 8 * i);
                         }
                     }
                     __syncwarp();
                 }
             }
-            if (!alive) atomicExch(error_flag, 55);
         }
+        if (!alive) atomicExch(error_flag, 55);
     } else {
         // ---------------------------------------------------------------- softmax and output: a thread per row
         const int i = warp >> 2, r = (warp & 3) * 32 + lane;   // tile, row = lane of tensor memory
         const int head = head0 + (head_pairs ? i : 0), row = row0 + (head_pairs ? 0 : i * FA_ROWS) + r;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t tm_s = tmem_base + i * 128 + lane_base, tm_o = tmem_base + 256 + i * 128 + lane_base;
+        const uint32_t tm_s = tmem_base + i * 128 + lane_base, tm_o = tmem_base + 256 + i * HD + lane_base;
+        const uint32_t tm_p = APART ? tmem_base + 384 + i * 64 + lane_base : tm_s;
         const int qpos = pos0 + row, lo = hb_oldest_visible(qpos, window, 0);
         const bool valid = row < n_new;
         const f32x2 scale2 = pair_of(scale_log2e, scale_log2e);
@@ -226,6 +241,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             float sv[128];
             tmem_ld64(tm_s, sv);
             tmem_ld64(tm_s + 64, sv + 64);
+            if (APART) {
+                tc_fence_before();
+                if (lane == 0) mbar_arrive(s_free0 + 8 * i);   // the warp's scores are in registers (the load is the warp's)
+            }
             // this row sees keys lo..qpos; as columns of the tile: [c_lo, c_hi]
             const int kbase = (jt0 + it) * FA_KEYS, c_lo = lo - kbase, c_hi = qpos - kbase;
             const bool edge = __any_sync(0xffffffffu, c_lo > 0 || c_hi < 127);      // the causal diagonal or the window's edge
@@ -241,12 +260,20 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 for (int u = 0; u < 4; u++) mx[u] = fmaxf(mx[u], fmaxf(sv[e + u], sv[e + 4 + u]));
             }
             const float m_tile = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2e;
+            if (APART && it > 0) {                             // the product before: it reads the weights and writes the accumulator
+                if (!__all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * i, (it - 1) & 1))) {
+                    atomicExch(error_flag, 59);
+                    ok = false;
+                    break;
+                }
+                tc_fence_after();
+            }
             if (it == 0) {
                 m_run = m_tile;
             } else {
                 const bool grow = m_tile > m_run + FA_RESCALE_THRESHOLD;
                 if (__any_sync(0xffffffffu, grow)) {
-                    // S of this tile is complete, so is every product issued before it: nothing touches the accumulator now
+                    // nothing touches the accumulator now (P over S: S of this tile is complete, so is every product issued before it)
                     const float m_new = fmaxf(m_run, m_tile);
                     const float corr = m_new == -INFINITY ? 1.0f : exp2f(m_run - m_new);
                     m_run = m_new;
@@ -281,8 +308,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             }
 #pragma unroll
             for (int half = 0; half < 2; half++) {
-                if (edge) chunk_weights<false>(sv + 64 * half, scale2, neg2, tm_s + half * 32, sum);
-                else chunk_weights<true>(sv + 64 * half, scale2, neg2, tm_s + half * 32, sum);
+                if (edge) chunk_weights<false>(sv + 64 * half, scale2, neg2, tm_p + half * 32, sum);
+                else chunk_weights<true>(sv + 64 * half, scale2, neg2, tm_p + half * 32, sum);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -293,7 +320,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             l += s0 + s1;
         }
         const size_t at = ((size_t)z * nh + head) * n_tokens + t_begin + row;
-        if (ok && !__all_sync(0xffffffffu, mbar_wait(o_full0 + 8 * i, 0))) {
+        if (ok && !__all_sync(0xffffffffu, mbar_wait(pv_done0 + 8 * i, APART ? (n_it - 1) & 1 : 0))) {
             atomicExch(error_flag, 58);
             ok = false;
         }
@@ -302,7 +329,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
             if (valid) {
                 if (S > 1) *reinterpret_cast<float2*>(sh.ml + at * 2) = make_float2(m_run, l);
-                else lse[head * lse_ld + place0 + row] = l > 0.0f ? m_run + log2f(l) : INFINITY;
+                else lse[head * lse_ld + place0 + row] = l > 0.0f ? -(m_run + log2f(l)) : -INFINITY;
             }
             bf16* dst = out + (size_t)(t_begin + row) * out_stride + (size_t)head * HD;
             float4* po = reinterpret_cast<float4*>(sh.o + at * HD);
@@ -340,7 +367,7 @@ template <int HD>
 static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width, const int* seq_start,
                         const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, Shares sh, int max_shares, int n_tokens, int n_seqs, int q_blocks,
                         int nh, int nkv, int head_pairs, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
-    constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 18 * 8 + 16 + 1024;
+    constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 22 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "attention tiles do not fit shared memory");
     static bool done[HB_MAX_DEVICES] = {};
     bool& set = done[hb_device_slot()];

@@ -224,7 +224,7 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
 }
 
 // out = sum_z o_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), lse = M + log2 of that sum, for the rows whose block has several shares; a
-// warp per (token, head)
+// block per token, a warp per head
 template <typename T>
 __global__ void __launch_bounds__(256)
 shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, int rounded,
@@ -233,34 +233,41 @@ shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* 
     __shared__ float ws[8][32];
     pdl_trigger();
     pdl_wait();
-    const int t = blockIdx.x, lane = threadIdx.x & 31, head = blockIdx.y * 8 + (threadIdx.x >> 5);
+    const int t = blockIdx.x, lane = threadIdx.x & 31;
     int b, i, place0;
     if (!mass_find_block(seq_start, n_seqs, t, 1, b, i, place0)) return;
     const int place = rounded ? place0 + i : t;
     const int n_new = seq_start[b + 1] - seq_start[b], row0 = (t - seq_start[b]) / span * span;
     int tile0;
     const int S = shares_of(sh, key_tiles_of(seq_pos0[b] + row0, seq_pos0[b] + min(row0 + span, n_new) - 1, window, keys, tile0));
-    if (S == 1 || head >= nh) return;
-    const size_t at = (size_t)head * n_tokens + t, step = (size_t)nh * n_tokens;
-    float2 ml = make_float2(-INFINITY, 0.0f);                  // of share `lane` (at most 32)
-    if (lane < S) ml = __ldcg(reinterpret_cast<const float2*>(sh.ml) + at + lane * step);
-    const float M = warp_max(ml.x);
-    const float w = ml.x != -INFINITY ? exp2f(ml.x - M) : 0.0f;
-    const float L = warp_sum(ml.y * w), inv = L > 0.0f ? 1.0f / L : 0.0f;
+    if (S == 1) return;
     float* mine = ws[threadIdx.x >> 5];
-    mine[lane] = w;
-    __syncwarp();
-    for (int d = lane; d < hd; d += 32) {
-        float acc = 0.0f;
-        for (int z = 0; z < S; z++) acc = fmaf(__ldcg(sh.o + (at + z * step) * hd + d), mine[z], acc);
-        out[(size_t)t * out_stride + (size_t)head * hd + d] = from_f32<T>(acc * inv);
+    for (int head = threadIdx.x >> 5; head < nh; head += 8) {
+        const size_t at = (size_t)head * n_tokens + t, step = (size_t)nh * n_tokens;
+        float2 ml = make_float2(-INFINITY, 0.0f);              // of share `lane` (at most 32)
+        if (lane < S) ml = __ldcg(reinterpret_cast<const float2*>(sh.ml) + at + lane * step);
+        const float M = warp_max(ml.x);
+        const float w = ml.x != -INFINITY ? exp2f(ml.x - M) : 0.0f;
+        const float L = warp_sum(ml.y * w), inv = L > 0.0f ? 1.0f / L : 0.0f;
+        mine[lane] = w;
+        __syncwarp();
+        for (int d = lane; d < hd; d += 32) {
+            float acc = 0.0f;
+#pragma unroll 4
+            for (int z = 0; z < S; z++) acc = fmaf(__ldcg(sh.o + (at + z * step) * hd + d), mine[z], acc);
+            out[(size_t)t * out_stride + (size_t)head * hd + d] = from_f32<T>(acc * inv);
+        }
+        if (lane == 0) {
+            const float total = L > 0.0f ? M + log2f(L) : INFINITY;
+            lse[head * lse_ld + place] = rounded ? -total : total;
+        }
+        __syncwarp();
     }
-    if (lane == 0) lse[head * lse_ld + place] = L > 0.0f ? M + log2f(L) : INFINITY;
 }
 
 int shares_join(Shares sh, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded, const int* seq_start,
                 const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s) {
-    const dim3 grid(n_tokens, (nh + 7) / 8);
+    const dim3 grid(n_tokens);                             // a block per token: most tokens of a step with unequal sequences have one share
     cudaError_t e = dtype == HB_BF16 ? hb_launch(shares_join_kernel<bf16>, grid, dim3(256), 0, s, sh, (bf16*)out, out_stride, lse, lse_ld, rounded,
                                                  seq_start, seq_pos0, span, keys, window, n_tokens, n_seqs, nh, hd)
                                      : hb_launch(shares_join_kernel<float>, grid, dim3(256), 0, s, sh, (float*)out, out_stride, lse, lse_ld, rounded,

@@ -122,12 +122,12 @@ __device__ __forceinline__ int key_tiles_of(int first, int last, int window, int
 }
 
 // joins the shares (attention_mass.cu): out and lse of the rows whose block has several.  Blocks of `span` tokens, tiles of `keys`
-// keys; lse[head * lse_ld + place], places in blocks of 128 per sequence (`rounded`) or the token's number
+// keys; lse[head * lse_ld + place], places in blocks of 128 per sequence and the log-sums negated (`rounded`), or the token's number
 int shares_join(Shares sh, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded, const int* seq_start,
                 const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s);
 
 // The first half of a step of many tokens on the tensor cores (attention_chunk_tc.cu): writes out and the rows'
-// log-sums, lse[head][place]: a sequence's places begin at a multiple of 128, behind those of the sequences in front.  q_blocks: sum
+// log-sums, negated, lse[head][place]: a sequence's places begin at a multiple of 128, behind those of the sequences in front.  q_blocks: sum
 // over sequences of ceil(new tokens / span), span 128 with an even group of heads and 256 with an odd one; max_shares: the most CTAs
 // that a block of queries takes, share_tiles: the most tiles of 128 keys of one of them; parts: max_shares * n_heads * n_tokens *
 // (head_dim + 2) floats when max_shares > 1.

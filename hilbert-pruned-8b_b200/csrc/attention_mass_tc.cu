@@ -7,8 +7,10 @@
 //   warp 0      TMA producer: the two key tiles once, then query tiles with their log-sums (three stages)
 //   warp 1      owns tensor memory; one thread issues S = K Q^T of the two key tiles (head size / 16 steps each) into two pairs of buffers
 //   warps 2-17  weights: 8 warps per key tile, a thread has 64 queries of its key: w = 2^(s scale log2(e) - lse), added up
+//               (the log-sums come negated)
 // What bounds it: 16 exponentials a clock and SM (1024 clocks for 128 x 128 weights, against 512 for the product at head size
-// 128), so three pairs in eight are computed on the FMA pipe instead.  Two key tiles share a query tile because an SM takes about 32
+// 128), so a pair in eight is computed on the FMA pipe instead (none: 684, one: 654, three: 697 us for 2048 tokens behind 30001 rows of the
+// 8B sizes, where the products alone take 418).  Two key tiles share a query tile because an SM takes about 32
 // bytes a clock from L2: with one, loading a 32 KB query tile would last as long as its exponentials.
 //
 // Every wait is bounded; a wait that runs out sets *error_flag and the CTA drains and leaves.
@@ -154,7 +156,7 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const int hf = (w >> 2) & 1;                           // which 64 queries of a tile
         const int key = key0 + k * 128 + r;
         const uint32_t lane_base = (uint32_t)(quarter * 32) << 16;
-        const f32x2 scale2 = pair_of(scale_log2e, scale_log2e), minus = pair_of(-1.0f, -1.0f);
+        const f32x2 scale2 = pair_of(scale_log2e, scale_log2e);
         f32x2 sum[4] = {0ull, 0ull, 0ull, 0ull};
         bool ok = true;
         for (int it = 0; it < n_it; it++) {
@@ -187,11 +189,10 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                         const float4 l4 = ls[c >> 2];
 #pragma unroll
                         for (int u = 0; u < 2; u++) {
-                            const f32x2 x = pair_fma(pair_of(sv[c + 2 * u], sv[c + 2 * u + 1]), scale2,
-                                                     pair_fma(pair_of(u ? l4.z : l4.x, u ? l4.w : l4.y), minus, 0ull));
+                            const f32x2 x = pair_fma(pair_of(sv[c + 2 * u], sv[c + 2 * u + 1]), scale2, pair_of(u ? l4.z : l4.x, u ? l4.w : l4.y));
                             const int pair = (c >> 1) + u;     // 0..15
                             float a, d;
-                            if ((pair & 7) == 1 || (pair & 7) == 4 || (pair & 7) == 6) {
+                            if ((pair & 7) == 4) {
                                 exp2_pair<5>(x, a, d);
                             } else {
                                 pair_parts(x, a, d);
@@ -204,8 +205,8 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 } else if (lo <= 31 && hi >= 0) {              // the causal diagonal, the window's edge, the last queries
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
-                        const float a = c >= lo && c <= hi ? exp2_approx(fmaf(sv[c], scale_log2e, -xlse[s * 128 + hf * 64 + part * 32 + c])) : 0.0f;
-                        const float d = c + 1 >= lo && c + 1 <= hi ? exp2_approx(fmaf(sv[c + 1], scale_log2e, -xlse[s * 128 + hf * 64 + part * 32 + c + 1])) : 0.0f;
+                        const float a = c >= lo && c <= hi ? exp2_approx(fmaf(sv[c], scale_log2e, xlse[s * 128 + hf * 64 + part * 32 + c])) : 0.0f;
+                        const float d = c + 1 >= lo && c + 1 <= hi ? exp2_approx(fmaf(sv[c + 1], scale_log2e, xlse[s * 128 + hf * 64 + part * 32 + c + 1])) : 0.0f;
                         sum[(c >> 1) & 3] = pair_add(sum[(c >> 1) & 3], pair_of(a, d));
                     }
                 }
