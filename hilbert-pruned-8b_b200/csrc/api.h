@@ -325,11 +325,12 @@ int hb_attention_mass_tc(const void* q, long long q_stride, const void* k_cache,
 int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_dim, int max_new);
 int hb_attention_few_pairs(void);
 long long hb_attention_mass_few_floats(int n_tokens, int n_heads, int head_dim, int splits, int max_len);
+int hb_attention_few_block_pairs(void);
 int hb_attention_mass_few(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
-                          int pt_width, const int* tok_seq, const int* positions, const int* seq_start, const int* seq_pos0, void* out,
-                          long long out_stride, float* scratch, const float* before, float* mass, int splits, int share_pages,
-                          int n_tokens, int n_seqs, int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages,
-                          int token_blocks, int* status, void* stream);
+                          int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* scratch,
+                          const float* before, float* mass, int splits, int share_pages, int blocks, int tensor_cores, int n_tokens, int n_seqs,
+                          int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* status,
+                          void* stream);
 int hb_evict_select(const float* mass, const int* page_table, int pt_width, const int* lengths, int* kept, int entries, int n_seqs,
                     int n_kv_heads, int n_pages, int first, int recent, int budget, int threads, int cluster, int* status, void* stream);
 int hb_evict_rows(const int* kept, void* k, int k_row_bytes, void* v, int v_row_bytes, float* mass, const int* from_table, int from_width,

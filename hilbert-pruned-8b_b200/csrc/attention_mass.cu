@@ -15,6 +15,7 @@
 // Softmax statistics, scores, sums and mass are float32; lse is in units of log 2.
 #include "api.h"
 #include "attention_mass.cuh"
+#include "mma.cuh"
 
 // ------------------------------------------------------------------------------------------- many tokens, every head size
 // Tiles of 64 queries (of one head) x 64 keys, 256 threads, 4 x 4 scores a thread (rows ty + 16 i, keys tx + 16 j), operands
@@ -448,142 +449,218 @@ extern "C" int hb_attention_mass(const void* q, int dtype, long long q_stride, c
 }
 
 // -------------------------------------------------------------------------------------------- few tokens, every head size
-// A block per (share of the token's pages, kv head and up to 8 of its query heads, token).  Scores: 4 threads per key, 16 bytes
-// of the key's row each at a time; softmax: a warp per head; values: a thread per column (and share of the keys), 8 heads each.
+// A block per (share of the pages, kv head, eight (token, head) pairs of a sequence's new tokens and the kv head's group).  Keys and values
+// stream through shared memory in tiles of 32 rows, three cp.async stages, as they are stored.  Scores: a warp per pair, a lane per
+// key, so that the softmax is a warp's; values: a thread per two columns (and share of the tile's keys), all eight pairs at once.
+// Rows in shared memory lie an odd number of 16-byte units apart: the lanes' 16-byte reads of 32 rows then fall into different banks.
+// Bound by the FP32 pipe or by memory: 32 keys of head size 152 take about 900 clocks of instructions and 20 KB.  (Keys and values
+// read where they are used, a page at a time, took 404 us for five sequences of 8000 to 14000 rows, 16 heads of size
+// 152, instead of 113, with 16 shares each.)
 #define AF_THREADS 256
-#define AF_HEADS 8
+#define AF_PAIRS 8
+#define AF_KEYS 32
+#define AF_STAGES 3
+
+static __host__ __device__ constexpr int af_row_bytes(int hd, int es) {
+    const int units = (hd * es + 15) / 16;
+    return (units | 1) * 16;
+}
+static __host__ __device__ constexpr int af_smem(int hd, int es) {
+    return AF_STAGES * 2 * AF_KEYS * af_row_bytes(hd, es) + AF_PAIRS * ((hd + 7) & ~7) * 4;
+}
+
+// eight (bfloat16) or four (float32) elements of a 16-byte unit
+__device__ __forceinline__ void unpack16(const uint4& u, float (&x)[8], const bf16*) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+__device__ __forceinline__ void unpack16(const uint4& u, float (&x)[4], const float*) {
+    x[0] = __uint_as_float(u.x), x[1] = __uint_as_float(u.y), x[2] = __uint_as_float(u.z), x[3] = __uint_as_float(u.w);
+}
+__device__ __forceinline__ float2 two_columns(const uint8_t* p, const float*) { return *reinterpret_cast<const float2*>(p); }
+__device__ __forceinline__ float2 two_columns(const uint8_t* p, const bf16*) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
 
 template <typename T>
 __global__ void __launch_bounds__(AF_THREADS)
 few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict__ kc, const T* __restrict__ vc, const int* __restrict__ page_table,
-                int pt_width, const int* __restrict__ tok_seq, const int* __restrict__ positions, float* __restrict__ part_o,
-                float* __restrict__ part_ml, float* __restrict__ scores, long long score_ld, int nh, int nkv, int hd, int head_blocks,
-                int share_pages, float scale_log2e, int window, int n_pages, int* status) {
-    extern __shared__ __align__(16) float am_smem[];
-    __shared__ float sc[AF_HEADS][HB_PAGE_TOKENS + 1];   // a page's scores
-    __shared__ float w8[HB_PAGE_TOKENS][AF_HEADS];       // and weights
-    __shared__ float corr[AF_HEADS], stat[2][AF_HEADS];
+                int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* __restrict__ part_o,
+                float* __restrict__ part_ml, float* __restrict__ scores, long long score_ld, int n_seqs, int nh, int nkv, int hd, int share_pages,
+                float scale_log2e, int window, int n_pages, int vec, int* status) {
+    extern __shared__ __align__(16) uint8_t af_raw[];
+    __shared__ float4 w8[AF_KEYS][AF_PAIRS / 4];         // a tile's weights
+    __shared__ float corr[AF_PAIRS], stat[2][AF_PAIRS];
+    constexpr int UNIT = 16 / sizeof(T);
     pdl_trigger();
     pdl_wait();
     q = pdl_fresh(q);
     kc = pdl_fresh(kc);
     vc = pdl_fresh(vc);
-    const int G = nh / nkv, t = blockIdx.z, S = gridDim.x, z = blockIdx.x;
-    const int g = blockIdx.y / head_blocks, h0 = (blockIdx.y % head_blocks) * AF_HEADS, H = min(AF_HEADS, G - h0);
+    const int G = nh / nkv, S = gridDim.x, z = blockIdx.x, g = blockIdx.y;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int b = tok_seq[t], p = positions[t], lo = hb_oldest_visible(p, window, 0);
+    const int row_bytes = af_row_bytes(hd, sizeof(T)), hd8 = (hd + 7) & ~7;
+    uint8_t* tiles = af_raw;                             // [stages][keys, values][32][row_bytes]
+    float* qs = reinterpret_cast<float*>(af_raw + AF_STAGES * 2 * AF_KEYS * row_bytes);        // [8][hd8]
+    int b, blk, unused;
+    if (!mass_find(n_seqs, blockIdx.z, [&](int i) { return ((seq_start[i + 1] - seq_start[i]) * G + AF_PAIRS - 1) / AF_PAIRS; }, [](int) { return 0; },
+                   b, blk, unused))
+        return;
+    const int t0 = seq_start[b], n_new = seq_start[b + 1] - t0, pos0 = seq_pos0[b];
+    const int pair0 = blk * AF_PAIRS, pairs = min(AF_PAIRS, n_new * G - pair0);          // pair i is head i % G of token i / G
+    const int p_first = pos0 + pair0 / G, p_last = pos0 + (pair0 + pairs - 1) / G;
     const int* pt = page_table + (size_t)b * pt_width;
-    const int width = (int)min((long long)pt_width, score_ld / HB_PAGE_TOKENS);      // no score is written behind its head's
-    const int first = lo / HB_PAGE_TOKENS, last = min(p / HB_PAGE_TOKENS + 1, width);
-    int p_begin, p_end;
-    mass_share(first, last, z, S, share_pages, p_begin, p_end);
-    if (z == 0 && tid == 0 && p >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
-    const int hd4 = (hd + 3) & ~3;
-    float* qs = am_smem;                                  // [8][hd4]
-    float* so = qs + AF_HEADS * hd4;                      // [slices][8][hd]: at the end
-    for (int i = tid; i < AF_HEADS * hd4; i += AF_THREADS) {
-        const int h = i / hd4, d = i - h * hd4;
-        qs[i] = (h < H && d < hd) ? to_f32(q[(size_t)t * q_stride + (size_t)(g * G + h0 + h) * hd + d]) : 0.0f;
-    }
-    float m = -INFINITY, l = 0.0f;                        // of head `warp`, in every lane
-    const int slices = max(1, AF_THREADS / hd), d_own = tid % hd, slice = tid / hd;      // hd <= 256
-    float acc[AF_HEADS];
-#pragma unroll
-    for (int h = 0; h < AF_HEADS; h++) acc[h] = 0.0f;
-    const bool vec = hd % 4 == 0 && ((uintptr_t)kc & 15) == 0;
-    for (int pi = p_begin; pi < p_end; pi++) {
-        int page = pt[pi];
-        if (page < 0 || page >= n_pages) {
-            if (tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + b);
-            page = -1;
+    const int width = (int)min((long long)pt_width, score_ld / HB_PAGE_TOKENS);          // no score is written behind its pair's
+    const int oldest = hb_oldest_visible(p_first, window, 0);
+    int page0, page1;
+    mass_share(oldest / HB_PAGE_TOKENS, min(p_last / HB_PAGE_TOKENS + 1, width), z, S, share_pages, page0, page1);
+    if (z == 0 && tid == 0 && p_last >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
+    auto at_of = [&](int r) -> size_t { return (size_t)(t0 + (pair0 + r) / G) * nh + g * G + (pair0 + r) % G; };
+    if (page0 >= page1) {                                // a share without keys
+        if (tid < pairs) {
+            part_ml[(at_of(tid) * S + z) * 2] = -INFINITY;
+            part_ml[(at_of(tid) * S + z) * 2 + 1] = 0.0f;
         }
-        const size_t row0 = ((size_t)max(page, 0) * nkv + g) * HB_PAGE_TOKENS;
-        __syncthreads();
-        {
-            const int e = tid >> 2, sub = tid & 3, key = pi * HB_PAGE_TOKENS + e;
-            const bool seen = page >= 0 && key >= lo && key <= p;
-            float dot[AF_HEADS];
-#pragma unroll
-            for (int h = 0; h < AF_HEADS; h++) dot[h] = 0.0f;
-            if (seen) {
-                const T* kr = kc + (row0 + e) * hd;
-                for (int d = sub * 4; d < hd4; d += 16) {
-                    float x[4];
-                    if (vec) {
-                        load4(kr + d, x);
-                    } else {
-#pragma unroll
-                        for (int u = 0; u < 4; u++) x[u] = d + u < hd ? to_f32(kr[d + u]) : 0.0f;
-                    }
-#pragma unroll
-                    for (int h = 0; h < AF_HEADS; h++) {
-                        const float4 y = *reinterpret_cast<const float4*>(qs + h * hd4 + d);
-                        dot[h] = fmaf(x[0], y.x, fmaf(x[1], y.y, fmaf(x[2], y.z, fmaf(x[3], y.w, dot[h]))));
-                    }
+        return;
+    }
+    // what no copy fills (the columns behind hd) is read times zero
+    for (int i = tid; i < AF_STAGES * 2 * AF_KEYS * row_bytes / 16; i += AF_THREADS) reinterpret_cast<uint4*>(tiles)[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = tid; i < AF_PAIRS * hd8; i += AF_THREADS) {
+        const int r = i / hd8, d = i - r * hd8;
+        qs[i] = r < pairs && d < hd ? to_f32(q[(size_t)(t0 + (pair0 + r) / G) * q_stride + (size_t)(g * G + (pair0 + r) % G) * hd + d]) : 0.0f;
+    }
+    __syncthreads();
+    const int n_tiles = (page1 - page0) * (HB_PAGE_TOKENS / AF_KEYS);
+    bool bad = false;
+    auto load_tile = [&](int it) {
+        if (it < n_tiles) {
+            const int key0 = page0 * HB_PAGE_TOKENS + it * AF_KEYS;
+            int page = pt[key0 / HB_PAGE_TOKENS];
+            const bool held = page >= 0 && page < n_pages;
+            if (!held) {
+                bad = true;
+                page = 0;                                // never read outside the cache; its keys count as not there
+            }
+            const size_t row0 = ((size_t)page * nkv + g) * HB_PAGE_TOKENS + (key0 & (HB_PAGE_TOKENS - 1));
+            uint8_t* dst = tiles + (size_t)(it % AF_STAGES) * 2 * AF_KEYS * row_bytes;
+            if (vec) {
+                const int units = hd / UNIT;             // whole, and aligned
+                for (int i = tid; i < 2 * AF_KEYS * units; i += AF_THREADS) {
+                    const int r = i / units, u = i - r * units, key = r & (AF_KEYS - 1);
+                    const bool there = held && key0 + key >= oldest && key0 + key <= p_last;
+                    const T* src = (r < AF_KEYS ? kc : vc) + (row0 + key) * hd + u * UNIT;
+                    cp_async_16_or_zero((uint32_t)__cvta_generic_to_shared(dst + r * row_bytes + u * 16), src, there);
+                }
+            } else {
+                for (int i = tid; i < 2 * AF_KEYS * hd; i += AF_THREADS) {
+                    const int r = i / hd, d = i - r * hd, key = r & (AF_KEYS - 1);
+                    const bool there = held && key0 + key >= oldest && key0 + key <= p_last;
+                    reinterpret_cast<T*>(dst + r * row_bytes)[d] = there ? ((r < AF_KEYS ? kc : vc) + (row0 + key) * hd)[d] : from_f32<T>(0.0f);
                 }
             }
-#pragma unroll
-            for (int h = 0; h < AF_HEADS; h++) {
-                dot[h] += __shfl_xor_sync(0xffffffffu, dot[h], 1);
-                dot[h] += __shfl_xor_sync(0xffffffffu, dot[h], 2);
-            }
-            if (sub == 0) {
-#pragma unroll
-                for (int h = 0; h < AF_HEADS; h++) sc[h][e] = seen ? dot[h] * scale_log2e : -INFINITY;
-            }
         }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int i = 0; i < AF_STAGES - 1; i++) load_tile(i);
+    const int pos = pos0 + (pair0 + min(warp, pairs - 1)) / G, lo = hb_oldest_visible(pos, window, 0);      // of this warp's pair
+    float* my_scores = scores + at_of(min(warp, pairs - 1)) * score_ld;
+    float m = -INFINITY, l = 0.0f;                        // in every lane
+    const int columns = (hd + 1) / 2, slices = AF_THREADS / columns, slice = tid / columns, column = (tid - slice * columns) * 2;
+    float2 acc[AF_PAIRS];
+#pragma unroll
+    for (int r = 0; r < AF_PAIRS; r++) acc[r] = make_float2(0.0f, 0.0f);
+    for (int it = 0; it < n_tiles; it++) {
+        cp_async_wait<AF_STAGES - 2>();
         __syncthreads();
-        {
-            const float a = sc[warp][lane], c = sc[warp][lane + 32];
-            const float m_new = fmaxf(m, warp_max(fmaxf(a, c))), m_safe = m_new == -INFINITY ? 0.0f : m_new;
-            const float f = exp2f(m - m_safe), wa = exp2f(a - m_safe), wc = exp2f(c - m_safe);
-            m = m_new;
-            l = l * f + warp_sum(wa + wc);
-            w8[lane][warp] = wa;
-            w8[lane + 32][warp] = wc;
-            if (lane == 0) corr[warp] = f;
-            if (warp < H) {
-                float* dst = scores + ((size_t)t * nh + g * G + h0 + warp) * score_ld + (size_t)pi * HB_PAGE_TOKENS;
-                dst[lane] = a;
-                dst[lane + 32] = c;
+        load_tile(it + AF_STAGES - 1);
+        const uint8_t* kt = tiles + (size_t)(it % AF_STAGES) * 2 * AF_KEYS * row_bytes;
+        const uint8_t* vt = kt + AF_KEYS * row_bytes;
+        const int key0 = page0 * HB_PAGE_TOKENS + it * AF_KEYS, key = key0 + lane;
+        if (warp < pairs) {
+            const uint4* kr = reinterpret_cast<const uint4*>(kt + lane * row_bytes);
+            const float4* qr = reinterpret_cast<const float4*>(qs + warp * hd8);
+            float dot[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+            for (int u = 0; u < (hd + UNIT - 1) / UNIT; u++) {
+                float x[UNIT];
+                unpack16(kr[u], x, (const T*)nullptr);
+#pragma unroll
+                for (int c = 0; c < UNIT / 4; c++) {
+                    const float4 y = qr[u * (UNIT / 4) + c];
+                    dot[0] = fmaf(x[4 * c], y.x, dot[0]);
+                    dot[1] = fmaf(x[4 * c + 1], y.y, dot[1]);
+                    dot[2] = fmaf(x[4 * c + 2], y.z, dot[2]);
+                    dot[3] = fmaf(x[4 * c + 3], y.w, dot[3]);
+                }
             }
+            // a page that is missing: its keys are not there
+            const int page = pt[key0 / HB_PAGE_TOKENS];
+            const bool seen = key >= lo && key <= pos && page >= 0 && page < n_pages;
+            const float s = seen ? ((dot[0] + dot[1]) + (dot[2] + dot[3])) * scale_log2e : -INFINITY;
+            my_scores[key] = s;
+            const float m_new = fmaxf(m, warp_max(s)), m_safe = m_new == -INFINITY ? 0.0f : m_new;
+            const float f = exp2f(m - m_safe), w = exp2f(s - m_safe);
+            m = m_new;
+            l = l * f + warp_sum(w);
+            reinterpret_cast<float*>(&w8[lane][0])[warp] = w;
+            if (lane == 0) corr[warp] = f;
+        } else {
+            reinterpret_cast<float*>(&w8[lane][0])[warp] = 0.0f;
+            if (lane == 0) corr[warp] = 1.0f;
         }
         __syncthreads();
         if (slice < slices) {
 #pragma unroll
-            for (int h = 0; h < AF_HEADS; h++) acc[h] *= corr[h];
-            const int e_end = min(HB_PAGE_TOKENS, p - pi * HB_PAGE_TOKENS + 1);
-            if (page >= 0) {
-                for (int e = slice; e < e_end; e += slices) {
-                    const float x = to_f32(vc[(row0 + e) * hd + d_own]);
-                    const float4 wa = *reinterpret_cast<const float4*>(&w8[e][0]), wb = *reinterpret_cast<const float4*>(&w8[e][4]);
-                    const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
-                    if (pi * HB_PAGE_TOKENS + e < lo) continue;
+            for (int r = 0; r < AF_PAIRS; r++) {
+                acc[r].x *= corr[r];
+                acc[r].y *= corr[r];
+            }
+#pragma unroll 4
+            for (int e = slice; e < AF_KEYS; e += slices) {
+                const float2 x = two_columns(vt + e * row_bytes + column * sizeof(T), (const T*)nullptr);
+                const float4 wa = w8[e][0], wb = w8[e][1];
+                const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
-                    for (int h = 0; h < AF_HEADS; h++) acc[h] = fmaf(w[h], x, acc[h]);
+                for (int r = 0; r < AF_PAIRS; r++) {
+                    acc[r].x = fmaf(w[r], x.x, acc[r].x);
+                    acc[r].y = fmaf(w[r], x.y, acc[r].y);
                 }
             }
         }
     }
-    __syncthreads();
-    if (slice < slices) {
+    cp_async_wait<0>();
+    if (bad && tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + b);
+    // join the slices: one after another adds to the first's sums, in shared memory over the tiles
+    float* so = reinterpret_cast<float*>(af_raw);         // [8][2 columns]
+    for (int c = 0; c < slices; c++) {
+        __syncthreads();
+        if (slice == c) {
 #pragma unroll
-        for (int h = 0; h < AF_HEADS; h++) so[((size_t)slice * AF_HEADS + h) * hd + d_own] = acc[h];
+            for (int r = 0; r < AF_PAIRS; r++) {
+                float2* o = reinterpret_cast<float2*>(so + r * 2 * columns + column);
+                const float2 old = c > 0 ? *o : make_float2(0.0f, 0.0f);
+                *o = make_float2(old.x + acc[r].x, old.y + acc[r].y);
+            }
+        }
     }
     if (lane == 0) {
         stat[0][warp] = m;
         stat[1][warp] = l;
     }
     __syncthreads();
-    for (int i = tid; i < H * hd; i += AF_THREADS) {
-        const int h = i / hd, d = i - h * hd;
-        float s = 0.0f;
-        for (int c = 0; c < slices; c++) s += so[((size_t)c * AF_HEADS + h) * hd + d];
-        const size_t base = ((size_t)t * nh + g * G + h0 + h) * S + z;
-        part_o[base * hd + d] = s;
+    for (int i = tid; i < pairs * hd; i += AF_THREADS) {
+        const int r = i / hd, d = i - r * hd;
+        const size_t base = at_of(r) * S + z;
+        part_o[base * hd + d] = so[r * 2 * columns + d];
         if (d == 0) {
-            part_ml[base * 2] = stat[0][h];
-            part_ml[base * 2 + 1] = stat[1][h];
+            part_ml[base * 2] = stat[0][r];
+            part_ml[base * 2 + 1] = stat[1][r];
         }
     }
 }
@@ -699,15 +776,16 @@ extern "C" long long hb_attention_mass_few_floats(int n_tokens, int n_heads, int
 }
 
 template <typename T>
-static int launch_few(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* tok_seq,
-                      const int* positions, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int n_tokens, int nh,
-                      int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
-    const int hd4 = (hd + 3) & ~3, slices = AF_THREADS / hd > 1 ? AF_THREADS / hd : 1, hb = (nh / nkv + AF_HEADS - 1) / AF_HEADS;
-    const int smem = (AF_HEADS * hd4 + slices * AF_HEADS * hd) * 4;        // at most 16 KB
-    HB_REQUIRE((long long)nkv * hb <= 65535, "attention_mass: too many heads for one launch");
-    cudaError_t e = hb_launch(few_rows_kernel<T>, dim3(splits, nkv * hb, n_tokens), dim3(AF_THREADS), smem, s, (const T*)q, q_stride, (const T*)kc,
-                              (const T*)vc, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, nh, nkv, hd, hb, share_pages,
-                              scale * MASS_LOG2E, window, n_pages, status);
+static int launch_few(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
+                      const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int blocks,
+                      int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+    static_assert(af_smem(256, 4) <= 227 * 1024, "tiles do not fit shared memory");
+    static bool done[HB_MAX_DEVICES] = {};
+    if (am_reserve(few_rows_kernel<T>, af_smem(256, sizeof(T)), done)) return 1;
+    const int vec = hd % (16 / (int)sizeof(T)) == 0 && (((uintptr_t)kc | (uintptr_t)vc) & 15) == 0;
+    cudaError_t e = hb_launch(few_rows_kernel<T>, dim3(splits, nkv, blocks), dim3(AF_THREADS), af_smem(hd, sizeof(T)), s, (const T*)q, q_stride, (const T*)kc,
+                              (const T*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, n_seqs, nh, nkv, hd, share_pages,
+                              scale * MASS_LOG2E, window, n_pages, vec, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (few tokens)");
 }
@@ -724,21 +802,28 @@ static int launch_finish(const float* part_o, const float* part_ml, const float*
     return hb_check_launch("attention_mass (finish)");
 }
 
+// Pairs of a token and a head that a block of the kernel for every head size takes.
+extern "C" int hb_attention_few_block_pairs(void) { return AF_PAIRS; }
+
 // Steps of few tokens (at most hb_attention_few_pairs() pairs of a sequence's tokens and a group's heads).  `scratch` holds
-// hb_attention_mass_few_floats floats; token_blocks: 0, or for the tensor cores as attention_few_tc; a
-// sequence's pages go into at most `splits` shares, of share_pages or more; max_len bounds the rows of every sequence, max_new their new tokens.
+// hb_attention_mass_few_floats floats; blocks: the sum over sequences of ceil(pairs / hb_attention_few_block_pairs()), or with
+// tensor_cores of ceil(new tokens / hb_attention_few_tc_tokens(...)); a sequence's pages go into at most `splits` shares, of share_pages
+// or more; max_len bounds the rows of every sequence, max_new their new tokens.
 extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
-                                     int pt_width, const int* tok_seq, const int* positions, const int* seq_start, const int* seq_pos0, void* out,
-                                     long long out_stride, float* scratch, const float* before, float* mass, int splits, int share_pages, int n_tokens,
-                                     int n_seqs, int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages,
-                                     int token_blocks, int* status, void* stream) {
+                                     int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* scratch,
+                                     const float* before, float* mass, int splits, int share_pages, int blocks, int tensor_cores, int n_tokens,
+                                     int n_seqs, int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window,
+                                     int n_pages, int* status, void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0 && head_dim <= 256 && n_pages > 0 && pt_width > 0,
                "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, head_dim);
     HB_REQUIRE((long long)max_new * (n_heads / n_kv_heads) <= MASS_FEW_PAIRS, "attention_mass: %d tokens of %d heads are no step of few tokens",
                max_new, n_heads / n_kv_heads);
-    HB_REQUIRE(n_tokens <= 65535 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && max_len >= 1 && share_pages >= 1 && scratch != nullptr && mass != nullptr,
+    HB_REQUIRE(n_tokens > 0 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && share_pages >= 1 && blocks >= 1 && blocks <= 65535 && max_len >= 1 &&
+                   scratch != nullptr && mass != nullptr,
                "attention_mass: bad sizes");
+    HB_REQUIRE(dtype == HB_F32 || dtype == HB_BF16, "attention_mass: unsupported dtype %d", dtype);
+    HB_REQUIRE(!tensor_cores || dtype == HB_BF16, "attention_mass: the tensor cores take bfloat16");
     const size_t rows = (size_t)n_tokens * n_heads * splits;
     const long long score_ld = mass_score_ld(max_len);
     float *scores = scratch, *part_ml = scores + (size_t)n_tokens * n_heads * score_ld, *part_o = part_ml + rows * 2;
@@ -746,18 +831,15 @@ extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_strid
     cudaStream_t s = (cudaStream_t)stream;
     MassOut mo = {before, mass, nullptr};
     int rc;
-    if (token_blocks > 0) {
-        HB_REQUIRE(dtype == HB_BF16, "attention_mass: the tensor cores take bfloat16");
+    if (tensor_cores)
         rc = attention_few_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, share_pages,
-                              token_blocks, max_new, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
-    } else if (dtype == HB_F32)
-        rc = launch_few<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits, share_pages,
-                               n_tokens, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
-    else if (dtype == HB_BF16)
-        rc = launch_few<bf16>(q, q_stride, k_cache, v_cache, page_table, pt_width, tok_seq, positions, part_o, part_ml, scores, score_ld, splits, share_pages, n_tokens,
-                              n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
+                              blocks, max_new, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
+    else if (dtype == HB_F32)
+        rc = launch_few<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, share_pages,
+                               blocks, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     else
-        return hb_fail("attention_mass: unsupported dtype %d", dtype);
+        rc = launch_few<bf16>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, share_pages,
+                              blocks, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     if (rc) return rc;
     if (dtype == HB_F32)
         return launch_finish<float>(part_o, part_ml, scores, score_ld, page_table, pt_width, seq_start, seq_pos0, out, out_stride, mo, max_len, max_new,

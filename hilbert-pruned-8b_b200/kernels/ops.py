@@ -83,9 +83,9 @@ _SIGNATURES = {
                           _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_tc": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr,
                              _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
-    "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr,
-                              _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int,
-                              _c_int, _c_ptr, _c_ptr],
+    "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr,
+                              _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int,
+                              _c_ptr, _c_ptr],
     "hb_evict_select": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr,
                         _c_ptr],
     "hb_evict_rows": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
@@ -189,6 +189,7 @@ def load_library():
             getattr(lib, name).argtypes, getattr(lib, name).restype = [_c_int, _c_int, _c_int], _c_int
         lib.hb_attention_mass_tc_keys.argtypes, lib.hb_attention_mass_tc_keys.restype = [], _c_int
         lib.hb_attention_few_tc_tokens.argtypes, lib.hb_attention_few_tc_tokens.restype = [_c_int] * 4, _c_int
+        lib.hb_attention_few_block_pairs.argtypes, lib.hb_attention_few_block_pairs.restype = [], _c_int
         lib.hb_attention_few_pairs.argtypes, lib.hb_attention_few_pairs.restype = [], _c_int
         lib.hb_attention_mass_few_floats.argtypes, lib.hb_attention_mass_few_floats.restype = [_c_int] * 5, _c_ll
         lib.hb_attention_sink_prefill_supported.argtypes, lib.hb_attention_sink_prefill_supported.restype = [_c_int] * 4, _c_int
@@ -1262,28 +1263,32 @@ class Ops:
             raise KernelError(f"attention: {what} must be a contiguous float32 {list(want)} (pages, kv heads, rows of a page), got {t.dtype} "
                               f"{tuple(t.shape)}")
 
-    def _mass_plan(self, few: bool, tc: bool, heads: int, kv_heads: int, head_dim: int, win: int, step, splits: Optional[int]):
-        """How a step of ``attention_mass`` is cut, from its sizes alone: few tokens: (blocks of tokens for the tensor cores or 0, most
+    def _mass_plan(self, few: bool, tc: bool, bf16: bool, heads: int, kv_heads: int, head_dim: int, win: int, step, splits: Optional[int]):
+        """How a step of ``attention_mass`` is cut, from its sizes alone: few tokens: (blocks, whether on the tensor cores, most
         shares of the pages, fewest pages of one, floats of scratch); many: (shares of the keys' sums, blocks of queries, tiles of keys, most shares of a block of
         queries, tiles of keys in one, distance of two heads' log-sums, floats of the log-sums, of the sums' shares, of the partial results)."""
         T, group = step.num_tokens, heads // kv_heads
         # (single tokens: from the page table's width alone, so that a captured step and an eager one sum alike)
         single = step.max_new == 1 and few
-        key = (few, tc, heads, kv_heads, head_dim, win, splits, T, step.num_seqs, step.max_len, step.max_new,
+        key = (few, tc, bf16, heads, kv_heads, head_dim, win, splits, T, step.num_seqs, step.max_len, step.max_new,
                None if single else (tuple(step.host_new), tuple(step.host_len)))
         plan = self._mass_plans.get(key)
         if plan is not None:
             return plan
         if few:
             at_once = self.lib.hb_attention_few_tc_tokens(heads, kv_heads, head_dim, step.max_new) if tc else 0
-            blocks = 0 if not at_once else step.num_seqs if single else sum(-(-n // at_once) for n in step.host_new)
+            # blocks of a sequence: of so many tokens, or without the tensor cores of so many pairs of a token and a head of the group
+            per, each = (at_once, 1) if at_once else (self.lib.hb_attention_few_block_pairs(), group)
+            new = [1] * step.num_seqs if single else step.host_new
+            blocks = sum(-(-n * each // per) for n in new)
             least = 1
             if splits is None:
-                seqs = [(1, step.max_len)] * step.num_seqs if single else zip(step.host_new, step.host_len)
-                seen = [-(-(min(ln, win + n) if win else ln) // 64) for n, ln in seqs for _ in range(-(-n // (at_once or 1)))]
-                splits, least = few_splits(seen, kv_heads if at_once else kv_heads * -(-group // 8), (2 if at_once else 3) * self.sm_count)
+                lens = [step.max_len] * step.num_seqs if single else step.host_len
+                seen = [-(-(min(ln, win + n) if win else ln) // 64) for n, ln in zip(new, lens) for _ in range(-(-n * each // per))]
+                slots = 2 if at_once else max(1, min(4, 200_000 // (6 * 32 * head_dim * (2 if tc or bf16 else 4))))
+                splits, least = few_splits(seen, kv_heads, slots * self.sm_count)
             splits = max(1, min(splits, (step.max_len + 63) // 64))
-            plan = (blocks, splits, least, self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len))
+            plan = (blocks, int(at_once > 0), splits, least, self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len))
         else:
             # the tensor cores take two tiles of 128 queries at a time: two heads, or with an odd group two blocks of tokens
             rows, keys = (128 if group % 2 == 0 else 256, self.lib.hb_attention_mass_tc_keys()) if tc else (64, 64)
@@ -1343,16 +1348,16 @@ class Ops:
         old, new, status, stream = before.data_ptr() if before is not None else None, mass.data_ptr(), self.status.data_ptr(), self._stream()
         # scratch of the call's own, from torch's allocator: two calls on two streams, or two captured graphs, share nothing
         if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * (heads // kv_heads) <= self.MASS_FEW_PAIRS:
-            blocks, splits, least, floats = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, heads, kv_heads, head_dim, win, step, splits)
+            blocks, tc, splits, least, floats = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
             scratch = torch.empty(floats, dtype=torch.float32, device=self.device)
-            self._call("hb_attention_mass_few", q_at, code, q_ld, k_at, v_at, pt.data_ptr(), pt.shape[1], step.tok_seq.data_ptr(),
-                       step.positions.data_ptr(), step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out_at, out_ld, scratch.data_ptr(), old, new,
-                       splits, least, T, step.num_seqs, step.max_new, step.max_len, heads, kv_heads, head_dim, scale, win, pages, blocks, status, stream)
+            self._call("hb_attention_mass_few", q_at, code, q_ld, k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(),
+                       step.seq_pos0.data_ptr(), out_at, out_ld, scratch.data_ptr(), old, new, splits, least, blocks, tc, T, step.num_seqs,
+                       step.max_new, step.max_len, heads, kv_heads, head_dim, scale, win, pages, status, stream)
             self.launches += 2
             return
         tc = bool(fast and self.use_tcgen05_attention and (q_at | out_at) % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0
                   and self.lib.hb_attention_prefill_tc_supported(heads, kv_heads, head_dim))
-        splits, q_blocks, key_tiles, shares, tiles, lse_ld, n_lse, n_parts, n_cut = self._mass_plan(False, tc, heads, kv_heads, head_dim, win, step, splits)
+        splits, q_blocks, key_tiles, shares, tiles, lse_ld, n_lse, n_parts, n_cut = self._mass_plan(False, tc, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
         scratch = torch.empty(n_lse + n_parts + n_cut, dtype=torch.float32, device=self.device)
         lse = scratch.data_ptr()
         parts, cut = lse + 4 * n_lse if n_parts else None, lse + 4 * (n_lse + n_parts) if n_cut else None

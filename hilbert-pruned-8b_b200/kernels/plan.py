@@ -30,13 +30,13 @@ def decode_splits(sequences: int, kv_heads: int, max_pages: int, cta_slots: int)
 
 def few_splits(pages, kv_heads: int, cta_slots: int):
     """Shares of a sequence's pages in a step of few tokens that keeps its scores: (the most of a sequence, the fewest pages of one);
-    ``pages``: how many each block of tokens sees.  As ``decode_splits``, but down to a page each while the device has room, since a second
-    kernel follows in any case.  With blocks of unequal lengths shares of about equal size that take one round of the device (32 of a
+    ``pages``: how many each block of tokens sees.  As ``decode_splits``, but down to a page each (64 shares at most) while the device has room, since
+    a second kernel follows in any case.  With blocks of unequal lengths shares of about equal size that take one round of the device (32 of a
     sequence at most)."""
     blocks, most, total = max(1, len(pages)), max(pages, default=1), sum(pages)
     if 4 * most * blocks <= 5 * total or total == 0:
         room = max(1, cta_slots) // (blocks * kv_heads)
-        return max(1, min(max(decode_splits(blocks, kv_heads, most, cta_slots), min(most, 16, room)), most)), 1
+        return max(1, min(max(decode_splits(blocks, kv_heads, most, cta_slots), min(most, 64, room)), most)), 1
     size = max(1, -(-total * kv_heads // cta_slots), -(-most // 32))
     while size < most and kv_heads * sum(-(-n // size) for n in pages) > cta_slots:
         size += 1

@@ -167,6 +167,9 @@ FEW = [
     (33, 1, 64, [500], [1], None),
     (6, 2, 128, [2000, 0, 61, 63], [8, 7, 6, 1], 50),
     (12, 1, 64, [130, 1000], [3, 8], None),
+    (16, 2, 152, [1434, 31, 32], [1, 1, 1], None),
+    (3, 1, 20, [40, 95], [7, 8], 30),
+    (7, 1, 1, [70], [3], None),
 ]
 TYPES = [torch.bfloat16, torch.float32]
 
