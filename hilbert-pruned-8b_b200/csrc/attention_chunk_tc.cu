@@ -203,6 +203,20 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                                                                  (APART || i > 0 || half == 0 || !more || mbar_wait(next_k, next_parity)));
                     if (!alive) break;
                     tc_fence_after();
+                    const int kbase = (jt0 + it) * FA_KEYS;
+                    if (i + half == 0 && (kbase < lo_cta || kbase + FA_KEYS > pos0 + n_new)) {
+                        // The tile that holds the sequence's end, or begins in front of the window: the values there are whatever a
+                        // page held before, or of a page that was given back, and 0 * NaN is NaN.
+                        const int from = lo_cta - kbase, to = pos0 + n_new - kbase;          // rows [from, to) stay; 128 bytes in each half
+                        for (int u = lane; u < FA_KEYS * 8 * HALVES; u += 32) {
+                            const int vr = u / (8 * HALVES), c = u % (8 * HALVES);
+                            if (vr < from || vr >= to)
+                                *reinterpret_cast<uint4*>(smem + (2 + CT_STAGES + sv) * TILE + (c >> 3) * FA_HALF_BYTES + vr * 128 + (c & 7) * 16) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                        }
+                        fence_async_shared();                  // before the tensor core reads them
+                        __syncwarp();
+                    }
                     if (elect_one()) {
 #pragma unroll
                         for (int kk = half * 4; kk < half * 4 + 4; kk++)
@@ -293,19 +307,6 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const float neg_m = m_run == -INFINITY ? 0.0f : -m_run;
             f32x2 sum[2] = {0ull, 0ull};
             const f32x2 neg2 = pair_of(neg_m, neg_m);
-            if (i == 0 && (jt0 + it + 1) * FA_KEYS > pos0 + n_new) {
-                // the tile that holds the sequence's end: values behind it are whatever a page held before, and 0 * NaN is NaN
-                const int s = it % CT_STAGES;
-                if (!mbar_wait(v_full0 + 8 * s, (it / CT_STAGES) & 1)) atomicExch(error_flag, 57);
-                const int from = pos0 + n_new - kbase;         // rows from..127, 128 bytes of each half
-                for (int u = threadIdx.x + from * 8 * HALVES; u < FA_KEYS * 8 * HALVES; u += 128) {
-                    const int vr = u / (8 * HALVES), c = u % (8 * HALVES);
-                    *reinterpret_cast<uint4*>(smem + (2 + CT_STAGES + s) * TILE + (c >> 3) * FA_HALF_BYTES + vr * 128 + (c & 7) * 16) =
-                        make_uint4(0u, 0u, 0u, 0u);
-                }
-                fence_async_shared();                          // before the tensor core reads them (tile 0's product is issued first)
-                __syncwarp();
-            }
 #pragma unroll
             for (int half = 0; half < 2; half++) {
                 if (edge) chunk_weights<false>(sv + 64 * half, scale2, neg2, tm_p + half * 32, sum);

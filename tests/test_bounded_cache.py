@@ -274,6 +274,27 @@ def test_attention_mass_notes_a_missing_page(ops, dtype, hd, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("new", [[300], [90], [5], [1]])
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.bfloat16, 80), (torch.float32, 64)])
+def test_pages_given_back_in_front_of_the_window(ops, dtype, hd, new):
+    """Pages that no token sees any more may be gone from the table, whatever the cache holds elsewhere (NaN here, in page 0 too)."""
+    seed = next(s for s in range(100) if 0 not in _tables([700 + new[0]], s)[0].tolist()[0])
+    c = Case(dtype, 6, 2, hd, [700], new, 100, seed=seed)
+    start = torch.zeros(c.pages, 2, PAGE, device=DEV)
+    full = start.clone()
+    want = c.run(ops, full, before=c.before)
+    gone = (700 - 100 + 1) // PAGE                       # whole pages in front of the oldest row that the first token sees
+    freed = c.table[0, :gone].clone()
+    c.table[0, :gone] = -1
+    mass = start.clone()
+    got = c.run(ops, mass, before=c.before)
+    assert torch.isfinite(got).all() and torch.equal(got, want)
+    full[freed.long()] = 0.0
+    assert torch.equal(mass, full)
+    ops.check_errors()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [[90, 40], [1, 3]])
 def test_captured_and_replayed(ops, new):
     """A captured call follows its inputs; two graphs that are replayed on two streams share nothing."""
@@ -490,7 +511,7 @@ def _attention_args(**kw):
     a = dict(qkv=torch.zeros(3, 64 * 6), heads=4, kv_heads=2, head_dim=64, k=torch.zeros(5, 2, 64, 64), v=torch.zeros(5, 2, 64, 64),
              out=torch.zeros(3, 256), mass=torch.zeros(5, 2, 64), before=None, tokens=3)
     a.update(kw)
-    step = n(num_tokens=a.pop("tokens"), num_seqs=1, page_tables=[torch.zeros(1, 2, dtype=torch.int32)], max_new=3, max_len=3, host_new=[3], host_len=[3])
+    step = n(num_tokens=a.pop("tokens"), num_seqs=1, page_tables=[a.pop("table", torch.zeros(1, 2, dtype=torch.int32))], max_new=3, max_len=3, host_new=[3], host_len=[3])
     cache = n(k=a.pop("k"), v=a.pop("v"), group=0, window=None)
     return dict(dict(scale=0.125, window=None, cache=cache, step=step), **a)
 
@@ -501,7 +522,8 @@ def _attention_args(**kw):
     (dict(k=torch.zeros(5, 2, 32, 64)), "cache"), (dict(v=torch.zeros(5, 64, 2, 64).transpose(1, 2)), "cache"),
     (dict(out=torch.zeros(3, 256, dtype=torch.bfloat16)), "dtype"), (dict(k=torch.zeros(5, 2, 64, 64).half()), "dtype"),
     (dict(mass=torch.zeros(4, 2, 64)), "mass"), (dict(mass=torch.zeros(5, 2, 64).double()), "mass"), (dict(mass=torch.zeros(5, 64, 2).mT), "mass"),
-    (dict(before=torch.zeros(5, 2, 63)), "before"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=NAN), "scale")])
+    (dict(before=torch.zeros(5, 2, 63)), "before"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=NAN), "scale"),
+    (dict(table=torch.zeros(1, 2, dtype=torch.int64)), "page table"), (dict(table=torch.zeros(1, 4, dtype=torch.int32)[:, ::2]), "page table")])
 def test_attention_mass_refuses(change, text):
     from hilbert_pruned_8b_b200.kernels.ops import KernelError
     with pytest.raises(KernelError, match=text):
