@@ -386,7 +386,7 @@ static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
 
 int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
                        const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts,
-                       int max_shares, int share_tiles, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale,
+                       int max_shares, int share_tiles, int join_tokens, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale,
                        int window, int n_pages, int* error_flag, cudaStream_t s) {
     HB_REQUIRE(hb_attention_prefill_tc_supported(n_heads, n_kv_heads, head_dim), "attention_mass: head size %d is not built for the tensor cores (64, 128)",
                head_dim);
@@ -413,6 +413,6 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
                                                       max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_pairs, scale, window, n_pages,
                                                       error_flag, s);
     if (rc || max_shares == 1) return rc;
-    return shares_join(sh, HB_BF16, out, out_stride, lse, lse_ld, 1, seq_start, seq_pos0, head_pairs ? FA_ROWS : 2 * FA_ROWS, FA_KEYS, window, n_tokens,
+    return shares_join(sh, join_tokens, HB_BF16, out, out_stride, lse, lse_ld, 1, seq_start, seq_pos0, head_pairs ? FA_ROWS : 2 * FA_ROWS, FA_KEYS, window, n_tokens,
                        n_seqs, n_heads, head_dim, s);
 }

@@ -225,7 +225,7 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
 }
 
 // out = sum_z o_z 2^(m_z - M) / sum_z l_z 2^(m_z - M), lse = M + log2 of that sum, for the rows whose block has several shares; a
-// block per token, a warp per head
+// warp per (token, head)
 template <typename T>
 __global__ void __launch_bounds__(256)
 shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, int rounded,
@@ -234,16 +234,23 @@ shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* 
     __shared__ float ws[8][32];
     pdl_trigger();
     pdl_wait();
-    const int t = blockIdx.x, lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31;
     int b, i, place0;
-    if (!mass_find_block(seq_start, n_seqs, t, 1, b, i, place0)) return;
-    const int place = rounded ? place0 + i : t;
-    const int n_new = seq_start[b + 1] - seq_start[b], row0 = (t - seq_start[b]) / span * span;
+    if (!mass_find(n_seqs, blockIdx.x,
+                   [&](int s) {
+                       const int n = seq_start[s + 1] - seq_start[s];
+                       return shares_may_cut(sh, seq_pos0[s] + n, span, window, keys) ? n : 0;
+                   },
+                   [&](int s) { return mass_round128(seq_start[s + 1] - seq_start[s]); }, b, i, place0))
+        return;
+    const int t = seq_start[b] + i, place = rounded ? place0 + i : t;
+    const int n_new = seq_start[b + 1] - seq_start[b], row0 = i / span * span;
     int tile0;
     const int S = shares_of(sh, key_tiles_of(seq_pos0[b] + row0, seq_pos0[b] + min(row0 + span, n_new) - 1, window, keys, tile0));
     if (S == 1) return;
     float* mine = ws[threadIdx.x >> 5];
-    for (int head = threadIdx.x >> 5; head < nh; head += 8) {
+    const int head = blockIdx.y * 8 + (threadIdx.x >> 5);
+    if (head < nh) {
         const size_t at = (size_t)head * n_tokens + t, step = (size_t)nh * n_tokens;
         float2 ml = make_float2(-INFINITY, 0.0f);              // of share `lane` (at most 32)
         if (lane < S) ml = __ldcg(reinterpret_cast<const float2*>(sh.ml) + at + lane * step);
@@ -262,13 +269,13 @@ shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* 
             const float total = L > 0.0f ? M + log2f(L) : INFINITY;
             lse[head * lse_ld + place] = rounded ? -total : total;
         }
-        __syncwarp();
     }
 }
 
-int shares_join(Shares sh, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded, const int* seq_start,
+int shares_join(Shares sh, int join_tokens, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded, const int* seq_start,
                 const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s) {
-    const dim3 grid(n_tokens);                             // a block per token: most tokens of a step with unequal sequences have one share
+    if (join_tokens == 0) return 0;
+    const dim3 grid(join_tokens, (nh + 7) / 8);
     cudaError_t e = dtype == HB_BF16 ? hb_launch(shares_join_kernel<bf16>, grid, dim3(256), 0, s, sh, (bf16*)out, out_stride, lse, lse_ld, rounded,
                                                  seq_start, seq_pos0, span, keys, window, n_tokens, n_seqs, nh, hd)
                                      : hb_launch(shares_join_kernel<float>, grid, dim3(256), 0, s, sh, (float*)out, out_stride, lse, lse_ld, rounded,
@@ -393,7 +400,7 @@ static int am_reserve(F* kernel, int bytes, bool (&done)[HB_MAX_DEVICES]) {
 
 template <typename T, int NC>
 static int launch_rows(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                       const int* seq_pos0, void* out, long long out_stride, float* lse, Shares sh, int max_shares, MassOut mo, int splits, int n_tokens,
+                       const int* seq_pos0, void* out, long long out_stride, float* lse, Shares sh, int max_shares, int join_tokens, MassOut mo, int splits, int n_tokens,
                        int n_seqs, int q_blocks, int key_tiles, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
     static_assert(AM_SMEM_ROWS(256) <= 227 * 1024, "attention tiles do not fit shared memory");
     static bool done[HB_MAX_DEVICES] = {}, done_mass[HB_MAX_DEVICES] = {};
@@ -407,7 +414,7 @@ static int launch_rows(const void* q, long long q_stride, const void* kc, const 
                               nkv, hd, scale * MASS_LOG2E, window, n_pages, vec_q, vec_kv, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     if (hb_check_launch("attention_mass (rows)")) return 1;
-    if (max_shares > 1 && shares_join(sh, sizeof(T) == 4 ? HB_F32 : HB_BF16, out, out_stride, lse, n_tokens, 0, seq_start, seq_pos0, AM_ROWS,
+    if (max_shares > 1 && shares_join(sh, join_tokens, sizeof(T) == 4 ? HB_F32 : HB_BF16, out, out_stride, lse, n_tokens, 0, seq_start, seq_pos0, AM_ROWS,
                                       HB_PAGE_TOKENS, window, n_tokens, n_seqs, nh, hd, s))
         return 1;
     e = hb_launch(mass_rows_kernel<T, NC>, dim3(key_tiles, nkv, splits), dim3(AM_THREADS), AM_SMEM_MASS(hd), s, (const T*)q, q_stride, (const T*)kc,
@@ -420,11 +427,12 @@ static int launch_rows(const void* q, long long q_stride, const void* kc, const 
 
 // Steps of many tokens.  q_blocks: sum over sequences of ceil(new tokens / 64); key_tiles: sum of ceil(rows / 64); lse:
 // n_heads * n_tokens floats; max_shares: the most blocks that a block of queries takes, share_tiles: the most pages of one of them;
+// join_tokens: the new tokens of the sequences that shares_may_cut;
 // chunk_parts: max_shares * n_heads * n_tokens * (head_dim + 2) floats when max_shares > 1; parts: splits * n_kv_heads * key_tiles * 64
 // floats when splits > 1.  before may be null or mass.
 extern "C" int hb_attention_mass(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
                                  int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse,
-                                 const float* before, float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int splits,
+                                 const float* before, float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int join_tokens, int splits,
                                  int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window,
                                  int n_pages, int* status, void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
@@ -441,7 +449,7 @@ extern "C" int hb_attention_mass(const void* q, int dtype, long long q_stride, c
                        max_shares == 1 ? 0x3fffffff : share_tiles};
     cudaStream_t s = (cudaStream_t)stream;
 #define HB_AM_LAUNCH(T, NC)                                                                                                                     \
-    launch_rows<T, NC>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, sh, max_shares, mo, splits, \
+    launch_rows<T, NC>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, sh, max_shares, join_tokens, mo, splits, \
                        n_tokens, n_seqs, q_blocks, key_tiles, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s)
     if (dtype == HB_F32) return head_dim <= 64 ? HB_AM_LAUNCH(float, 4) : head_dim <= 128 ? HB_AM_LAUNCH(float, 8) : HB_AM_LAUNCH(float, 16);
     return head_dim <= 64 ? HB_AM_LAUNCH(bf16, 4) : head_dim <= 128 ? HB_AM_LAUNCH(bf16, 8) : HB_AM_LAUNCH(bf16, 16);

@@ -255,14 +255,14 @@ static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const in
 
 extern "C" int hb_attention_mass_tc_keys(void) { return MT_KEYS; }
 
-// Sizes and types of hb_attention_prefill_tc, with the same alignment of queries and output.  q_blocks, chunk_parts, max_shares, share_tiles: as
-// attention_chunk_tc (attention_mass.cuh); key_tiles: sum over sequences of ceil(rows / 256); lse: n_heads * lse_ld
+// Sizes and types of hb_attention_prefill_tc, with the same alignment of queries and output.  q_blocks, chunk_parts, max_shares, share_tiles,
+// join_tokens: as attention_chunk_tc (attention_mass.cuh); key_tiles: sum over sequences of ceil(rows / 256); lse: n_heads * lse_ld
 // floats, lse_ld 128 * the sum of ceil(new tokens / 128); parts:
 // splits * n_kv_heads * key_tiles * 256 floats when splits > 1.
 extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
                                     const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, const float* before,
-                                    float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int splits, int n_tokens, int n_seqs, int q_blocks,
-                                    int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
+                                    float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int join_tokens,
+                                    int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
                                     void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(((uintptr_t)lse & 15) == 0 && lse_ld % 128 == 0, "attention_mass: the log-sums must be aligned");
@@ -271,7 +271,7 @@ extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const voi
                "attention_mass: bad sizes");
     cudaStream_t s = (cudaStream_t)stream;
     if (attention_chunk_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, chunk_parts, max_shares, share_tiles,
-                           n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s))
+                           join_tokens, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s))
         return 1;
     CUtensorMap mq, mk;
     if (tc_make_map(&mq, q, n_tokens, (long long)n_heads * head_dim, q_stride, 128)) return 1;

@@ -80,9 +80,11 @@ _SIGNATURES = {
     "hb_attention_prefill_tc": [_c_ptr, _c_ll, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_int,
                                 _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
-                          _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
+                          _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int,
+                          _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_tc": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr,
-                             _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
+                             _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int,
+                             _c_int, _c_ptr, _c_ptr],
     "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr,
                               _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int,
                               _c_ptr, _c_ptr],
@@ -1268,7 +1270,7 @@ class Ops:
     def _mass_plan(self, few: bool, tc: bool, bf16: bool, heads: int, kv_heads: int, head_dim: int, win: int, step, splits: Optional[int]):
         """How a step of ``attention_mass`` is cut, from its sizes alone: few tokens: (blocks, whether on the tensor cores, most
         shares of the pages, fewest pages of one, floats of scratch); many: (shares of the keys' sums, blocks of queries, tiles of keys, most shares of a block of
-        queries, tiles of keys in one, distance of two heads' log-sums, floats of the log-sums, of the sums' shares, of the partial results)."""
+        queries, tiles of keys in one, tokens whose blocks may be cut, distance of two heads' log-sums, floats of the log-sums, of the sums' shares, of the partial results)."""
         T, group = step.num_tokens, heads // kv_heads
         # (single tokens: from the page table's width alone, so that a captured step and an eager one sum alike)
         single = step.max_new == 1 and few
@@ -1298,13 +1300,13 @@ class Ops:
             key_tiles = sum(-(-n // keys) for n in step.host_len)
             if splits is None:
                 splits = mass_splits(key_tiles, kv_heads, group * -(-step.max_new // (128 if tc else 64)), self.sm_count * (1 if tc else 2))
-            shares, tiles = chunk_shares(step.host_new, step.host_len, win, rows, 128 if tc else 64, heads // 2 if tc and group % 2 == 0 else heads,
-                                         heads * (head_dim + 2), self.sm_count * (1 if tc or head_dim > 64 else 2))
+            shares, tiles, cut = chunk_shares(step.host_new, step.host_len, win, rows, 128 if tc else 64, heads // 2 if tc and group % 2 == 0 else heads,
+                                         heads * (head_dim + 2), self.sm_count * (1 if tc or head_dim > 64 else 2), *((4.5, 8.0) if tc else (1.0, 2.0)))
             lse_ld = 128 * sum(-(-n // 128) for n in step.host_new) if tc else T
 
             def round128(n: int) -> int:
                 return (n + 127) & ~127
-            plan = (splits, q_blocks, key_tiles, shares, tiles, lse_ld, round128(heads * lse_ld),
+            plan = (splits, q_blocks, key_tiles, shares, tiles, cut, lse_ld, round128(heads * lse_ld),
                     round128(splits * kv_heads * key_tiles * keys) if splits > 1 else 0,
                     shares * heads * T * (head_dim + 2) if shares > 1 else 0)
         if len(self._mass_plans) >= self.MASS_PLANS:
@@ -1361,12 +1363,12 @@ class Ops:
             return
         tc = bool(fast and self.use_tcgen05_attention and (q_at | out_at) % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0
                   and self.lib.hb_attention_prefill_tc_supported(heads, kv_heads, head_dim))
-        splits, q_blocks, key_tiles, shares, tiles, lse_ld, n_lse, n_parts, n_cut = self._mass_plan(False, tc, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
+        splits, q_blocks, key_tiles, shares, tiles, cut, lse_ld, n_lse, n_parts, n_cut = self._mass_plan(False, tc, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
         scratch = torch.empty(n_lse + n_parts + n_cut, dtype=torch.float32, device=self.device)
         lse = scratch.data_ptr()
-        parts, cut = lse + 4 * n_lse if n_parts else None, lse + 4 * (n_lse + n_parts) if n_cut else None
+        parts, partial = lse + 4 * n_lse if n_parts else None, lse + 4 * (n_lse + n_parts) if n_cut else None
         where = (k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out_at, out_ld, lse)
-        sizes = (old, new, parts, cut, shares, tiles, splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim, scale, win, pages, status,
+        sizes = (old, new, parts, partial, shares, tiles, cut, splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim, scale, win, pages, status,
                  stream)
         if tc:
             self._call("hb_attention_mass_tc", q_at, q_ld, *where, lse_ld, *sizes)

@@ -43,42 +43,42 @@ def few_splits(pages, kv_heads: int, cta_slots: int):
     return -(-most // size), size
 
 
-def chunk_shares(new, lengths, window: int, span: int, keys: int, units: int, row_floats: int, slots: int):
+def chunk_shares(new, lengths, window: int, span: int, keys: int, units: int, row_floats: int, slots: int, own: float, join: float):
     """How the keys of blocks of queries are shared out over blocks of threads: (the most shares of one block of queries, the most tiles of
-    ``keys`` keys in a share).  ``new`` tokens and ``lengths`` of the sequences, blocks of ``span`` tokens, ``units`` heads or pairs of heads,
+    ``keys`` keys in a share, the new tokens of sequences that may be cut).  ``new`` tokens and ``lengths`` of the sequences, blocks of ``span`` tokens, ``units`` heads or pairs of heads,
     ``row_floats`` floats that a share leaves per token, on a device with ``slots`` places.
 
     Blocks start with the ones that see the most keys, so a step lasts about as long as its work divided by the places, or as its
     longest block.  Where that is the longer of the two, blocks are cut: with shares of at most t tiles a step lasts about the lesser of
-    (work / places + t) and t times the rounds that its shares need.  A share costs about three tiles' time to start and end, and the kernel
-    that joins the shares four.  The partial results are at most 256 MB in all."""
-    blocks = []                                                            # per sequence: blocks, tiles that the last one sees
+    (work / places + t) and t times the rounds that its shares need.  To start and end a share takes the time of ``own``
+    tiles, the kernel that joins the shares that of ``join``.  (Measured: the tensor-core kernel 7 to 9 us against 1.6 to 2 us for a tile of 128
+    keys, the kernel for every type about 3 us like its tile of 64.)  The partial results are at most 256 MB in all."""
+    blocks = []                                                            # per sequence: blocks, tiles that one may see, new tokens
     work = 0.0
     for n, ln in zip(new, lengths):
         if n > 0:
             nb = -(-n // span)
             most = -(-min(ln, window + span if window else ln) // keys) + (1 if window else 0)
             least = min(most, -(-(ln - n + 1) // keys))
-            blocks.append((nb * units, most))
+            blocks.append((nb * units, most, n))
             work += nb * units * (most + least) / 2
     if not blocks:
-        return 1, 1
-    longest = max(t for _, t in blocks)
-    own = 3.0
-    count = sum(c for c, _ in blocks)
+        return 1, 1, 0
+    longest = max(t for _, t, _ in blocks)
+    count = sum(c for c, _, _ in blocks)
     ideal = (work + own * count) / slots
     if longest <= 4 or longest + own <= 1.25 * ideal:
-        return 1, longest
+        return 1, longest, 0
     best, shares, tiles = max(longest + own, min(ideal + longest / 2, (longest + own) * -(-count // slots))), 1, longest
     for s in (2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32):
         t = -(-longest // s)
-        if t < 2 or s * row_floats * sum(new) > 64 << 20:
+        if s > longest or s * row_floats * sum(new) > 64 << 20:
             break
-        count = sum(c * -(-m // t) for c, m in blocks)
-        cost = min((work + own * count) / slots + t, (t + own) * -(-count // slots)) + 4
+        count = sum(c * -(-m // t) for c, m, _ in blocks)
+        cost = min((work + own * count) / slots + t, (t + own) * -(-count // slots)) + join
         if cost < best:
             best, shares, tiles = cost, s, t
-    return shares, tiles
+    return shares, tiles, sum(n for _, m, n in blocks if m > tiles)
 
 
 def mass_splits(key_tiles: int, kv_heads: int, items: int, cta_slots: int) -> int:

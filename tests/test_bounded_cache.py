@@ -572,14 +572,15 @@ def test_shapes_of_the_launches():
         splits, least = few_splits(pages, 8, 296)
         assert 1 <= splits <= 32 and splits * least >= max(pages)
     assert mass_splits(1000, 8, 100, 296) == 1 and mass_splits(1, 1, 1, 296) == 1 and mass_splits(1, 1, 100, 296) == 16
-    assert chunk_shares([4096], [4096], 0, 128, 128, 16, 4160, 148) == (1, 32)                 # enough blocks for everybody
-    shares, tiles = chunk_shares([128], [100000], 0, 128, 128, 16, 4160, 148)                  # 16 blocks of 782 tiles
-    assert 8 <= shares <= 32 and (shares - 1) * tiles < 782 <= shares * tiles
-    assert chunk_shares([10, 0], [100, 7], 0, 128, 128, 16, 4160, 148) == (1, 1) and chunk_shares([], [], 0, 128, 128, 16, 4160, 148) == (1, 1)
+    assert chunk_shares([4096], [4096], 0, 128, 128, 16, 4160, 148, 4.5, 8.0) == (1, 32, 0)                 # enough blocks for everybody
+    shares, tiles, cut = chunk_shares([128], [100000], 0, 128, 128, 16, 4160, 148, 4.5, 8.0)                  # 16 blocks of 782 tiles
+    assert 8 <= shares <= 32 and (shares - 1) * tiles < 782 <= shares * tiles and cut == 128
+    assert chunk_shares([10, 0], [100, 7], 0, 128, 128, 16, 4160, 148, 4.5, 8.0) == (1, 1, 0) and chunk_shares([], [], 0, 128, 128, 16, 4160, 148, 4.5, 8.0) == (1, 1, 0)
     for window in (0, 1000):
         for new, lens in (([700, 33, 1], [700, 550, 5000]), ([2000] * 5, [9000] * 5), ([9], [10 ** 6])):
-            shares, tiles = chunk_shares(new, lens, window, 256, 64, 5, 100, 148)
+            shares, tiles, cut = chunk_shares(new, lens, window, 256, 64, 5, 100, 148, 1.0, 2.0)
             seen = max(min(ln, window + 256) if window else ln for ln in lens)
+            assert 0 <= cut <= sum(new) and (shares == 1 or cut > 0)
             assert 1 <= shares <= 32 and shares * tiles * 64 >= seen               # the device cuts a block into at most that many
     for rows in (1, 64, 1000, 16384, 16385, 70000, 131072, 300000, 10 ** 7):
         for lists in (1, 2, 16, 74, 75, 148, 256, 4096):
