@@ -326,6 +326,7 @@ int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_dim, int ma
 int hb_attention_few_pairs(void);
 long long hb_attention_mass_few_floats(int n_tokens, int n_heads, int head_dim, int splits, int max_len);
 int hb_attention_few_block_pairs(void);
+int hb_attention_few_blocks_per_sm(int head_dim, int dtype);
 int hb_attention_mass_few(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
                           int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* scratch,
                           const float* before, float* mass, int splits, int share_pages, int blocks, int tensor_cores, int n_tokens, int n_seqs,

@@ -458,7 +458,7 @@ extern "C" int hb_attention_mass(const void* q, int dtype, long long q_stride, c
 
 // -------------------------------------------------------------------------------------------- few tokens, every head size
 // A block per (share of the pages, kv head, eight (token, head) pairs of a sequence's new tokens and the kv head's group).  Keys and values
-// stream through shared memory in tiles of 32 rows, three cp.async stages, as they are stored.  Scores: a warp per pair, a lane per
+// stream through shared memory in tiles of 32 rows, cp.async stages, as they are stored.  Scores: a warp per pair, a lane per
 // key, so that the softmax is a warp's; values: a thread per two columns (and share of the tile's keys), all eight pairs at once.
 // Rows in shared memory lie an odd number of 16-byte units apart: the lanes' 16-byte reads of 32 rows then fall into different banks.
 // Bound by the FP32 pipe or by memory: 32 keys of head size 152 take about 900 clocks of instructions and 20 KB.  (Keys and values
@@ -467,15 +467,16 @@ extern "C" int hb_attention_mass(const void* q, int dtype, long long q_stride, c
 #define AF_THREADS 256
 #define AF_PAIRS 8
 #define AF_KEYS 32
-#define AF_STAGES 3
 
 static __host__ __device__ constexpr int af_row_bytes(int hd, int es) {
     const int units = (hd * es + 15) / 16;
     return (units | 1) * 16;
 }
-static __host__ __device__ constexpr int af_smem(int hd, int es) {
-    return AF_STAGES * 2 * AF_KEYS * af_row_bytes(hd, es) + AF_PAIRS * ((hd + 7) & ~7) * 4;
+static __host__ __device__ constexpr int af_smem(int hd, int es, int stages) {
+    return stages * 2 * AF_KEYS * af_row_bytes(hd, es) + AF_PAIRS * ((hd + 7) & ~7) * 4;
 }
+// three stages where two blocks of them fit an SM, else two (32-bit, head size 176: a second block hides more than a third stage)
+static __host__ __device__ constexpr int af_stages(int hd, int es) { return 2 * (af_smem(hd, es, 3) + 3 * 1024) <= 227 * 1024 ? 3 : 2; }
 
 // eight (bfloat16) or four (float32) elements of a 16-byte unit
 __device__ __forceinline__ void unpack16(const uint4& u, float (&x)[8], const bf16*) {
@@ -495,8 +496,8 @@ __device__ __forceinline__ float2 two_columns(const uint8_t* p, const bf16*) {
     return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(AF_THREADS)
+template <typename T, int AF_STAGES>
+__global__ void __launch_bounds__(AF_THREADS, 2)
 few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict__ kc, const T* __restrict__ vc, const int* __restrict__ page_table,
                 int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* __restrict__ part_o,
                 float* __restrict__ part_ml, float* __restrict__ scores, long long score_ld, int n_seqs, int nh, int nkv, int hd, int share_pages,
@@ -787,13 +788,16 @@ template <typename T>
 static int launch_few(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                       const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int blocks,
                       int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
-    static_assert(af_smem(256, 4) <= 227 * 1024, "tiles do not fit shared memory");
-    static bool done[HB_MAX_DEVICES] = {};
-    if (am_reserve(few_rows_kernel<T>, af_smem(256, sizeof(T)), done)) return 1;
-    const int vec = hd % (16 / (int)sizeof(T)) == 0 && (((uintptr_t)kc | (uintptr_t)vc) & 15) == 0;
-    cudaError_t e = hb_launch(few_rows_kernel<T>, dim3(splits, nkv, blocks), dim3(AF_THREADS), af_smem(hd, sizeof(T)), s, (const T*)q, q_stride, (const T*)kc,
-                              (const T*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, n_seqs, nh, nkv, hd, share_pages,
-                              scale * MASS_LOG2E, window, n_pages, vec, status);
+    static_assert(af_smem(256, 4, 2) <= 227 * 1024, "tiles do not fit shared memory");
+    static bool done[2][HB_MAX_DEVICES] = {};
+    if (am_reserve(few_rows_kernel<T, 2>, af_smem(256, sizeof(T), 2), done[0]) || am_reserve(few_rows_kernel<T, 3>, 114 * 1024, done[1])) return 1;
+    const int vec = hd % (16 / (int)sizeof(T)) == 0 && (((uintptr_t)kc | (uintptr_t)vc) & 15) == 0, stages = af_stages(hd, sizeof(T));
+#define HB_AF_LAUNCH(ST)                                                                                                                           \
+    hb_launch(few_rows_kernel<T, ST>, dim3(splits, nkv, blocks), dim3(AF_THREADS), af_smem(hd, sizeof(T), ST), s, (const T*)q, q_stride, (const T*)kc, \
+              (const T*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, n_seqs, nh, nkv, hd, share_pages,            \
+              scale * MASS_LOG2E, window, n_pages, vec, status)
+    cudaError_t e = stages == 3 ? HB_AF_LAUNCH(3) : HB_AF_LAUNCH(2);
+#undef HB_AF_LAUNCH
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (few tokens)");
 }
@@ -810,8 +814,12 @@ static int launch_finish(const float* part_o, const float* part_ml, const float*
     return hb_check_launch("attention_mass (finish)");
 }
 
-// Pairs of a token and a head that a block of the kernel for every head size takes.
+// Pairs of a token and a head that a block of the kernel for every head size takes, and how many of its blocks an SM holds.
 extern "C" int hb_attention_few_block_pairs(void) { return AF_PAIRS; }
+extern "C" int hb_attention_few_blocks_per_sm(int head_dim, int dtype) {
+    const int es = dtype == HB_F32 ? 4 : 2, bytes = af_smem(head_dim, es, af_stages(head_dim, es)) + 3 * 1024, n = 227 * 1024 / bytes;
+    return n < 1 ? 1 : n > 2 ? 2 : n;                      // registers hold two
+}
 
 // Steps of few tokens (at most hb_attention_few_pairs() pairs of a sequence's tokens and a group's heads).  `scratch` holds
 // hb_attention_mass_few_floats floats; blocks: the sum over sequences of ceil(pairs / hb_attention_few_block_pairs()), or with

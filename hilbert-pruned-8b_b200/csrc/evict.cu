@@ -412,6 +412,7 @@ evict_rows_kernel(EvictRows p, U* k, int k_units, int k_slices, U* v, int v_unit
     const int parts = k_slices + v_slices + (mass != nullptr ? 1 : 0);
     const int part = blockIdx.x % parts, row = blockIdx.y;
     const int j0 = (blockIdx.x / parts) * rows_per_block, j1 = min(j0 + rows_per_block, p.budget);
+    if (p.kept[(size_t)row * p.budget + j0] < 0) return;      // behind the last kept row
     if (part < k_slices) {
         const int a = k_units * part / k_slices, z = k_units * (part + 1) / k_slices;
         evict_move<U>(p, k, k_units, a, z - a, row, j0, j1);

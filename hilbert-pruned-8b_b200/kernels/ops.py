@@ -192,6 +192,7 @@ def load_library():
         lib.hb_attention_mass_tc_keys.argtypes, lib.hb_attention_mass_tc_keys.restype = [], _c_int
         lib.hb_attention_few_tc_tokens.argtypes, lib.hb_attention_few_tc_tokens.restype = [_c_int] * 4, _c_int
         lib.hb_attention_few_block_pairs.argtypes, lib.hb_attention_few_block_pairs.restype = [], _c_int
+        lib.hb_attention_few_blocks_per_sm.argtypes, lib.hb_attention_few_blocks_per_sm.restype = [_c_int] * 2, _c_int
         lib.hb_attention_few_pairs.argtypes, lib.hb_attention_few_pairs.restype = [], _c_int
         lib.hb_attention_mass_few_floats.argtypes, lib.hb_attention_mass_few_floats.restype = [_c_int] * 5, _c_ll
         lib.hb_attention_sink_prefill_supported.argtypes, lib.hb_attention_sink_prefill_supported.restype = [_c_int] * 4, _c_int
@@ -1289,7 +1290,7 @@ class Ops:
             if splits is None:
                 lens = [step.max_len] * step.num_seqs if single else step.host_len
                 seen = [-(-(min(ln, win + n) if win else ln) // 64) for n, ln in zip(new, lens) for _ in range(-(-n * each // per))]
-                slots = 2 if at_once else max(1, min(4, 200_000 // (6 * 32 * head_dim * (2 if tc or bf16 else 4))))
+                slots = 2 if at_once else self.lib.hb_attention_few_blocks_per_sm(head_dim, int(bf16))
                 splits, least = few_splits(seen, kv_heads, slots * self.sm_count)
             splits = max(1, min(splits, (step.max_len + 63) // 64))
             plan = (blocks, int(at_once > 0), splits, least, self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len))
