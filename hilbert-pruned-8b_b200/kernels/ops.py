@@ -1339,8 +1339,9 @@ class Ops:
         self._mass_like(mass, "mass", want[:3])
         if before is not None:
             self._mass_like(before, "before", want[:3])
-        if not 0.0 < scale < float("inf"):
-            raise KernelError(f"attention: the scale must be positive and finite, got {scale}")
+        scale, win = float(scale), int(window) if window else 0
+        if not 0.0 < scale < float("inf") or win < 0:
+            raise KernelError(f"attention: the scale must be positive and finite and the window none or positive, got {scale} and {window}")
         pt = step.page_tables[cache.group]
         self._tables("attention", pt)
         if T == 0:
@@ -1348,7 +1349,6 @@ class Ops:
         if self._elsewhere():
             with torch.cuda.device(self._index):
                 return self.attention_mass(qkv, heads, kv_heads, head_dim, cache, step, out, scale, window, mass, before, splits)
-        win = int(window) if window else 0
         code, q_ld, out_ld = _code(qkv), _rows(qkv, "attention queries"), _rows(out, "attention output")
         q_at, k_at, v_at, out_at = qkv.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
         fast = self.use_fast_attention and dtype == torch.bfloat16 and (k_at | v_at) % 16 == 0

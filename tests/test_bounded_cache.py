@@ -213,6 +213,23 @@ def test_shares_of_the_work(ops, dtype, heads, kv, hd, past, new, window, splits
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("most", [1, 3, 20])
+def test_many_sequences(ops, dtype, most):
+    """More sequences than a warp has lanes, some of them without new tokens, one much longer than the others."""
+    rng = random.Random(most)
+    past = [rng.choice([0, 1, 63, 64, 100]) for _ in range(70)]
+    new = [rng.randint(0, most) if p else rng.randint(1, most) for p in past]
+    new[-1] = most
+    past[40] = 3000
+    c = Case(dtype, 4, 2, 64, past, new, None, seed=most)
+    start = torch.zeros(c.pages, 2, PAGE, device=DEV)
+    mass = start.clone()
+    c.check(c.run(ops, mass, before=c.before), mass, c.before, start)
+    ops.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("new", [[70, 5], [1, 1]])
 def test_peaked_and_flat_rows(ops, dtype, new):
     """Scores far apart (one row has nearly all the weight) and all alike."""
@@ -523,7 +540,7 @@ def _attention_args(**kw):
     (dict(out=torch.zeros(3, 256, dtype=torch.bfloat16)), "dtype"), (dict(k=torch.zeros(5, 2, 64, 64).half()), "dtype"),
     (dict(mass=torch.zeros(4, 2, 64)), "mass"), (dict(mass=torch.zeros(5, 2, 64).double()), "mass"), (dict(mass=torch.zeros(5, 64, 2).mT), "mass"),
     (dict(before=torch.zeros(5, 2, 63)), "before"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=NAN), "scale"),
-    (dict(table=torch.zeros(1, 2, dtype=torch.int64)), "page table"), (dict(table=torch.zeros(1, 4, dtype=torch.int32)[:, ::2]), "page table")])
+    (dict(window=-5), "window"), (dict(table=torch.zeros(1, 2, dtype=torch.int64)), "page table"), (dict(table=torch.zeros(1, 4, dtype=torch.int32)[:, ::2]), "page table")])
 def test_attention_mass_refuses(change, text):
     from hilbert_pruned_8b_b200.kernels.ops import KernelError
     with pytest.raises(KernelError, match=text):
