@@ -5,9 +5,9 @@
 //   s = scale q_th . k_jg,  lse_th = log sum_j exp(s),  w = exp(s - lse_th),  out_th = sum_j w v_jg,
 //   mass_jg = (j appended by this step ? 0 : before_jg) + sum over the sequence's tokens t of the step and the heads h of g of w.
 // A row's weight is known only once the token has seen all its keys, and then the scores are gone.  Two ways:
-//   steps of few tokens   (memory-bound: keys and values are read once per token, a page at a time, by several blocks) the scores
-//                         themselves are written beside the partial results, 4 bytes per (head, row) against the 2 head sizes of a
-//                         key and a value; one more launch joins the partial results and turns the scores into weights.
+//   steps of few tokens   (memory-bound) the scores themselves are written beside the partial results, 4 bytes per (head, row) against
+//                         the 2 head sizes of a key and a value; one more launch joins the partial results and turns the scores into
+//                         weights.  Keys and values are read once for a block of (token, head) pairs.
 //   steps of many tokens  (bound by arithmetic) the tokens' log-sums are kept and a second kernel, a block per tile of keys,
 //                         computes its keys' scores with all queries once more: half as much arithmetic again instead of
 //                         writing and reading a weight for every (token, head, row).  Every key's sum belongs to one thread from
