@@ -314,7 +314,8 @@ int hb_attention_mass(const void* q, int dtype, long long q_stride, const void* 
                       const float* before, float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int join_tokens, int splits,
                       int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window,
                       int n_pages, int* status, void* stream);
-// the same on tcgen05 (attention_mass_tc.cu), sizes of hb_attention_prefill_tc; key tiles of hb_attention_mass_tc_keys() rows
+// the same on tcgen05 (attention_chunk_tc.cu, attention_mass_tc.cu), bfloat16, head sizes up to 128 in steps of 8; key tiles of hb_attention_mass_tc_keys() rows
+int hb_attention_mass_tc_supported(int n_heads, int n_kv_heads, int head_dim);
 int hb_attention_mass_tc_keys(void);
 int hb_attention_mass_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
                          const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld,

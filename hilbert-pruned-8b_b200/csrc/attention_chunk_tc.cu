@@ -1,5 +1,5 @@
 // Attention of a chunk of new tokens over the paged cache on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), bfloat16, head
-// size 64 or 128, that leaves each row's log-sum, negated, for the weights' kernel (attention_mass_tc.cu): causal, grouped, with a window,
+// sizes up to 128 in steps of 8, that leaves each row's log-sum, negated, for the weights' kernel (attention_mass_tc.cu): causal, grouped, with a window,
 // sequences with unequal numbers of new tokens, the keys cut into shares where there are few rows.
 //
 // One CTA = two tiles of 128 query rows that read the same keys and values: two heads of a kv head with an even group, else two
@@ -17,6 +17,7 @@
 //   warp 8          TMA producer: the query tiles once, then key and value tiles of 128 rows (two pages), two stages each
 //   warp 9          owns tensor memory; one thread issues, per key tile and in this order: O0 += P0 V, S0 = Q0 K' (the next keys),
 //                   O1 += P1 V, S1 = Q1 K'; with head size 64, whose weights do not lie over the scores, a tile's S before its O.
+// Built for tiles of HD = 64 and 128 columns; a smaller head size hd has the rest of its tiles filled with zeros by the copies.
 // Weights are rounded to bfloat16 for the product with the values (the sum they are divided by is taken before that).
 //
 // Every wait is bounded; a wait that runs out sets *error_flag and the CTA drains and leaves.
@@ -57,7 +58,7 @@ template <int HD>
 __global__ void __launch_bounds__(CT_THREADS, 1)
 chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
-                bf16* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, Shares sh, int n_tokens, int n_seqs, int nh, int nkv, int head_pairs, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
+                bf16* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, Shares sh, int n_tokens, int n_seqs, int nh, int nkv, int hd, int head_pairs, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // [Q tiles 2][K stages][V stages][barriers]; a tile is 128 rows x HD
@@ -123,7 +124,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             mbar_expect_tx(q_full, 2 * TILE);
             for (int i = 0; i < 2; i++)
                 for (int half = 0; half < HALVES; half++)
-                    tma_load_2d(smem_base + i * TILE + half * FA_HALF_BYTES, &map_q, q_full, (head0 + (head_pairs ? i : 0)) * HD + half * 64,
+                    tma_load_3d(smem_base + i * TILE + half * FA_HALF_BYTES, &map_q, q_full, half * 64, head0 + (head_pairs ? i : 0),
                                 t_begin + row0 + (head_pairs ? 0 : i * FA_ROWS));
             auto load_tile = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int it) {
                 mbar_expect_tx(bar, TILE);
@@ -172,6 +173,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
             const int st = it % CT_STAGES;
 #pragma unroll
             for (int kk = 0; kk < HD / 16; kk++) {
+                if (kk * 16 >= hd) break;
                 const uint32_t off = (kk >> 2) * FA_HALF_BYTES + (kk & 3) * 32;
                 umma_bf16(tmem_base + i * 128, q_desc + ((i * TILE + off) >> 4), k_desc + ((st * TILE + off) >> 4), idesc_qk, kk ? 1u : 0u);
             }
@@ -334,19 +336,21 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 if (S > 1) *reinterpret_cast<float2*>(sh.ml + at * 2) = make_float2(m_run, l);
                 else lse[head * lse_ld + place0 + row] = l > 0.0f ? -(m_run + log2f(l)) : -INFINITY;
             }
-            bf16* dst = out + (size_t)(t_begin + row) * out_stride + (size_t)head * HD;
-            float4* po = reinterpret_cast<float4*>(sh.o + at * HD);
+            bf16* dst = out + (size_t)(t_begin + row) * out_stride + (size_t)head * hd;
+            float4* po = reinterpret_cast<float4*>(sh.o + at * hd);
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; c++) {
+            for (int c = 0; c * 32 < hd; c++) {
                 float v[32];
                 tmem_ld32(tm_o + c * 32, v);
                 if (!valid) continue;
                 if (S > 1) {
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) po[c * 8 + (e >> 2)] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    for (int e = 0; e < 32; e += 4)
+                        if (c * 32 + e < hd) po[c * 8 + (e >> 2)] = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
+                        if (c * 32 + e >= hd) break;
                         uint4 o4;
                         o4.x = pack_bf16_pair(v[e] * inv, v[e + 1] * inv);
                         o4.y = pack_bf16_pair(v[e + 2] * inv, v[e + 3] * inv);
@@ -369,7 +373,7 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 template <int HD>
 static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width, const int* seq_start,
                         const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, Shares sh, int max_shares, int n_tokens, int n_seqs, int q_blocks,
-                        int nh, int nkv, int head_pairs, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
+                        int nh, int nkv, int hd, int head_pairs, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
     constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 22 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "attention tiles do not fit shared memory");
     static bool done[HB_MAX_DEVICES] = {};
@@ -380,18 +384,22 @@ static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
         set = true;
     }
     cudaError_t e = hb_launch(chunk_tc_kernel<HD>, dim3(head_pairs ? nh / 2 : nh, q_blocks, max_shares), dim3(CT_THREADS), SMEM, s, mq, mk, mv, page_table,
-                              pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, sh, n_tokens, n_seqs, nh, nkv, head_pairs,
+                              pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, sh, n_tokens, n_seqs, nh, nkv, hd, head_pairs,
                               scale * FA_LOG2E, window, n_pages, error_flag);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (chunk)");
+}
+
+extern "C" int hb_attention_mass_tc_supported(int n_heads, int n_kv_heads, int head_dim) {
+    return head_dim > 0 && head_dim <= 128 && head_dim % 8 == 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0;
 }
 
 int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
                        const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts,
                        int max_shares, int share_tiles, int join_tokens, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale,
                        int window, int n_pages, int* error_flag, cudaStream_t s) {
-    HB_REQUIRE(hb_attention_prefill_tc_supported(n_heads, n_kv_heads, head_dim), "attention_mass: head size %d is not built for the tensor cores (64, 128)",
-               head_dim);
+    HB_REQUIRE(hb_attention_mass_tc_supported(n_heads, n_kv_heads, head_dim),
+               "attention_mass: %d heads over %d of size %d are not built for the tensor cores (sizes up to 128 in steps of 8)", n_heads, n_kv_heads, head_dim);
     HB_REQUIRE(q_blocks > 0 && q_blocks <= 65535 && error_flag != nullptr && max_shares >= 1 && max_shares <= 32 && share_tiles >= 1 &&
                    (max_shares == 1 || parts != nullptr),
                "attention_mass: the step is too large for one launch");
@@ -401,18 +409,18 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
     CUtensorMap mq, mk, mv;
     const long long cache_rows = (long long)n_pages * n_kv_heads * HB_PAGE_TOKENS;
     HB_REQUIRE(cache_rows <= 0x7fffffffLL, "attention_mass: the cache has too many rows for a tensor map");
-    if (tc_make_map(&mq, q, n_tokens, (long long)n_heads * head_dim, q_stride, FA_ROWS)) return 1;
+    if (tc_make_map_heads(&mq, q, n_tokens, n_heads, head_dim, q_stride, FA_ROWS)) return 1;
     if (tc_make_map(&mk, k_cache, cache_rows, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     if (tc_make_map(&mv, v_cache, cache_rows, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     const int head_pairs = (n_heads / n_kv_heads) % 2 == 0;
     // one share: no block is cut, whatever it sees
     const Shares sh = {parts, parts == nullptr ? nullptr : parts + (size_t)max_shares * n_heads * n_tokens * head_dim,
                        max_shares == 1 ? 0x3fffffff : share_tiles};
-    const int rc = head_dim == 128 ? launch_chunk<128>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, sh,
-                                                       max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_pairs, scale, window, n_pages,
+    const int rc = head_dim > 64 ? launch_chunk<128>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, sh,
+                                                       max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, head_pairs, scale, window, n_pages,
                                                        error_flag, s)
                                    : launch_chunk<64>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, sh,
-                                                      max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_pairs, scale, window, n_pages,
+                                                      max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, head_pairs, scale, window, n_pages,
                                                       error_flag, s);
     if (rc || max_shares == 1) return rc;
     return shares_join(sh, join_tokens, HB_BF16, out, out_stride, lse, lse_ld, 1, seq_start, seq_pos0, head_pairs ? FA_ROWS : 2 * FA_ROWS, FA_KEYS, window, n_tokens,

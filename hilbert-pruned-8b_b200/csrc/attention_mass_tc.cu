@@ -1,5 +1,5 @@
-// The weights of steps of many tokens on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), bfloat16, head size 64 or 128:
-// the second half of attention_mass.cu's arithmetic, behind the attention that leaves each row's log-sum (attention_chunk_tc.cu).
+// The weights of steps of many tokens on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), bfloat16, head sizes up to 128
+// in steps of 8 (as attention_chunk_tc.cu): the second half of attention_mass.cu's arithmetic, behind the attention that leaves each row's log-sum (attention_chunk_tc.cu).
 //
 // One CTA = 256 consecutive rows of a sequence's cache x one kv head x a share of the (head, 128 queries) tiles that see them.
 // Keys are the M operand: a tile's 128 keys are the 128 lanes of tensor memory and the queries its columns, so that a key's sum over
@@ -34,7 +34,7 @@ template <int HD>
 __global__ void __launch_bounds__(MT_THREADS, 1)
 mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const int* __restrict__ page_table, int pt_width,
                const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* lse, long long lse_ld, MassOut mo, int n_seqs, int nh,
-               int nkv, float scale_log2e, int window, int n_pages, int S, int* __restrict__ error_flag) {
+               int nkv, int hd, float scale_log2e, int window, int n_pages, int S, int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // [K tiles 2][Q stages 3][log-sums of the stages][barriers]; a tile is 128 rows x HD
@@ -112,7 +112,7 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 const int item = it0 + it, head = g * G + item / blocks, q0 = (item % blocks) * 128;
                 mbar_expect_tx(q_full0 + 8 * s, TILE + 512);
                 for (int half = 0; half < HALVES; half++)
-                    tma_load_2d(q_smem + s * TILE + half * FA_HALF_BYTES, &map_q, q_full0 + 8 * s, head * HD + half * 64, t_begin + n0 + q0);
+                    tma_load_3d(q_smem + s * TILE + half * FA_HALF_BYTES, &map_q, q_full0 + 8 * s, half * 64, head, t_begin + n0 + q0);
                 bulk_load(smem_u32(xlse + s * 128), lse + (size_t)head * lse_ld + lse0 + q0, 512, q_full0 + 8 * s);
                 issued = it + 1;
             }
@@ -141,6 +141,7 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 for (int k = 0; k < 2; k++)
 #pragma unroll
                     for (int kk = 0; kk < HD / 16; kk++) {
+                        if (kk * 16 >= hd) break;
                         const uint32_t off = (kk >> 2) * FA_HALF_BYTES + (kk & 3) * 32;
                         umma_bf16(tmem_base + (2 * sb + k) * 128, k_desc + ((k * TILE + off) >> 4), q_desc + ((s * TILE + off) >> 4), idesc, kk ? 1u : 0u);
                     }
@@ -236,7 +237,7 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 
 template <int HD>
 static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0,
-                          const float* lse, long long lse_ld, MassOut mo, int splits, int n_seqs, int key_tiles, int nh, int nkv, float scale, int window,
+                          const float* lse, long long lse_ld, MassOut mo, int splits, int n_seqs, int key_tiles, int nh, int nkv, int hd, float scale, int window,
                           int n_pages, int* error_flag, cudaStream_t s) {
     constexpr int SMEM = (2 + MT_STAGES) * (HD / 64) * FA_HALF_BYTES + (MT_STAGES * 128 + 256) * 4 + 16 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "key and query tiles do not fit shared memory");
@@ -248,14 +249,14 @@ static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const in
         set = true;
     }
     cudaError_t e = hb_launch(mass_tc_kernel<HD>, dim3(key_tiles * nkv * splits), dim3(MT_THREADS), SMEM, s, mq, mk, page_table, pt_width, seq_start,
-                              seq_pos0, lse, lse_ld, mo, n_seqs, nh, nkv, scale * FA_LOG2E, window, n_pages, splits, error_flag);
+                              seq_pos0, lse, lse_ld, mo, n_seqs, nh, nkv, hd, scale * FA_LOG2E, window, n_pages, splits, error_flag);
     if (e != cudaSuccess) return hb_fail("attention_mass_tc: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass_tc");
 }
 
 extern "C" int hb_attention_mass_tc_keys(void) { return MT_KEYS; }
 
-// Sizes and types of hb_attention_prefill_tc, with the same alignment of queries and output.  q_blocks, chunk_parts, max_shares, share_tiles,
+// bfloat16, sizes of hb_attention_mass_tc_supported, queries and output with 16-byte aligned rows.  q_blocks, chunk_parts, max_shares, share_tiles,
 // join_tokens: as attention_chunk_tc (attention_mass.cuh); key_tiles: sum over sequences of ceil(rows / 256); lse: n_heads * lse_ld
 // floats, lse_ld 128 * the sum of ceil(new tokens / 128); parts:
 // splits * n_kv_heads * key_tiles * 256 floats when splits > 1.
@@ -274,13 +275,13 @@ extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const voi
                            join_tokens, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s))
         return 1;
     CUtensorMap mq, mk;
-    if (tc_make_map(&mq, q, n_tokens, (long long)n_heads * head_dim, q_stride, 128)) return 1;
+    if (tc_make_map_heads(&mq, q, n_tokens, n_heads, head_dim, q_stride, 128)) return 1;
     if (tc_make_map(&mk, k_cache, (long long)n_pages * n_kv_heads * HB_PAGE_TOKENS, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
     MassOut mo = {before, mass, parts};
-    const int rc = head_dim == 128 ? launch_mass_tc<128>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, lse_ld, mo, splits, n_seqs, key_tiles,
-                                                         n_heads, n_kv_heads, scale, window, n_pages, error_flag, s)
+    const int rc = head_dim > 64 ? launch_mass_tc<128>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, lse_ld, mo, splits, n_seqs, key_tiles,
+                                                         n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s)
                                    : launch_mass_tc<64>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, lse_ld, mo, splits, n_seqs, key_tiles,
-                                                        n_heads, n_kv_heads, scale, window, n_pages, error_flag, s);
+                                                        n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s);
     if (rc) return rc;
     return splits > 1 ? mass_join(page_table, pt_width, seq_start, seq_pos0, mo, n_seqs, n_kv_heads, n_pages, MT_KEYS, key_tiles, splits, s) : 0;
 }

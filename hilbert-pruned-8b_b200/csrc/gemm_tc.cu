@@ -88,6 +88,20 @@ int tc_make_map_blocks(CUtensorMap* map, const void* base, long long rows, long 
     return 0;
 }
 
+int tc_make_map_heads(CUtensorMap* map, const void* base, long long rows, long long heads, long long hd, long long ld, int box_rows) {
+    EncodeTiledFn enc = get_encode();
+    if (!enc) return hb_fail("gemm_tc: cuTensorMapEncodeTiled is not available from this driver");
+    cuuint64_t dims[3] = {(cuuint64_t)hd, (cuuint64_t)heads, (cuuint64_t)rows};
+    cuuint64_t strides[2] = {(cuuint64_t)hd * 2, (cuuint64_t)ld * 2};
+    cuuint32_t box[3] = {TC_BK, 1, (cuuint32_t)box_rows};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, (void*)base, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS)
+        return hb_fail("gemm_tc: tensor map encode failed with code %d (%lld rows of %lld heads of size %lld)", (int)r, rows, heads, hd);
+    return 0;
+}
+
 int tc_make_out_map(CUtensorMap* map, const void* base, int elem_bytes, long long rows, long long cols, long long ld,
                     int box_rows, int box_cols) {
     EncodeTiledFn enc = get_encode();

@@ -512,6 +512,9 @@ int tc_make_map(CUtensorMap* map, const void* base, long long rows, long long co
 // Tensor map of a bf16 matrix stored in column blocks, [block][rows][64 columns]: boxes of box_blocks x box_rows x 64 elements, so
 // that one copy brings several column blocks of some rows, each as a tile of its own; zeros outside.
 int tc_make_map_blocks(CUtensorMap* map, const void* base, long long rows, long long blocks, int box_rows, int box_blocks);
+// Tensor map of rows of bf16 heads, [rows][heads][hd] with row stride ld (elements): boxes of box_rows x one head x 64 columns, zeros
+// behind a head's columns (hd a multiple of 8).
+int tc_make_map_heads(CUtensorMap* map, const void* base, long long rows, long long heads, long long hd, long long ld, int box_rows);
 // Tensor map of a row-major output [rows, cols] of float32 (elem_bytes 4) or bfloat16 (2) with
 // row stride ld (elements), for stores of boxes of box_rows x box_cols elements, no swizzle.
 // The base must be 16-byte aligned and ld * elem_bytes a multiple of 16.

@@ -189,6 +189,7 @@ def load_library():
         lib.hb_gemm_tc2_resident_pairs.argtypes, lib.hb_gemm_tc2_resident_pairs.restype = [_c_int], _c_int
         for name in ("hb_attention_decode_supported", "hb_attention_prefill_supported", "hb_attention_prefill_tc_supported"):
             getattr(lib, name).argtypes, getattr(lib, name).restype = [_c_int, _c_int, _c_int], _c_int
+        lib.hb_attention_mass_tc_supported.argtypes, lib.hb_attention_mass_tc_supported.restype = [_c_int] * 3, _c_int
         lib.hb_attention_mass_tc_keys.argtypes, lib.hb_attention_mass_tc_keys.restype = [], _c_int
         lib.hb_attention_few_tc_tokens.argtypes, lib.hb_attention_few_tc_tokens.restype = [_c_int] * 4, _c_int
         lib.hb_attention_few_block_pairs.argtypes, lib.hb_attention_few_block_pairs.restype = [], _c_int
@@ -1300,7 +1301,7 @@ class Ops:
             q_blocks = sum(-(-n // rows) for n in step.host_new)
             key_tiles = sum(-(-n // keys) for n in step.host_len)
             if splits is None:
-                splits = mass_splits(key_tiles, kv_heads, group * -(-step.max_new // (128 if tc else 64)), self.sm_count * (1 if tc else 2))
+                splits = mass_splits(step.host_new, step.host_len, win, keys, 128 if tc else 64, kv_heads, group, self.sm_count * (1 if tc else 2))
             shares, tiles, cut = chunk_shares(step.host_new, step.host_len, win, rows, 128 if tc else 64, heads // 2 if tc and group % 2 == 0 else heads,
                                          heads * (head_dim + 2), self.sm_count * (1 if tc or head_dim > 64 else 2), *((4.5, 8.0) if tc else (1.0, 2.0)))
             lse_ld = 128 * sum(-(-n // 128) for n in step.host_new) if tc else T
@@ -1363,7 +1364,7 @@ class Ops:
             self.launches += 2
             return
         tc = bool(fast and self.use_tcgen05_attention and (q_at | out_at) % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0
-                  and self.lib.hb_attention_prefill_tc_supported(heads, kv_heads, head_dim))
+                  and self.lib.hb_attention_mass_tc_supported(heads, kv_heads, head_dim))
         splits, q_blocks, key_tiles, shares, tiles, cut, lse_ld, n_lse, n_parts, n_cut = self._mass_plan(False, tc, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
         scratch = torch.empty(n_lse + n_parts + n_cut, dtype=torch.float32, device=self.device)
         lse = scratch.data_ptr()

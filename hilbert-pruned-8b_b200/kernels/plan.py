@@ -81,12 +81,24 @@ def chunk_shares(new, lengths, window: int, span: int, keys: int, units: int, ro
     return shares, tiles, sum(n for _, m, n in blocks if m > tiles)
 
 
-def mass_splits(key_tiles: int, kv_heads: int, items: int, cta_slots: int) -> int:
-    """Shares of the weights' kernel for ``key_tiles`` x ``kv_heads`` (tile of keys, kv head) pairs with up to ``items`` tiles of
-    queries each: under a causal mask the first keys are seen by every query and the last by few, so the work evens out only
-    over several blocks per slot.  Four times as many blocks as slots, at most 16 shares, and a share has work."""
-    pairs = max(1, key_tiles * kv_heads)
-    return max(1, min(16, items, -(-4 * max(1, cta_slots) // pairs)))
+def mass_splits(new, lengths, window: int, tile: int, span: int, kv_heads: int, group: int, cta_slots: int) -> int:
+    """Shares of the weights' kernel, whose block takes a tile of keys and goes through the tiles of ``span`` queries of each head that see
+    it.  Under a causal mask the first keys are seen by every query and the last by few, and the heaviest tiles start first: shares so
+    that a heaviest one is about an even share of the work (4096-token prompt: 2, 227 us in all, against 313 with 1 and 239 with 5)."""
+    most = total = 0
+    for n, ln in zip(new, lengths):
+        if n > 0:
+            blocks = -(-n // span)
+            seen = min(blocks, (window + tile) // span + 1) if window else blocks
+            most = max(most, seen)
+            old, fresh = (ln - n) // tile, n // tile + 1                  # tiles of older rows, of the step's own
+            if window:
+                old = min(old, -(-window // tile))
+            total += old * seen + fresh * (seen + 1) / 2 if not window else (old + fresh) * (seen + 1) / 2
+    if not most:
+        return 1
+    even = max(1.0, total * group * kv_heads / max(1, cta_slots))
+    return max(1, min(16, most * group, round(most * group / even)))
 
 
 def select_shape(lists: int, rows: int, sms: int):

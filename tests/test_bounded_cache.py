@@ -149,6 +149,10 @@ MANY = [
     (3, 1, 64, [5000, 100], [30, 10], 2000),
     (8, 8, 64, [0, 300], [513, 129], None),
     (6, 2, 128, [0, 131], [400, 255], 130),
+    (24, 8, 72, [0, 130], [290, 11], None),      # head sizes between the tensor cores' tiles
+    (4, 2, 120, [300, 0], [30, 140], 90),
+    (6, 1, 56, [1000], [129], None),
+    (2, 1, 16, [0, 5000], [300, 20], None),
 ]
 FEW = [
     (4, 2, 64, [0], [1], None),
@@ -588,7 +592,9 @@ def test_shapes_of_the_launches():
     for pages in ([33, 126, 9, 65], [1, 1, 2000], [7] * 50 + [900]):
         splits, least = few_splits(pages, 8, 296)
         assert 1 <= splits <= 32 and splits * least >= max(pages)
-    assert mass_splits(1000, 8, 100, 296) == 1 and mass_splits(1, 1, 1, 296) == 1 and mass_splits(1, 1, 100, 296) == 16
+    assert mass_splits([4096], [4096], 0, 256, 128, 8, 4, 148) == 2 and mass_splits([2048], [32049], 0, 256, 128, 8, 4, 148) == 1
+    assert mass_splits([1], [1], 0, 64, 64, 1, 1, 296) == 1 and mass_splits([9000], [9000], 0, 64, 64, 1, 1, 296) == 4
+    assert mass_splits([], [], 0, 64, 64, 1, 1, 296) == 1 and 1 <= mass_splits([0, 500], [7, 900], 30, 64, 64, 2, 3, 296) <= 6
     assert chunk_shares([4096], [4096], 0, 128, 128, 16, 4160, 148, 4.5, 8.0) == (1, 32, 0)                 # enough blocks for everybody
     shares, tiles, cut = chunk_shares([128], [100000], 0, 128, 128, 16, 4160, 148, 4.5, 8.0)                  # 16 blocks of 782 tiles
     assert 8 <= shares <= 32 and (shares - 1) * tiles < 782 <= shares * tiles and cut == 128
