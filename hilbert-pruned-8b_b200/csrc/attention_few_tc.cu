@@ -1,5 +1,5 @@
-// The first half of a step of few tokens with accumulated weights (attention_mass.cu) on the tensor cores, bfloat16, head size 64 or
-// 128: partial results over shares of the keys, and the scores themselves, for the kernel that joins the shares and turns the
+// The first half of a step of few tokens with accumulated weights (attention_mass.cu) on the tensor cores, bfloat16, head sizes up to
+// 128 in steps of 8: partial results over shares of the keys, and the scores themselves, for the kernel that joins the shares and turns the
 // scores into weights.
 //
 // A CTA = a share of the pages x one kv head x a block of a sequence's new tokens: the rows of the mma.sync tiles (16 RT of them) are the
@@ -16,13 +16,15 @@
 
 #define FT_STAGES 3
 
-template <int HD, int RT>
+// FULL: the head size is HD; else it is hd < HD, and the columns behind it are zeros in the tiles and in the queries.
+template <int HD, int RT, bool FULL>
 __global__ void __launch_bounds__(128 * RT, 2)
 few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __restrict__ kc, const bf16* __restrict__ vc,
               const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* part_o,
-              float* part_ml, float* scores, long long score_ld, int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, float scale_log2e,
-              int window, int n_pages, int* status) {
+              float* part_ml, float* scores, long long score_ld, int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd_given,
+              float scale_log2e, int window, int n_pages, int* status) {
     constexpr int ROW_BYTES = HD * 2, TILE_BYTES = HB_PAGE_TOKENS * ROW_BYTES, CHUNKS = ROW_BYTES / 16, KSTEPS = HD / 16, ROWS = 16 * RT, THREADS = 128 * RT;
+    const int hd = FULL ? HD : hd_given, chunks = FULL ? CHUNKS : hd / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_trigger();
     pdl_wait();
@@ -58,12 +60,12 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
                 bad_page = true;
                 page = 0;                                   // never read outside the cache
             }
-            const uint8_t* ksrc = (const uint8_t*)(kc + ((size_t)page * nkv + g) * HB_PAGE_TOKENS * HD);
-            const uint8_t* vsrc = (const uint8_t*)(vc + ((size_t)page * nkv + g) * HB_PAGE_TOKENS * HD);
+            const uint8_t* ksrc = (const uint8_t*)(kc + ((size_t)page * nkv + g) * HB_PAGE_TOKENS * hd);
+            const uint8_t* vsrc = (const uint8_t*)(vc + ((size_t)page * nkv + g) * HB_PAGE_TOKENS * hd);
             const uint32_t kdst = smem_base + stage * 2 * TILE_BYTES, vdst = kdst + TILE_BYTES;
 #pragma unroll
-            for (int i = tid; i < HB_PAGE_TOKENS * CHUNKS; i += THREADS) {
-                const int row = i / CHUNKS, ch = i % CHUNKS;
+            for (int i = tid; i < HB_PAGE_TOKENS * chunks; i += THREADS) {
+                const int row = i / chunks, ch = i - row * chunks;
                 const uint32_t off = swizzled<ROW_BYTES>(row, ch);
                 cp_async_16(kdst + off, ksrc + (size_t)i * 16);
                 // values behind the last key are whatever the page held before, and 0 * NaN is NaN
@@ -72,6 +74,10 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
         }
         cp_async_commit();
     };
+    if (!FULL) {
+        for (int i = tid; i < FT_STAGES * 2 * TILE_BYTES / 16; i += THREADS) reinterpret_cast<uint4*>(smem)[i] = make_uint4(0u, 0u, 0u, 0u);
+        __syncthreads();
+    }
 #pragma unroll
     for (int s = 0; s < FT_STAGES - 1; s++) load_page(s, page0 + s);
 
@@ -87,11 +93,11 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
         row_lo[h] = hb_oldest_visible(p0 + i, window, 0);
         row_end[h] = there ? p0 + i + 1 : 0;
         row_scores[h] = scores + ((size_t)(t0 + i) * nh + head) * score_ld;
-        const unsigned int* src = reinterpret_cast<const unsigned int*>(q + (size_t)(t0 + i) * q_stride + (size_t)head * HD + (lane & 3) * 2);
+        const unsigned int* src = reinterpret_cast<const unsigned int*>(q + (size_t)(t0 + i) * q_stride + (size_t)head * hd + (lane & 3) * 2);
 #pragma unroll
         for (int ks = 0; ks < KSTEPS; ks++) {
-            qf[ks][h] = there ? __ldcg(src + ks * 8) : 0u;
-            qf[ks][h + 2] = there ? __ldcg(src + ks * 8 + 4) : 0u;
+            qf[ks][h] = there && (FULL || ks * 16 < hd) ? __ldcg(src + ks * 8) : 0u;
+            qf[ks][h + 2] = there && (FULL || ks * 16 + 8 < hd) ? __ldcg(src + ks * 8 + 4) : 0u;
         }
     }
     float o[HD / 8][4], m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
@@ -182,8 +188,8 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
         }
     }
     __syncthreads();
-    for (int idx = tid; idx < pairs * HD; idx += THREADS) {
-        const int r = idx / HD, d = idx - r * HD, i = r / G;
+    for (int idx = tid; idx < pairs * hd; idx += THREADS) {
+        const int r = idx / hd, d = idx - r * hd, i = r / G;
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < 4; w++) M = fmaxf(M, sm[w * ROWS + r]);
@@ -197,7 +203,7 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
             }
         }
         const size_t base = ((size_t)(t0 + i) * nh + g * G + (r - i * G)) * S + z;
-        part_o[base * HD + d] = acc;
+        part_o[base * hd + d] = acc;
         if (d == 0) {
             part_ml[base * 2] = M;
             part_ml[base * 2 + 1] = L;
@@ -205,27 +211,27 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
     }
 }
 
-template <int HD, int RT>
+template <int HD, int RT, bool FULL>
 static int launch_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                          const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks,
-                         int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+                         int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
     constexpr int PIPE = FT_STAGES * 2 * HB_PAGE_TOKENS * HD * 2, MERGE = (4 * 16 * RT * HD + 2 * 4 * 16 * RT) * 4, SMEM = PIPE > MERGE ? PIPE : MERGE;
     static bool done[HB_MAX_DEVICES] = {};
     bool& set = done[hb_device_slot()];
     if (!set) {
-        cudaError_t e = cudaFuncSetAttribute(few_tc_kernel<HD, RT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+        cudaError_t e = cudaFuncSetAttribute(few_tc_kernel<HD, RT, FULL>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
         if (e != cudaSuccess) return hb_fail("attention_mass: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
         set = true;
     }
-    cudaError_t e = hb_launch(few_tc_kernel<HD, RT>, dim3(splits, nkv, token_blocks), dim3(128 * RT), SMEM, s, (const bf16*)q, q_stride,
+    cudaError_t e = hb_launch(few_tc_kernel<HD, RT, FULL>, dim3(splits, nkv, token_blocks), dim3(128 * RT), SMEM, s, (const bf16*)q, q_stride,
                               (const bf16*)kc, (const bf16*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld,
-                              tokens_per_block, share_pages, n_seqs, nh, nkv, scale * MASS_LOG2E, window, n_pages, status);
+                              tokens_per_block, share_pages, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window, n_pages, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (few tokens, tensor cores)");
 }
 
 extern "C" int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_dim, int max_new) {
-    if ((head_dim != 64 && head_dim != 128) || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 32 || max_new < 1) return 0;
+    if (head_dim < 8 || head_dim > 128 || head_dim % 8 != 0 || n_kv_heads < 1 || n_heads % n_kv_heads != 0 || n_heads / n_kv_heads > 32 || max_new < 1) return 0;
     const int G = n_heads / n_kv_heads, rows = G * max_new <= 16 ? 16 : 32;
     return rows / G;
 }
@@ -234,16 +240,19 @@ int attention_few_tc(const void* q, long long q_stride, const void* kc, const vo
                      const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int token_blocks, int max_new,
                      int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s) {
     const int tokens = hb_attention_few_tc_tokens(nh, nkv, head_dim, max_new);
-    HB_REQUIRE(tokens > 0, "attention_mass: head size %d with %d heads over %d kv heads is not built for the tensor cores (64 or 128, groups up to 32)",
+    HB_REQUIRE(tokens > 0, "attention_mass: head size %d with %d heads over %d kv heads is not built for the tensor cores (up to 128 in steps of 8, groups up to"
+               " 32)",
                head_dim, nh, nkv);
     HB_REQUIRE(q_stride % 2 == 0 && ((uintptr_t)q & 3) == 0 && (((uintptr_t)kc | (uintptr_t)vc) & 15) == 0,
                "attention_mass: queries must be 4-byte and the cache 16-byte aligned");
     HB_REQUIRE(token_blocks <= 65535, "attention_mass: too many tokens for one launch");
     const bool two = nh / nkv * tokens > 16;
-#define HB_FT_LAUNCH(HD, RT)                                                                                                                  \
-    launch_few_tc<HD, RT>(q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, token_blocks, \
-                          tokens, share_pages, n_seqs, nh, nkv, scale, window, n_pages, status, s)
-    if (head_dim == 128) return two ? HB_FT_LAUNCH(128, 2) : HB_FT_LAUNCH(128, 1);
-    return two ? HB_FT_LAUNCH(64, 2) : HB_FT_LAUNCH(64, 1);
+#define HB_FT_LAUNCH(HD, RT, FULL)                                                                                                                  \
+    launch_few_tc<HD, RT, FULL>(q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, token_blocks, \
+                                tokens, share_pages, n_seqs, nh, nkv, head_dim, scale, window, n_pages, status, s)
+    if (head_dim == 128) return two ? HB_FT_LAUNCH(128, 2, true) : HB_FT_LAUNCH(128, 1, true);
+    if (head_dim > 64) return two ? HB_FT_LAUNCH(128, 2, false) : HB_FT_LAUNCH(128, 1, false);
+    if (head_dim == 64) return two ? HB_FT_LAUNCH(64, 2, true) : HB_FT_LAUNCH(64, 1, true);
+    return two ? HB_FT_LAUNCH(64, 2, false) : HB_FT_LAUNCH(64, 1, false);
 #undef HB_FT_LAUNCH
 }

@@ -174,6 +174,10 @@ FEW = [
     (16, 2, 152, [1434, 31, 32], [1, 1, 1], None),
     (3, 1, 20, [40, 95], [7, 8], 30),
     (7, 1, 1, [70], [3], None),
+    (24, 8, 112, [1500, 63], [1, 1], None),
+    (8, 2, 72, [700, 5], [5, 8], 300),
+    (3, 1, 8, [200, 64], [1, 2], None),
+    (20, 1, 40, [130], [1], None),
 ]
 TYPES = [torch.bfloat16, torch.float32]
 
