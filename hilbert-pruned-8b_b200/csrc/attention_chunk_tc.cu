@@ -1,6 +1,6 @@
 // Attention of a chunk of new tokens over the paged cache on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), bfloat16, head
-// sizes up to 128 in steps of 8, that leaves each row's log-sum, negated, for the weights' kernel (attention_mass_tc.cu): causal, grouped, with a window,
-// sequences with unequal numbers of new tokens, the keys cut into shares where there are few rows.
+// sizes up to 128 in steps of 8, that leaves each row's log-sum, negated, for the weights' kernel (attention_mass_tc.cu): causal,
+// grouped, with a window, sequences with unequal numbers of new tokens, the keys cut into shares where there are few rows.
 //
 // One CTA = two tiles of 128 query rows that read the same keys and values: two heads of a kv head with an even group, else two
 // neighbouring blocks of one head's tokens.  A tile's rows are the 128 lanes of tensor memory.  What bounds it, per 128 x 128 scores at
@@ -58,7 +58,8 @@ template <int HD>
 __global__ void __launch_bounds__(CT_THREADS, 1)
 chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                 const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
-                bf16* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, Shares sh, int n_tokens, int n_seqs, int nh, int nkv, int hd, int head_pairs, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
+                bf16* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, Shares sh, int n_tokens, int n_seqs, int nh,
+                int nkv, int hd, int head_pairs, float scale_log2e, int window, int n_pages, int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // [Q tiles 2][K stages][V stages][barriers]; a tile is 128 rows x HD
@@ -168,7 +169,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
         constexpr uint32_t idesc_qk = instr_desc_bf16_mn(128, FA_KEYS);
         constexpr uint32_t idesc_pv = instr_desc_bf16_mn(128, HD) | (1u << 16);               // B is MN-major
         // descriptors of the tiles' beginnings; a step along a tile adds its bytes / 16
-        const uint64_t q_desc = smem_desc_sw128(smem_base), k_desc = smem_desc_sw128(k_smem), v_desc = smem_desc_mn_sw128(v_smem, FA_HALF_BYTES, 1024);
+        const uint64_t q_desc = smem_desc_sw128(smem_base), k_desc = smem_desc_sw128(k_smem), v_desc = smem_desc_mn_sw128(v_smem, FA_HALF_BYTES,
+                                                                                                                          1024);
         auto scores = [&](int i, int it) {
             const int st = it % CT_STAGES;
 #pragma unroll
@@ -371,8 +373,10 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 }
 
 template <int HD>
-static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width, const int* seq_start,
-                        const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, Shares sh, int max_shares, int n_tokens, int n_seqs, int q_blocks,
+static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width,
+                        const int* seq_start,
+                        const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, Shares sh, int max_shares, int n_tokens,
+                        int n_seqs, int q_blocks,
                         int nh, int nkv, int hd, int head_pairs, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
     constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 22 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "attention tiles do not fit shared memory");
@@ -383,7 +387,8 @@ static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUte
         if (e != cudaSuccess) return hb_fail("attention_mass: cannot reserve %d bytes of shared memory: %s", SMEM, cudaGetErrorString(e));
         set = true;
     }
-    cudaError_t e = hb_launch(chunk_tc_kernel<HD>, dim3(head_pairs ? nh / 2 : nh, q_blocks, max_shares), dim3(CT_THREADS), SMEM, s, mq, mk, mv, page_table,
+    cudaError_t e = hb_launch(chunk_tc_kernel<HD>, dim3(head_pairs ? nh / 2 : nh, q_blocks, max_shares), dim3(CT_THREADS), SMEM, s, mq, mk, mv,
+                              page_table,
                               pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, sh, n_tokens, n_seqs, nh, nkv, hd, head_pairs,
                               scale * FA_LOG2E, window, n_pages, error_flag);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
@@ -396,7 +401,8 @@ extern "C" int hb_attention_mass_tc_supported(int n_heads, int n_kv_heads, int h
 
 int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
                        const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts,
-                       int max_shares, int share_tiles, int join_tokens, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads, int head_dim, float scale,
+                       int max_shares, int share_tiles, int join_tokens, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads,
+                       int head_dim, float scale,
                        int window, int n_pages, int* error_flag, cudaStream_t s) {
     HB_REQUIRE(hb_attention_mass_tc_supported(n_heads, n_kv_heads, head_dim),
                "attention_mass: %d heads over %d of size %d are not built for the tensor cores (sizes up to 128 in steps of 8)", n_heads, n_kv_heads, head_dim);
@@ -417,12 +423,15 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
     const Shares sh = {parts, parts == nullptr ? nullptr : parts + (size_t)max_shares * n_heads * n_tokens * head_dim,
                        max_shares == 1 ? 0x3fffffff : share_tiles};
     const int rc = head_dim > 64 ? launch_chunk<128>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, sh,
-                                                       max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, head_pairs, scale, window, n_pages,
+                                                       max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, head_pairs, scale,
+                                                       window, n_pages,
                                                        error_flag, s)
                                    : launch_chunk<64>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, sh,
-                                                      max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, head_pairs, scale, window, n_pages,
+                                                      max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, head_pairs, scale,
+                                                      window, n_pages,
                                                       error_flag, s);
     if (rc || max_shares == 1) return rc;
-    return shares_join(sh, join_tokens, HB_BF16, out, out_stride, lse, lse_ld, 1, seq_start, seq_pos0, head_pairs ? FA_ROWS : 2 * FA_ROWS, FA_KEYS, window, n_tokens,
+    return shares_join(sh, join_tokens, HB_BF16, out, out_stride, lse, lse_ld, 1, seq_start, seq_pos0, head_pairs ? FA_ROWS : 2 * FA_ROWS, FA_KEYS,
+                       window, n_tokens,
                        n_seqs, n_heads, head_dim, s);
 }

@@ -23,7 +23,8 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
               const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* part_o,
               float* part_ml, float* scores, long long score_ld, int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd_given,
               float scale_log2e, int window, int n_pages, int* status) {
-    constexpr int ROW_BYTES = HD * 2, TILE_BYTES = HB_PAGE_TOKENS * ROW_BYTES, CHUNKS = ROW_BYTES / 16, KSTEPS = HD / 16, ROWS = 16 * RT, THREADS = 128 * RT;
+    constexpr int ROW_BYTES = HD * 2, TILE_BYTES = HB_PAGE_TOKENS * ROW_BYTES, CHUNKS = ROW_BYTES / 16, KSTEPS = HD / 16, ROWS = 16 * RT,
+    THREADS = 128 * RT;
     const int hd = FULL ? HD : hd_given, chunks = FULL ? CHUNKS : hd / 8;
     extern __shared__ __align__(128) uint8_t smem[];
     pdl_trigger();
@@ -214,8 +215,10 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
 template <int HD, int RT, bool FULL>
 static int launch_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                          const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks,
-                         int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
-    constexpr int PIPE = FT_STAGES * 2 * HB_PAGE_TOKENS * HD * 2, MERGE = (4 * 16 * RT * HD + 2 * 4 * 16 * RT) * 4, SMEM = PIPE > MERGE ? PIPE : MERGE;
+                         int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages,
+                         int* status, cudaStream_t s) {
+    constexpr int PIPE = FT_STAGES * 2 * HB_PAGE_TOKENS * HD * 2, MERGE = (4 * 16 * RT * HD + 2 * 4 * 16 * RT) * 4,
+    SMEM = PIPE > MERGE ? PIPE : MERGE;
     static bool done[HB_MAX_DEVICES] = {};
     bool& set = done[hb_device_slot()];
     if (!set) {
@@ -237,7 +240,8 @@ extern "C" int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_
 }
 
 int attention_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int token_blocks, int max_new,
+                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages,
+                     int token_blocks, int max_new,
                      int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s) {
     const int tokens = hb_attention_few_tc_tokens(nh, nkv, head_dim, max_new);
     HB_REQUIRE(tokens > 0, "attention_mass: head size %d with %d heads over %d kv heads is not built for the tensor cores (up to 128 in steps of 8, groups up to"

@@ -92,7 +92,8 @@ template <typename T, int NC>
 __global__ void __launch_bounds__(AM_THREADS)
 attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict__ kc, const T* __restrict__ vc,
                       const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
-                      T* __restrict__ out, long long out_stride, float* __restrict__ lse, Shares sh, int n_tokens, int n_seqs, int nh, int nkv, int hd,
+                      T* __restrict__ out, long long out_stride, float* __restrict__ lse, Shares sh, int n_tokens, int n_seqs, int nh, int nkv,
+                      int hd,
                       float scale_log2e, int window, int n_pages, int vec_q, int vec_kv, int* status) {
     extern __shared__ __align__(16) float am_smem[];
     pdl_trigger();
@@ -229,7 +230,8 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
 template <typename T>
 __global__ void __launch_bounds__(256)
 shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, int rounded,
-                   const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh,
+                   const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs,
+                   int nh,
                    int hd) {
     __shared__ float ws[8][32];
     pdl_trigger();
@@ -272,7 +274,8 @@ shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* 
     }
 }
 
-int shares_join(Shares sh, int join_tokens, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded, const int* seq_start,
+int shares_join(Shares sh, int join_tokens, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded,
+                const int* seq_start,
                 const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s) {
     if (join_tokens == 0) return 0;
     const dim3 grid(join_tokens, (nh + 7) / 8);
@@ -400,8 +403,10 @@ static int am_reserve(F* kernel, int bytes, bool (&done)[HB_MAX_DEVICES]) {
 
 template <typename T, int NC>
 static int launch_rows(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                       const int* seq_pos0, void* out, long long out_stride, float* lse, Shares sh, int max_shares, int join_tokens, MassOut mo, int splits, int n_tokens,
-                       int n_seqs, int q_blocks, int key_tiles, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+                       const int* seq_pos0, void* out, long long out_stride, float* lse, Shares sh, int max_shares, int join_tokens, MassOut mo,
+                       int splits, int n_tokens,
+                       int n_seqs, int q_blocks, int key_tiles, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status,
+                       cudaStream_t s) {
     static_assert(AM_SMEM_ROWS(256) <= 227 * 1024, "attention tiles do not fit shared memory");
     static bool done[HB_MAX_DEVICES] = {}, done_mass[HB_MAX_DEVICES] = {};
     if (am_reserve(attention_rows_kernel<T, NC>, AM_SMEM_ROWS(16 * NC), done)) return 1;
@@ -409,16 +414,20 @@ static int launch_rows(const void* q, long long q_stride, const void* kc, const 
     const uintptr_t four = 4 * sizeof(T);                      // four elements at a time where rows and heads begin at a multiple of that
     const int vec_kv = hd % 4 == 0 && (((uintptr_t)kc | (uintptr_t)vc) & (four - 1)) == 0;
     const int vec_q = hd % 4 == 0 && q_stride % 4 == 0 && ((uintptr_t)q & (four - 1)) == 0;
-    cudaError_t e = hb_launch(attention_rows_kernel<T, NC>, dim3(nh, q_blocks, max_shares), dim3(AM_THREADS), AM_SMEM_ROWS(hd), s, (const T*)q, q_stride,
-                              (const T*)kc, (const T*)vc, page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, lse, sh, n_tokens, n_seqs, nh,
+    cudaError_t e = hb_launch(attention_rows_kernel<T, NC>, dim3(nh, q_blocks, max_shares), dim3(AM_THREADS), AM_SMEM_ROWS(hd), s, (const T*)q,
+                              q_stride,
+                              (const T*)kc, (const T*)vc, page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, lse, sh, n_tokens, n_seqs,
+                              nh,
                               nkv, hd, scale * MASS_LOG2E, window, n_pages, vec_q, vec_kv, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     if (hb_check_launch("attention_mass (rows)")) return 1;
-    if (max_shares > 1 && shares_join(sh, join_tokens, sizeof(T) == 4 ? HB_F32 : HB_BF16, out, out_stride, lse, n_tokens, 0, seq_start, seq_pos0, AM_ROWS,
+    if (max_shares > 1 && shares_join(sh, join_tokens, sizeof(T) == 4 ? HB_F32 : HB_BF16, out, out_stride, lse, n_tokens, 0, seq_start, seq_pos0,
+                                      AM_ROWS,
                                       HB_PAGE_TOKENS, window, n_tokens, n_seqs, nh, hd, s))
         return 1;
     e = hb_launch(mass_rows_kernel<T, NC>, dim3(key_tiles, nkv, splits), dim3(AM_THREADS), AM_SMEM_MASS(hd), s, (const T*)q, q_stride, (const T*)kc,
-                  page_table, pt_width, seq_start, seq_pos0, (const float*)lse, mo, n_tokens, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window, n_pages,
+                  page_table, pt_width, seq_start, seq_pos0, (const float*)lse, mo, n_tokens, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window,
+                  n_pages,
                   vec_q, vec_kv, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     if (hb_check_launch("attention_mass (weights)")) return 1;
@@ -432,8 +441,10 @@ static int launch_rows(const void* q, long long q_stride, const void* kc, const 
 // floats when splits > 1.  before may be null or mass.
 extern "C" int hb_attention_mass(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
                                  int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse,
-                                 const float* before, float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int join_tokens, int splits,
-                                 int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window,
+                                 const float* before, float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles,
+                                 int join_tokens, int splits,
+                                 int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale,
+                                 int window,
                                  int n_pages, int* status, void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0 && head_dim <= 256 && n_pages > 0 && pt_width > 0,
@@ -517,7 +528,8 @@ few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict
     uint8_t* tiles = af_raw;                             // [stages][keys, values][32][row_bytes]
     float* qs = reinterpret_cast<float*>(af_raw + AF_STAGES * 2 * AF_KEYS * row_bytes);        // [8][hd8]
     int b, blk, unused;
-    if (!mass_find(n_seqs, blockIdx.z, [&](int i) { return ((seq_start[i + 1] - seq_start[i]) * G + AF_PAIRS - 1) / AF_PAIRS; }, [](int) { return 0; },
+    if (!mass_find(n_seqs, blockIdx.z, [&](int i) { return ((seq_start[i + 1] - seq_start[i]) * G + AF_PAIRS - 1) / AF_PAIRS; },
+                   [](int) { return 0; },
                    b, blk, unused))
         return;
     const int t0 = seq_start[b], n_new = seq_start[b + 1] - t0, pos0 = seq_pos0[b];
@@ -699,7 +711,8 @@ __device__ __forceinline__ void join_stats(const float* __restrict__ part_ml, si
 template <typename T>
 __global__ void __launch_bounds__(FF_THREADS)
 few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const float* __restrict__ scores, long long score_ld,
-                  const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, T* __restrict__ out,
+                  const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
+                  T* __restrict__ out,
                   long long out_stride, MassOut mo, int token_rows, int nh, int nkv, int hd, int S, int window, int n_pages, int vec) {
     __shared__ float lse[MASS_FEW_PAIRS];
     pdl_trigger();
@@ -740,6 +753,7 @@ few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
         }
         return;
     }
+    if (n_new * G > MASS_FEW_PAIRS) return;                    // no step of few tokens: the host refuses it
     const int n = (int)min((long long)(pos0 + n_new), score_ld), key0 = ((int)blockIdx.x - token_rows) * FF_KEYS;
     if (key0 >= n) return;
     for (int i = warp; i < n_new * G; i += FF_THREADS / 32) {
@@ -808,7 +822,8 @@ static int launch_finish(const float* part_o, const float* part_ml, const float*
                          int nh, int nkv, int hd, int splits, int window, int n_pages, cudaStream_t s) {
     const int key_blocks = (max_len + FF_KEYS - 1) / FF_KEYS;
     const int vec = (((uintptr_t)mo.before | (uintptr_t)mo.mass) & 15) == 0;
-    cudaError_t e = hb_launch(few_finish_kernel<T>, dim3(max_new + key_blocks, nkv, n_seqs), dim3(FF_THREADS), 0, s, part_o, part_ml, scores, score_ld,
+    cudaError_t e = hb_launch(few_finish_kernel<T>, dim3(max_new + key_blocks, nkv, n_seqs), dim3(FF_THREADS), 0, s, part_o, part_ml, scores,
+                              score_ld,
                               page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, mo, max_new, nh, nkv, hd, splits, window, n_pages, vec);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (finish)");
@@ -848,18 +863,23 @@ extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_strid
     MassOut mo = {before, mass, nullptr};
     int rc;
     if (tensor_cores)
-        rc = attention_few_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, share_pages,
+        rc = attention_few_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits,
+                              share_pages,
                               blocks, max_new, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     else if (dtype == HB_F32)
-        rc = launch_few<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, share_pages,
+        rc = launch_few<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits,
+                               share_pages,
                                blocks, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     else
-        rc = launch_few<bf16>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, share_pages,
+        rc = launch_few<bf16>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits,
+                              share_pages,
                               blocks, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
     if (rc) return rc;
     if (dtype == HB_F32)
-        return launch_finish<float>(part_o, part_ml, scores, score_ld, page_table, pt_width, seq_start, seq_pos0, out, out_stride, mo, max_len, max_new,
+        return launch_finish<float>(part_o, part_ml, scores, score_ld, page_table, pt_width, seq_start, seq_pos0, out, out_stride, mo, max_len,
+                                    max_new,
                                     n_seqs, n_heads, n_kv_heads, head_dim, splits, window, n_pages, s);
-    return launch_finish<bf16>(part_o, part_ml, scores, score_ld, page_table, pt_width, seq_start, seq_pos0, out, out_stride, mo, max_len, max_new, n_seqs,
+    return launch_finish<bf16>(part_o, part_ml, scores, score_ld, page_table, pt_width, seq_start, seq_pos0, out, out_stride, mo, max_len, max_new,
+                               n_seqs,
                                n_heads, n_kv_heads, head_dim, splits, window, n_pages, s);
 }

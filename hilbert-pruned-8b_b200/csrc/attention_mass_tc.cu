@@ -1,5 +1,6 @@
 // The weights of steps of many tokens on the 5th-generation tensor cores (tcgen05 + TMEM + TMA), bfloat16, head sizes up to 128
-// in steps of 8 (as attention_chunk_tc.cu): the second half of attention_mass.cu's arithmetic, behind the attention that leaves each row's log-sum (attention_chunk_tc.cu).
+// in steps of 8 (as attention_chunk_tc.cu): the second half of attention_mass.cu's arithmetic, behind the attention that leaves each
+// row's log-sum.
 //
 // One CTA = 256 consecutive rows of a sequence's cache x one kv head x a share of the (head, 128 queries) tiles that see them.
 // Keys are the M operand: a tile's 128 keys are the 128 lanes of tensor memory and the queries its columns, so that a key's sum over
@@ -33,7 +34,8 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 template <int HD>
 __global__ void __launch_bounds__(MT_THREADS, 1)
 mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const int* __restrict__ page_table, int pt_width,
-               const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* lse, long long lse_ld, MassOut mo, int n_seqs, int nh,
+               const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* lse, long long lse_ld, MassOut mo, int n_seqs,
+               int nh,
                int nkv, int hd, float scale_log2e, int window, int n_pages, int S, int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -143,7 +145,8 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                     for (int kk = 0; kk < HD / 16; kk++) {
                         if (kk * 16 >= hd) break;
                         const uint32_t off = (kk >> 2) * FA_HALF_BYTES + (kk & 3) * 32;
-                        umma_bf16(tmem_base + (2 * sb + k) * 128, k_desc + ((k * TILE + off) >> 4), q_desc + ((s * TILE + off) >> 4), idesc, kk ? 1u : 0u);
+                        umma_bf16(tmem_base + (2 * sb + k) * 128, k_desc + ((k * TILE + off) >> 4), q_desc + ((s * TILE + off) >> 4), idesc,
+                                  kk ? 1u : 0u);
                     }
                 umma_commit(q_empty0 + 8 * s);
                 umma_commit(s_full0 + 8 * sb);
@@ -207,7 +210,8 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 #pragma unroll
                     for (int c = 0; c < 32; c += 2) {
                         const float a = c >= lo && c <= hi ? exp2_approx(fmaf(sv[c], scale_log2e, xlse[s * 128 + hf * 64 + part * 32 + c])) : 0.0f;
-                        const float d = c + 1 >= lo && c + 1 <= hi ? exp2_approx(fmaf(sv[c + 1], scale_log2e, xlse[s * 128 + hf * 64 + part * 32 + c + 1])) : 0.0f;
+                        const float d = c + 1 >= lo && c + 1 <= hi ? exp2_approx(fmaf(sv[c + 1], scale_log2e,
+                                                                                      xlse[s * 128 + hf * 64 + part * 32 + c + 1])) : 0.0f;
                         sum[(c >> 1) & 3] = pair_add(sum[(c >> 1) & 3], pair_of(a, d));
                     }
                 }
@@ -236,8 +240,10 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 }
 
 template <int HD>
-static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const int* page_table, int pt_width, const int* seq_start, const int* seq_pos0,
-                          const float* lse, long long lse_ld, MassOut mo, int splits, int n_seqs, int key_tiles, int nh, int nkv, int hd, float scale, int window,
+static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const int* page_table, int pt_width, const int* seq_start,
+                          const int* seq_pos0,
+                          const float* lse, long long lse_ld, MassOut mo, int splits, int n_seqs, int key_tiles, int nh, int nkv, int hd,
+                          float scale, int window,
                           int n_pages, int* error_flag, cudaStream_t s) {
     constexpr int SMEM = (2 + MT_STAGES) * (HD / 64) * FA_HALF_BYTES + (MT_STAGES * 128 + 256) * 4 + 16 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "key and query tiles do not fit shared memory");
@@ -261,9 +267,11 @@ extern "C" int hb_attention_mass_tc_keys(void) { return MT_KEYS; }
 // floats, lse_ld 128 * the sum of ceil(new tokens / 128); parts:
 // splits * n_kv_heads * key_tiles * 256 floats when splits > 1.
 extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
-                                    const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, const float* before,
+                                    const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld,
+                                    const float* before,
                                     float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int join_tokens,
-                                    int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
+                                    int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim,
+                                    float scale, int window, int n_pages, int* error_flag,
                                     void* stream) {
     if (n_seqs == 0 || n_tokens == 0) return 0;
     HB_REQUIRE(((uintptr_t)lse & 15) == 0 && lse_ld % 128 == 0, "attention_mass: the log-sums must be aligned");
@@ -271,7 +279,8 @@ extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const voi
                    (splits == 1 || parts != nullptr),
                "attention_mass: bad sizes");
     cudaStream_t s = (cudaStream_t)stream;
-    if (attention_chunk_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, chunk_parts, max_shares, share_tiles,
+    if (attention_chunk_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, chunk_parts,
+                           max_shares, share_tiles,
                            join_tokens, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s))
         return 1;
     CUtensorMap mq, mk;

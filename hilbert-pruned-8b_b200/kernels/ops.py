@@ -1270,9 +1270,10 @@ class Ops:
                               f"{tuple(t.shape)}")
 
     def _mass_plan(self, few: bool, tc: bool, bf16: bool, heads: int, kv_heads: int, head_dim: int, win: int, step, splits: Optional[int]):
-        """How a step of ``attention_mass`` is cut, from its sizes alone: few tokens: (blocks, whether on the tensor cores, most
-        shares of the pages, fewest pages of one, floats of scratch); many: (shares of the keys' sums, blocks of queries, tiles of keys, most shares of a block of
-        queries, tiles of keys in one, tokens whose blocks may be cut, distance of two heads' log-sums, floats of the log-sums, of the sums' shares, of the partial results)."""
+        """How a step of ``attention_mass`` is cut, from its sizes alone.  Few tokens: (blocks, whether on the tensor cores, most
+        shares of the pages, fewest pages of one, floats of scratch).  Many: (shares of the keys' sums, blocks of queries, tiles of
+        keys, most shares of a block of queries, tiles of keys in one, tokens whose blocks may be cut, distance of two heads'
+        log-sums, floats of the log-sums, of the sums' shares, of the partial results)."""
         T, group = step.num_tokens, heads // kv_heads
         # (single tokens: from the page table's width alone, so that a captured step and an eager one sum alike)
         single = step.max_new == 1 and few
@@ -1302,8 +1303,9 @@ class Ops:
             key_tiles = sum(-(-n // keys) for n in step.host_len)
             if splits is None:
                 splits = mass_splits(step.host_new, step.host_len, win, keys, 128 if tc else 64, kv_heads, group, self.sm_count * (1 if tc else 2))
-            shares, tiles, cut = chunk_shares(step.host_new, step.host_len, win, rows, 128 if tc else 64, heads // 2 if tc and group % 2 == 0 else heads,
-                                         heads * (head_dim + 2), self.sm_count * (1 if tc or head_dim > 64 else 2), *((4.5, 8.0) if tc else (1.0, 2.0)))
+            units, costs = heads // 2 if tc and group % 2 == 0 else heads, (4.5, 8.0) if tc else (1.0, 2.0)
+            shares, tiles, cut = chunk_shares(step.host_new, step.host_len, win, rows, 128 if tc else 64, units, heads * (head_dim + 2),
+                                              self.sm_count * (1 if tc or head_dim > 64 else 2), *costs)
             lse_ld = 128 * sum(-(-n // 128) for n in step.host_new) if tc else T
 
             def round128(n: int) -> int:
@@ -1322,8 +1324,9 @@ class Ops:
         ``mass[page of j, g, j % 64] = before[the same] + the sum over the sequence's tokens in this step and the query heads of g of
         their softmax weight of j`` in 32-bit; rows that this step itself appended start from zero, whatever ``before`` holds
         there.  ``before``: None (this step's weights alone), another tensor, or ``mass`` itself (a running sum).  A page belongs to
-        one sequence; rows that no sequence of the step holds are neither read nor written.  The step's new keys and values are in the cache already, as for
-        ``attention``; queries, cache and output have one type.  The sums do not depend on what else runs (fixed order)."""
+        one sequence; rows that no sequence of the step holds are neither read nor written.  The step's new keys and values are in
+        the cache already, as for ``attention``; queries, cache and output have one type.  The sums do not depend on what else runs
+        (fixed order)."""
         k, v = cache.k, cache.v
         self._on(qkv, k, v, out, mass, before)
         T, pages = qkv.shape[0], k.shape[0]
@@ -1356,7 +1359,8 @@ class Ops:
         old, new, status, stream = before.data_ptr() if before is not None else None, mass.data_ptr(), self.status.data_ptr(), self._stream()
         # scratch of the call's own, from torch's allocator: two calls on two streams, or two captured graphs, share nothing
         if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * (heads // kv_heads) <= self.MASS_FEW_PAIRS:
-            blocks, tc, splits, least, floats = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
+            blocks, tc, splits, least, floats = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, dtype == torch.bfloat16, heads,
+                                                                kv_heads, head_dim, win, step, splits)
             scratch = torch.empty(floats, dtype=torch.float32, device=self.device)
             self._call("hb_attention_mass_few", q_at, code, q_ld, k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(),
                        step.seq_pos0.data_ptr(), out_at, out_ld, scratch.data_ptr(), old, new, splits, least, blocks, tc, T, step.num_seqs,
@@ -1365,7 +1369,8 @@ class Ops:
             return
         tc = bool(fast and self.use_tcgen05_attention and (q_at | out_at) % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0
                   and self.lib.hb_attention_mass_tc_supported(heads, kv_heads, head_dim))
-        splits, q_blocks, key_tiles, shares, tiles, cut, lse_ld, n_lse, n_parts, n_cut = self._mass_plan(False, tc, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
+        splits, q_blocks, key_tiles, shares, tiles, cut, lse_ld, n_lse, n_parts, n_cut = self._mass_plan(
+            False, tc, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
         scratch = torch.empty(n_lse + n_parts + n_cut, dtype=torch.float32, device=self.device)
         lse = scratch.data_ptr()
         parts, partial = lse + 4 * n_lse if n_parts else None, lse + 4 * (n_lse + n_parts) if n_cut else None
