@@ -308,31 +308,69 @@ int hb_side_unit(const float* s, long long lds, const int* tokens, const void* t
 
 // A bounded cache (attention_mass.cu, evict.cu): attention that also adds up every cached row's weight, for steps of many and of
 // few tokens; the choice of the rows that stay (kept, ascending, -1 behind the last); their move, in place (to_table null) or into
-// pages of their own.  before may be null or mass.
-int hb_attention_mass(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
-                      int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse,
-                      const float* before, float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int join_tokens, int splits,
-                      int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window,
-                      int n_pages, int* status, void* stream);
-// the same on tcgen05 (attention_chunk_tc.cu, attention_mass_tc.cu), bfloat16, head sizes up to 128 in steps of 8; key tiles of hb_attention_mass_tc_keys() rows
+// pages of their own.  before may be null or mass.  The caller of
+// attention_mass packs the fields, 8 bytes each in this order, and says how many.
+typedef struct {
+    const void* q;
+    long long dtype, q_stride;
+    const void *k_cache, *v_cache;
+    const int* page_table;
+    long long pt_width;
+    const int *seq_start, *seq_pos0;
+    void* out;
+    long long out_stride;
+    float* lse;                 // n_heads * lse_ld floats; lse_ld: the tokens, or on the tensor cores 128 * the sum of ceil(new tokens / 128)
+    long long lse_ld;
+    const float* before;
+    float *mass, *parts;        // parts: splits * n_kv_heads * key_tiles * (keys of a tile) floats when splits > 1
+    float* chunk_parts;         // max_shares * n_heads * n_tokens * (head_dim + 2) floats when max_shares > 1
+    long long max_shares;       // the most blocks of threads that a block of queries takes
+    long long share_tiles;      // the most tiles of keys of one of them
+    long long join_tokens;      // the new tokens of the sequences that shares_may_cut (attention_mass.cuh)
+    long long splits;           // shares of the weights' work
+    long long n_tokens, n_seqs;
+    long long q_blocks;         // sum over sequences of ceil(new tokens / queries of a block)
+    long long key_tiles;        // sum over sequences of ceil(rows / keys of a tile)
+    long long n_heads, n_kv_heads, head_dim, window, n_pages;
+    int* status;
+    void* stream;
+} HbMassMany;
+int hb_attention_mass(const HbMassMany* a, int fields, float scale);
+// the same on tcgen05 (attention_chunk_tc.cu, attention_mass_tc.cu), bfloat16, head sizes up to 128 in steps of 8; key tiles of
+// hb_attention_mass_tc_keys() rows
 int hb_attention_mass_tc_supported(int n_heads, int n_kv_heads, int head_dim);
 int hb_attention_mass_tc_keys(void);
-int hb_attention_mass_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
-                         const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld,
-                         const float* before, float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int join_tokens,
-                         int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* error_flag,
-                         void* stream);
+int hb_attention_mass_tc(const HbMassMany* a, int fields, float scale);
 // new tokens of a sequence that a block of the tensor-core kernel takes at once (0: sizes that it is not built for)
 int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_dim, int max_new);
 int hb_attention_few_pairs(void);
 long long hb_attention_mass_few_floats(int n_tokens, int n_heads, int head_dim, int splits, int max_len);
 int hb_attention_few_block_pairs(void);
 int hb_attention_few_blocks_per_sm(int head_dim, int dtype);
-int hb_attention_mass_few(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
-                          int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* scratch,
-                          const float* before, float* mass, int splits, int share_pages, int blocks, int tensor_cores, int n_tokens, int n_seqs,
-                          int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window, int n_pages, int* status,
-                          void* stream);
+typedef struct {
+    const void* q;
+    long long dtype, q_stride;
+    const void *k_cache, *v_cache;
+    const int* page_table;
+    long long pt_width;
+    const int *seq_start, *seq_pos0;
+    void* out;
+    long long out_stride;
+    float* scratch;             // hb_attention_mass_few_floats floats
+    const float* before;
+    float* mass;
+    long long splits;           // a sequence's pages go into at most so many shares,
+    long long share_pages;      // of so many pages or more
+    long long blocks;           // sum over sequences of ceil(pairs / hb_attention_few_block_pairs()), or with
+    long long tensor_cores;     // tensor_cores of ceil(new tokens / hb_attention_few_tc_tokens(...))
+    long long whole;            // one share and one block for every sequence, each with new tokens: no second kernel
+    long long n_tokens, n_seqs;
+    long long max_new, max_len; // bounds of the sequences' new tokens and rows
+    long long n_heads, n_kv_heads, head_dim, window, n_pages;
+    int* status;
+    void* stream;
+} HbMassFew;
+int hb_attention_mass_few(const HbMassFew* a, int fields, float scale);
 int hb_evict_select(const float* mass, const int* page_table, int pt_width, const int* lengths, int* kept, int entries, int n_seqs,
                     int n_kv_heads, int n_pages, int first, int recent, int budget, int threads, int cluster, int* status, void* stream);
 int hb_evict_rows(const int* kept, void* k, int k_row_bytes, void* v, int v_row_bytes, float* mass, const int* from_table, int from_width,

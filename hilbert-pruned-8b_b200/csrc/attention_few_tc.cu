@@ -1,6 +1,6 @@
 // The first half of a step of few tokens with accumulated weights (attention_mass.cu) on the tensor cores, bfloat16, head sizes up to
 // 128 in steps of 8: partial results over shares of the keys, and the scores themselves, for the kernel that joins the shares and turns the
-// scores into weights.
+// scores into weights; or, of short sequences, everything in one block (mass_whole).
 //
 // A CTA = a share of the pages x one kv head x a block of a sequence's new tokens: the rows of the mma.sync tiles (16 RT of them) are the
 // (token, head) pairs of the block, so a page is read once for all of them.  Bound by memory: 2 head sizes of keys and values per row of
@@ -22,11 +22,12 @@ __global__ void __launch_bounds__(128 * RT, 2)
 few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __restrict__ kc, const bf16* __restrict__ vc,
               const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* part_o,
               float* part_ml, float* scores, long long score_ld, int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd_given,
-              float scale_log2e, int window, int n_pages, int* status) {
+              float scale_log2e, int window, int n_pages, MassWhole whole, int* status) {
     constexpr int ROW_BYTES = HD * 2, TILE_BYTES = HB_PAGE_TOKENS * ROW_BYTES, CHUNKS = ROW_BYTES / 16, KSTEPS = HD / 16, ROWS = 16 * RT,
     THREADS = 128 * RT;
     const int hd = FULL ? HD : hd_given, chunks = FULL ? CHUNKS : hd / 8;
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ float lse[ROWS];                            // of a whole sequence's pairs
     pdl_trigger();
     pdl_wait();
     q = pdl_fresh(q);
@@ -44,7 +45,7 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
     const int* pt = page_table + (size_t)b * pt_width;
     if (z == 0 && tid == 0 && p_last >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
     const int pairs = n_tok * G;                           // row r is head r % G of token r / G
-    if (page0 >= page1) {                                  // a share without keys
+    if (page0 >= page1 && whole.out == nullptr) {          // a share without keys
         for (int r = tid; r < pairs; r += THREADS) {
             float* ml = part_ml + (((size_t)(t0 + r / G) * nh + g * G + r % G) * S + z) * 2;
             ml[0] = -INFINITY;
@@ -203,6 +204,12 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
                 L += sl[w * ROWS + r] * e;
             }
         }
+        if (whole.out != nullptr) {
+            ((bf16*)whole.out)[(size_t)(t0 + i) * whole.out_stride + (size_t)(g * G + (r - i * G)) * hd + d] =
+                __float2bfloat16_rn(acc * (L > 0.0f ? 1.0f / L : 0.0f));
+            if (d == 0) lse[r] = L > 0.0f ? M + log2f(L) : INFINITY;
+            continue;
+        }
         const size_t base = ((size_t)(t0 + i) * nh + g * G + (r - i * G)) * S + z;
         part_o[base * hd + d] = acc;
         if (d == 0) {
@@ -210,10 +217,14 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
             part_ml[base * 2 + 1] = L;
         }
     }
+    if (whole.out != nullptr) {
+        __syncthreads();
+        mass_whole(whole.mo, scores, score_ld, lse, n_tok, G, g, t0, nh, nkv, p0, window, pt, pt_width, n_pages);
+    }
 }
 
 template <int HD, int RT, bool FULL>
-static int launch_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
+static int launch_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                          const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks,
                          int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages,
                          int* status, cudaStream_t s) {
@@ -228,7 +239,7 @@ static int launch_few_tc(const void* q, long long q_stride, const void* kc, cons
     }
     cudaError_t e = hb_launch(few_tc_kernel<HD, RT, FULL>, dim3(splits, nkv, token_blocks), dim3(128 * RT), SMEM, s, (const bf16*)q, q_stride,
                               (const bf16*)kc, (const bf16*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld,
-                              tokens_per_block, share_pages, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window, n_pages, status);
+                              tokens_per_block, share_pages, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window, n_pages, whole, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (few tokens, tensor cores)");
 }
@@ -239,7 +250,7 @@ extern "C" int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_
     return rows / G;
 }
 
-int attention_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
+int attention_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                      const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages,
                      int token_blocks, int max_new,
                      int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s) {
@@ -252,7 +263,7 @@ int attention_few_tc(const void* q, long long q_stride, const void* kc, const vo
     HB_REQUIRE(token_blocks <= 65535, "attention_mass: too many tokens for one launch");
     const bool two = nh / nkv * tokens > 16;
 #define HB_FT_LAUNCH(HD, RT, FULL)                                                                                                                  \
-    launch_few_tc<HD, RT, FULL>(q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, token_blocks, \
+    launch_few_tc<HD, RT, FULL>(whole, q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, token_blocks, \
                                 tokens, share_pages, n_seqs, nh, nkv, head_dim, scale, window, n_pages, status, s)
     if (head_dim == 128) return two ? HB_FT_LAUNCH(128, 2, true) : HB_FT_LAUNCH(128, 1, true);
     if (head_dim > 64) return two ? HB_FT_LAUNCH(128, 2, false) : HB_FT_LAUNCH(128, 1, false);

@@ -7,7 +7,7 @@
 // A row's weight is known only once the token has seen all its keys, and then the scores are gone.  Two ways:
 //   steps of few tokens   (memory-bound) the scores themselves are written beside the partial results, 4 bytes per (head, row) against
 //                         the 2 head sizes of a key and a value; one more launch joins the partial results and turns the scores into
-//                         weights.  Keys and values are read once for a block of (token, head) pairs.
+//                         weights (short sequences: the same block does it).  Keys and values are read once for a block of (token, head) pairs.
 //   steps of many tokens  (bound by arithmetic) the tokens' log-sums are kept and a second kernel, a block per tile of keys,
 //                         computes its keys' scores with all queries once more: half as much arithmetic again instead of
 //                         writing and reading a weight for every (token, head, row).  Every key's sum belongs to one thread from
@@ -434,36 +434,32 @@ static int launch_rows(const void* q, long long q_stride, const void* kc, const 
     return splits > 1 ? mass_join(page_table, pt_width, seq_start, seq_pos0, mo, n_seqs, nkv, n_pages, AM_KEYS, key_tiles, splits, s) : 0;
 }
 
-// Steps of many tokens.  q_blocks: sum over sequences of ceil(new tokens / 64); key_tiles: sum of ceil(rows / 64); lse:
-// n_heads * n_tokens floats; max_shares: the most blocks that a block of queries takes, share_tiles: the most pages of one of them;
-// join_tokens: the new tokens of the sequences that shares_may_cut;
-// chunk_parts: max_shares * n_heads * n_tokens * (head_dim + 2) floats when max_shares > 1; parts: splits * n_kv_heads * key_tiles * 64
-// floats when splits > 1.  before may be null or mass.
-extern "C" int hb_attention_mass(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
-                                 int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse,
-                                 const float* before, float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles,
-                                 int join_tokens, int splits,
-                                 int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim, float scale,
-                                 int window,
-                                 int n_pages, int* status, void* stream) {
+// Steps of many tokens (HbMassMany in api.h): blocks of 64 queries, tiles of 64 keys.
+extern "C" int hb_attention_mass(const HbMassMany* a, int fields, float scale) {
+    HB_REQUIRE(fields * sizeof(long long) == sizeof(*a), "attention_mass: %d fields given", fields);
+    const int n_tokens = (int)a->n_tokens, n_seqs = (int)a->n_seqs, n_heads = (int)a->n_heads, n_kv_heads = (int)a->n_kv_heads, hd = (int)a->head_dim;
+    const int splits = (int)a->splits, max_shares = (int)a->max_shares, n_pages = (int)a->n_pages, pt_width = (int)a->pt_width, dtype = (int)a->dtype;
+    const int q_blocks = (int)a->q_blocks, key_tiles = (int)a->key_tiles, share_tiles = (int)a->share_tiles, join_tokens = (int)a->join_tokens;
+    const int window = (int)a->window;
     if (n_seqs == 0 || n_tokens == 0) return 0;
-    HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0 && head_dim <= 256 && n_pages > 0 && pt_width > 0,
-               "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, head_dim);
-    HB_REQUIRE(n_kv_heads <= 65535 && q_blocks <= 65535 && key_tiles > 0 && splits >= 1 && splits <= 65535 && (splits == 1 || parts != nullptr) &&
-                   max_shares >= 1 && max_shares <= 32 && share_tiles >= 1 && (max_shares == 1 || chunk_parts != nullptr),
+    HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && hd > 0 && hd <= 256 && n_pages > 0 && pt_width > 0,
+               "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, hd);
+    HB_REQUIRE(n_kv_heads <= 65535 && q_blocks <= 65535 && key_tiles > 0 && splits >= 1 && splits <= 65535 && (splits == 1 || a->parts != nullptr) &&
+                   max_shares >= 1 && max_shares <= 32 && share_tiles >= 1 && (max_shares == 1 || a->chunk_parts != nullptr),
                "attention_mass: the step is too large for one launch");
-    HB_REQUIRE(lse != nullptr && mass != nullptr, "attention_mass: missing buffers");
+    HB_REQUIRE(a->lse != nullptr && a->mass != nullptr, "attention_mass: missing buffers");
     HB_REQUIRE(dtype == HB_F32 || dtype == HB_BF16, "attention_mass: unsupported dtype %d", dtype);
-    MassOut mo = {before, mass, parts};
+    MassOut mo = {a->before, a->mass, a->parts};
     // (maximum, sum) pairs in front: 8-byte aligned whatever the head size; one share: no block is cut, whatever it sees
-    const Shares sh = {chunk_parts == nullptr ? nullptr : chunk_parts + (size_t)max_shares * n_heads * n_tokens * 2, chunk_parts,
+    const Shares sh = {a->chunk_parts == nullptr ? nullptr : a->chunk_parts + (size_t)max_shares * n_heads * n_tokens * 2, a->chunk_parts,
                        max_shares == 1 ? 0x3fffffff : share_tiles};
-    cudaStream_t s = (cudaStream_t)stream;
-#define HB_AM_LAUNCH(T, NC)                                                                                                                     \
-    launch_rows<T, NC>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, sh, max_shares, join_tokens, mo, splits, \
-                       n_tokens, n_seqs, q_blocks, key_tiles, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s)
-    if (dtype == HB_F32) return head_dim <= 64 ? HB_AM_LAUNCH(float, 4) : head_dim <= 128 ? HB_AM_LAUNCH(float, 8) : HB_AM_LAUNCH(float, 16);
-    return head_dim <= 64 ? HB_AM_LAUNCH(bf16, 4) : head_dim <= 128 ? HB_AM_LAUNCH(bf16, 8) : HB_AM_LAUNCH(bf16, 16);
+    cudaStream_t s = (cudaStream_t)a->stream;
+#define HB_AM_LAUNCH(T, NC)                                                                                                                       \
+    launch_rows<T, NC>(a->q, a->q_stride, a->k_cache, a->v_cache, a->page_table, pt_width, a->seq_start, a->seq_pos0, a->out, a->out_stride, a->lse, sh, \
+                       max_shares, join_tokens, mo, splits, n_tokens, n_seqs, q_blocks, key_tiles, n_heads, n_kv_heads, hd, scale, window, n_pages,   \
+                       a->status, s)
+    if (dtype == HB_F32) return hd <= 64 ? HB_AM_LAUNCH(float, 4) : hd <= 128 ? HB_AM_LAUNCH(float, 8) : HB_AM_LAUNCH(float, 16);
+    return hd <= 64 ? HB_AM_LAUNCH(bf16, 4) : hd <= 128 ? HB_AM_LAUNCH(bf16, 8) : HB_AM_LAUNCH(bf16, 16);
 #undef HB_AM_LAUNCH
 }
 
@@ -512,7 +508,8 @@ __global__ void __launch_bounds__(AF_THREADS, 2)
 few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict__ kc, const T* __restrict__ vc, const int* __restrict__ page_table,
                 int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* __restrict__ part_o,
                 float* __restrict__ part_ml, float* __restrict__ scores, long long score_ld, int n_seqs, int nh, int nkv, int hd, int share_pages,
-                float scale_log2e, int window, int n_pages, int vec, int* status) {
+                float scale_log2e, int window, int n_pages, int vec, MassWhole whole,
+                int* status) {
     extern __shared__ __align__(16) uint8_t af_raw[];
     __shared__ float4 w8[AF_KEYS][AF_PAIRS / 4];         // a tile's weights
     __shared__ float corr[AF_PAIRS], stat[2][AF_PAIRS];
@@ -542,7 +539,7 @@ few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict
     mass_share(oldest / HB_PAGE_TOKENS, min(p_last / HB_PAGE_TOKENS + 1, width), z, S, share_pages, page0, page1);
     if (z == 0 && tid == 0 && p_last >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
     auto at_of = [&](int r) -> size_t { return (size_t)(t0 + (pair0 + r) / G) * nh + g * G + (pair0 + r) % G; };
-    if (page0 >= page1) {                                // a share without keys
+    if (page0 >= page1 && whole.out == nullptr) {        // a share without keys
         if (tid < pairs) {
             part_ml[(at_of(tid) * S + z) * 2] = -INFINITY;
             part_ml[(at_of(tid) * S + z) * 2 + 1] = 0.0f;
@@ -675,6 +672,18 @@ few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict
         stat[1][warp] = l;
     }
     __syncthreads();
+    if (whole.out != nullptr) {
+        for (int i = tid; i < pairs * hd; i += AF_THREADS) {
+            const int r = i / hd, d = i - r * hd;
+            const float L = stat[1][r];
+            ((T*)whole.out)[(size_t)(t0 + r / G) * whole.out_stride + (size_t)(g * G + r % G) * hd + d] =
+                from_f32<T>(so[r * 2 * columns + d] * (L > 0.0f ? 1.0f / L : 0.0f));
+        }
+        if (tid < pairs) corr[tid] = stat[1][tid] > 0.0f ? stat[0][tid] + log2f(stat[1][tid]) : INFINITY;      // now the pairs' log-sums
+        __syncthreads();
+        mass_whole(whole.mo, scores, score_ld, corr, n_new, G, g, t0, nh, nkv, pos0, window, pt, pt_width, n_pages);
+        return;
+    }
     for (int i = tid; i < pairs * hd; i += AF_THREADS) {
         const int r = i / hd, d = i - r * hd;
         const size_t base = at_of(r) * S + z;
@@ -799,8 +808,8 @@ extern "C" long long hb_attention_mass_few_floats(int n_tokens, int n_heads, int
 }
 
 template <typename T>
-static int launch_few(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                      const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int blocks,
+static int launch_few(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width,
+                      const int* seq_start, const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int blocks,
                       int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
     static_assert(af_smem(256, 4, 2) <= 227 * 1024, "tiles do not fit shared memory");
     static bool done[2][HB_MAX_DEVICES] = {};
@@ -809,7 +818,7 @@ static int launch_few(const void* q, long long q_stride, const void* kc, const v
 #define HB_AF_LAUNCH(ST)                                                                                                                           \
     hb_launch(few_rows_kernel<T, ST>, dim3(splits, nkv, blocks), dim3(AF_THREADS), af_smem(hd, sizeof(T), ST), s, (const T*)q, q_stride, (const T*)kc, \
               (const T*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, n_seqs, nh, nkv, hd, share_pages,            \
-              scale * MASS_LOG2E, window, n_pages, vec, status)
+              scale * MASS_LOG2E, window, n_pages, vec, whole, status)
     cudaError_t e = stages == 3 ? HB_AF_LAUNCH(3) : HB_AF_LAUNCH(2);
 #undef HB_AF_LAUNCH
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
@@ -836,50 +845,45 @@ extern "C" int hb_attention_few_blocks_per_sm(int head_dim, int dtype) {
     return n < 1 ? 1 : n > 2 ? 2 : n;                      // registers hold two
 }
 
-// Steps of few tokens (at most hb_attention_few_pairs() pairs of a sequence's tokens and a group's heads).  `scratch` holds
-// hb_attention_mass_few_floats floats; blocks: the sum over sequences of ceil(pairs / hb_attention_few_block_pairs()), or with
-// tensor_cores of ceil(new tokens / hb_attention_few_tc_tokens(...)); a sequence's pages go into at most `splits` shares, of share_pages
-// or more; max_len bounds the rows of every sequence, max_new their new tokens.
-extern "C" int hb_attention_mass_few(const void* q, int dtype, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table,
-                                     int pt_width, const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* scratch,
-                                     const float* before, float* mass, int splits, int share_pages, int blocks, int tensor_cores, int n_tokens,
-                                     int n_seqs, int max_new, int max_len, int n_heads, int n_kv_heads, int head_dim, float scale, int window,
-                                     int n_pages, int* status, void* stream) {
+// Steps of few tokens (at most hb_attention_few_pairs() pairs of a sequence's tokens and a group's heads); HbMassFew in api.h.
+extern "C" int hb_attention_mass_few(const HbMassFew* a, int fields, float scale) {
+    HB_REQUIRE(fields * sizeof(long long) == sizeof(*a), "attention_mass: %d fields given", fields);
+    const int n_tokens = (int)a->n_tokens, n_seqs = (int)a->n_seqs, n_heads = (int)a->n_heads, n_kv_heads = (int)a->n_kv_heads, hd = (int)a->head_dim;
+    const int max_new = (int)a->max_new, max_len = (int)a->max_len, splits = (int)a->splits, window = (int)a->window, n_pages = (int)a->n_pages;
+    const int pt_width = (int)a->pt_width, share_pages = (int)a->share_pages, blocks = (int)a->blocks, dtype = (int)a->dtype;
     if (n_seqs == 0 || n_tokens == 0) return 0;
-    HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && head_dim > 0 && head_dim <= 256 && n_pages > 0 && pt_width > 0,
-               "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, head_dim);
+    HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && hd > 0 && hd <= 256 && n_pages > 0 && pt_width > 0,
+               "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, hd);
     HB_REQUIRE((long long)max_new * (n_heads / n_kv_heads) <= MASS_FEW_PAIRS, "attention_mass: %d tokens of %d heads are no step of few tokens",
                max_new, n_heads / n_kv_heads);
     HB_REQUIRE(n_tokens > 0 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && share_pages >= 1 && blocks >= 1 && blocks <= 65535 && max_len >= 1 &&
-                   scratch != nullptr && mass != nullptr,
+                   a->scratch != nullptr && a->mass != nullptr,
                "attention_mass: bad sizes");
+    HB_REQUIRE(!a->whole || (splits == 1 && blocks == n_seqs), "attention_mass: a whole sequence to a block needs one share and one block each");
     HB_REQUIRE(dtype == HB_F32 || dtype == HB_BF16, "attention_mass: unsupported dtype %d", dtype);
-    HB_REQUIRE(!tensor_cores || dtype == HB_BF16, "attention_mass: the tensor cores take bfloat16");
+    HB_REQUIRE(!a->tensor_cores || dtype == HB_BF16, "attention_mass: the tensor cores take bfloat16");
+    HB_REQUIRE(((uintptr_t)a->scratch & 15) == 0, "attention_mass: scratch must be 16-byte aligned");
     const size_t rows = (size_t)n_tokens * n_heads * splits;
     const long long score_ld = mass_score_ld(max_len);
-    float *scores = scratch, *part_ml = scores + (size_t)n_tokens * n_heads * score_ld, *part_o = part_ml + rows * 2;
-    HB_REQUIRE(((uintptr_t)scratch & 15) == 0, "attention_mass: scratch must be 16-byte aligned");
-    cudaStream_t s = (cudaStream_t)stream;
-    MassOut mo = {before, mass, nullptr};
+    float *scores = a->scratch, *part_ml = scores + (size_t)n_tokens * n_heads * score_ld, *part_o = part_ml + rows * 2;
+    cudaStream_t s = (cudaStream_t)a->stream;
+    MassOut mo = {a->before, a->mass, nullptr};
+    const MassWhole whole = {a->whole ? a->out : nullptr, a->out_stride, mo};
+#define HB_FEW_ARGS                                                                                                                              \
+    whole, a->q, a->q_stride, a->k_cache, a->v_cache, a->page_table, pt_width, a->seq_start, a->seq_pos0, part_o, part_ml, scores, score_ld, splits, \
+        share_pages, blocks
     int rc;
-    if (tensor_cores)
-        rc = attention_few_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits,
-                              share_pages,
-                              blocks, max_new, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
+    if (a->tensor_cores)
+        rc = attention_few_tc(HB_FEW_ARGS, max_new, n_seqs, n_heads, n_kv_heads, hd, scale, window, n_pages, a->status, s);
     else if (dtype == HB_F32)
-        rc = launch_few<float>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits,
-                               share_pages,
-                               blocks, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
+        rc = launch_few<float>(HB_FEW_ARGS, n_seqs, n_heads, n_kv_heads, hd, scale, window, n_pages, a->status, s);
     else
-        rc = launch_few<bf16>(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits,
-                              share_pages,
-                              blocks, n_seqs, n_heads, n_kv_heads, head_dim, scale, window, n_pages, status, s);
-    if (rc) return rc;
+        rc = launch_few<bf16>(HB_FEW_ARGS, n_seqs, n_heads, n_kv_heads, hd, scale, window, n_pages, a->status, s);
+#undef HB_FEW_ARGS
+    if (rc || a->whole) return rc;
     if (dtype == HB_F32)
-        return launch_finish<float>(part_o, part_ml, scores, score_ld, page_table, pt_width, seq_start, seq_pos0, out, out_stride, mo, max_len,
-                                    max_new,
-                                    n_seqs, n_heads, n_kv_heads, head_dim, splits, window, n_pages, s);
-    return launch_finish<bf16>(part_o, part_ml, scores, score_ld, page_table, pt_width, seq_start, seq_pos0, out, out_stride, mo, max_len, max_new,
-                               n_seqs,
-                               n_heads, n_kv_heads, head_dim, splits, window, n_pages, s);
+        return launch_finish<float>(part_o, part_ml, scores, score_ld, a->page_table, pt_width, a->seq_start, a->seq_pos0, a->out, a->out_stride, mo, max_len,
+                                    max_new, n_seqs, n_heads, n_kv_heads, hd, splits, window, n_pages, s);
+    return launch_finish<bf16>(part_o, part_ml, scores, score_ld, a->page_table, pt_width, a->seq_start, a->seq_pos0, a->out, a->out_stride, mo, max_len, max_new,
+                               n_seqs, n_heads, n_kv_heads, hd, splits, window, n_pages, s);
 }

@@ -80,6 +80,33 @@ __device__ __forceinline__ void mass_write(const MassOut& mo, float sum, int g, 
     mo.mass[at] = old + sum;
 }
 
+// For blocks that have all of a sequence's new tokens and all of its keys (short sequences): they write the outputs and the weights
+// themselves and no second kernel follows.  out null: a second kernel joins the shares.
+struct MassWhole {
+    void* out;
+    long long out_stride;
+    MassOut mo;
+};
+
+// The weights of a sequence's n keys from the scores that this block wrote, in the order of the second kernel's sums; lse: of pair r, which is
+// head r % G of token r / G.
+__device__ __forceinline__ void mass_whole(const MassOut& mo, const float* scores, long long score_ld, const float* lse, int n_new, int G, int g, int t0,
+                                           int nh, int nkv, int pos0, int window, const int* __restrict__ pt, int pt_width, int n_pages) {
+    const int n = (int)min((long long)(pos0 + n_new), score_ld);
+    for (int key = threadIdx.x; key < n; key += blockDim.x) {
+        float s = 0.0f;
+        for (int i = 0; i < n_new; i++) {
+            const int p = pos0 + i;
+            if (key > p || key < hb_oldest_visible(p, window, 0)) continue;
+            const float* row = scores + ((size_t)(t0 + i) * nh + g * G) * score_ld + key;
+#pragma unroll 4
+            for (int h = 0; h < G; h++) s += exp2f(row[h * score_ld] - lse[i * G + h]);
+        }
+        const int pi = key / HB_PAGE_TOKENS;
+        mass_write(mo, s, g, key, pi < pt_width ? pt[pi] : -1, nkv, n_pages, pos0, n_new);
+    }
+}
+
 // a key's sum, or with several shares (S) share z of it
 __device__ __forceinline__ void mass_store(const MassOut& mo, float sum, int b, int g, int key, int page, int nkv, int n_pages, int pos0, int n_new,
                                            int z, int S, size_t place, size_t places) {
@@ -147,7 +174,7 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
 
 // The first half of a step of few tokens on the tensor cores (attention_few_tc.cu): token_blocks, the sum over sequences of ceil(new
 // tokens / hb_attention_few_tc_tokens(...)); queries 4-byte, keys and values 16-byte aligned.
-int attention_few_tc(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
+int attention_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                      const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages,
                      int token_blocks, int max_new,
                      int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);

@@ -262,35 +262,31 @@ static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const in
 
 extern "C" int hb_attention_mass_tc_keys(void) { return MT_KEYS; }
 
-// bfloat16, sizes of hb_attention_mass_tc_supported, queries and output with 16-byte aligned rows.  q_blocks, chunk_parts, max_shares, share_tiles,
-// join_tokens: as attention_chunk_tc (attention_mass.cuh); key_tiles: sum over sequences of ceil(rows / 256); lse: n_heads * lse_ld
-// floats, lse_ld 128 * the sum of ceil(new tokens / 128); parts:
-// splits * n_kv_heads * key_tiles * 256 floats when splits > 1.
-extern "C" int hb_attention_mass_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
-                                    const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld,
-                                    const float* before,
-                                    float* mass, float* parts, float* chunk_parts, int max_shares, int share_tiles, int join_tokens,
-                                    int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles, int n_heads, int n_kv_heads, int head_dim,
-                                    float scale, int window, int n_pages, int* error_flag,
-                                    void* stream) {
+// Steps of many tokens (HbMassMany in api.h), bfloat16, sizes of hb_attention_mass_tc_supported, queries and output with 16-byte aligned
+// rows: blocks of queries as attention_chunk_tc (attention_mass.cuh), tiles of 256 keys.
+extern "C" int hb_attention_mass_tc(const HbMassMany* a, int fields, float scale) {
+    HB_REQUIRE(fields * sizeof(long long) == sizeof(*a), "attention_mass: %d fields given", fields);
+    const int n_tokens = (int)a->n_tokens, n_seqs = (int)a->n_seqs, n_heads = (int)a->n_heads, n_kv_heads = (int)a->n_kv_heads, hd = (int)a->head_dim;
+    const int splits = (int)a->splits, n_pages = (int)a->n_pages, pt_width = (int)a->pt_width, key_tiles = (int)a->key_tiles, window = (int)a->window;
     if (n_seqs == 0 || n_tokens == 0) return 0;
-    HB_REQUIRE(((uintptr_t)lse & 15) == 0 && lse_ld % 128 == 0, "attention_mass: the log-sums must be aligned");
-    HB_REQUIRE(lse != nullptr && mass != nullptr && n_kv_heads > 0 && n_kv_heads <= 65535 && key_tiles > 0 && splits >= 1 && (long long)key_tiles * n_kv_heads * splits <= 0x7fffffffLL &&
-                   (splits == 1 || parts != nullptr),
+    HB_REQUIRE(((uintptr_t)a->lse & 15) == 0 && a->lse_ld % 128 == 0, "attention_mass: the log-sums must be aligned");
+    HB_REQUIRE(a->dtype == HB_BF16 && a->lse != nullptr && a->mass != nullptr && n_kv_heads > 0 && n_kv_heads <= 65535 && key_tiles > 0 && splits >= 1 &&
+                   (long long)key_tiles * n_kv_heads * splits <= 0x7fffffffLL && (splits == 1 || a->parts != nullptr),
                "attention_mass: bad sizes");
-    cudaStream_t s = (cudaStream_t)stream;
-    if (attention_chunk_tc(q, q_stride, k_cache, v_cache, page_table, pt_width, seq_start, seq_pos0, out, out_stride, lse, lse_ld, chunk_parts,
-                           max_shares, share_tiles,
-                           join_tokens, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s))
+    cudaStream_t s = (cudaStream_t)a->stream;
+    if (attention_chunk_tc(a->q, a->q_stride, a->k_cache, a->v_cache, a->page_table, pt_width, a->seq_start, a->seq_pos0, a->out, a->out_stride, a->lse,
+                           a->lse_ld, a->chunk_parts, (int)a->max_shares, (int)a->share_tiles, (int)a->join_tokens, n_tokens, n_seqs, (int)a->q_blocks,
+                           n_heads, n_kv_heads, hd, scale, window, n_pages, a->status, s))
         return 1;
     CUtensorMap mq, mk;
-    if (tc_make_map_heads(&mq, q, n_tokens, n_heads, head_dim, q_stride, 128)) return 1;
-    if (tc_make_map(&mk, k_cache, (long long)n_pages * n_kv_heads * HB_PAGE_TOKENS, head_dim, head_dim, HB_PAGE_TOKENS)) return 1;
-    MassOut mo = {before, mass, parts};
-    const int rc = head_dim > 64 ? launch_mass_tc<128>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, lse_ld, mo, splits, n_seqs, key_tiles,
-                                                         n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s)
-                                   : launch_mass_tc<64>(mq, mk, page_table, pt_width, seq_start, seq_pos0, lse, lse_ld, mo, splits, n_seqs, key_tiles,
-                                                        n_heads, n_kv_heads, head_dim, scale, window, n_pages, error_flag, s);
+    if (tc_make_map_heads(&mq, a->q, n_tokens, n_heads, hd, a->q_stride, 128)) return 1;
+    if (tc_make_map(&mk, a->k_cache, (long long)n_pages * n_kv_heads * HB_PAGE_TOKENS, hd, hd, HB_PAGE_TOKENS)) return 1;
+    MassOut mo = {a->before, a->mass, a->parts};
+#define HB_MT_LAUNCH(HD)                                                                                                                   \
+    launch_mass_tc<HD>(mq, mk, a->page_table, pt_width, a->seq_start, a->seq_pos0, a->lse, a->lse_ld, mo, splits, n_seqs, key_tiles, n_heads, \
+                       n_kv_heads, hd, scale, window, n_pages, a->status, s)
+    const int rc = hd > 64 ? HB_MT_LAUNCH(128) : HB_MT_LAUNCH(64);
+#undef HB_MT_LAUNCH
     if (rc) return rc;
-    return splits > 1 ? mass_join(page_table, pt_width, seq_start, seq_pos0, mo, n_seqs, n_kv_heads, n_pages, MT_KEYS, key_tiles, splits, s) : 0;
+    return splits > 1 ? mass_join(a->page_table, pt_width, a->seq_start, a->seq_pos0, mo, n_seqs, n_kv_heads, n_pages, MT_KEYS, key_tiles, splits, s) : 0;
 }

@@ -14,6 +14,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+from array import array
 from typing import Optional
 
 import torch
@@ -79,15 +80,9 @@ _SIGNATURES = {
                              _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
     "hb_attention_prefill_tc": [_c_ptr, _c_ll, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_int,
                                 _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int, _c_ptr, _c_ptr],
-    "hb_attention_mass": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_ptr,
-                          _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int,
-                          _c_int, _c_ptr, _c_ptr],
-    "hb_attention_mass_tc": [_c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr,
-                             _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int,
-                             _c_int, _c_ptr, _c_ptr],
-    "hb_attention_mass_few": [_c_ptr, _c_int, _c_ll, _c_ptr, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_ptr, _c_ll, _c_ptr, _c_ptr, _c_ptr,
-                              _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_float, _c_int, _c_int,
-                              _c_ptr, _c_ptr],
+    "hb_attention_mass": [_c_ptr, _c_int, _c_float],
+    "hb_attention_mass_tc": [_c_ptr, _c_int, _c_float],
+    "hb_attention_mass_few": [_c_ptr, _c_int, _c_float],
     "hb_evict_select": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int, _c_ptr,
                         _c_ptr],
     "hb_evict_rows": [_c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_ptr, _c_ptr, _c_int, _c_ptr, _c_int, _c_int, _c_int, _c_int, _c_int, _c_int,
@@ -1270,10 +1265,10 @@ class Ops:
                               f"{tuple(t.shape)}")
 
     def _mass_plan(self, few: bool, tc: bool, bf16: bool, heads: int, kv_heads: int, head_dim: int, win: int, step, splits: Optional[int]):
-        """How a step of ``attention_mass`` is cut, from its sizes alone.  Few tokens: (blocks, whether on the tensor cores, most
-        shares of the pages, fewest pages of one, floats of scratch).  Many: (shares of the keys' sums, blocks of queries, tiles of
-        keys, most shares of a block of queries, tiles of keys in one, tokens whose blocks may be cut, distance of two heads'
-        log-sums, floats of the log-sums, of the sums' shares, of the partial results)."""
+        """How a step of ``attention_mass`` is cut, from its sizes alone.  Few tokens: (blocks, whether on the tensor cores, whether
+        a block has a whole sequence, most shares of the pages, fewest pages of one, floats of scratch).  Many: (shares of the keys'
+        sums, blocks of queries, tiles of keys, most shares of a block of queries, tiles of keys in one, tokens whose blocks may be
+        cut, distance of two heads' log-sums, floats of the log-sums, of the sums' shares, of the partial results)."""
         T, group = step.num_tokens, heads // kv_heads
         # (single tokens: from the page table's width alone, so that a captured step and an eager one sum alike)
         single = step.max_new == 1 and few
@@ -1288,14 +1283,20 @@ class Ops:
             per, each = (at_once, 1) if at_once else (self.lib.hb_attention_few_block_pairs(), group)
             new = [1] * step.num_seqs if single else step.host_new
             blocks = sum(-(-n * each // per) for n in new)
-            least = 1
+            given, least = splits, 1
             if splits is None:
                 lens = [step.max_len] * step.num_seqs if single else step.host_len
                 seen = [-(-(min(ln, win + n) if win else ln) // 64) for n, ln in zip(new, lens) for _ in range(-(-n * each // per))]
                 slots = 2 if at_once else self.lib.hb_attention_few_blocks_per_sm(head_dim, int(bf16))
                 splits, least = few_splits(seen, kv_heads, slots * self.sm_count)
-            splits = max(1, min(splits, (step.max_len + 63) // 64))
-            plan = (blocks, int(at_once > 0), splits, least, self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len))
+            # short sequences, each in one block: it sees all of the keys and no second kernel follows.  (Captured, device time of 32 heads
+            # over 8: size 64, one sequence of 300 rows 7.1 in two kernels and 7.4 us in one, of 440 rows 7.8 and 9.1; eight with four
+            # tokens each 15.8 and 12.6; size 128, 250 rows 8.2 and 8.3, 500 rows 8.9 and 12.6; in 32-bit 60 rows 10.9 and 8.5, 120 rows
+            # 10.9 and 11.3.  The host's part of a call is 2.4 us shorter.)
+            rows = 64 if not at_once else 256 if head_dim > 64 else 384
+            whole = (given is None and step.max_len <= rows and blocks == step.num_seqs == sum(n > 0 for n in new) and T >= step.num_seqs)
+            splits, least = (1, 1) if whole else (max(1, min(splits, (step.max_len + 63) // 64)), least)
+            plan = (blocks, int(at_once > 0), int(whole), splits, least, self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len))
         else:
             # the tensor cores take two tiles of 128 queries at a time: two heads, or with an odd group two blocks of tokens
             rows, keys = (128 if group % 2 == 0 else 256, self.lib.hb_attention_mass_tc_keys()) if tc else (64, 64)
@@ -1356,16 +1357,18 @@ class Ops:
         code, q_ld, out_ld = _code(qkv), _rows(qkv, "attention queries"), _rows(out, "attention output")
         q_at, k_at, v_at, out_at = qkv.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
         fast = self.use_fast_attention and dtype == torch.bfloat16 and (k_at | v_at) % 16 == 0
-        old, new, status, stream = before.data_ptr() if before is not None else None, mass.data_ptr(), self.status.data_ptr(), self._stream()
+        old, new, status, stream = before.data_ptr() if before is not None else 0, mass.data_ptr(), self.status.data_ptr(), self._stream()
         # scratch of the call's own, from torch's allocator: two calls on two streams, or two captured graphs, share nothing
         if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * (heads // kv_heads) <= self.MASS_FEW_PAIRS:
-            blocks, tc, splits, least, floats = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, dtype == torch.bfloat16, heads,
-                                                                kv_heads, head_dim, win, step, splits)
+            blocks, tc, whole, splits, least, floats = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, dtype == torch.bfloat16, heads,
+                                                                       kv_heads, head_dim, win, step, splits)
             scratch = torch.empty(floats, dtype=torch.float32, device=self.device)
-            self._call("hb_attention_mass_few", q_at, code, q_ld, k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(),
-                       step.seq_pos0.data_ptr(), out_at, out_ld, scratch.data_ptr(), old, new, splits, least, blocks, tc, T, step.num_seqs,
-                       step.max_new, step.max_len, heads, kv_heads, head_dim, scale, win, pages, status, stream)
-            self.launches += 2
+            # (the fields of HbMassFew, 8 bytes each: a third of the time of as many arguments)
+            a = array("q", (q_at, code, q_ld, k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out_at,
+                            out_ld, scratch.data_ptr(), old, new, splits, least, blocks, tc, whole, T, step.num_seqs, step.max_new, step.max_len, heads,
+                            kv_heads, head_dim, win, pages, status, stream))
+            self._call("hb_attention_mass_few", *a.buffer_info(), scale)
+            self.launches += 2 - whole
             return
         tc = bool(fast and self.use_tcgen05_attention and (q_at | out_at) % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0
                   and self.lib.hb_attention_mass_tc_supported(heads, kv_heads, head_dim))
@@ -1373,14 +1376,12 @@ class Ops:
             False, tc, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
         scratch = torch.empty(n_lse + n_parts + n_cut, dtype=torch.float32, device=self.device)
         lse = scratch.data_ptr()
-        parts, partial = lse + 4 * n_lse if n_parts else None, lse + 4 * (n_lse + n_parts) if n_cut else None
-        where = (k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out_at, out_ld, lse)
-        sizes = (old, new, parts, partial, shares, tiles, cut, splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads, head_dim, scale, win, pages, status,
-                 stream)
-        if tc:
-            self._call("hb_attention_mass_tc", q_at, q_ld, *where, lse_ld, *sizes)
-        else:
-            self._call("hb_attention_mass", q_at, code, q_ld, *where, *sizes)
+        parts, partial = lse + 4 * n_lse if n_parts else 0, lse + 4 * (n_lse + n_parts) if n_cut else 0
+        # (the fields of HbMassMany)
+        a = array("q", (q_at, code, q_ld, k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out_at, out_ld,
+                        lse, lse_ld, old, new, parts, partial, shares, tiles, cut, splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads,
+                        head_dim, win, pages, status, stream))
+        self._call("hb_attention_mass_tc" if tc else "hb_attention_mass", *a.buffer_info(), scale)
         self.launches += 2 + (splits > 1) + (shares > 1)
 
     def evict_select(self, mass, page_table, lengths, first: int, recent: int, kept) -> None:

@@ -267,6 +267,30 @@ def test_output_rows_apart_and_unaligned_queries(ops, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("window", [None, 1, 50])
+@pytest.mark.parametrize("dtype,heads,kv,hd,past,new", [
+    (torch.bfloat16, 8, 2, 64, [0, 383, 64, 5], [1, 1, 1, 1]), (torch.bfloat16, 32, 1, 64, [380], [1]), (torch.bfloat16, 6, 2, 80, [252, 0], [4, 1]),
+    (torch.bfloat16, 8, 8, 128, [63, 128, 9], [8, 2, 8]), (torch.float32, 8, 1, 64, [63, 0], [1, 1]), (torch.float32, 3, 3, 7, [61, 40], [3, 2]),
+    (torch.bfloat16, 4, 2, 256, [60] * 40, [4] * 40)])
+def test_short_sequences_in_one_kernel(ops, dtype, heads, kv, hd, past, new, window):
+    """A block with a whole sequence gives what two kernels give, bit for bit: one share, the same order of sums."""
+    c = Case(dtype, heads, kv, hd, past, new, window, seed=6)
+    start = torch.randn(c.pages, kv, PAGE, device=DEV)
+    two, one, was = start.clone(), start.clone(), ops.launches
+    want = c.run(ops, two, before=c.before, splits=1)
+    assert ops.launches == was + 2
+    got = c.run(ops, one, before=c.before)
+    assert ops.launches == was + 3
+    c.check(got, one, c.before, start)
+    assert torch.equal(got, want) and torch.equal(one, two)
+    own = c.before.clone()                                   # a running sum in place
+    c.run(ops, own, before=own)
+    held = two != start
+    assert torch.equal(own[held], two[held])
+    ops.check_errors()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [[90, 3], [1, 2]])
 def test_a_sequence_without_new_tokens(ops, new):
     """Rows of a sequence that brings nothing keep their earlier sum."""
