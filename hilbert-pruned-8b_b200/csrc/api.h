@@ -364,8 +364,9 @@ typedef struct {
     long long blocks;           // sum over sequences of ceil(pairs / hb_attention_few_block_pairs()), or with
     long long tensor_cores;     // tensor_cores of ceil(new tokens / hb_attention_few_tc_tokens(...))
     long long whole;            // one share and one block for every sequence, each with new tokens: no second kernel
-    long long n_tokens, n_seqs;
-    long long max_new, max_len; // bounds of the sequences' new tokens and rows
+    long long n_tokens, n_seqs; // of this call: a step's sequences from first_seq on, whose first token is the step's first_token
+    long long first_seq, first_token;
+    long long max_new, max_len; // bounds of the step's new tokens of a sequence, of the rows of this call's sequences
     long long n_heads, n_kv_heads, head_dim, window, n_pages;
     int* status;
     void* stream;

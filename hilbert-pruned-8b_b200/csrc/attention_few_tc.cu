@@ -22,7 +22,7 @@ __global__ void __launch_bounds__(128 * RT, 2)
 few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __restrict__ kc, const bf16* __restrict__ vc,
               const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* part_o,
               float* part_ml, float* scores, long long score_ld, int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd_given,
-              float scale_log2e, int window, int n_pages, MassWhole whole, int* status) {
+              float scale_log2e, int window, int n_pages, MassWhole whole, int seq0, int* status) {
     constexpr int ROW_BYTES = HD * 2, TILE_BYTES = HB_PAGE_TOKENS * ROW_BYTES, CHUNKS = ROW_BYTES / 16, KSTEPS = HD / 16, ROWS = 16 * RT,
     THREADS = 128 * RT;
     const int hd = FULL ? HD : hd_given, chunks = FULL ? CHUNKS : hd / 8;
@@ -43,7 +43,7 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
     int page0, page1;
     mass_share(first, last, z, S, share_pages, page0, page1);
     const int* pt = page_table + (size_t)b * pt_width;
-    if (z == 0 && tid == 0 && p_last >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
+    if (z == 0 && tid == 0 && p_last >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + seq0 + b);
     const int pairs = n_tok * G;                           // row r is head r % G of token r / G
     if (page0 >= page1 && whole.out == nullptr) {          // a share without keys
         for (int r = tid; r < pairs; r += THREADS) {
@@ -170,7 +170,7 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
     }
     cp_async_wait<0>();
     __syncthreads();
-    if (bad_page && tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + b);
+    if (bad_page && tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + seq0 + b);
 
     float* so = reinterpret_cast<float*>(smem);                        // [4 quarters][ROWS][HD]
     float* sm = so + 4 * ROWS * HD;                                    // [4][ROWS]
@@ -227,7 +227,7 @@ template <int HD, int RT, bool FULL>
 static int launch_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                          const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks,
                          int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages,
-                         int* status, cudaStream_t s) {
+                         int seq0, int* status, cudaStream_t s) {
     constexpr int PIPE = FT_STAGES * 2 * HB_PAGE_TOKENS * HD * 2, MERGE = (4 * 16 * RT * HD + 2 * 4 * 16 * RT) * 4,
     SMEM = PIPE > MERGE ? PIPE : MERGE;
     static bool done[HB_MAX_DEVICES] = {};
@@ -239,7 +239,7 @@ static int launch_few_tc(MassWhole whole, const void* q, long long q_stride, con
     }
     cudaError_t e = hb_launch(few_tc_kernel<HD, RT, FULL>, dim3(splits, nkv, token_blocks), dim3(128 * RT), SMEM, s, (const bf16*)q, q_stride,
                               (const bf16*)kc, (const bf16*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld,
-                              tokens_per_block, share_pages, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window, n_pages, whole, status);
+                              tokens_per_block, share_pages, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window, n_pages, whole, seq0, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (few tokens, tensor cores)");
 }
@@ -253,7 +253,7 @@ extern "C" int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_
 int attention_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                      const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages,
                      int token_blocks, int max_new,
-                     int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+                     int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int seq0, int* status, cudaStream_t s) {
     const int tokens = hb_attention_few_tc_tokens(nh, nkv, head_dim, max_new);
     HB_REQUIRE(tokens > 0, "attention_mass: head size %d with %d heads over %d kv heads is not built for the tensor cores (up to 128 in steps of 8, groups up to"
                " 32)",
@@ -264,7 +264,7 @@ int attention_few_tc(MassWhole whole, const void* q, long long q_stride, const v
     const bool two = nh / nkv * tokens > 16;
 #define HB_FT_LAUNCH(HD, RT, FULL)                                                                                                                  \
     launch_few_tc<HD, RT, FULL>(whole, q, q_stride, kc, vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, token_blocks, \
-                                tokens, share_pages, n_seqs, nh, nkv, head_dim, scale, window, n_pages, status, s)
+                                tokens, share_pages, n_seqs, nh, nkv, head_dim, scale, window, n_pages, seq0, status, s)
     if (head_dim == 128) return two ? HB_FT_LAUNCH(128, 2, true) : HB_FT_LAUNCH(128, 1, true);
     if (head_dim > 64) return two ? HB_FT_LAUNCH(128, 2, false) : HB_FT_LAUNCH(128, 1, false);
     if (head_dim == 64) return two ? HB_FT_LAUNCH(64, 2, true) : HB_FT_LAUNCH(64, 1, true);

@@ -508,8 +508,7 @@ __global__ void __launch_bounds__(AF_THREADS, 2)
 few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict__ kc, const T* __restrict__ vc, const int* __restrict__ page_table,
                 int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, float* __restrict__ part_o,
                 float* __restrict__ part_ml, float* __restrict__ scores, long long score_ld, int n_seqs, int nh, int nkv, int hd, int share_pages,
-                float scale_log2e, int window, int n_pages, int vec, MassWhole whole,
-                int* status) {
+                float scale_log2e, int window, int n_pages, int vec, MassWhole whole, int seq0, int* status) {
     extern __shared__ __align__(16) uint8_t af_raw[];
     __shared__ float4 w8[AF_KEYS][AF_PAIRS / 4];         // a tile's weights
     __shared__ float corr[AF_PAIRS], stat[2][AF_PAIRS];
@@ -537,7 +536,7 @@ few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict
     const int oldest = hb_oldest_visible(p_first, window, 0);
     int page0, page1;
     mass_share(oldest / HB_PAGE_TOKENS, min(p_last / HB_PAGE_TOKENS + 1, width), z, S, share_pages, page0, page1);
-    if (z == 0 && tid == 0 && p_last >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + b);
+    if (z == 0 && tid == 0 && p_last >= width * HB_PAGE_TOKENS) hb_note(status, HB_STATUS_PAGE, 1 + seq0 + b);
     auto at_of = [&](int r) -> size_t { return (size_t)(t0 + (pair0 + r) / G) * nh + g * G + (pair0 + r) % G; };
     if (page0 >= page1 && whole.out == nullptr) {        // a share without keys
         if (tid < pairs) {
@@ -653,7 +652,7 @@ few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict
         }
     }
     cp_async_wait<0>();
-    if (bad && tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + b);
+    if (bad && tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + seq0 + b);
     // join the slices: one after another adds to the first's sums, in shared memory over the tiles
     float* so = reinterpret_cast<float*>(af_raw);         // [8][2 columns]
     for (int c = 0; c < slices; c++) {
@@ -810,7 +809,7 @@ extern "C" long long hb_attention_mass_few_floats(int n_tokens, int n_heads, int
 template <typename T>
 static int launch_few(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width,
                       const int* seq_start, const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int blocks,
-                      int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status, cudaStream_t s) {
+                      int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages, int seq0, int* status, cudaStream_t s) {
     static_assert(af_smem(256, 4, 2) <= 227 * 1024, "tiles do not fit shared memory");
     static bool done[2][HB_MAX_DEVICES] = {};
     if (am_reserve(few_rows_kernel<T, 2>, af_smem(256, sizeof(T), 2), done[0]) || am_reserve(few_rows_kernel<T, 3>, 114 * 1024, done[1])) return 1;
@@ -818,7 +817,7 @@ static int launch_few(MassWhole whole, const void* q, long long q_stride, const 
 #define HB_AF_LAUNCH(ST)                                                                                                                           \
     hb_launch(few_rows_kernel<T, ST>, dim3(splits, nkv, blocks), dim3(AF_THREADS), af_smem(hd, sizeof(T), ST), s, (const T*)q, q_stride, (const T*)kc, \
               (const T*)vc, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, n_seqs, nh, nkv, hd, share_pages,            \
-              scale * MASS_LOG2E, window, n_pages, vec, whole, status)
+              scale * MASS_LOG2E, window, n_pages, vec, whole, seq0, status)
     cudaError_t e = stages == 3 ? HB_AF_LAUNCH(3) : HB_AF_LAUNCH(2);
 #undef HB_AF_LAUNCH
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
@@ -850,40 +849,46 @@ extern "C" int hb_attention_mass_few(const HbMassFew* a, int fields, float scale
     HB_REQUIRE(fields * sizeof(long long) == sizeof(*a), "attention_mass: %d fields given", fields);
     const int n_tokens = (int)a->n_tokens, n_seqs = (int)a->n_seqs, n_heads = (int)a->n_heads, n_kv_heads = (int)a->n_kv_heads, hd = (int)a->head_dim;
     const int max_new = (int)a->max_new, max_len = (int)a->max_len, splits = (int)a->splits, window = (int)a->window, n_pages = (int)a->n_pages;
-    const int pt_width = (int)a->pt_width, share_pages = (int)a->share_pages, blocks = (int)a->blocks, dtype = (int)a->dtype;
+    const int pt_width = (int)a->pt_width, share_pages = (int)a->share_pages, blocks = (int)a->blocks, dtype = (int)a->dtype, seq0 = (int)a->first_seq;
     if (n_seqs == 0 || n_tokens == 0) return 0;
+    const int* page_table = a->page_table + (size_t)seq0 * pt_width;
+    const int *seq_start = a->seq_start + seq0, *seq_pos0 = a->seq_pos0 + seq0;
     HB_REQUIRE(n_heads > 0 && n_kv_heads > 0 && n_heads % n_kv_heads == 0 && hd > 0 && hd <= 256 && n_pages > 0 && pt_width > 0,
                "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, hd);
     HB_REQUIRE((long long)max_new * (n_heads / n_kv_heads) <= MASS_FEW_PAIRS, "attention_mass: %d tokens of %d heads are no step of few tokens",
                max_new, n_heads / n_kv_heads);
-    HB_REQUIRE(n_tokens > 0 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && share_pages >= 1 && blocks >= 1 && blocks <= 65535 && max_len >= 1 &&
+    HB_REQUIRE(n_tokens > 0 && seq0 >= 0 && a->first_token >= 0 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && share_pages >= 1 && blocks >= 1 && blocks <= 65535 && max_len >= 1 &&
                    a->scratch != nullptr && a->mass != nullptr,
                "attention_mass: bad sizes");
     HB_REQUIRE(!a->whole || (splits == 1 && blocks == n_seqs), "attention_mass: a whole sequence to a block needs one share and one block each");
     HB_REQUIRE(dtype == HB_F32 || dtype == HB_BF16, "attention_mass: unsupported dtype %d", dtype);
     HB_REQUIRE(!a->tensor_cores || dtype == HB_BF16, "attention_mass: the tensor cores take bfloat16");
     HB_REQUIRE(((uintptr_t)a->scratch & 15) == 0, "attention_mass: scratch must be 16-byte aligned");
-    const size_t rows = (size_t)n_tokens * n_heads * splits;
     const long long score_ld = mass_score_ld(max_len);
-    float *scores = a->scratch, *part_ml = scores + (size_t)n_tokens * n_heads * score_ld, *part_o = part_ml + rows * 2;
+    // Scores, (maximum, sum) pairs and partial outputs of this call's (token, head) pairs.  The kernels number tokens from the step's
+    // first, of which this call's are [first_token, first_token + n_tokens): each part's address is that of the step's first pair.
+    const long long pairs = (long long)n_tokens * n_heads, in_front = a->first_token * n_heads;
+    auto part = [&](long long begin, long long floats) { return (float*)((uintptr_t)a->scratch + 4 * (begin - in_front * floats)); };
+    float *scores = part(0, score_ld), *part_ml = part(pairs * score_ld, 2LL * splits),
+          *part_o = part(pairs * (score_ld + 2LL * splits), (long long)splits * hd);
     cudaStream_t s = (cudaStream_t)a->stream;
     MassOut mo = {a->before, a->mass, nullptr};
     const MassWhole whole = {a->whole ? a->out : nullptr, a->out_stride, mo};
 #define HB_FEW_ARGS                                                                                                                              \
-    whole, a->q, a->q_stride, a->k_cache, a->v_cache, a->page_table, pt_width, a->seq_start, a->seq_pos0, part_o, part_ml, scores, score_ld, splits, \
+    whole, a->q, a->q_stride, a->k_cache, a->v_cache, page_table, pt_width, seq_start, seq_pos0, part_o, part_ml, scores, score_ld, splits, \
         share_pages, blocks
     int rc;
     if (a->tensor_cores)
-        rc = attention_few_tc(HB_FEW_ARGS, max_new, n_seqs, n_heads, n_kv_heads, hd, scale, window, n_pages, a->status, s);
+        rc = attention_few_tc(HB_FEW_ARGS, max_new, n_seqs, n_heads, n_kv_heads, hd, scale, window, n_pages, seq0, a->status, s);
     else if (dtype == HB_F32)
-        rc = launch_few<float>(HB_FEW_ARGS, n_seqs, n_heads, n_kv_heads, hd, scale, window, n_pages, a->status, s);
+        rc = launch_few<float>(HB_FEW_ARGS, n_seqs, n_heads, n_kv_heads, hd, scale, window, n_pages, seq0, a->status, s);
     else
-        rc = launch_few<bf16>(HB_FEW_ARGS, n_seqs, n_heads, n_kv_heads, hd, scale, window, n_pages, a->status, s);
+        rc = launch_few<bf16>(HB_FEW_ARGS, n_seqs, n_heads, n_kv_heads, hd, scale, window, n_pages, seq0, a->status, s);
 #undef HB_FEW_ARGS
     if (rc || a->whole) return rc;
     if (dtype == HB_F32)
-        return launch_finish<float>(part_o, part_ml, scores, score_ld, a->page_table, pt_width, a->seq_start, a->seq_pos0, a->out, a->out_stride, mo, max_len,
+        return launch_finish<float>(part_o, part_ml, scores, score_ld, page_table, pt_width, seq_start, seq_pos0, a->out, a->out_stride, mo, max_len,
                                     max_new, n_seqs, n_heads, n_kv_heads, hd, splits, window, n_pages, s);
-    return launch_finish<bf16>(part_o, part_ml, scores, score_ld, a->page_table, pt_width, a->seq_start, a->seq_pos0, a->out, a->out_stride, mo, max_len, max_new,
+    return launch_finish<bf16>(part_o, part_ml, scores, score_ld, page_table, pt_width, seq_start, seq_pos0, a->out, a->out_stride, mo, max_len, max_new,
                                n_seqs, n_heads, n_kv_heads, hd, splits, window, n_pages, s);
 }

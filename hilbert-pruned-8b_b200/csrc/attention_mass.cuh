@@ -177,4 +177,4 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
 int attention_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                      const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages,
                      int token_blocks, int max_new,
-                     int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int* status, cudaStream_t s);
+                     int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int seq0, int* status, cudaStream_t s);

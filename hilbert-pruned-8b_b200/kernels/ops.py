@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 
 from . import build
-from .plan import chunk_shares, decode_splits, few_splits, mass_splits, select_shape
+from .plan import chunk_shares, decode_splits, few_groups, few_splits, mass_splits, select_shape
 
 _c_int, _c_ll, _c_float, _c_ptr = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
 
@@ -1248,6 +1248,7 @@ class Ops:
     # ------------------------------------------------------------------ a bounded cache
     MASS_FEW_TOKENS = 8             # a step whose sequences bring more tokens than this takes the kernels for many tokens
     MASS_PLANS = 512                # plans kept: steps of the same sizes are cut alike
+    MASS_SCORES = 64 << 20          # floats of scores that a step of few tokens keeps at once (256 MB)
 
     def _on(self, *tensors) -> None:
         for t in tensors:
@@ -1265,14 +1266,14 @@ class Ops:
                               f"{tuple(t.shape)}")
 
     def _mass_plan(self, few: bool, tc: bool, bf16: bool, heads: int, kv_heads: int, head_dim: int, win: int, step, splits: Optional[int]):
-        """How a step of ``attention_mass`` is cut, from its sizes alone.  Few tokens: (blocks, whether on the tensor cores, whether
-        a block has a whole sequence, most shares of the pages, fewest pages of one, floats of scratch).  Many: (shares of the keys'
+        """How a step of ``attention_mass`` is cut, from its sizes alone.  Few tokens: (floats of scratch, whether on the tensor cores,
+        kernels, per group of sequences that run at once what ``_few_plan`` gives).  Many: (shares of the keys'
         sums, blocks of queries, tiles of keys, most shares of a block of queries, tiles of keys in one, tokens whose blocks may be
         cut, distance of two heads' log-sums, floats of the log-sums, of the sums' shares, of the partial results)."""
         T, group = step.num_tokens, heads // kv_heads
-        # (single tokens: from the page table's width alone, so that a captured step and an eager one sum alike)
-        single = step.max_new == 1 and few
-        key = (few, tc, bf16, heads, kv_heads, head_dim, win, splits, T, step.num_seqs, step.max_len, step.max_new,
+        # (a step of single tokens goes by max_len alone, which a captured step gives as the bound of its replays)
+        single = few and step.max_new == 1 and T == step.num_seqs
+        key = (few, tc, bf16, heads, kv_heads, head_dim, win, splits, self.MASS_SCORES, T, step.num_seqs, step.max_len, step.max_new,
                None if single else (tuple(step.host_new), tuple(step.host_len)))
         plan = self._mass_plans.get(key)
         if plan is not None:
@@ -1281,22 +1282,15 @@ class Ops:
             at_once = self.lib.hb_attention_few_tc_tokens(heads, kv_heads, head_dim, step.max_new) if tc else 0
             # blocks of a sequence: of so many tokens, or without the tensor cores of so many pairs of a token and a head of the group
             per, each = (at_once, 1) if at_once else (self.lib.hb_attention_few_block_pairs(), group)
-            new = [1] * step.num_seqs if single else step.host_new
-            blocks = sum(-(-n * each // per) for n in new)
-            given, least = splits, 1
-            if splits is None:
-                lens = [step.max_len] * step.num_seqs if single else step.host_len
-                seen = [-(-(min(ln, win + n) if win else ln) // 64) for n, ln in zip(new, lens) for _ in range(-(-n * each // per))]
-                slots = 2 if at_once else self.lib.hb_attention_few_blocks_per_sm(head_dim, int(bf16))
-                splits, least = few_splits(seen, kv_heads, slots * self.sm_count)
-            # short sequences, each in one block: it sees all of the keys and no second kernel follows.  (Captured, device time of 32 heads
-            # over 8: size 64, one sequence of 300 rows 7.1 in two kernels and 7.4 us in one, of 440 rows 7.8 and 9.1; eight with four
-            # tokens each 15.8 and 12.6; size 128, 250 rows 8.2 and 8.3, 500 rows 8.9 and 12.6; in 32-bit 60 rows 10.9 and 8.5, 120 rows
-            # 10.9 and 11.3.  The host's part of a call is 2.4 us shorter.)
-            rows = 64 if not at_once else 256 if head_dim > 64 else 384
-            whole = (given is None and step.max_len <= rows and blocks == step.num_seqs == sum(n > 0 for n in new) and T >= step.num_seqs)
-            splits, least = (1, 1) if whole else (max(1, min(splits, (step.max_len + 63) // 64)), least)
-            plan = (blocks, int(at_once > 0), int(whole), splits, least, self.lib.hb_attention_mass_few_floats(T, heads, head_dim, splits, step.max_len))
+            if single:
+                new, lens = [1] * step.num_seqs, [step.max_len] * step.num_seqs
+            else:
+                new, lens = step.host_new, step.host_len
+            # (max_len is a bound: a captured step's sequences may grow to it)
+            bound = lens if max(lens) == step.max_len else [step.max_len] * step.num_seqs
+            groups = [self._few_plan(new[b: b + n], lens[b: b + n], b, n, t, tokens, rows, at_once, per, each, bf16, heads, kv_heads, head_dim, win, splits)
+                      for b, n, t, tokens, rows in few_groups(new, bound, heads, self.MASS_SCORES)]
+            plan = (max(g[0] for g in groups), int(at_once > 0), sum(2 - g[1] for g in groups), [g[1:] for g in groups])
         else:
             # the tensor cores take two tiles of 128 queries at a time: two heads, or with an odd group two blocks of tokens
             rows, keys = (128 if group % 2 == 0 else 256, self.lib.hb_attention_mass_tc_keys()) if tc else (64, 64)
@@ -1318,6 +1312,26 @@ class Ops:
             self._mass_plans.clear()
         self._mass_plans[key] = plan
         return plan
+
+    def _few_plan(self, new, lens, first: int, seqs: int, token: int, tokens: int, max_len: int, at_once: int, per: int, each: int, bf16: bool,
+                  heads: int, kv_heads: int, head_dim: int, win: int, splits: Optional[int]):
+        """How ``seqs`` sequences of a step of few tokens are cut: (floats of scratch, whether a block has a whole sequence, first sequence, their
+        number, first token, their number, rows of the longest, most shares of the pages, fewest pages of one, blocks of tokens)."""
+        blocks = sum(-(-n * each // per) for n in new)
+        given, least = splits, 1
+        if splits is None:
+            seen = [-(-(min(ln, win + n) if win else ln) // 64) for n, ln in zip(new, lens) for _ in range(-(-n * each // per))]
+            slots = 2 if at_once else self.lib.hb_attention_few_blocks_per_sm(head_dim, int(bf16))
+            splits, least = few_splits(seen, kv_heads, slots * self.sm_count)
+        # short sequences, each in one block: it sees all of the keys and no second kernel follows.  (Captured, device time of 32 heads
+        # over 8: size 64, one sequence of 300 rows 7.1 in two kernels and 7.4 us in one, of 440 rows 7.8 and 9.1; eight with four
+        # tokens each 15.8 and 12.6; size 128, 250 rows 8.2 and 8.3, 500 rows 8.9 and 12.6; in 32-bit 60 rows 10.9 and 8.5, 120 rows
+        # 10.9 and 11.3.  The host's part of a call is 2.4 us shorter.)
+        rows = 64 if not at_once else 256 if head_dim > 64 else 384
+        whole = given is None and max_len <= rows and blocks == seqs == sum(n > 0 for n in new) and tokens >= seqs
+        splits, least = (1, 1) if whole else (max(1, min(splits, (max_len + 63) // 64)), least)
+        return (self.lib.hb_attention_mass_few_floats(tokens, heads, head_dim, splits, max_len), int(whole), first, seqs, token, tokens, max_len, splits,
+                least, blocks)
 
     def attention_mass(self, qkv, heads: int, kv_heads: int, head_dim: int, cache, step, out, scale: float, window: Optional[int], mass,
                        before=None, splits: Optional[int] = None) -> None:
@@ -1359,16 +1373,20 @@ class Ops:
         fast = self.use_fast_attention and dtype == torch.bfloat16 and (k_at | v_at) % 16 == 0
         old, new, status, stream = before.data_ptr() if before is not None else 0, mass.data_ptr(), self.status.data_ptr(), self._stream()
         # scratch of the call's own, from torch's allocator: two calls on two streams, or two captured graphs, share nothing
-        if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * (heads // kv_heads) <= self.MASS_FEW_PAIRS:
-            blocks, tc, whole, splits, least, floats = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, dtype == torch.bfloat16, heads,
-                                                                       kv_heads, head_dim, win, step, splits)
+        if step.max_new <= self.MASS_FEW_TOKENS and step.max_new * (heads // kv_heads) <= self.MASS_FEW_PAIRS \
+                and (step.max_new == 1 or heads * step.max_new * step.max_len <= self.MASS_SCORES or max(step.host_len) < step.max_len):
+            floats, tc, kernels, groups = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, dtype == torch.bfloat16, heads, kv_heads,
+                                                          head_dim, win, step, splits)
             scratch = torch.empty(floats, dtype=torch.float32, device=self.device)
-            # (the fields of HbMassFew, 8 bytes each: a third of the time of as many arguments)
-            a = array("q", (q_at, code, q_ld, k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out_at,
-                            out_ld, scratch.data_ptr(), old, new, splits, least, blocks, tc, whole, T, step.num_seqs, step.max_new, step.max_len, heads,
-                            kv_heads, head_dim, win, pages, status, stream))
-            self._call("hb_attention_mass_few", *a.buffer_info(), scale)
-            self.launches += 2 - whole
+            at, tables, width = scratch.data_ptr(), pt.data_ptr(), pt.shape[1]
+            starts, places = step.seq_start.data_ptr(), step.seq_pos0.data_ptr()
+            # (groups of sequences one after another through the same scratch; nearly always one.)
+            for whole, seq, seqs, token, tokens, rows, shares, least, blocks in groups:
+                # (the fields of HbMassFew, 8 bytes each: a third of the time of as many arguments)
+                a = array("q", (q_at, code, q_ld, k_at, v_at, tables, width, starts, places, out_at, out_ld, at, old, new, shares, least, blocks, tc, whole,
+                                tokens, seqs, seq, token, step.max_new, rows, heads, kv_heads, head_dim, win, pages, status, stream))
+                self._call("hb_attention_mass_few", *a.buffer_info(), scale)
+            self.launches += kernels
             return
         tc = bool(fast and self.use_tcgen05_attention and (q_at | out_at) % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0
                   and self.lib.hb_attention_mass_tc_supported(heads, kv_heads, head_dim))

@@ -28,6 +28,31 @@ def decode_splits(sequences: int, kv_heads: int, max_pages: int, cta_slots: int)
     return best
 
 
+def few_groups(new, lengths, heads: int, limit: int):
+    """Which sequences of a step of few tokens run at once: ``[(first sequence, their number, first token, their number, rows of the longest)]``,
+    neighbours, in order.  The scores of a group (``heads`` times its tokens times its longest sequence's rows, in whole pages) are at most
+    ``limit`` floats, or those of one sequence's tokens: one long sequence among many short ones would else cost every token a row of its
+    length (64 single tokens, one of them behind 131072 rows, 32 heads: 1 GB).  A sequence without new tokens goes with one that has some."""
+    parts, first, longest = [], 0, 1                              # [first sequence, their number, their tokens, rows of the longest]
+    for b, (n, ln) in enumerate(zip(new, lengths)):
+        longest = max(longest, ln)
+        if n > 0:
+            parts.append([first, b + 1 - first, n, longest])
+            first, longest = b + 1, 1
+    if parts:
+        parts[-1][1] += len(new) - first
+        parts[-1][3] = max(parts[-1][3], longest)
+    groups, at = [], 0
+    for b, count, n, ln in parts:
+        if groups and heads * (groups[-1][3] + n) * (-(-max(groups[-1][4], ln) // 64) * 64) <= limit:
+            b0, seqs, t0, tokens, rows = groups[-1]
+            groups[-1] = (b0, seqs + count, t0, tokens + n, max(rows, ln))
+        else:
+            groups.append((b, count, at, n, ln))
+        at += n
+    return groups
+
+
 def few_splits(pages, kv_heads: int, cta_slots: int):
     """Shares of a sequence's pages in a step of few tokens that keeps its scores: (the most of a sequence, the fewest pages of one);
     ``pages``: how many each block of tokens sees.  As ``decode_splits``, but down to a page each (64 shares at most) while the device has room, since

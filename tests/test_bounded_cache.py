@@ -291,6 +291,75 @@ def test_short_sequences_in_one_kernel(ops, dtype, heads, kv, hd, past, new, win
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,heads,kv,hd,window", [(torch.bfloat16, 8, 2, 64, None), (torch.bfloat16, 6, 2, 80, 100), (torch.float32, 4, 2, 33, None)])
+@pytest.mark.parametrize("past,new", [
+    ([700, 3, 64, 0, 5000, 200, 1], [1, 1, 1, 1, 1, 1, 1]), ([700, 3, 64, 300, 5000, 200, 1], [2, 1, 8, 0, 3, 1, 5]),
+    ([40, 3, 64, 0, 20], [1, 1, 1, 1, 1]), ([700, 900, 64, 300, 2000], [0, 3, 1, 1, 0]), ([100, 3000], [1, 0])])
+def test_sequences_in_groups(ops, dtype, heads, kv, hd, window, past, new):
+    """Scores of a few rows at a time: sequences run one group after another through the same scratch."""
+    from hilbert_pruned_8b_b200.kernels.plan import few_groups
+    c = Case(dtype, heads, kv, hd, past, new, window, seed=12)
+    start = torch.randn(c.pages, kv, PAGE, device=DEV)
+    for limit in (1, heads * 2 * 800, heads * 4 * 5100):
+        # (a limit below one sequence's scores would send several tokens to the kernels for many)
+        ops.MASS_SCORES = max(limit, heads * c.step.max_new * c.step.max_len) if c.step.max_new > 1 else limit
+        groups, mass, again, own = few_groups(c.new, c.lens, heads, ops.MASS_SCORES), start.clone(), start.clone(), c.before.clone()
+        ops.call_log, log = [], ops.call_log
+        try:
+            c.check(c.run(ops, mass, before=c.before), mass, c.before, start)
+            assert limit > 1 or c.step.max_new > 1 or len(groups) == sum(n > 0 for n in new)
+            assert sum(new) == len(new) or ops.call_log == ["hb_attention_mass_few"] * len(groups)
+            c.run(ops, again, before=c.before)
+            c.run(ops, own, before=own)
+        finally:
+            ops.call_log = log
+            del ops.MASS_SCORES
+        assert torch.equal(again, mass) and torch.equal(own[mass != start], mass[mass != start])
+    ops.check_errors()
+
+
+@pytest.mark.gpu
+def test_scores_of_one_long_sequence_among_short_ones(ops):
+    """64 single tokens, one of them behind 131072 rows: scratch within its limit, captured and eager."""
+    past = [50 + b for b in range(64)]
+    past[20] = 131072
+    c = Case(torch.bfloat16, 32, 1, 64, past, [1] * 64, None, seed=3, garbage=0.0)
+    mass, out = torch.zeros(c.pages, 1, PAGE, device=DEV), torch.empty(64, 32 * 64, dtype=torch.bfloat16, device=DEV)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    c.run(ops, mass, out=out)
+    torch.cuda.synchronize()
+    assert torch.cuda.max_memory_allocated() - held < 300 << 20
+    want, sums = out.clone(), mass.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        c.run(ops, mass, out=out)
+    out.zero_(), mass.zero_()
+    graph.replay()
+    assert torch.equal(out, want) and torch.equal(mass, sums)
+    c.check(out, mass, None, torch.zeros_like(mass))
+    ops.check_errors()
+
+
+@pytest.mark.gpu
+def test_many_drafted_tokens_of_a_sequence_too_long_for_its_scores(ops):
+    """Several tokens of one sequence whose scores alone are above the limit: the kernels that keep none."""
+    c = Case(torch.bfloat16, 8, 2, 64, [900, 100], [5, 2], None, seed=3)
+    mass = torch.zeros(c.pages, 2, PAGE, device=DEV)
+    ops.MASS_SCORES = 8 * 5 * 800
+    try:
+        ops.call_log, log = [], ops.call_log
+        c.check(c.run(ops, mass, before=c.before), mass, c.before, torch.zeros_like(mass))
+        assert ops.call_log == ["hb_attention_mass_tc"]
+    finally:
+        ops.call_log = log
+        del ops.MASS_SCORES
+    ops.check_errors()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [[90, 3], [1, 2]])
 def test_a_sequence_without_new_tokens(ops, new):
     """Rows of a sequence that brings nothing keep their earlier sum."""
@@ -611,6 +680,36 @@ def test_evict_rows_refuses(change, text):
              page_table=_i32(4, 2), to_table=None)
     with pytest.raises(KernelError, match=text):
         _Fake().evict_rows(**dict(a, **change))
+
+
+def test_groups_of_sequences():
+    """Every sequence once and in order, with its tokens, within the limit unless a group has one sequence with new tokens."""
+    from hilbert_pruned_8b_b200.kernels.plan import few_groups
+    assert few_groups([1] * 8, [300] * 8, 32, 64 << 20) == [(0, 8, 0, 8, 300)]
+    assert few_groups([1, 1, 1], [131072, 5, 131072], 32, 32 * 131072) == [(0, 1, 0, 1, 131072), (1, 1, 1, 1, 5), (2, 1, 2, 1, 131072)]
+    assert few_groups([0, 1, 0, 2, 0], [7, 1, 900, 2, 65], 4, 1) == [(0, 2, 0, 1, 7), (2, 3, 1, 2, 900)]
+    assert few_groups([0, 0], [7, 1], 4, 1) == [] and few_groups([], [], 4, 1) == []
+    rng = random.Random(1)
+    for _ in range(300):
+        n = rng.randint(1, 40)
+        new, heads = [rng.choice([0, 1, 1, rng.randint(1, 8)]) for _ in range(n)], rng.choice([1, 8, 32])
+        lens = [m + (rng.randint(0, 131072) if rng.random() < 0.2 else rng.randint(0, 900)) for m in new]
+        limit = rng.choice([1, 10 ** 6, 64 << 20])
+        groups = few_groups(new, lens, heads, limit)
+        if sum(new) == 0:
+            assert groups == []
+            continue
+        seq = token = 0
+        for first, count, t0, tokens, rows in groups:
+            assert (first, t0) == (seq, token) and count > 0 and tokens > 0
+            inside = list(range(first, first + count))
+            assert tokens == sum(new[b] for b in inside) and rows == max(max(1, lens[b]) for b in inside)
+            assert heads * tokens * -(-rows // 64) * 64 <= limit or sum(new[b] > 0 for b in inside) == 1
+            seq, token = seq + count, token + tokens
+        assert seq == n and token == sum(new)
+    # 64 single tokens, one long sequence: 1 GB in one group
+    groups = few_groups([1] * 64, [131072] * 64, 32, 64 << 20)
+    assert len(groups) == 4 and max(32 * g[3] * g[4] for g in groups) <= 64 << 20
 
 
 def test_shapes_of_the_launches():
