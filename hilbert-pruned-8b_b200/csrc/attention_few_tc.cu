@@ -39,7 +39,7 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
     const int t0 = seq_start[b] + blk * tokens_per_block, n_tok = min(tokens_per_block, seq_start[b + 1] - t0);
     const int p0 = seq_pos0[b] + blk * tokens_per_block, p_last = p0 + n_tok - 1;
     const int width = (int)min((long long)pt_width, score_ld / HB_PAGE_TOKENS);       // no score is written behind its head's
-    const int first = hb_oldest_visible(p0, window, 0) / HB_PAGE_TOKENS, last = min(p_last / HB_PAGE_TOKENS + 1, width);
+    const int oldest = hb_oldest_visible(p0, window, 0), first = oldest / HB_PAGE_TOKENS, last = min(p_last / HB_PAGE_TOKENS + 1, width);
     int page0, page1;
     mass_share(first, last, z, S, share_pages, page0, page1);
     const int* pt = page_table + (size_t)b * pt_width;
@@ -70,8 +70,9 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
                 const int row = i / chunks, ch = i - row * chunks;
                 const uint32_t off = swizzled<ROW_BYTES>(row, ch);
                 cp_async_16(kdst + off, ksrc + (size_t)i * 16);
-                // values behind the last key are whatever the page held before, and 0 * NaN is NaN
-                cp_async_16_or_zero(vdst + off, vsrc + (size_t)i * 16, pi * HB_PAGE_TOKENS + row <= p_last);
+                // values behind the last key and in front of the oldest are whatever is there, and 0 * NaN is NaN
+                const int key = pi * HB_PAGE_TOKENS + row;
+                cp_async_16_or_zero(vdst + off, vsrc + (size_t)i * 16, key >= oldest && key <= p_last);
             }
         }
         cp_async_commit();

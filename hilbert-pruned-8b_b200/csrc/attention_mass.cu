@@ -26,18 +26,18 @@
 #define AM_THREADS 256
 
 // 64 rows of a tensor as float32 in shared memory, `ld` apart (a multiple of 4), in two halves so that the loads can be in flight while
-// something else is computed: registers (up to 4 NC numbers a thread), then shared memory.  Rows from `rows` on and columns
+// something else is computed: registers (up to 4 NC numbers a thread), then shared memory.  Rows outside [from, rows) and columns
 // behind hd are zero.  vec: rows are aligned for four elements at a time.
 template <typename T, int NC>
 struct AmTile {
     float4 x[NC];
-    __device__ __forceinline__ void load(const T* src, long long stride, int hd, int rows, bool vec, int tid) {
+    __device__ __forceinline__ void load(const T* src, long long stride, int hd, int rows, bool vec, int tid, int from = 0) {
         const int per = (hd + 3) >> 2;
 #pragma unroll
         for (int u = 0; u < NC; u++) {
             const int i = tid + u * AM_THREADS, r = i / per, d = (i - r * per) * 4;
             x[u] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (r < rows) {
+            if (r >= from && r < rows) {
                 const T* p = src + (size_t)r * stride + d;
                 if (vec) {
                     float v[4];
@@ -112,7 +112,7 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
     if (!mass_find_block(seq_start, n_seqs, gridDim.y - 1 - blockIdx.y, AM_ROWS, b, blk, place0)) return;
     const int t0 = seq_start[b] + blk * AM_ROWS;
     const int rows = min(AM_ROWS, seq_start[b + 1] - t0);
-    const int p0 = seq_pos0[b] + blk * AM_ROWS, p_last = p0 + rows - 1;
+    const int p0 = seq_pos0[b] + blk * AM_ROWS, p_last = p0 + rows - 1, oldest = hb_oldest_visible(p0, window, 0);
     int page0;
     const int n_all = key_tiles_of(p0, p_last, window, HB_PAGE_TOKENS, page0), S = shares_of(sh, n_all);
     if (z >= S) return;
@@ -144,7 +144,8 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
     for (int pi = page0; pi < page1; pi++) {
         if (held == 0 && tid == 0) hb_note(status, HB_STATUS_PAGE, 1 + b);
         __syncthreads();                                 // the keys are there; values and weights of the page before are used up
-        tile.load(vc + row0 * hd, hd, hd, held, vec_kv, tid);
+        // (values in front of the oldest key that the first row sees may be anything, and 0 * NaN is NaN)
+        tile.load(vc + row0 * hd, hd, hd, held, vec_kv, tid, oldest - pi * HB_PAGE_TOKENS);
         float s[4][4];
         am_scores(s, qs, ks, ld, tx, ty);
 #pragma unroll

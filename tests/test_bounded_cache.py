@@ -413,6 +413,27 @@ def test_pages_given_back_in_front_of_the_window(ops, dtype, hd, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("past,window", [(700, 100), (700, 1), (150, 20), (5000, 1500)])
+@pytest.mark.parametrize("new", [[300], [90], [5], [1]])
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 128), (torch.bfloat16, 64), (torch.bfloat16, 80), (torch.bfloat16, 200), (torch.float32, 64)])
+def test_rows_in_front_of_the_window_do_not_count(ops, dtype, hd, new, past, window):
+    """Rows that no token sees any more may hold anything, those of the first visible page too: NaN and infinities there change no bit."""
+    c = Case(dtype, 6, 2, hd, [past], new, window, seed=4)
+    start = torch.randn(c.pages, 2, PAGE, device=DEV)
+    full = start.clone()
+    want = c.run(ops, full, before=c.before)
+    c.check(want, full, c.before, start)
+    j = torch.arange(past - window + 1, device=DEV)       # all rows in front of the oldest that the first token sees
+    page = c.table[0].long()[j // PAGE]
+    for junk in (NAN, math.inf, -math.inf):
+        c.k[page, :, j % PAGE] = junk
+        c.v[page, :, j % PAGE] = junk
+        mass = start.clone()
+        assert torch.equal(c.run(ops, mass, before=c.before), want) and torch.equal(mass, full)
+    ops.check_errors()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [[90, 40], [1, 3]])
 def test_captured_and_replayed(ops, new):
     """A captured call follows its inputs; two graphs that are replayed on two streams share nothing."""
