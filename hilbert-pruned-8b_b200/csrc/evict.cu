@@ -414,10 +414,10 @@ __device__ __forceinline__ void evict_move(const EvictRows& p, U* data, int row_
     if (bad) hb_note(p.status, HB_STATUS_PAGE, 1 + b);
 }
 
-// grid: (parts, lists); a list's parts are, for every range of rows, the slices of the keys, those of the values, the mass
+// grid: `blocks` of each list, list by list; a list's blocks are, for every range of rows, the slices of the keys, those of the values, the mass
 template <typename U>
 __global__ void __launch_bounds__(ER_THREADS)
-evict_rows_kernel(EvictRows p, U* k, int k_units, int k_slices, U* v, int v_units, int v_slices, uint32_t* mass, int rows_per_block) {
+evict_rows_kernel(EvictRows p, U* k, int k_units, int k_slices, U* v, int v_units, int v_slices, uint32_t* mass, int rows_per_block, int blocks) {
     // no pdl_trigger(): the decode attention kernels read pages of older tokens before their griddepcontrol.wait, and
     // with small kernels in between they could be resident while rows still move.  Without the trigger, nothing behind this
     // kernel starts before it has finished.
@@ -426,8 +426,8 @@ evict_rows_kernel(EvictRows p, U* k, int k_units, int k_slices, U* v, int v_unit
     p.from_table = pdl_fresh(p.from_table);
     p.to_table = pdl_fresh(p.to_table);
     const int parts = k_slices + v_slices + (mass != nullptr ? 1 : 0);
-    const int part = blockIdx.x % parts, row = blockIdx.y;
-    const int j0 = (blockIdx.x / parts) * rows_per_block, j1 = min(j0 + rows_per_block, p.budget);
+    const int row = blockIdx.x / blocks, block = blockIdx.x % blocks, part = block % parts;
+    const int j0 = (block / parts) * rows_per_block, j1 = min(j0 + rows_per_block, p.budget);
     if (p.kept[(size_t)row * p.budget + j0] < 0) return;      // behind the last kept row
     if (part < k_slices) {
         const int a = k_units * part / k_slices, z = k_units * (part + 1) / k_slices;
@@ -450,7 +450,6 @@ extern "C" int hb_evict_rows(const int* kept, void* k, int k_row_bytes, void* v,
     HB_REQUIRE(entries > 0 && n_seqs > 0 && n_kv_heads > 0 && n_pages > 0 && from_width > 0 && budget > 0 && sm_count > 0, "evict_rows: bad sizes");
     HB_REQUIRE(k_row_bytes > 0 && v_row_bytes > 0 && k_row_bytes % 2 == 0 && v_row_bytes % 2 == 0, "evict_rows: bad row sizes");
     const long long lists = (long long)entries * n_seqs * n_kv_heads;
-    HB_REQUIRE(lists <= 65535, "evict_rows: %lld lists of rows are too many for one launch", lists);
     EvictRows p = {kept, from_table, to_table != nullptr ? to_table : from_table, from_width, to_table != nullptr ? to_width : from_width,
                    n_seqs, n_kv_heads, n_pages, budget, to_table == nullptr, status};
     HB_REQUIRE(p.in_place || budget <= (long long)p.to_width * HB_PAGE_TOKENS, "evict_rows: %d rows do not fit a page table of width %d", budget, p.to_width);
@@ -472,11 +471,11 @@ extern "C" int hb_evict_rows(const int* kept, void* k, int k_row_bytes, void* v,
         rows_per_block = rows_per_block < 64 ? 64 : rows_per_block;
     }
     const long long blocks = (long long)((budget + rows_per_block - 1) / rows_per_block) * (ks + vs + (mass != nullptr ? 1 : 0));
-    HB_REQUIRE(blocks <= 0x7fffffffLL, "evict_rows: too many rows for one launch");
-    dim3 grid((unsigned)blocks, (unsigned)lists);
+    HB_REQUIRE(blocks * lists <= 0x7fffffffLL, "evict_rows: %lld lists of %d rows are too many for one launch", lists, budget);
+    dim3 grid((unsigned)(blocks * lists));
     cudaStream_t s = (cudaStream_t)stream;
 #define HB_ER_LAUNCH(U) \
-    hb_launch(evict_rows_kernel<U>, grid, dim3(ER_THREADS), 0, s, p, (U*)k, ku, ks, (U*)v, vu, vs, (uint32_t*)mass, rows_per_block)
+    hb_launch(evict_rows_kernel<U>, grid, dim3(ER_THREADS), 0, s, p, (U*)k, ku, ks, (U*)v, vu, vs, (uint32_t*)mass, rows_per_block, (int)blocks)
     cudaError_t e = unit == 32 ? HB_ER_LAUNCH(Unit32) : unit == 16 ? HB_ER_LAUNCH(uint4) : unit == 4 ? HB_ER_LAUNCH(uint32_t) : HB_ER_LAUNCH(unsigned short);
 #undef HB_ER_LAUNCH
     if (e != cudaSuccess) return hb_fail("evict_rows: launch failed: %s", cudaGetErrorString(e));

@@ -568,6 +568,28 @@ def test_evict_rows(ops, dtype, E, kv, hd, v_hd, lengths, budget, first, recent,
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("apart", [False, True])
+def test_evict_rows_of_very_many_lists(ops, apart):
+    """More lists of rows (entries x sequences x kv heads) than a grid's second axis holds."""
+    E, B, kv, hd = 32, 1100, 2, 4                         # 70400 lists
+    pages = 2 * B
+    table = torch.arange(B, dtype=torch.int32, device=DEV).view(B, 1)
+    to = (table + B).contiguous() if apart else None
+    k, v = (torch.randn(E, pages, kv, PAGE, hd, device=DEV) for _ in range(2))
+    mass = torch.rand(E, pages, kv, PAGE, device=DEV)
+    kept = torch.empty(E, B, kv, 2, dtype=torch.int32, device=DEV)
+    ops.evict_select(mass, table, _ints([3] * B), 0, 1, kept)
+    want = [x.clone() for x in (k, v, mass)]
+    e, b, h, j = torch.nonzero(kept >= 0, as_tuple=True)
+    for x, y in zip((k, v, mass), want):
+        y[e, b + (B if apart else 0), h, j] = x[e, b, h, kept[e, b, h, j].long()]
+    ops.evict_rows(kept, k, v, mass, table, to_table=to)
+    for x, y in zip((k, v, mass), want):
+        assert torch.equal(x, y)
+    ops.check_errors()
+
+
+@pytest.mark.gpu
 def test_evict_rows_skips_what_has_no_page(ops):
     from hilbert_pruned_8b_b200.kernels.ops import KernelError
     table, pages, _ = _tables([200], 1)
