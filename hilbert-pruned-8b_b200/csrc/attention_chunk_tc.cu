@@ -71,6 +71,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                    v_empty0 = smem_u32(bars + 7), s_full0 = smem_u32(bars + 9), p_full0 = smem_u32(bars + 11), pv_done0 = smem_u32(bars + 15),
                    s_free0 = smem_u32(bars + 17);              // p_full: [2 tiles][2 halves of the keys]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    mass_fresh(page_table, seq_start, seq_pos0);
 
     // The two tiles: heads head0 and head0 + 1 (head_pairs) of one block of tokens, or blocks 2 blk and 2 blk + 1 of head0.  Blocks
     // are taken from the back and heads are the fast index: what sees the most keys starts first.
@@ -79,7 +81,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     const int span = head_pairs ? FA_ROWS : 2 * FA_ROWS;
     int b, blk, place0;
     const bool has_work = mass_find_block(seq_start, n_seqs, gridDim.y - 1 - blockIdx.y, span, b, blk, place0);
-    const int t_begin = has_work ? seq_start[b] : 0, n_new = has_work ? seq_start[b + 1] - t_begin : 1, pos0 = has_work ? seq_pos0[b] : 0;
+    const int t_begin = mass_uniform(has_work ? seq_start[b] : 0), n_new = mass_uniform(has_work ? seq_start[b + 1] - t_begin : 1),
+              pos0 = mass_uniform(has_work ? seq_pos0[b] : 0);
     const int row0 = blk * span;                               // the first of the CTA's new tokens
     const int first_pos = pos0 + row0, last_pos = pos0 + min(row0 + span, n_new) - 1;
     int jt0, n_it = key_tiles_of(first_pos, last_pos, window, FA_KEYS, jt0);
@@ -116,7 +119,6 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     constexpr bool APART = HD == 64;
     const uint32_t tmem_base = *tmem_slot;
     pdl_trigger();
-    pdl_wait();
 
     if (warp == 8) {
         // ---------------------------------------------------------------- TMA producer
@@ -127,35 +129,52 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
                 for (int half = 0; half < HALVES; half++)
                     tma_load_3d(smem_base + i * TILE + half * FA_HALF_BYTES, &map_q, q_full, half * 64, head0 + (head_pairs ? i : 0),
                                 t_begin + row0 + (head_pairs ? 0 : i * FA_ROWS));
-            auto load_tile = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int it) {
-                mbar_expect_tx(bar, TILE);
+            // the pages of tile `it` of the keys and the values: both numbers asked for at once, a tile ahead
+            int page[2], next_page[2];
+            auto ask = [&](int it) {
+#pragma unroll
                 for (int pg = 0; pg < 2; pg++) {
                     const int pi = (jt0 + it) * 2 + pg;
-                    int page = pi < pt_width ? pt[pi] : -1;
-                    if (page < 0 || page >= n_pages) {
-                        // a page behind the last row's key or in front of the oldest that the first row sees may be missing
-                        if (page >= n_pages || (pi >= lo_cta / HB_PAGE_TOKENS && pi <= last_pos / HB_PAGE_TOKENS))
-                            hb_note(error_flag, HB_STATUS_PAGE, 1 + b);
-                        page = 0;                                   // never read outside the cache
-                    }
-                    for (int half = 0; half < HALVES; half++)
-                        tma_load_2d(dst + half * FA_HALF_BYTES + pg * (FA_HALF_BYTES / 2), map, bar, half * 64, (page * nkv + g) * HB_PAGE_TOKENS);
+                    next_page[pg] = it < n_it && pi < pt_width ? pt[pi] : -1;
                 }
             };
+            auto take = [&](int it) {
+#pragma unroll
+                for (int pg = 0; pg < 2; pg++) {
+                    const int pi = (jt0 + it) * 2 + pg;
+                    page[pg] = next_page[pg];
+                    if (page[pg] < 0 || page[pg] >= n_pages) {
+                        // a page behind the last row's key or in front of the oldest that the first row sees may be missing
+                        if (page[pg] >= n_pages || (pi >= lo_cta / HB_PAGE_TOKENS && pi <= last_pos / HB_PAGE_TOKENS))
+                            hb_note(error_flag, HB_STATUS_PAGE, 1 + b);
+                        page[pg] = 0;                               // never read outside the cache
+                    }
+                }
+            };
+            auto load_tile = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar) {
+                mbar_expect_tx(bar, TILE);
+#pragma unroll
+                for (int pg = 0; pg < 2; pg++)
+                    for (int half = 0; half < HALVES; half++)
+                        tma_load_2d(dst + half * FA_HALF_BYTES + pg * (FA_HALF_BYTES / 2), map, bar, half * 64, (page[pg] * nkv + g) * HB_PAGE_TOKENS);
+            };
+            ask(0);
             int k_issued = 0, v_issued = 0;
             for (int it = 0; it < n_it; it++) {
                 const int s = it % CT_STAGES;
+                take(it);
+                ask(it + 1);
                 if (!mbar_wait(k_empty0 + 8 * s, ((it / CT_STAGES) & 1) ^ 1)) {
                     atomicExch(error_flag, 51);
                     break;
                 }
-                load_tile(k_smem + s * TILE, &map_k, k_full0 + 8 * s, it);
+                load_tile(k_smem + s * TILE, &map_k, k_full0 + 8 * s);
                 k_issued = it + 1;
                 if (!mbar_wait(v_empty0 + 8 * s, ((it / CT_STAGES) & 1) ^ 1)) {
                     atomicExch(error_flag, 52);
                     break;
                 }
-                load_tile(v_smem + s * TILE, &map_v, v_full0 + 8 * s, it);
+                load_tile(v_smem + s * TILE, &map_v, v_full0 + 8 * s);
                 v_issued = it + 1;
             }
             for (int it = max(0, k_issued - CT_STAGES); it < k_issued; it++)

@@ -30,6 +30,7 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
     __shared__ float lse[ROWS];                            // of a whole sequence's pairs
     pdl_trigger();
     pdl_wait();
+    mass_fresh(page_table, seq_start, seq_pos0);
     q = pdl_fresh(q);
     const int z = blockIdx.x, g = blockIdx.y, S = gridDim.x;
     const int tid = threadIdx.x, lane = tid & 31, warp = (tid >> 5) & 3, rt = tid >> 7;       // quarter of a page's keys, tile of rows

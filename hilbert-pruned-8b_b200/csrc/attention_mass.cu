@@ -13,6 +13,8 @@
 //                         writing and reading a weight for every (token, head, row).  Every key's sum belongs to one thread from
 //                         beginning to end, so the order of the additions is fixed.
 // Softmax statistics, scores, sums and mass are float32; lse is in units of log 2.
+#include <type_traits>
+
 #include "api.h"
 #include "attention_mass.cuh"
 #include "mma.cuh"
@@ -98,6 +100,7 @@ attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __re
     extern __shared__ __align__(16) float am_smem[];
     pdl_trigger();
     pdl_wait();
+    mass_fresh(page_table, seq_start, seq_pos0);
     q = pdl_fresh(q);
     kc = pdl_fresh(kc);
     vc = pdl_fresh(vc);
@@ -237,6 +240,8 @@ shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* 
     __shared__ float ws[8][32];
     pdl_trigger();
     pdl_wait();
+    seq_start = pdl_fresh(seq_start);
+    seq_pos0 = pdl_fresh(seq_pos0);
     const int lane = threadIdx.x & 31;
     int b, i, place0;
     if (!mass_find(n_seqs, blockIdx.x,
@@ -298,6 +303,7 @@ mass_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restric
     extern __shared__ __align__(16) float am_smem[];
     pdl_trigger();
     pdl_wait();
+    mass_fresh(page_table, seq_start, seq_pos0);
     q = pdl_fresh(q);
     kc = pdl_fresh(kc);
     lse = pdl_fresh(lse);
@@ -370,6 +376,7 @@ __global__ void mass_join_kernel(const int* __restrict__ page_table, int pt_widt
                                  const int* __restrict__ seq_pos0, MassOut mo, int n_seqs, int nkv, int n_pages, int tile, int S) {
     pdl_trigger();
     pdl_wait();
+    mass_fresh(page_table, seq_start, seq_pos0);
     const int g = blockIdx.y, tid = threadIdx.x;
     int b, kt, place0;
     if (!mass_find_keys(seq_start, seq_pos0, n_seqs, blockIdx.x, tile, b, kt, place0)) return;
@@ -516,6 +523,7 @@ few_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict
     constexpr int UNIT = 16 / sizeof(T);
     pdl_trigger();
     pdl_wait();
+    mass_fresh(page_table, seq_start, seq_pos0);
     q = pdl_fresh(q);
     kc = pdl_fresh(kc);
     vc = pdl_fresh(vc);
@@ -726,6 +734,7 @@ few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
     __shared__ float lse[MASS_FEW_PAIRS];
     pdl_trigger();
     pdl_wait();
+    mass_fresh(page_table, seq_start, seq_pos0);
     part_o = pdl_fresh(part_o);
     part_ml = pdl_fresh(part_ml);
     scores = pdl_fresh(scores);
@@ -740,19 +749,31 @@ few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
             float M, L;
             join_stats(part_ml, base, S, lane, M, L);
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-            for (int d0 = 0; d0 < hd; d0 += 128) {             // four columns a lane, all shares' loads in flight
+            for (int d0 = 0; d0 < hd; d0 += 128) {             // four columns a lane, the loads of four shares in flight
                 float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-                for (int z = 0; z < S; z++) {
-                    const float mz = __ldcg(part_ml + (base + z) * 2);
-                    const float w = mz != -INFINITY ? exp2f(mz - M) : 0.0f;
+auto shares = [&](int z0, auto count) {
+                    constexpr int N = decltype(count)::value;
+                    float mz[N], x[N][4];
 #pragma unroll
-                    for (int u = 0; u < 4; u++) {
-                        const int d = d0 + u * 32 + lane;
-                        const float x = d < hd ? __ldcg(part_o + (base + z) * hd + d) : 0.0f;
-                        if (w != 0.0f) acc[u] = fmaf(x, w, acc[u]);          // a share without keys has written no output
+                    for (int k = 0; k < N; k++) {
+                        mz[k] = __ldcg(part_ml + (base + z0 + k) * 2);
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            const int d = d0 + u * 32 + lane;
+                            x[k][u] = d < hd ? __ldcg(part_o + (base + z0 + k) * hd + d) : 0.0f;
+                        }
                     }
-                }
+#pragma unroll
+                    for (int k = 0; k < N; k++) {
+                        const float w = mz[k] != -INFINITY ? exp2f(mz[k] - M) : 0.0f;
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+                            if (w != 0.0f) acc[u] = fmaf(x[k][u], w, acc[u]);          // a share without keys has written no output
+                    }
+                };
+                int z = 0;
+                for (; z + 4 <= S; z += 4) shares(z, std::integral_constant<int, 4>());
+                for (; z < S; z++) shares(z, std::integral_constant<int, 1>());
 #pragma unroll
                 for (int u = 0; u < 4; u++) {
                     const int d = d0 + u * 32 + lane;
@@ -771,8 +792,9 @@ few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
         if (lane == 0) lse[i] = L > 0.0f ? M + log2f(L) : INFINITY;
     }
     __syncthreads();
-    const int key = key0 + tid * 4;                            // this thread's four keys, on one page
+    const int key = key0 + tid * 4, pi = key / HB_PAGE_TOKENS; // this thread's four keys, on one page
     if (key >= n) return;
+    const int page = pi < pt_width ? page_table[(size_t)b * pt_width + pi] : -1;
     float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int i = 0; i < n_new; i++) {
         const int p = pos0 + i, lo = hb_oldest_visible(p, window, 0);
@@ -788,8 +810,6 @@ few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
             s[3] += key + 3 >= lo && key + 3 <= p ? exp2f(x.w - e) : 0.0f;
         }
     }
-    const int pi = key / HB_PAGE_TOKENS;
-    const int page = pi < pt_width ? page_table[(size_t)b * pt_width + pi] : -1;
     if (vec && key + 3 < pos0 && page >= 0 && page < n_pages) {
         const size_t at = ((size_t)page * nkv + g) * HB_PAGE_TOKENS + (key & (HB_PAGE_TOKENS - 1));
         const float4 old = mo.before != nullptr ? __ldcg(reinterpret_cast<const float4*>(mo.before + at)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);

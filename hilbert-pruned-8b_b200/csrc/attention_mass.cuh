@@ -17,6 +17,13 @@ struct MassOut {
 // distance, in floats, of the scores of two heads
 static __host__ __device__ inline long long mass_score_ld(int max_len) { return ((long long)max_len + 63) / 64 * 64; }
 
+// A step's metadata may come from the kernel in front (lengths that a program works out on the device): read behind pdl_wait() only
+__device__ __forceinline__ void mass_fresh(const int* __restrict__& page_table, const int* __restrict__& seq_start, const int* __restrict__& seq_pos0) {
+    page_table = pdl_fresh(page_table);
+    seq_start = pdl_fresh(seq_start);
+    seq_pos0 = pdl_fresh(seq_pos0);
+}
+
 // A step's sequences are looked through 32 at a time, a lane each: which of them element number `at` of `count(b)` elements each belongs
 // to, its number there, and the sum of `other(b)` over the sequences in front.  Called by whole warps; the same answer in every lane.
 template <typename F, typename H>
@@ -147,6 +154,9 @@ __device__ __forceinline__ int key_tiles_of(int first, int last, int window, int
     tile0 = hb_oldest_visible(first, window, 0) / keys;
     return last / keys + 1 - tile0;
 }
+
+// A number that every lane of a warp has loaded alike, as one for the warp (the compiler then keeps it in a uniform register)
+__device__ __forceinline__ int mass_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // whether blocks of `span` tokens of a sequence of `rows` rows may see more tiles than go into one share (by the host's bound)
 __device__ __forceinline__ bool shares_may_cut(const Shares& sh, int rows, int span, int window, int keys) {

@@ -53,16 +53,6 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     // heaviest ones start first and what ends last is light.
     const int z = blockIdx.x % S, g = blockIdx.x / S % nkv, G = nh / nkv, tile = blockIdx.x / (S * nkv);
 
-    int b, kt, place0;
-    const bool has_work = mass_find_keys(seq_start, seq_pos0, n_seqs, tile, MT_KEYS, b, kt, place0);
-    const int t_begin = has_work ? seq_start[b] : 0, n_new = has_work ? seq_start[b + 1] - t_begin : 0, pos0 = has_work ? seq_pos0[b] : 0;
-    const int key0 = kt * MT_KEYS;
-    int n0 = 0, n1 = 0;
-    if (has_work) mass_queries(key0, MT_KEYS, pos0, n_new, window, n0, n1);
-    n0 &= ~127;                                                // whole blocks of 128 new tokens, as the log-sums lie
-    const int blocks = (n1 - n0 + 127) / 128;
-    const int it0 = (int)((long long)blocks * G * z / S), n_it = (int)((long long)blocks * G * (z + 1) / S) - it0;
-
     if (threadIdx.x == 0) {
         mbar_init(k_full, 1);
         for (int s = 0; s < MT_STAGES; s++) {
@@ -83,15 +73,34 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint32_t tmem_base = *tmem_slot;                    // buffer s of key tile k at columns (2 s + k) * 128
     pdl_trigger();
     pdl_wait();
+    mass_fresh(page_table, seq_start, seq_pos0);
+
+    int b, kt, place0;
+    const bool has_work = mass_find_keys(seq_start, seq_pos0, n_seqs, tile, MT_KEYS, b, kt, place0);
+    const int t_begin = mass_uniform(has_work ? seq_start[b] : 0), n_new = mass_uniform(has_work ? seq_start[b + 1] - t_begin : 0),
+              pos0 = mass_uniform(has_work ? seq_pos0[b] : 0);
+    const int key0 = kt * MT_KEYS;
+    int n0 = 0, n1 = 0;
+    if (has_work) mass_queries(key0, MT_KEYS, pos0, n_new, window, n0, n1);
+    n0 &= ~127;                                                // whole blocks of 128 new tokens, as the log-sums lie
+    const int blocks = (n1 - n0 + 127) / 128;
+    const int it0 = (int)((long long)blocks * G * z / S), n_it = (int)((long long)blocks * G * (z + 1) / S) - it0;
 
     if (warp == 0) {
         // ---------------------------------------------------------------- TMA producer
         if (lane == 0 && n_it > 0) {
             const int* pt = page_table + (size_t)b * pt_width;
             mbar_expect_tx(k_full, 2 * TILE);
+            int pages[MT_KEYS / HB_PAGE_TOKENS];                    // asked for at once
+#pragma unroll
             for (int pg = 0; pg < MT_KEYS / HB_PAGE_TOKENS; pg++) {
                 const int pi = kt * (MT_KEYS / HB_PAGE_TOKENS) + pg;
-                int page = pi < pt_width ? pt[pi] : -1;
+                pages[pg] = pi < pt_width ? pt[pi] : -1;
+            }
+#pragma unroll
+            for (int pg = 0; pg < MT_KEYS / HB_PAGE_TOKENS; pg++) {
+                const int pi = kt * (MT_KEYS / HB_PAGE_TOKENS) + pg;
+                int page = pages[pg];
                 if (page < 0 || page >= n_pages) {
                     // a page that no token of the step sees (behind the end, or given back) may be missing
                     int a, e;

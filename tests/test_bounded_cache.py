@@ -462,6 +462,36 @@ def test_captured_and_replayed(ops, new):
         c.check(out, mass, c.before, torch.zeros_like(mass))
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd,past,new", [(torch.bfloat16, 128, [300, 64], [90, 40]), (torch.bfloat16, 64, [3000, 10], [300, 20]),
+                                               (torch.float32, 64, [300, 64], [90, 40]), (torch.bfloat16, 64, [300, 64], [1, 3]),
+                                               (torch.float32, 80, [300, 64], [1, 1]), (torch.bfloat16, 64, [1500, 900], [1, 1])])
+def test_metadata_from_the_kernel_in_front(ops, dtype, hd, past, new):
+    """A step whose table, starts and places the kernel right in front of the call writes (they held other values before)."""
+    c = Case(dtype, 8, 2, hd, past, new, None, seed=13)
+    mass = torch.zeros(c.pages, 2, PAGE, device=DEV)
+    want, sums = c.run(ops, mass), mass.clone()
+    right = [x.clone() for x in (c.step.page_tables[0], c.step.seq_start, c.step.seq_pos0)]
+    held = [c.step.page_tables[0], c.step.seq_start, c.step.seq_pos0]
+    work = torch.randn(2048, 2048, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    out = torch.empty_like(want)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        for x, y in zip(held, right):
+            torch.add(y, 0, out=x)
+        c.run(ops, mass, out=out)
+        held[0].fill_(-1)
+        held[1].fill_(0)
+        held[2].fill_(0)
+    for _ in range(10):
+        out.zero_(), mass.zero_()
+        torch.mm(work, work)
+        graph.replay()
+        assert torch.equal(out, want) and torch.equal(mass, sums)
+    ops.check_errors()
+
+
 # ------------------------------------------------------------------------------------------------------- the choice
 def _chosen(values, n, first, recent, budget):
     """values: the rows' masses (a list)."""
