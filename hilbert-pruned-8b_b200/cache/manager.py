@@ -57,6 +57,8 @@ class Sequence:
     pages: List[List[Optional[int]]] = field(default_factory=list)
     open: bool = True
     pages_version: int = 0      # counts the changes of `pages`: who keeps a copy compares this
+    evicted: int = 0            # rows that were evicted: the token in row i of the newest ones stands at position i + evicted
+    kept: int = 0               # rows that the last eviction left: they are not the first `kept` tokens any more
 
 
 @dataclass
@@ -66,6 +68,7 @@ class Snapshot:
     seq_id: int
     length: int
     state: Dict[int, torch.Tensor]
+    evicted: int = 0
 
 
 class CacheGroup:
@@ -242,11 +245,31 @@ class CacheManager:
                              "(take a snapshot and restore it)")
         self._forget_after(seq, length)
 
-    def _forget_after(self, seq: Sequence, length: int) -> None:
+    def evict(self, seq: Sequence, rows: int) -> None:
+        """Notes that all but ``rows`` rows of a sequence were evicted: in every entry and kv head the rows that stay have been
+        moved to the front (``Ops.evict_rows`` in place, for every group), the pages behind them are given back.  The tokens
+        that come next are appended behind the kept rows and keep their positions (``Sequence.evicted`` rows further on), by
+        which queries and keys are rotated.  Rows of a group with a window or a stride stand for positions: refused."""
+        if not seq.open:
+            raise ValueError(f"cache: sequence {seq.seq_id} is closed")
+        if not 0 < rows <= seq.length:
+            raise ValueError(f"cache: {rows} rows of a sequence of {seq.length} cannot stay")
+        if any(g.need.window is not None or g.stride > 1 for g in self.groups):
+            raise ValueError("cache: rows of a group with a window or a stride cannot be evicted")
+        if rows == seq.length:
+            return
+        gone = seq.length - rows
+        self._forget_after(seq, rows, evicting=True)
+        seq.evicted += gone
+        seq.kept = rows
+
+    def _forget_after(self, seq: Sequence, length: int, evicting: bool = False) -> None:
         if not seq.open:
             raise ValueError(f"cache: sequence {seq.seq_id} is closed")
         if length > seq.length or length < 0:
             raise ValueError("cache: truncate needs 0 <= length <= current length")
+        if not evicting and 0 < length < seq.kept:
+            raise ValueError(f"cache: rows were evicted down to {seq.kept}, a sequence cannot be rewound to {length} of them")
         for gi, g in enumerate(self.groups):
             w = g.need.window
             keep = g.pages_for(length)
@@ -260,6 +283,8 @@ class CacheManager:
             del seq.pages[gi][keep:]
         seq.pages_version += 1
         seq.length = length
+        if length == 0:
+            seq.evicted = seq.kept = 0
 
     def snapshot(self, seq: Sequence) -> "Snapshot":
         """Remembers where a sequence stands: its length and a copy of its fixed-size state (the
@@ -267,13 +292,15 @@ class CacheManager:
         cpu_backend.c:265-277).  Keys and values are not copied: a restore forgets the later ones."""
         if not seq.open:
             raise ValueError(f"cache: sequence {seq.seq_id} is closed")
-        return Snapshot(seq.seq_id, seq.length, {e: t[seq.state_slot].clone() for e, t in self.state.items()})
+        return Snapshot(seq.seq_id, seq.length, {e: t[seq.state_slot].clone() for e, t in self.state.items()}, seq.evicted)
 
     def restore(self, seq: Sequence, snap: "Snapshot") -> None:
         """Takes a sequence back to a snapshot of itself: later keys and values are forgotten,
         the fixed-size state is the snapshot's again."""
         if snap.seq_id != seq.seq_id:
             raise ValueError(f"cache: the snapshot is of sequence {snap.seq_id}, not of {seq.seq_id}")
+        if snap.length > 0 and snap.evicted != seq.evicted:
+            raise ValueError("cache: rows were evicted since the snapshot")
         self._forget_after(seq, snap.length)
         for e, t in self.state.items():
             t[seq.state_slot].copy_(snap.state[e])

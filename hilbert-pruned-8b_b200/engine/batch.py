@@ -1,7 +1,9 @@
 """One step's batch: which tokens run, where they sit in their sequences, what is wanted.
 
 Tokens of all sequences are packed one after another without padding.  Per token the
-device holds its sequence's row in the batch and its absolute position; per sequence the
+device holds its sequence's row in the batch, its place (the row of the cache that it takes,
+``positions``) and its absolute position (``rope_positions``: the same, plus the rows that were
+evicted from the sequence: ``CacheManager.evict``); per sequence the
 offsets of its tokens, its length before and after the step, its state slot and, per cache
 group, the physical pages of its logical pages.  All of it travels in one host-to-device
 copy of one int32 array.
@@ -48,6 +50,7 @@ class StepBatch:
     host_len: List[int]
     host_state_slots: List[int] = field(default_factory=list)
     shared: Dict[str, Any] = field(default_factory=dict)
+    rope_positions: Optional[torch.Tensor] = None
     tag: str = ""               # suffix of buffers whose size follows the batch (captured steps keep their own)
 
 
@@ -75,7 +78,7 @@ def build_step(entries: List[StepEntry], cache: CacheManager, workspace, device,
     # layout of the packed int32 array (every segment starts on a 16-byte boundary)
     off: Dict[str, int] = {}
     cur = 0
-    for name, n in (("tokens", T), ("positions", T), ("tok_seq", T), ("seq_start", B + 1), ("seq_pos0", B),
+    for name, n in (("tokens", T), ("positions", T), ("rope_positions", T), ("tok_seq", T), ("seq_start", B + 1), ("seq_pos0", B),
                     ("seq_len", B), ("state_slots", B), ("want", max(n_want, 1))):
         off[name] = cur
         cur = _round4(cur + n)
@@ -94,6 +97,7 @@ def build_step(entries: List[StepEntry], cache: CacheManager, workspace, device,
         n = new[b]
         a[off["tokens"] + t0: off["tokens"] + t0 + n] = np.asarray(e.tokens, dtype=np.int64)
         a[off["positions"] + t0: off["positions"] + t0 + n] = np.arange(pos0[b], pos0[b] + n)
+        a[off["rope_positions"] + t0: off["rope_positions"] + t0 + n] = np.arange(pos0[b], pos0[b] + n) + e.seq.evicted
         a[off["tok_seq"] + t0: off["tok_seq"] + t0 + n] = b
         for w in e.want:
             if not 0 <= w < n:
@@ -123,7 +127,7 @@ def build_step(entries: List[StepEntry], cache: CacheManager, workspace, device,
 
     return StepBatch(
         num_tokens=T, num_seqs=B, num_wanted=n_want,
-        tokens=seg("tokens", T), positions=seg("positions", T), tok_seq=seg("tok_seq", T),
+        tokens=seg("tokens", T), positions=seg("positions", T), rope_positions=seg("rope_positions", T), tok_seq=seg("tok_seq", T),
         seq_start=seg("seq_start", B + 1), seq_pos0=seg("seq_pos0", B), seq_len=seg("seq_len", B),
         state_slots=seg("state_slots", B), want_rows=seg("want", n_want) if n_want else None,
         page_tables=[seg(f"pt{gi}", B * w).view(B, w) for gi, w in enumerate(widths)],
@@ -147,7 +151,7 @@ class DecodeMeta:
         self.n_groups = len(cache.groups)
         off: Dict[str, int] = {}
         cur = 0
-        for name, n in (("tokens", B), ("positions", B), ("tok_seq", B), ("seq_start", B + 1), ("seq_pos0", B),
+        for name, n in (("tokens", B), ("positions", B), ("rope_positions", B), ("tok_seq", B), ("seq_start", B + 1), ("seq_pos0", B),
                         ("seq_len", B), ("state_slots", B), ("want", B)):
             off[name] = cur
             cur = _round4(cur + n)
@@ -170,7 +174,7 @@ class DecodeMeta:
 
         self.batch = StepBatch(
             num_tokens=B, num_seqs=B, num_wanted=B, tokens=seg("tokens", B), positions=seg("positions", B),
-            tok_seq=seg("tok_seq", B), seq_start=seg("seq_start", B + 1), seq_pos0=seg("seq_pos0", B),
+            rope_positions=seg("rope_positions", B), tok_seq=seg("tok_seq", B), seq_start=seg("seq_start", B + 1), seq_pos0=seg("seq_pos0", B),
             seq_len=seg("seq_len", B), state_slots=seg("state_slots", B), want_rows=seg("want", B),
             page_tables=[seg(f"pt{gi}", B * width).view(B, width) for gi in range(self.n_groups)],
             max_new=1, max_len=width * PAGE_TOKENS, is_decode=True, host_new=[1] * B, host_len=[0] * B)
@@ -210,6 +214,7 @@ class DecodeMeta:
         pos0 = [s.length for s in seqs]
         a[off["tokens"]: off["tokens"] + B] = [e.tokens[0] for e in entries]
         a[off["positions"]: off["positions"] + B] = pos0
+        a[off["rope_positions"]: off["rope_positions"] + B] = [p + s.evicted for p, s in zip(pos0, seqs)]
         a[off["seq_pos0"]: off["seq_pos0"] + B] = pos0
         lens = [p + 1 for p in pos0]
         a[off["seq_len"]: off["seq_len"] + B] = lens

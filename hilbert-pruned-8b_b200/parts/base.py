@@ -233,7 +233,8 @@ class PositionEncoding(Part):
       changes ``q [tokens, heads, head_dim]`` and ``k [tokens, kv_heads, head_dim]`` (views of
       the step's projections) in place before the keys are cached; no kernel rotates.
 
-    ``prepare(step)`` may compute what all layers of a step share into ``step.shared``."""
+    ``prepare(step)`` may compute what all layers of a step share into ``step.shared``.  A token's position is
+    ``step.rope_positions[t]``; ``step.positions[t]`` is its place in the cache, which lies behind it once rows were evicted."""
 
     fusable = True
 

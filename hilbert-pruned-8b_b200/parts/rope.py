@@ -113,7 +113,8 @@ class RotaryEmbedding(PositionEncoding):
         half = self.rotary_dim // 2
         table = self.ctx.workspace.buffer(self._key, (self.ctx.max_step_tokens, half, 2), torch.float32)
         table = table[: step.num_tokens]
-        self.ctx.ops.rope_table(step.positions, self.inv_freq, table, self.amplitude)
+        positions = getattr(step, "rope_positions", None)          # None: of a step whose places are its positions
+        self.ctx.ops.rope_table(step.positions if positions is None else positions, self.inv_freq, table, self.amplitude)
         step.shared[self._key] = table
 
     def rotation_table(self, step):

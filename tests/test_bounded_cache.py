@@ -681,6 +681,186 @@ def test_a_conversation_with_a_bounded_cache(ops, dtype, hd):
     ops.check_errors()
 
 
+def _hidden_attention(hidden):
+    """Grouped attention of one whole sequence in 64 bits over what is not hidden: ``hidden`` [kv heads, tokens, tokens]."""
+    def attention(q, k, v, window=None):
+        T, nh, hd = q.shape
+        G = nh // k.shape[1]
+        out = torch.empty_like(q)
+        for h in range(nh):
+            s = (q[:, h] @ k[:, h // G].T / math.sqrt(hd)).masked_fill(hidden[h // G], -math.inf)
+            out[:, h] = torch.softmax(s, dim=-1) @ v[:, h // G]
+        return out
+    return attention
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("model", ["strong_a", "strong_b", "strong_c", "strong_d"])
+def test_the_engine_goes_on_behind_an_eviction(model_folders, monkeypatch, model, dtype):
+    """Prompts, two evictions in place with tokens between and behind them, in steps of several tokens and in captured ones: the logits
+    are those of a plain model whose later tokens see the rows that stayed, rotated by their true positions."""
+    require_gpu()
+    import plain_llama as pl
+    import trace_tools as tt
+    from hilbert_pruned_8b_b200.engine.batch import StepEntry
+    from hilbert_pruned_8b_b200.engine.step import Engine
+    eng = Engine.from_folder(model_folders[model], dtype, max_tokens=1024)
+    ops, cfg = eng.ctx.ops, pl.read_config(model_folders[model])
+    L, kv = cfg["num_hidden_layers"], cfg["num_key_value_heads"]
+    (group,) = eng.cache.groups
+    tokens = {b: tt.random_tokens(n, cfg["vocab_size"], 40 + b) for b, n in enumerate((260, 90))}
+    seqs = [eng.open_sequence() for _ in tokens]
+    done, got = [0, 0], {}
+    stood = {(b, e, g): [] for b in tokens for e in range(L) for g in range(kv)}          # positions of a list's rows
+    hidden = {b: torch.ones(len(t), len(t), dtype=torch.bool).triu(1).repeat(L, kv, 1, 1) for b, t in tokens.items()}
+
+    def feed(counts):
+        entries = [StepEntry(s, tokens[b][done[b]: done[b] + n], list(range(n))) for b, (s, n) in enumerate(zip(seqs, counts))]
+        logits = eng.step(entries).double().cpu()
+        rows = [(b, done[b] + i) for b, n in enumerate(counts) for i in range(n)]
+        got.update({key: row for key, row in zip(rows, logits)})
+        for b, n in enumerate(counts):
+            for e in range(L):
+                for g in range(kv):
+                    stood[b, e, g] += range(done[b], done[b] + n)
+            done[b] += n
+
+    def cut(budget, first, recent, seed):
+        width = max(len(s.pages[0]) for s in seqs)
+        table = torch.tensor([s.pages[0] + [-1] * (width - len(s.pages[0])) for s in seqs], dtype=torch.int32, device=DEV)
+        mass = torch.rand(group.k.shape[:-1], generator=torch.Generator(device=DEV).manual_seed(seed), device=DEV)
+        kept = torch.empty(L, len(seqs), kv, budget, dtype=torch.int32, device=DEV)
+        ops.evict_select(mass, table, _ints([s.length for s in seqs]), first, recent, kept)
+        ops.evict_rows(kept, group.k, group.v, mass, table)
+        for b, s in enumerate(seqs):
+            before = len(s.pages[0])
+            eng.cache.evict(s, min(s.length, budget))
+            assert len(s.pages[0]) == min(before, _pages(budget)) and s.length + s.evicted == done[b]
+            for e in range(L):
+                for g in range(kv):
+                    was = stood[b, e, g]
+                    stood[b, e, g] = [was[j] for j in kept[e, b, g].tolist() if j >= 0]
+                    gone = sorted(set(range(done[b])) - set(stood[b, e, g]))
+                    hidden[b][e, g, done[b]:, gone] = True
+
+    feed([200, 40])
+    cut(70, 2, 8, 1)                        # the second sequence is shorter than its budget
+    for _ in range(5):
+        feed([1, 1])
+    feed([9, 30])
+    cut(40, 0, 5, 2)
+    feed([3, 2])
+    for _ in range(6):
+        feed([1, 1])
+    assert eng.graph_replays > 0 and seqs[0].evicted == 130 + 44 and seqs[1].evicted == 35
+    ops.check_errors()
+    plain = pl.PlainLlama(model_folders[model], round_to=torch.bfloat16 if dtype == "bfloat16" else None)
+    for b, s in enumerate(seqs):
+        layer = [0]
+
+        def attention(q, k, v, window=None):
+            layer[0] += 1
+            return _hidden_attention(hidden[b][layer[0] - 1][:, :done[b], :done[b]])(q, k, v)
+        monkeypatch.setattr(pl, "attention", attention)
+        want = plain.logits(tokens[b][:done[b]])
+        tt.compare({k: v for k, v in got.items() if k[0] == b}, {(b, i): row for i, row in enumerate(want)}, dtype, "behind an eviction")
+
+
+# ------------------------------------------------------------------------------------------- the cache's bookkeeping
+def _manager(max_tokens=1024, window=None, stride=1, state=False):
+    from hilbert_pruned_8b_b200.cache import CacheManager
+    from hilbert_pruned_8b_b200.parts.base import CacheNeed, StateNeed
+    needs = {0: CacheNeed(2, 16), 1: CacheNeed(1, 32, window, stride=stride)}
+    return CacheManager(needs, {0: StateNeed((3,))} if state else {}, max_tokens, torch.device("cpu"), torch.float32)
+
+
+def test_an_evicted_sequence_keeps_its_positions():
+    from hilbert_pruned_8b_b200.engine.batch import DecodeMeta, StepEntry, build_step
+    from hilbert_pruned_8b_b200.engine.workspace import Workspace
+    cpu = torch.device("cpu")
+    m, ws = _manager(), Workspace(cpu)
+    a, b = m.open(), m.open()
+    for s, n in ((a, 300), (b, 70)):
+        m.reserve([(s, n)])
+        m.commit(s, n)
+    free = m.pages_free()
+    m.evict(a, 130)
+    assert (a.length, a.evicted, a.kept) == (130, 170, 130) and (b.length, b.evicted) == (70, 0)
+    assert m.pages_free() == [f + 2 for f in free] and [len(p) for p in a.pages] == [3, 3]
+    meta = DecodeMeta(2, 8, m, ws, cpu, "meta")
+    for n in (3, 1, 1):
+        entries = [StepEntry(a, [5] * n, [0]), StepEntry(b, [7], [0])]
+        m.reserve([(e.seq, e.seq.length + len(e.tokens)) for e in entries])
+        steps = [build_step(entries, m, ws, cpu)] + ([meta.fill(entries)] if n == 1 else [])
+        for st in steps:
+            assert st.positions.tolist() == [a.length + i for i in range(n)] + [b.length]
+            assert st.rope_positions.tolist() == [a.length + 170 + i for i in range(n)] + [b.length]
+            assert st.seq_pos0.tolist() == [a.length, b.length]
+        for e in entries:
+            m.commit(e.seq, e.seq.length + len(e.tokens))
+    m.evict(a, 64)
+    assert (a.length, a.evicted, a.kept) == (64, 241, 64)
+    m.evict(a, 64)                                           # nothing goes
+    assert (a.length, a.evicted, a.kept) == (64, 241, 64)
+    m.close(a), m.close(b)
+    assert m.pages_free() == [16, 16]
+
+
+def test_rewinds_of_an_evicted_sequence():
+    m = _manager()
+    s = m.open()
+    for n in (100, 200):
+        m.reserve([(s, n)])
+        m.commit(s, n)
+        snap = m.snapshot(s) if n == 100 else snap
+    m.evict(s, 120)
+    with pytest.raises(ValueError, match="evicted since"):
+        m.restore(s, snap)
+    m.reserve([(s, 150)])
+    m.commit(s, 150)
+    later = m.snapshot(s)
+    m.reserve([(s, 160)])
+    m.commit(s, 160)
+    m.restore(s, later)                                      # tokens behind the kept rows may be taken back
+    assert (s.length, s.evicted) == (150, 80)
+    m.truncate(s, 120)
+    for n in (119, 1):
+        with pytest.raises(ValueError, match="rewound"):
+            m.truncate(s, n)
+    assert (s.length, s.evicted, s.kept) == (120, 80, 120)
+    m.truncate(s, 0)                                         # a new beginning
+    assert (s.length, s.evicted, s.kept) == (0, 0, 0)
+
+
+def test_evictions_that_are_refused():
+    m = _manager()
+    s = m.open()
+    m.reserve([(s, 100)])
+    m.commit(s, 100)
+    for rows in (0, -1, 101):
+        with pytest.raises(ValueError, match="cannot stay"):
+            m.evict(s, rows)
+    m.close(s)
+    with pytest.raises(ValueError, match="closed"):
+        m.evict(s, 50)
+    for kw in (dict(window=70), dict(stride=4)):
+        n = _manager(**kw)
+        s = n.open()
+        n.reserve([(s, 100)])
+        n.commit(s, 100)
+        with pytest.raises(ValueError, match="window or a stride"):
+            n.evict(s, 50)
+        assert s.length == 100
+    n = _manager(state=True)                                 # state of fixed size goes on
+    s = n.open()
+    n.reserve([(s, 100)])
+    n.commit(s, 100)
+    n.state_view(0)[s.state_slot] += 2.0
+    n.evict(s, 50)
+    assert (s.length, s.evicted) == (50, 50) and n.state_view(0)[s.state_slot].tolist() == [2.0] * 3
+
+
 # ------------------------------------------------------------------------------------------------------- refusals
 class _Fake:
     """An ``Ops`` without a device: the checks of arguments run, a call of the library would fail the test."""
