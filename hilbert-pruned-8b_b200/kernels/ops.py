@@ -1365,6 +1365,9 @@ class Ops:
         self._tables("attention", pt)
         if T == 0:
             return
+        self._on(pt, step.seq_start, step.seq_pos0)
+        if pt.shape[0] < step.num_seqs or step.seq_start.shape[0] <= step.num_seqs or step.seq_pos0.shape[0] < step.num_seqs:
+            raise KernelError(f"attention: the page table, starts and places are of fewer than the step's {step.num_seqs} sequences")
         if self._elsewhere():
             with torch.cuda.device(self._index):
                 return self.attention_mass(qkv, heads, kv_heads, head_dim, cache, step, out, scale, window, mass, before, splits)

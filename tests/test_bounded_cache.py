@@ -901,6 +901,31 @@ def test_attention_mass_refuses(change, text):
         _Fake().attention_mass(**_attention_args(**change))
 
 
+@pytest.mark.parametrize("short", ["table", "seq_start", "seq_pos0"])
+def test_attention_mass_refuses_a_step_of_fewer_rows_than_sequences(short):
+    """What the kernels would read behind the end of."""
+    from hilbert_pruned_8b_b200.kernels.ops import KernelError
+    a = _attention_args(table=_i32(2, 2))
+    st = a["step"]
+    st.num_seqs, st.host_new, st.host_len, st.seq_start, st.seq_pos0 = 2, [2, 1], [2, 1], _i32(3), _i32(2)
+    if short == "table":
+        st.page_tables = [_i32(1, 2)]
+    else:
+        setattr(st, short, getattr(st, short)[:-1])
+    with pytest.raises(KernelError, match="2 sequences"):
+        _Fake().attention_mass(**a)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["page_tables", "seq_start", "seq_pos0"])
+def test_attention_mass_refuses_metadata_of_another_device(ops, what):
+    from hilbert_pruned_8b_b200.kernels.ops import KernelError
+    c = Case(torch.bfloat16, 4, 2, 64, [100], [3], None)
+    setattr(c.step, what, [c.table.cpu()] if what == "page_tables" else getattr(c.step, what).cpu())
+    with pytest.raises(KernelError, match="tensor on cpu"):
+        c.run(ops, torch.zeros(c.pages, 2, PAGE, device=DEV))
+
+
 def test_attention_mass_of_no_tokens():
     _Fake().attention_mass(**_attention_args(qkv=torch.zeros(0, 384), out=torch.zeros(0, 256), tokens=0))
 
