@@ -1358,7 +1358,7 @@ class Ops:
         self._mass_like(mass, "mass", want[:3])
         if before is not None:
             self._mass_like(before, "before", want[:3])
-        scale, win = float(scale), int(window) if window else 0
+        scale, win = float(scale), min(int(window), 0x7fffffff) if window else 0           # (no sequence is longer)
         if not 0.0 < scale < float("inf") or win < 0:
             raise KernelError(f"attention: the scale must be positive and finite and the window none or positive, got {scale} and {window}")
         pt = step.page_tables[cache.group]

@@ -434,6 +434,22 @@ def test_rows_in_front_of_the_window_do_not_count(ops, dtype, hd, new, past, win
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.float32, 33)])
+@pytest.mark.parametrize("new", [[90, 40], [1, 3]])
+def test_windows_longer_than_any_sequence(ops, dtype, hd, new):
+    """A window that no 32-bit number holds is no window."""
+    c = Case(dtype, 4, 2, hd, [300, 64], new, None, seed=7)
+    start = torch.zeros(c.pages, 2, PAGE, device=DEV)
+    full = start.clone()
+    want = c.run(ops, full, before=c.before)
+    c.check(want, full, c.before, start)
+    for c.window in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 5, 2 ** 40):
+        mass = start.clone()
+        c.check(c.run(ops, mass, before=c.before), mass, c.before, start)
+    ops.check_errors()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("new", [[90, 40], [1, 3]])
 def test_captured_and_replayed(ops, new):
     """A captured call follows its inputs; two graphs that are replayed on two streams share nothing."""
