@@ -117,7 +117,7 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             for (int it = 0; it < n_it; it++) {
                 const int s = it % MT_STAGES;
                 if (!mbar_wait(q_empty0 + 8 * s, ((it / MT_STAGES) & 1) ^ 1)) {
-                    atomicExch(error_flag, 41);
+                    atomicExch(error_flag, 61);
                     break;
                 }
                 const int item = it0 + it, head = g * G + item / blocks, q0 = (item % blocks) * 128;
@@ -128,8 +128,8 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
                 issued = it + 1;
             }
             for (int it = max(0, issued - MT_STAGES); it < issued; it++)
-                if (!mbar_wait(q_full0 + 8 * (it % MT_STAGES), (it / MT_STAGES) & 1)) atomicExch(error_flag, 42);
-            if (!mbar_wait(k_full, 0)) atomicExch(error_flag, 42);
+                if (!mbar_wait(q_full0 + 8 * (it % MT_STAGES), (it / MT_STAGES) & 1)) atomicExch(error_flag, 62);
+            if (!mbar_wait(k_full, 0)) atomicExch(error_flag, 62);
         }
     } else if (warp == 1) {
         // ---------------------------------------------------------------- MMA issuer: the warp waits, one lane issues
@@ -137,13 +137,13 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
         const uint64_t k_desc = smem_desc_sw128(smem_base), q_desc = smem_desc_sw128(q_smem);     // a step along a tile adds its bytes / 16
         bool alive = n_it > 0;
         if (alive && !__all_sync(0xffffffffu, mbar_wait(k_full, 0))) {
-            atomicExch(error_flag, 43);
+            atomicExch(error_flag, 63);
             alive = false;
         }
         for (int it = 0; it < n_it && alive; it++) {
             const int s = it % MT_STAGES, sb = it & 1;
             if (!__all_sync(0xffffffffu, mbar_wait(q_full0 + 8 * s, (it / MT_STAGES) & 1) && mbar_wait(s_empty0 + 8 * sb, ((it >> 1) & 1) ^ 1))) {
-                atomicExch(error_flag, 44);
+                atomicExch(error_flag, 64);
                 break;
             }
             tc_fence_after();
@@ -176,7 +176,7 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
             const int sb = it & 1, s = it % MT_STAGES;
             // (the queries' barrier too: it says that the log-sums have arrived)
             if (!__all_sync(0xffffffffu, mbar_wait(s_full0 + 8 * sb, (it >> 1) & 1) && mbar_wait(q_full0 + 8 * s, (it / MT_STAGES) & 1))) {
-                atomicExch(error_flag, 45);
+                atomicExch(error_flag, 65);
                 ok = false;
                 break;
             }

@@ -976,6 +976,22 @@ def test_evict_rows_refuses(change, text):
         _Fake().evict_rows(**dict(a, **change))
 
 
+def test_codes_of_waits_that_ran_out_name_their_kernel():
+    """The status word holds a code and nothing else: no other kernel notes the codes of these two."""
+    import glob
+    import os
+    import re
+    import hilbert_pruned_8b_b200.kernels.build as build
+    codes = {}
+    for path in glob.glob(os.path.join(os.path.dirname(os.path.dirname(build.__file__)), "csrc", "*.cu*")):
+        with open(path) as f:
+            codes[os.path.basename(path)] = set(re.findall(r"atomicExch\(\w+, (\d+)\)", f.read()))
+    for mine in ("attention_chunk_tc.cu", "attention_mass_tc.cu"):
+        assert codes[mine] and codes["moe_tc.cu"]
+        for other, theirs in codes.items():
+            assert other == mine or not theirs & codes[mine], (mine, other)
+
+
 def test_groups_of_sequences():
     """Every sequence once and in order, with its tokens, within the limit unless a group has one sequence with new tokens."""
     from hilbert_pruned_8b_b200.kernels.plan import few_groups
