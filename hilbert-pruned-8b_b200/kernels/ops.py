@@ -1391,8 +1391,9 @@ class Ops:
                 self._call("hb_attention_mass_few", *a.buffer_info(), scale)
             self.launches += kernels
             return
+        # (tensor maps: rows of queries that lie apart, a cache of fewer than 2^31 rows; the kernel for every size takes any)
         tc = bool(fast and self.use_tcgen05_attention and (q_at | out_at) % 16 == 0 and q_ld % 8 == 0 and out_ld % 8 == 0
-                  and self.lib.hb_attention_mass_tc_supported(heads, kv_heads, head_dim))
+                  and q_ld >= heads * head_dim and pages * kv_heads * 64 < 1 << 31 and self.lib.hb_attention_mass_tc_supported(heads, kv_heads, head_dim))
         splits, q_blocks, key_tiles, shares, tiles, cut, lse_ld, n_lse, n_parts, n_cut = self._mass_plan(
             False, tc, dtype == torch.bfloat16, heads, kv_heads, head_dim, win, step, splits)
         scratch = torch.empty(n_lse + n_parts + n_cut, dtype=torch.float32, device=self.device)

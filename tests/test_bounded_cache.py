@@ -942,6 +942,50 @@ def test_attention_mass_refuses_metadata_of_another_device(ops, what):
         c.run(ops, torch.zeros(c.pages, 2, PAGE, device=DEV))
 
 
+@pytest.mark.parametrize("pages,q,called", [(5, None, "hb_attention_mass_tc"), (1 << 22, None, "hb_attention_mass"), ((1 << 22) - 1, None, "hb_attention_mass_tc"),
+                                            (5, torch.zeros(1, 256, dtype=torch.bfloat16).expand(20, 256), "hb_attention_mass")])
+def test_what_a_tensor_map_does_not_take(pages, q, called):
+    """Caches of 2^31 rows and more and one query row for all tokens go to the kernel for every size."""
+    o, calls, n = _Fake(), [], types.SimpleNamespace
+    o._call, o._elsewhere, o._stream, o.status = lambda name, *a: calls.append(name), lambda: False, lambda: 0, torch.zeros(4, dtype=torch.int32)
+    o.use_fast_attention = o.use_tcgen05_attention = True
+    o.MASS_FEW_PAIRS, o._mass_plans = 512, {}
+    o.lib = n(hb_attention_mass_tc_supported=lambda *a: 1, hb_attention_mass_tc_keys=lambda: 256)
+
+    class Held:
+        """Keys and values without memory."""
+        shape, dtype = (pages, 8, 64, 8), torch.bfloat16
+
+        def get_device(self):
+            return -1
+
+        def is_contiguous(self):
+            return True
+
+        def data_ptr(self):
+            return 1 << 20
+    q = q if q is not None else torch.zeros(20, 64 + 8, dtype=torch.bfloat16)
+    heads = 8 if q.shape[1] == 72 else 32
+
+    class Mass(Held):
+        shape, dtype = (pages, 8, 64), torch.float32
+    step = n(num_tokens=20, num_seqs=1, page_tables=[_i32(1, 2)], seq_start=_i32(2), seq_pos0=_i32(1), max_new=20, max_len=70, host_new=[20], host_len=[70])
+    o.attention_mass(q, heads, 8, 8, n(k=Held(), v=Held(), group=0), step, torch.zeros(20, heads * 8, dtype=torch.bfloat16), 0.3, None, Mass())
+    assert calls == [called]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 64)])
+@pytest.mark.parametrize("new", [[90, 40], [1, 3]])
+def test_one_query_row_for_all_tokens(ops, dtype, hd, new):
+    c = Case(dtype, 4, 2, hd, [300, 64], new, None, seed=17)
+    c.qkv = c.qkv[:1].expand(sum(new), -1)
+    start = torch.zeros(c.pages, 2, PAGE, device=DEV)
+    mass = start.clone()
+    c.check(c.run(ops, mass, before=c.before), mass, c.before, start)
+    ops.check_errors()
+
+
 def test_attention_mass_of_no_tokens():
     _Fake().attention_mass(**_attention_args(qkv=torch.zeros(0, 384), out=torch.zeros(0, 256), tokens=0))
 
