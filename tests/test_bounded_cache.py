@@ -615,6 +615,38 @@ def test_evict_rows(ops, dtype, E, kv, hd, v_hd, lengths, budget, first, recent,
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("apart", [False, True])
+@pytest.mark.parametrize("dtype,hd,v_hd,offset", [(torch.bfloat16, 72, 72, 0), (torch.bfloat16, 120, 120, 0), (torch.bfloat16, 24, 56, 0), (torch.float32, 36, 4, 0),
+                                                  (torch.bfloat16, 128, 128, 8), (torch.float32, 64, 64, 4), (torch.bfloat16, 80, 80, 2),
+                                                  (torch.bfloat16, 64, 64, 1)])
+def test_evict_rows_in_units_of_fewer_bytes(ops, dtype, hd, v_hd, offset, apart):
+    """Rows whose bytes are a multiple of 16 and not of 32, and storage that begins 16, 4 and 2 bytes behind a multiple of 32."""
+    E, kv, lengths, budget = 2, 3, [3000, 700, 65], 600
+    g = torch.Generator(device=DEV).manual_seed(2)
+    B, spare = len(lengths), _pages(budget)
+    table, pages, rest = _tables(lengths, 6, extra=B * spare + 2)
+
+    def storage(size):
+        n = E * pages * kv * PAGE * size
+        return torch.randn(n + offset, generator=g, device=DEV).to(dtype)[offset:].view(E, pages, kv, PAGE, size)
+    k, v = storage(hd), storage(v_hd)
+    mass = torch.rand(E, pages, kv, PAGE, generator=g, device=DEV)
+    kept = torch.empty(E, B, kv, budget, dtype=torch.int32, device=DEV)
+    ops.evict_select(mass, table, _ints(lengths), 4, 32, kept)
+    to = torch.tensor([rest[b * spare: (b + 1) * spare] for b in range(B)], dtype=torch.int32, device=DEV) if apart else None
+    want = [x.clone() for x in (k, v, mass)]
+    e, b, h, j = torch.nonzero(kept >= 0, as_tuple=True)
+    src = kept[e, b, h, j].long()
+    dest = (to if apart else table)[b, j // PAGE].long()
+    for x, y in zip((k, v, mass), want):
+        y[e, dest, h, j % PAGE] = x[e, table[b, src // PAGE].long(), h, src % PAGE]
+    ops.evict_rows(kept, k, v, mass, table, to_table=to)
+    for x, y in zip((k, v, mass), want):
+        assert torch.equal(x, y)
+    ops.check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("apart", [False, True])
 def test_evict_rows_of_very_many_lists(ops, apart):
     """More lists of rows (entries x sequences x kv heads) than a grid's second axis holds."""
     E, B, kv, hd = 32, 1100, 2, 4                         # 70400 lists
