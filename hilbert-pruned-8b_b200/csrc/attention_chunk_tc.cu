@@ -6,9 +6,9 @@
 // neighbouring blocks of one head's tokens.  A tile's rows are the 128 lanes of tensor memory.  What bounds it, per 128 x 128 scores at
 // head size 128: 1024 clocks of the two products, 1024 clocks of exponentials (16 a clock and SM), and 64 KB of keys and values, which at the
 // 32 bytes a clock that an SM takes from L2 would last 2048 clocks for one tile: hence two tiles, which halve that, and which take turns:
-// while one tile's weights are made, the tensor cores work on the other.  Measured: 893 us for 2048 tokens behind 30001 rows, 32 heads over 8
-// (1.17 PFLOP/s; with one tile to a CTA 1348 us), of which the products alone take 830; a tile's chain of products, softmax and
-// hand-overs bounds it.
+// while one tile's weights are made, the tensor cores work on the other.  Measured: 901 us for 2048 tokens behind 30001 rows, 32 heads over 8
+// (1.16 PFLOP/s; with one tile to a CTA 1348 us); the products alone, with the same loads and hand-overs, took 832 of then 892: a tile's chain
+// of products, softmax and hand-overs bounds it.
 //   warps 0-3, 4-7  softmax of tile 0 and 1, a thread per row: 128 scores from tensor memory into registers, running maximum and sum in
 //                   float32, weights as bfloat16, handed over in two halves.  No exchange between threads (two threads per row, which agree
 //                   on the maximum through shared memory: 2.09 instead of 1.77 us for the two tiles at head size 128, 1.73 instead of 1.62 at
@@ -75,7 +75,8 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
     mass_fresh(page_table, seq_start, seq_pos0);
 
     // The two tiles: heads head0 and head0 + 1 (head_pairs) of one block of tokens, or blocks 2 blk and 2 blk + 1 of head0.  Blocks
-    // are taken from the back and heads are the fast index: what sees the most keys starts first.
+    // are taken from the back and heads are the fast index: a sequence's blocks that see the most keys start first.  Sequences start in
+    // the opposite of the step's order, whatever they see (seven ragged sequences: 118 us with the longest last, 140 the other way round).
     const int z = blockIdx.z;
     const int head0 = head_pairs ? 2 * blockIdx.x : blockIdx.x, g = head0 / (nh / nkv);
     const int span = head_pairs ? FA_ROWS : 2 * FA_ROWS;
@@ -393,10 +394,9 @@ chunk_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant
 
 template <int HD>
 static int launch_chunk(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const int* page_table, int pt_width,
-                        const int* seq_start,
-                        const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, Shares sh, int max_shares, int n_tokens,
-                        int n_seqs, int q_blocks,
-                        int nh, int nkv, int hd, int head_pairs, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
+                        const int* seq_start, const int* seq_pos0, bf16* out, long long out_stride, float* lse, long long lse_ld, Shares sh,
+                        int max_shares, int n_tokens, int n_seqs, int q_blocks, int nh, int nkv, int hd, int head_pairs, float scale, int window,
+                        int n_pages, int* error_flag, cudaStream_t s) {
     constexpr int SMEM = (2 + 2 * CT_STAGES) * (HD / 64) * FA_HALF_BYTES + 22 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "attention tiles do not fit shared memory");
     static bool done[HB_MAX_DEVICES] = {};
@@ -421,8 +421,7 @@ extern "C" int hb_attention_mass_tc_supported(int n_heads, int n_kv_heads, int h
 int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
                        const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts,
                        int max_shares, int share_tiles, int join_tokens, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads,
-                       int head_dim, float scale,
-                       int window, int n_pages, int* error_flag, cudaStream_t s) {
+                       int head_dim, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
     HB_REQUIRE(hb_attention_mass_tc_supported(n_heads, n_kv_heads, head_dim),
                "attention_mass: %d heads over %d of size %d are not built for the tensor cores (sizes up to 128 in steps of 8)", n_heads, n_kv_heads, head_dim);
     HB_REQUIRE(q_blocks > 0 && q_blocks <= 65535 && error_flag != nullptr && max_shares >= 1 && max_shares <= 32 && share_tiles >= 1 &&
@@ -447,8 +446,7 @@ int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, c
                                                        error_flag, s)
                                    : launch_chunk<64>(mq, mk, mv, page_table, pt_width, seq_start, seq_pos0, (bf16*)out, out_stride, lse, lse_ld, sh,
                                                       max_shares, n_tokens, n_seqs, q_blocks, n_heads, n_kv_heads, head_dim, head_pairs, scale,
-                                                      window, n_pages,
-                                                      error_flag, s);
+                                                      window, n_pages, error_flag, s);
     if (rc || max_shares == 1) return rc;
     return shares_join(sh, join_tokens, HB_BF16, out, out_stride, lse, lse_ld, 1, seq_start, seq_pos0, head_pairs ? FA_ROWS : 2 * FA_ROWS, FA_KEYS,
                        window, n_tokens,

@@ -5,11 +5,9 @@
 // A CTA = a share of the pages x one kv head x a block of a sequence's new tokens: the rows of the mma.sync tiles (16 RT of them) are the
 // (token, head) pairs of the block, so a page is read once for all of them.  Bound by memory: 2 head sizes of keys and values per row of
 // the cache against 4 bytes of score per pair.  The pages stream through three cp.async stages; a warp takes a quarter of every page's
-// keys for one tile of 16 rows, with its own running maximum and sum, joined through shared memory at the end.  (Two tiles of rows in one
-// warp leave two warps to a quarter of the SM: 38 us for 17 drafted tokens of four sequences,
-// latencies unhidden, against 34.)
-// (With a CTA per token, as for single tokens, 17 drafted tokens of four sequences took 82 us in all instead of 46; their pages came
-// from L2 17 times.)
+// keys for one tile of 16 rows, with its own running maximum and sum, joined through shared memory at the end: 28 us for 17 drafted
+// tokens of four sequences.  (Two tiles of rows in one warp leave two warps to a quarter of the SM, latencies unhidden: a tenth slower.  With
+// a CTA per token, as for single tokens, those tokens took 82 us in all instead of 46; their pages came from L2 17 times.)
 #include "api.h"
 #include "attention_mass.cuh"
 #include "mma.cuh"
@@ -226,10 +224,10 @@ few_tc_kernel(const bf16* __restrict__ q, long long q_stride, const bf16* __rest
 }
 
 template <int HD, int RT, bool FULL>
-static int launch_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                         const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int token_blocks,
-                         int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages,
-                         int seq0, int* status, cudaStream_t s) {
+static int launch_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width,
+                         const int* seq_start, const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits,
+                         int token_blocks, int tokens_per_block, int share_pages, int n_seqs, int nh, int nkv, int hd, float scale, int window,
+                         int n_pages, int seq0, int* status, cudaStream_t s) {
     constexpr int PIPE = FT_STAGES * 2 * HB_PAGE_TOKENS * HD * 2, MERGE = (4 * 16 * RT * HD + 2 * 4 * 16 * RT) * 4,
     SMEM = PIPE > MERGE ? PIPE : MERGE;
     static bool done[HB_MAX_DEVICES] = {};
@@ -252,10 +250,10 @@ extern "C" int hb_attention_few_tc_tokens(int n_heads, int n_kv_heads, int head_
     return rows / G;
 }
 
-int attention_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages,
-                     int token_blocks, int max_new,
-                     int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int seq0, int* status, cudaStream_t s) {
+int attention_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width,
+                     const int* seq_start, const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits,
+                     int share_pages, int token_blocks, int max_new, int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages,
+                     int seq0, int* status, cudaStream_t s) {
     const int tokens = hb_attention_few_tc_tokens(nh, nkv, head_dim, max_new);
     HB_REQUIRE(tokens > 0, "attention_mass: head size %d with %d heads over %d kv heads is not built for the tensor cores (up to 128 in steps of 8, groups up to"
                " 32)",

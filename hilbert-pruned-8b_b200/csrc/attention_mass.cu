@@ -95,8 +95,7 @@ __global__ void __launch_bounds__(AM_THREADS)
 attention_rows_kernel(const T* __restrict__ q, long long q_stride, const T* __restrict__ kc, const T* __restrict__ vc,
                       const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
                       T* __restrict__ out, long long out_stride, float* __restrict__ lse, Shares sh, int n_tokens, int n_seqs, int nh, int nkv,
-                      int hd,
-                      float scale_log2e, int window, int n_pages, int vec_q, int vec_kv, int* status) {
+                      int hd, float scale_log2e, int window, int n_pages, int vec_q, int vec_kv, int* status) {
     extern __shared__ __align__(16) float am_smem[];
     pdl_trigger();
     pdl_wait();
@@ -235,8 +234,7 @@ template <typename T>
 __global__ void __launch_bounds__(256)
 shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* __restrict__ lse, long long lse_ld, int rounded,
                    const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs,
-                   int nh,
-                   int hd) {
+                   int nh, int hd) {
     __shared__ float ws[8][32];
     pdl_trigger();
     pdl_wait();
@@ -281,8 +279,7 @@ shares_join_kernel(Shares sh, T* __restrict__ out, long long out_stride, float* 
 }
 
 int shares_join(Shares sh, int join_tokens, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded,
-                const int* seq_start,
-                const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s) {
+                const int* seq_start, const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s) {
     if (join_tokens == 0) return 0;
     const dim3 grid(join_tokens, (nh + 7) / 8);
     cudaError_t e = dtype == HB_BF16 ? hb_launch(shares_join_kernel<bf16>, grid, dim3(256), 0, s, sh, (bf16*)out, out_stride, lse, lse_ld, rounded,
@@ -412,9 +409,8 @@ static int am_reserve(F* kernel, int bytes, bool (&done)[HB_MAX_DEVICES]) {
 template <typename T, int NC>
 static int launch_rows(const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
                        const int* seq_pos0, void* out, long long out_stride, float* lse, Shares sh, int max_shares, int join_tokens, MassOut mo,
-                       int splits, int n_tokens,
-                       int n_seqs, int q_blocks, int key_tiles, int nh, int nkv, int hd, float scale, int window, int n_pages, int* status,
-                       cudaStream_t s) {
+                       int splits, int n_tokens, int n_seqs, int q_blocks, int key_tiles, int nh, int nkv, int hd, float scale, int window,
+                       int n_pages, int* status, cudaStream_t s) {
     static_assert(AM_SMEM_ROWS(256) <= 227 * 1024, "attention tiles do not fit shared memory");
     static bool done[HB_MAX_DEVICES] = {}, done_mass[HB_MAX_DEVICES] = {};
     if (am_reserve(attention_rows_kernel<T, NC>, AM_SMEM_ROWS(16 * NC), done)) return 1;
@@ -423,10 +419,8 @@ static int launch_rows(const void* q, long long q_stride, const void* kc, const 
     const int vec_kv = hd % 4 == 0 && (((uintptr_t)kc | (uintptr_t)vc) & (four - 1)) == 0;
     const int vec_q = hd % 4 == 0 && q_stride % 4 == 0 && ((uintptr_t)q & (four - 1)) == 0;
     cudaError_t e = hb_launch(attention_rows_kernel<T, NC>, dim3(nh, q_blocks, max_shares), dim3(AM_THREADS), AM_SMEM_ROWS(hd), s, (const T*)q,
-                              q_stride,
-                              (const T*)kc, (const T*)vc, page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, lse, sh, n_tokens, n_seqs,
-                              nh,
-                              nkv, hd, scale * MASS_LOG2E, window, n_pages, vec_q, vec_kv, status);
+                              q_stride, (const T*)kc, (const T*)vc, page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, lse, sh,
+                              n_tokens, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window, n_pages, vec_q, vec_kv, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     if (hb_check_launch("attention_mass (rows)")) return 1;
     if (max_shares > 1 && shares_join(sh, join_tokens, sizeof(T) == 4 ? HB_F32 : HB_BF16, out, out_stride, lse, n_tokens, 0, seq_start, seq_pos0,
@@ -435,8 +429,7 @@ static int launch_rows(const void* q, long long q_stride, const void* kc, const 
         return 1;
     e = hb_launch(mass_rows_kernel<T, NC>, dim3(key_tiles, nkv, splits), dim3(AM_THREADS), AM_SMEM_MASS(hd), s, (const T*)q, q_stride, (const T*)kc,
                   page_table, pt_width, seq_start, seq_pos0, (const float*)lse, mo, n_tokens, n_seqs, nh, nkv, hd, scale * MASS_LOG2E, window,
-                  n_pages,
-                  vec_q, vec_kv, status);
+                  n_pages, vec_q, vec_kv, status);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     if (hb_check_launch("attention_mass (weights)")) return 1;
     return splits > 1 ? mass_join(page_table, pt_width, seq_start, seq_pos0, mo, n_seqs, nkv, n_pages, AM_KEYS, key_tiles, splits, s) : 0;
@@ -729,8 +722,8 @@ template <typename T>
 __global__ void __launch_bounds__(FF_THREADS)
 few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, const float* __restrict__ scores, long long score_ld,
                   const int* __restrict__ page_table, int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0,
-                  T* __restrict__ out,
-                  long long out_stride, MassOut mo, int token_rows, int nh, int nkv, int hd, int S, int window, int n_pages, int vec) {
+                  T* __restrict__ out, long long out_stride, MassOut mo, int token_rows, int nh, int nkv, int hd, int S, int window, int n_pages,
+                  int vec) {
     __shared__ float lse[MASS_FEW_PAIRS];
     pdl_trigger();
     pdl_wait();
@@ -749,7 +742,9 @@ few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
             float M, L;
             join_stats(part_ml, base, S, lane, M, L);
             const float inv = L > 0.0f ? 1.0f / L : 0.0f;
-            for (int d0 = 0; d0 < hd; d0 += 128) {             // four columns a lane, the loads of four shares in flight
+            // (four columns a lane, the loads of four shares in flight: asked for one share after another, 18 shares of two sequences of
+            // 100000 and 65538 rows held the kernel up for 35 us instead of 12.5)
+            for (int d0 = 0; d0 < hd; d0 += 128) {
                 float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 auto shares = [&](int z0, auto count) {
                     constexpr int N = decltype(count)::value;
@@ -829,8 +824,9 @@ extern "C" long long hb_attention_mass_few_floats(int n_tokens, int n_heads, int
 
 template <typename T>
 static int launch_few(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width,
-                      const int* seq_start, const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages, int blocks,
-                      int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages, int seq0, int* status, cudaStream_t s) {
+                      const int* seq_start, const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits,
+                      int share_pages, int blocks, int n_seqs, int nh, int nkv, int hd, float scale, int window, int n_pages, int seq0, int* status,
+                      cudaStream_t s) {
     static_assert(af_smem(256, 4, 2) <= 227 * 1024, "tiles do not fit shared memory");
     static bool done[2][HB_MAX_DEVICES] = {};
     if (am_reserve(few_rows_kernel<T, 2>, af_smem(256, sizeof(T), 2), done[0]) || am_reserve(few_rows_kernel<T, 3>, 114 * 1024, done[1])) return 1;
@@ -852,8 +848,8 @@ static int launch_finish(const float* part_o, const float* part_ml, const float*
     const int key_blocks = (max_len + FF_KEYS - 1) / FF_KEYS;
     const int vec = (((uintptr_t)mo.before | (uintptr_t)mo.mass) & 15) == 0;
     cudaError_t e = hb_launch(few_finish_kernel<T>, dim3(max_new + key_blocks, nkv, n_seqs), dim3(FF_THREADS), 0, s, part_o, part_ml, scores,
-                              score_ld,
-                              page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, mo, max_new, nh, nkv, hd, splits, window, n_pages, vec);
+                              score_ld, page_table, pt_width, seq_start, seq_pos0, (T*)out, out_stride, mo, max_new, nh, nkv, hd, splits, window,
+                              n_pages, vec);
     if (e != cudaSuccess) return hb_fail("attention_mass: launch failed: %s", cudaGetErrorString(e));
     return hb_check_launch("attention_mass (finish)");
 }

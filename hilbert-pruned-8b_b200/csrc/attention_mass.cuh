@@ -168,8 +168,7 @@ __device__ __forceinline__ bool shares_may_cut(const Shares& sh, int rows, int s
 // shares_may_cut.  Blocks of `span` tokens, tiles of `keys`
 // keys; lse[head * lse_ld + place], places in blocks of 128 per sequence and the log-sums negated (`rounded`), or the token's number
 int shares_join(Shares sh, int join_tokens, int dtype, void* out, long long out_stride, float* lse, long long lse_ld, int rounded,
-                const int* seq_start,
-                const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s);
+                const int* seq_start, const int* seq_pos0, int span, int keys, int window, int n_tokens, int n_seqs, int nh, int hd, cudaStream_t s);
 
 // The first half of a step of many tokens on the tensor cores (attention_chunk_tc.cu): writes out and the rows'
 // log-sums, negated, lse[head][place]: a sequence's places begin at a multiple of 128, behind those of the sequences in front.  q_blocks: sum
@@ -179,12 +178,11 @@ int shares_join(Shares sh, int join_tokens, int dtype, void* out, long long out_
 int attention_chunk_tc(const void* q, long long q_stride, const void* k_cache, const void* v_cache, const int* page_table, int pt_width,
                        const int* seq_start, const int* seq_pos0, void* out, long long out_stride, float* lse, long long lse_ld, float* parts,
                        int max_shares, int share_tiles, int join_tokens, int n_tokens, int n_seqs, int q_blocks, int n_heads, int n_kv_heads,
-                       int head_dim, float scale,
-                       int window, int n_pages, int* error_flag, cudaStream_t s);
+                       int head_dim, float scale, int window, int n_pages, int* error_flag, cudaStream_t s);
 
 // The first half of a step of few tokens on the tensor cores (attention_few_tc.cu): token_blocks, the sum over sequences of ceil(new
 // tokens / hb_attention_few_tc_tokens(...)); queries 4-byte, keys and values 16-byte aligned.
-int attention_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width, const int* seq_start,
-                     const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits, int share_pages,
-                     int token_blocks, int max_new,
-                     int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages, int seq0, int* status, cudaStream_t s);
+int attention_few_tc(MassWhole whole, const void* q, long long q_stride, const void* kc, const void* vc, const int* page_table, int pt_width,
+                     const int* seq_start, const int* seq_pos0, float* part_o, float* part_ml, float* scores, long long score_ld, int splits,
+                     int share_pages, int token_blocks, int max_new, int n_seqs, int nh, int nkv, int head_dim, float scale, int window, int n_pages,
+                     int seq0, int* status, cudaStream_t s);

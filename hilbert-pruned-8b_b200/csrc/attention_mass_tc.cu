@@ -11,7 +11,7 @@
 //               (the log-sums come negated)
 // What bounds it: 16 exponentials a clock and SM (1024 clocks for 128 x 128 weights, against 512 for the product at head size
 // 128), so a pair in eight is computed on the FMA pipe instead (none: 684, one: 654, three: 697 us for 2048 tokens behind 30001 rows of the
-// 8B sizes, where the products alone take 418).  Two key tiles share a query tile because an SM takes about 32
+// 8B sizes when that was chosen, 636 now; the products alone take 418).  Two key tiles share a query tile because an SM takes about 32
 // bytes a clock from L2: with one, loading a 32 KB query tile would last as long as its exponentials.
 //
 // Every wait is bounded; a wait that runs out sets *error_flag and the CTA drains and leaves.
@@ -33,10 +33,9 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_
 
 template <int HD>
 __global__ void __launch_bounds__(MT_THREADS, 1)
-mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const int* __restrict__ page_table, int pt_width,
-               const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* lse, long long lse_ld, MassOut mo, int n_seqs,
-               int nh,
-               int nkv, int hd, float scale_log2e, int window, int n_pages, int S, int* __restrict__ error_flag) {
+mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const int* __restrict__ page_table,
+               int pt_width, const int* __restrict__ seq_start, const int* __restrict__ seq_pos0, const float* lse, long long lse_ld, MassOut mo,
+               int n_seqs, int nh, int nkv, int hd, float scale_log2e, int window, int n_pages, int S, int* __restrict__ error_flag) {
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // [K tiles 2][Q stages 3][log-sums of the stages][barriers]; a tile is 128 rows x HD
@@ -49,8 +48,8 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
     const uint32_t k_full = smem_u32(bars), q_full0 = smem_u32(bars + 1), q_empty0 = smem_u32(bars + 4);
     const uint32_t s_full0 = smem_u32(bars + 7), s_empty0 = smem_u32(bars + 9);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    // Under a causal mask a sequence's first keys are seen by the most queries: with the tiles as the slowest index, the shares of the
-    // heaviest ones start first and what ends last is light.
+    // Under a causal mask a sequence's first keys are seen by the most queries: with the tiles as the slowest index, the shares of its
+    // heaviest ones start first and what ends last is light.  (Sequences start in the step's order.)
     const int z = blockIdx.x % S, g = blockIdx.x / S % nkv, G = nh / nkv, tile = blockIdx.x / (S * nkv);
 
     if (threadIdx.x == 0) {
@@ -250,10 +249,8 @@ mass_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 
 template <int HD>
 static int launch_mass_tc(const CUtensorMap& mq, const CUtensorMap& mk, const int* page_table, int pt_width, const int* seq_start,
-                          const int* seq_pos0,
-                          const float* lse, long long lse_ld, MassOut mo, int splits, int n_seqs, int key_tiles, int nh, int nkv, int hd,
-                          float scale, int window,
-                          int n_pages, int* error_flag, cudaStream_t s) {
+                          const int* seq_pos0, const float* lse, long long lse_ld, MassOut mo, int splits, int n_seqs, int key_tiles, int nh,
+                          int nkv, int hd, float scale, int window, int n_pages, int* error_flag, cudaStream_t s) {
     constexpr int SMEM = (2 + MT_STAGES) * (HD / 64) * FA_HALF_BYTES + (MT_STAGES * 128 + 256) * 4 + 16 * 8 + 16 + 1024;
     static_assert(SMEM <= 227 * 1024, "key and query tiles do not fit shared memory");
     static bool done[HB_MAX_DEVICES] = {};

@@ -1324,9 +1324,9 @@ class Ops:
             slots = 2 if at_once else self.lib.hb_attention_few_blocks_per_sm(head_dim, int(bf16))
             splits, least = few_splits(seen, kv_heads, slots * self.sm_count)
         # short sequences, each in one block: it sees all of the keys and no second kernel follows.  (Captured, device time of 32 heads
-        # over 8: size 64, one sequence of 300 rows 7.1 in two kernels and 7.4 us in one, of 440 rows 7.8 and 9.1; eight with four
-        # tokens each 15.8 and 12.6; size 128, 250 rows 8.2 and 8.3, 500 rows 8.9 and 12.6; in 32-bit 60 rows 10.9 and 8.5, 120 rows
-        # 10.9 and 11.3.  The host's part of a call is 2.4 us shorter.)
+        # over 8: size 64, one sequence of 300 rows 8.0 in two kernels and 7.4 us in one, of 384 rows 8.1 and 8.0, of 440 rows 7.8 and 9.1;
+        # eight of 304 rows with four tokens each 17.5 and 12.6; size 128, 256 rows 8.8 and 8.3, 500 rows 8.9 and 12.6; in 32-bit 60 rows
+        # 10.9 and 8.5, 120 rows 10.9 and 11.3.  The host's part of an eager call is 2.4 us shorter too.)
         rows = 64 if not at_once else 256 if head_dim > 64 else 384
         whole = given is None and max_len <= rows and blocks == seqs == sum(n > 0 for n in new) and tokens >= seqs
         splits, least = (1, 1) if whole else (max(1, min(splits, (max_len + 63) // 64)), least)
@@ -1340,8 +1340,13 @@ class Ops:
         their softmax weight of j`` in 32-bit; rows that this step itself appended start from zero, whatever ``before`` holds
         there.  ``before``: None (this step's weights alone), another tensor, or ``mass`` itself (a running sum).  A page belongs to
         one sequence; rows that no sequence of the step holds are neither read nor written.  The step's new keys and values are in
-        the cache already, as for ``attention``; queries, cache and output have one type.  The sums do not depend on what else runs
-        (fixed order)."""
+        the cache already, as for ``attention``; queries, cache and output have one type.  Values have to be finite in every row that a
+        token of the step sees; rows that none sees may hold anything.  A step without new tokens is left as it is.
+
+        The sums are added in a fixed order, which goes by the sizes of the step (all its sequences', and ``step.max_len``): the same
+        step gives the same bits, alone, beside other work or replayed from a graph; the same sequence in another step may be cut in
+        other places.  A captured step of single tokens may be replayed while its sequences grow to ``step.max_len`` rows, one of
+        more tokens with the lengths that it was captured with."""
         k, v = cache.k, cache.v
         self._on(qkv, k, v, out, mass, before)
         T, pages = qkv.shape[0], k.shape[0]

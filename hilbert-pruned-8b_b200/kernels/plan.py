@@ -73,8 +73,8 @@ def chunk_shares(new, lengths, window: int, span: int, keys: int, units: int, ro
     ``keys`` keys in a share, the new tokens of sequences that may be cut).  ``new`` tokens and ``lengths`` of the sequences, blocks of ``span`` tokens, ``units`` heads or pairs of heads,
     ``row_floats`` floats that a share leaves per token, on a device with ``slots`` places.
 
-    Blocks start with the ones that see the most keys, so a step lasts about as long as its work divided by the places, or as its
-    longest block.  Where that is the longer of the two, blocks are cut: with shares of at most t tiles a step lasts about the lesser of
+    A sequence's blocks start with the ones that see the most keys (sequences as the kernels take them: from the step's last to its
+    first, whatever they see), so a step lasts about as long as its work divided by the places, or as its longest block.  Where that is the longer of the two, blocks are cut: with shares of at most t tiles a step lasts about the lesser of
     (work / places + t) and t times the rounds that its shares need.  To start and end a share takes the time of ``own``
     tiles, the kernel that joins the shares that of ``join``.  (Measured: the tensor-core kernel 7 to 9 us against 1.6 to 2 us for a tile of 128
     keys, the kernel for every type about 3 us like its tile of 64.)  The partial results are at most 256 MB in all."""
@@ -108,8 +108,8 @@ def chunk_shares(new, lengths, window: int, span: int, keys: int, units: int, ro
 
 def mass_splits(new, lengths, window: int, tile: int, span: int, kv_heads: int, group: int, cta_slots: int) -> int:
     """Shares of the weights' kernel, whose block takes a tile of keys and goes through the tiles of ``span`` queries of each head that see
-    it.  Under a causal mask the first keys are seen by every query and the last by few, and the heaviest tiles start first: shares so
-    that a heaviest one is about an even share of the work (4096-token prompt: 2, 227 us in all, against 313 with 1 and 239 with 5)."""
+    it.  Under a causal mask the first keys are seen by every query and the last by few, and a sequence's heaviest tiles start first: shares
+    so that a heaviest one is about an even share of the work (4096-token prompt: 2, 242 us in all, against 323 with 1 and 255 with 5)."""
     most = total = 0
     for n, ln in zip(new, lengths):
         if n > 0:

@@ -1068,6 +1068,32 @@ def test_codes_of_waits_that_ran_out_name_their_kernel():
             assert other == mine or not theirs & codes[mine], (mine, other)
 
 
+@pytest.mark.parametrize("degree,bound", [(4, 2.7e-6), (5, 2.2e-7)])
+def test_the_polynomials_of_powers_of_two(degree, bound):
+    """2^x in 32-bit steps with the coefficients that stand in the kernels, against 64 bits: the relative errors that are stated there."""
+    import os
+    import re
+    import numpy as np
+    import hilbert_pruned_8b_b200.kernels.build as build
+    with open(os.path.join(os.path.dirname(os.path.dirname(build.__file__)), "csrc", "exp2_pair.cuh")) as f:
+        source = f.read()
+    body = source[source.index("if (DEG == 5)"): source.index("float r0, r1;")]
+    five, four = body.split("} else {")
+    coefficients = [float(a) for a, b in re.findall(r"pair_of\(([-\d.e]+)f, ([-\d.e]+)f\)", five if degree == 5 else four) if a == b]
+    assert len(coefficients) == degree + 1
+    f32 = np.float32
+    x = np.concatenate([np.linspace(-125, 127, 400001), np.linspace(-1, 1, 400001)]).astype(f32)
+    r = (x + f32(12582912.0)).astype(f32)
+    n = (r - f32(12582912.0)).astype(f32)
+    f = (x - n).astype(f32)                                  # exact: x and n lie within a half
+    assert np.abs(f).max() <= 0.5
+    p = np.full_like(f, f32(coefficients[0]))
+    for c in coefficients[1:]:
+        p = (f.astype(np.float64) * p.astype(np.float64) + np.float64(f32(c))).astype(f32)       # a fused product and sum, rounded once
+    got = p.astype(np.float64) * np.exp2(n.astype(np.float64))
+    assert np.abs(got / np.exp2(x.astype(np.float64)) - 1).max() <= bound
+
+
 def test_groups_of_sequences():
     """Every sequence once and in order, with its tokens, within the limit unless a group has one sequence with new tokens."""
     from hilbert_pruned_8b_b200.kernels.plan import few_groups
