@@ -1370,8 +1370,10 @@ class Ops:
         self._tables("attention", pt)
         if T == 0:
             return
-        self._on(pt, step.seq_start, step.seq_pos0)
-        if pt.shape[0] < step.num_seqs or step.seq_start.shape[0] <= step.num_seqs or step.seq_pos0.shape[0] < step.num_seqs:
+        starts, places, seqs = step.seq_start, step.seq_pos0, step.num_seqs
+        self._on(pt, starts, places)
+        height, width = pt.shape
+        if height < seqs or starts.numel() <= seqs or places.numel() < seqs:
             raise KernelError(f"attention: the page table, starts and places are of fewer than the step's {step.num_seqs} sequences")
         if self._elsewhere():
             with torch.cuda.device(self._index):
@@ -1386,8 +1388,7 @@ class Ops:
             floats, tc, kernels, groups = self._mass_plan(True, fast and q_ld % 2 == 0 and q_at % 4 == 0, dtype == torch.bfloat16, heads, kv_heads,
                                                           head_dim, win, step, splits)
             scratch = torch.empty(floats, dtype=torch.float32, device=self.device)
-            at, tables, width = scratch.data_ptr(), pt.data_ptr(), pt.shape[1]
-            starts, places = step.seq_start.data_ptr(), step.seq_pos0.data_ptr()
+            at, tables, starts, places = scratch.data_ptr(), pt.data_ptr(), starts.data_ptr(), places.data_ptr()
             # (groups of sequences one after another through the same scratch; nearly always one.)
             for whole, seq, seqs, token, tokens, rows, shares, least, blocks in groups:
                 # (the fields of HbMassFew, 8 bytes each: a third of the time of as many arguments)
@@ -1405,7 +1406,7 @@ class Ops:
         lse = scratch.data_ptr()
         parts, partial = lse + 4 * n_lse if n_parts else 0, lse + 4 * (n_lse + n_parts) if n_cut else 0
         # (the fields of HbMassMany)
-        a = array("q", (q_at, code, q_ld, k_at, v_at, pt.data_ptr(), pt.shape[1], step.seq_start.data_ptr(), step.seq_pos0.data_ptr(), out_at, out_ld,
+        a = array("q", (q_at, code, q_ld, k_at, v_at, pt.data_ptr(), width, starts.data_ptr(), places.data_ptr(), out_at, out_ld,
                         lse, lse_ld, old, new, parts, partial, shares, tiles, cut, splits, T, step.num_seqs, q_blocks, key_tiles, heads, kv_heads,
                         head_dim, win, pages, status, stream))
         self._call("hb_attention_mass_tc" if tc else "hb_attention_mass", *a.buffer_info(), scale)
