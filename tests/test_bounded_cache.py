@@ -319,6 +319,24 @@ def test_sequences_in_groups(ops, dtype, heads, kv, hd, window, past, new):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype,hd", [(torch.bfloat16, 64), (torch.float32, 33)])
+def test_groups_name_the_sequence_of_a_missing_page(ops, dtype, hd):
+    """The number in the message is the sequence's in the step, not in its group."""
+    from hilbert_pruned_8b_b200.kernels.ops import KernelError
+    c = Case(dtype, 4, 2, hd, [100, 200, 150, 300, 90], [1, 2, 1, 1, 1], None, seed=1, garbage=0.0)
+    c.table[3, 2] = -1
+    ops.MASS_SCORES = 4 * 2 * 320
+    try:
+        ops.reset_status()
+        c.run(ops, torch.zeros(c.pages, 2, PAGE, device=DEV))
+        with pytest.raises(KernelError, match="sequence 3 of a step"):
+            ops.check_errors()
+    finally:
+        del ops.MASS_SCORES
+        ops.reset_status()
+
+
+@pytest.mark.gpu
 def test_scores_of_one_long_sequence_among_short_ones(ops):
     """64 single tokens, one of them behind 131072 rows: scratch within its limit, captured and eager."""
     past = [50 + b for b in range(64)]
