@@ -746,7 +746,7 @@ few_finish_kernel(const float* __restrict__ part_o, const float* __restrict__ pa
             // 100000 and 65538 rows held the kernel up for 35 us instead of 12.5)
             for (int d0 = 0; d0 < hd; d0 += 128) {
                 float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-auto shares = [&](int z0, auto count) {
+                auto shares = [&](int z0, auto count) {
                     constexpr int N = decltype(count)::value;
                     float mz[N], x[N][4];
 #pragma unroll
@@ -874,7 +874,8 @@ extern "C" int hb_attention_mass_few(const HbMassFew* a, int fields, float scale
                "attention_mass: %d heads over %d kv heads of size %d are not built (sizes up to 256)", n_heads, n_kv_heads, hd);
     HB_REQUIRE((long long)max_new * (n_heads / n_kv_heads) <= MASS_FEW_PAIRS, "attention_mass: %d tokens of %d heads are no step of few tokens",
                max_new, n_heads / n_kv_heads);
-    HB_REQUIRE(n_tokens > 0 && seq0 >= 0 && a->first_token >= 0 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && share_pages >= 1 && blocks >= 1 && blocks <= 65535 && max_len >= 1 &&
+    HB_REQUIRE(n_tokens > 0 && seq0 >= 0 && a->first_token >= 0 && n_seqs <= 65535 && n_kv_heads <= 65535 && splits >= 1 && share_pages >= 1 &&
+                   blocks >= 1 && blocks <= 65535 && max_len >= 1 &&
                    a->scratch != nullptr && a->mass != nullptr,
                "attention_mass: bad sizes");
     HB_REQUIRE(!a->whole || (splits == 1 && blocks == n_seqs), "attention_mass: a whole sequence to a block needs one share and one block each");

@@ -1343,9 +1343,9 @@ class Ops:
         the cache already, as for ``attention``; queries, cache and output have one type.  Values have to be finite in every row that a
         token of the step sees; rows that none sees may hold anything.  A step without new tokens is left as it is.
 
-        The sums are added in a fixed order, which goes by the sizes of the step (all its sequences', and ``step.max_len``): the same
-        step gives the same bits, alone, beside other work or replayed from a graph; the same sequence in another step may be cut in
-        other places.  A captured step of single tokens may be replayed while its sequences grow to ``step.max_len`` rows, one of
+        The sums are added in a fixed order, which goes by the sizes of the step (all its sequences', and ``step.max_len``): a step of
+        the same sizes gives the same bits, alone, beside other work or replayed from a graph; the same sequence in another step may
+        be cut in other places.  A captured step of single tokens may be replayed while its sequences grow to ``step.max_len`` rows, one of
         more tokens with the lengths that it was captured with."""
         k, v = cache.k, cache.v
         self._on(qkv, k, v, out, mass, before)
